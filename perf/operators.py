@@ -11,7 +11,9 @@ The cache holds tiles of 16 values: 16 four-bit E2M1 elements (0, 0.5, 1,
 1.5, 2, 3, 4, 6 and their negatives) and one exponent byte E, value =
 element * 2^(E-127), E = 255 for a tile with a NaN or an infinity in it.  The
 exponent is the smallest at which the tile's largest element rounds to at
-most 6.  A page holds ``page`` tokens of every KV head.
+most 6.  A page holds ``page`` tokens of every KV head, tile by tile: k, v
+(pages, heads, hd/16, page, 8) bytes, the lower half of a byte first, and ke,
+ve (pages, heads, hd/16, page).
 """
 import math
 import sys
@@ -179,9 +181,9 @@ def _batch(case, g):
 def _empty_cache(case, pages):
     """Pages as they are found: whatever bytes were there."""
     g = _gen(pages)
-    shape = (pages, case["hkv"], case["page"])
-    r = lambda n: torch.randint(0, 256, (*shape, n), generator=g, device="cuda", dtype=torch.uint8)  # noqa: E731
-    return {"k": r(case["hd"] // 2), "ke": r(case["hd"] // TILE), "v": r(case["hd"] // 2), "ve": r(case["hd"] // TILE)}
+    shape = (pages, case["hkv"], case["hd"] // TILE, case["page"])
+    r = lambda *n: torch.randint(0, 256, (*shape, *n), generator=g, device="cuda", dtype=torch.uint8)  # noqa: E731
+    return {"k": r(TILE // 2), "ke": r(), "v": r(TILE // 2), "ve": r()}
 
 
 def _filled_cache(case, batch, g):
@@ -193,15 +195,16 @@ def _filled_cache(case, batch, g):
     step = max(1, (1 << 27) // (hkv * page * hd))
     for p in range(0, batch["pages"], step):
         n = min(step, batch["pages"] - p)
-        c["k"][p:p + n], c["ke"][p:p + n] = _quant4(_randn(g, n, hkv, page, hd) * strong)
-        c["v"][p:p + n], c["ve"][p:p + n] = _quant4(_randn(g, n, hkv, page, hd))
+        for data, exp, like in (("k", "ke", strong), ("v", "ve", 1.0)):
+            d, e = _quant4(_randn(g, n, hkv, page, hd) * like)
+            c[data][p:p + n], c[exp][p:p + n] = d.transpose(2, 3), e.transpose(2, 3)
     pos = torch.arange(batch["table"].shape[1] * page, device="cuda").view(1, -1, page)
     stale = (pos >= batch["lens"][:, None, None].long()) & (batch["table"][:, :, None] >= 0)
     b, w, off = stale.nonzero(as_tuple=True)
     ids = batch["table"][b, w].long()
     for name in ("k", "ke", "v", "ve"):
-        c[name][ids, :, off] = torch.randint(0, 256, (len(ids), hkv, c[name].shape[-1]), generator=g, device="cuda",
-                                             dtype=torch.uint8)
+        old = c[name][ids, :, :, off]
+        c[name][ids, :, :, off] = torch.randint(0, 256, old.shape, generator=g, device="cuda", dtype=torch.uint8)
     return c
 
 
@@ -314,7 +317,8 @@ def _rotate(x, cs, interleaved):
 
 
 def _quant4(v):
-    """Values to the cache's tiles: (bytes, exponent bytes)."""
+    """Values (..., hd) to the cache's tiles: bytes (..., hd/16, 8) and
+    exponent bytes (..., hd/16)."""
     t = v.unflatten(-1, (-1, TILE))
     amax = t.abs().amax(-1)
     good = amax.isfinite()
@@ -326,16 +330,16 @@ def _quant4(v):
     step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0)).to(a.dtype)
     a = (torch.round(a / step) * step).clamp(max=6)
     code = torch.where(a < 2, 2 * a, torch.where(a < 4, a + 2, a / 2 + 4)).to(torch.uint8)
-    code = (code | ((t < 0).to(torch.uint8) << 3)).flatten(-2)
+    code = code | ((t < 0).to(torch.uint8) << 3)
     return code[..., 0::2] | (code[..., 1::2] << 4), torch.where(good, e + 127, E_NAN).to(torch.uint8)
 
 
 def _values4(data, exp):
-    """The cache's tiles as float32."""
+    """Tiles (..., hd/16, 8) and their exponents as float32 (..., hd)."""
     lut = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6], device=data.device)
     v = lut[torch.stack([data & 15, data >> 4], -1).flatten(-2).int()]
     scale = torch.where(exp == E_NAN, torch.nan, torch.ldexp(torch.ones_like(exp, dtype=torch.float32), exp.int() - 127))
-    return (v.unflatten(-1, (-1, TILE)) * scale.unsqueeze(-1)).flatten(-2)
+    return (v * scale.unsqueeze(-1)).flatten(-2)
 
 
 def _slots(batch, page):
@@ -361,13 +365,18 @@ def _append(state, case):
     kd, ke = _quant4(k)
     vd, ve = _quant4(v)
     at = torch.where(ok, page, batch["spare"])      # a row without a slot goes to a page that nobody has
-    here = (at, slice(None), off)
+    here = (at, slice(None), slice(None), off)
     c["k"][here], c["ke"][here], c["v"][here], c["ve"][here] = kd, ke, vd, ve
     w, zero = ok[:, None, None], torch.zeros((), device="cuda")
     rk = torch.where(w, _values4(c["k"][here], c["ke"][here]), zero)
     rv = torch.where(w, _values4(c["v"][here], c["ve"][here]), zero)
     q = torch.where(w, q, zero)
     return q.to(DTYPES.get(case["dtype"], torch.float32)), rk.bfloat16(), rv.bfloat16()
+
+
+def _held_by(ids, data, exp):
+    """The tiles of the pages `ids` (seqs, width), token after token."""
+    return data[ids].permute(0, 2, 1, 4, 3, 5).flatten(2, 3), exp[ids].permute(0, 2, 1, 4, 3).flatten(2, 3)
 
 
 def _attend(state, case):
@@ -380,8 +389,8 @@ def _attend(state, case):
     key = torch.arange(width * page, device="cuda")
     there = (key[None] < lens[:, None])[:, None, :, None]                           # seqs, 1, keys, 1
     zero = torch.zeros((), device="cuda")
-    k = torch.where(there, _values4(c["k"][ids], c["ke"][ids]).transpose(1, 2).flatten(2, 3), zero)
-    v = torch.where(there, _values4(c["v"][ids], c["ve"][ids]).transpose(1, 2).flatten(2, 3), zero)
+    k = torch.where(there, _values4(*_held_by(ids, c["k"], c["ke"])), zero)         # seqs, hkv, keys, hd
+    v = torch.where(there, _values4(*_held_by(ids, c["v"], c["ve"])), zero)
     i = torch.arange(n, device="cuda")
     news = cu[1:] - cu[:-1]
     row = (cu[:-1, None] + i[None]).clamp(max=batch["rows"] - 1)                    # seqs, n
@@ -533,7 +542,8 @@ def _exact_attend(state, case):
     at = 0
 
     def held(data, exp, ids, n, h):
-        d, e = data[ids, h].reshape(len(ids) * page, -1)[:n], exp[ids, h].reshape(len(ids) * page, -1)[:n]
+        d = data[ids, h].transpose(1, 2).reshape(len(ids) * page, -1)[:n]
+        e = exp[ids, h].transpose(1, 2).reshape(len(ids) * page, -1)[:n]
         code = torch.stack([d % 16, d // 16], -1).flatten(-2)
         size = (code % 8).double()
         size = torch.where(size < 4, size / 2, torch.where(size < 6, size - 2, 2 * size - 8))
