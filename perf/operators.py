@@ -265,7 +265,7 @@ def _run_own(state, case):
     cache, batch = state["handle"]
     if case["kind"] == "append":
         q = cache.append(batch, state["k"], state["v"], state["cs"], interleaved=case["interleaved"], q=state["q"])
-        k, v = cache.read(batch, dtype=torch.bfloat16)
+        k, v = cache.read(batch, state["batch"]["rows"], dtype=torch.bfloat16)
         return q, k, v
     return cache.attend(batch, state["q"], window=case["window"])
 
