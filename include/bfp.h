@@ -518,6 +518,125 @@ long long bfp_vocab_decode(const bfp_vocab *v, const int32_t *ids, int n, char *
 int bfp_embed_gather_d(const void *lu_m, const void *lu_e, int vocab, int D, int e_row_bytes,
                        const int32_t *ids, int n, int16_t *out_m, int8_t *out_e, void *stream);
 
+/* ------------------------------------------- rows, rotary positions, 4-bit cache */
+/* No counterpart in the reference, whose cache is one float64 array per
+ * layer and whose rope_fp turns one 64-wide head: operators for serving many
+ * long sequences beside bfp_rope_fp_d, bfp_softmax_fp_d and bfp_kv_io.  All
+ * of them are stream-ordered, allocate nothing and keep nothing between
+ * calls, so they can be captured into a graph. */
+
+/* Element types of a bfp_rows. */
+enum bfp_type {
+  BFP_F32 = 0, BFP_BF16 = 1, BFP_F16 = 2,
+  BFP_TILES = 3                 /* 16 int16 mantissas and one int8 exponent a tile */
+};
+
+/* rows x heads x hd values on the device, the hd values of a head side by
+ * side: value (t, h, d) is p[t*row_stride + h*head_stride + d] (strides in
+ * values).  BFP_TILES: p holds mantissas and e one exponent for 16 of them,
+ * that of value offset o at e[o/16]; strides are then multiples of 16. */
+typedef struct bfp_rows {
+  void *p;
+  int8_t *e;
+  int type, heads;
+  long long row_stride, head_stride;
+} bfp_rows;
+
+/* How a context longer than the trained one gets its angles. */
+enum bfp_rope_scaling {
+  BFP_ROPE_NONE = 0,
+  BFP_ROPE_LINEAR = 1,  /* every frequency divided by factor */
+  BFP_ROPE_NTK = 2,     /* base * factor^(rot/(rot-2)): the slowest pair turns factor times slower */
+  BFP_ROPE_PARTS = 3,   /* pairs with more than 32 turns over orig_ctx stay, below one turn divided by
+                         * factor, linear in the pair's index between; mscale = 0.1 ln(factor) + 1 */
+  BFP_ROPE_BANDS = 4    /* more than 4 turns stay, below 1 divided, linear in the turns between */
+};
+/* The rot/2 angles per position inv_freq[j] (from base^(-2j/rot)) and the
+ * factor *mscale on cos and sin.  Host code.  rot even, 2..512; factor >= 1
+ * and orig_ctx > 0 where the scaling uses them. */
+int bfp_rope_freqs(int rot, double base, int scaling, double factor, int orig_ctx,
+                   double *inv_freq, double *mscale);
+/* table[i][j] = (cos, sin)((first + i) * inv_freq[j]) * mscale, evaluated in
+ * float64 and rounded once: n_pos x n_freq x 2 float32 on the device.
+ * inv_freq is a host array of n_freq <= 256 values (copied into the launch);
+ * first >= 0, first + n_pos <= 2^31. */
+int bfp_rope_table_d(const double *inv_freq, int n_freq, double mscale, long long first, int n_pos,
+                     float *table, void *stream);
+/* Rotates the first rot values of every head (rot even, 2 <= rot <= hd) and
+ * copies the rest: with (c, s) = table[pos[t]][j], y_a = a c - b s, y_b = b c +
+ * a s, in float64, where (a, b) are values (j, j + rot/2) of the head
+ * (interleaved 0, as rope_fp pairs them) or (2j, 2j + 1) (interleaved 1).
+ * x and y: n_rows rows, the same number of heads; y BFP_F32, BFP_BF16 or
+ * BFP_F16; y may be x.  pos: n_rows positions; a row whose position is
+ * outside [0, n_pos) gets NaN in its rotated part. */
+int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const float *table,
+               int n_pos, int rot, int interleaved, const bfp_rows *y, void *stream);
+
+/* A key/value cache in 4 bits, in pages of `page` tokens (16, 32, 64, 128 or
+ * 256) of every KV head.  A tile is 16 consecutive values of a head: 16 E2M1
+ * elements (sign, then 0 0.5 1 1.5 2 3 4 6) in 8 bytes, the first in the low
+ * half of the first byte, and one exponent byte E; value = element * 2^(E-127).
+ * Quantisation takes the smallest exponent in -100..100 at which the largest
+ * magnitude of the tile rounds to at most 6, and rounds to nearest, ties to
+ * the even code; a tile with a NaN or an infinity in it is kept as E = 255
+ * and reads as 16 NaNs.
+ *   k, v      (n_pages, heads, hd/16, page, 8) bytes, 16-byte aligned
+ *   k_e, v_e  (n_pages, heads, hd/16, page) bytes, 16-byte aligned
+ * hd: a multiple of 16 up to 256. */
+typedef struct bfp_kv4 {
+  uint8_t *k, *k_e, *v, *v_e;
+  int n_pages, page, heads, hd;
+} bfp_kv4;
+
+/* A batch of sequences with new tokens: rows start[b] .. start[b+1]-1 of the
+ * row arrays are sequence b's newest tokens in order, the last at position
+ * len[b] - 1 (len[b] counts them); token position p lies in page
+ * pages[b*width + p/page] at slot p % page.  start (n_seq + 1, ascending), len
+ * (n_seq) and pages are device arrays of int32.  max_q: no sequence has more
+ * new rows; max_len: no sequence is longer (0: width * page) -- it only
+ * chooses how the work is split.  n_rows bounds the row arrays.  A row whose
+ * position is negative (more rows than len) or whose page is outside
+ * [0, n_pages) has no slot.  Rows outside every sequence are left as they
+ * were. */
+typedef struct bfp_kv4_batch {
+  const int32_t *pages, *start, *len;
+  int n_seq, n_rows, width, max_q, max_len;
+} bfp_kv4_batch;
+
+/* Writes the new tokens' k and v (n_rows x heads x hd) into their slots, k
+ * rotated as bfp_rope_d does at its position first (table NULL: not
+ * rotated).  q and q_out (both or neither): queries rotated by the same
+ * table in the same launch, q_out as bfp_rope_d's y.  pos: positions to
+ * rotate at, per row (NULL: the position in the cache).  A row without a
+ * slot writes nothing, and its q_out is zero; a position outside
+ * [0, n_pos) gives NaN in the rotated part (whole tiles of k).  No two rows
+ * of a call may have the same slot. */
+int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *k,
+                     const bfp_rows *v, const bfp_rows *q, const bfp_rows *q_out, const int32_t *pos,
+                     const float *table, int n_pos, int rot, int interleaved, void *stream);
+/* Reads the batch's rows back: k and v (either may be NULL; BFP_F32, BFP_BF16
+ * or BFP_F16) hold the cached values, exact but for float16's range; a row
+ * without a slot gives zeros. */
+int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *k,
+                   const bfp_rows *v, void *stream);
+/* out = softmax(scale q k^T) v per row and query head over the cache: the
+ * query at position p sees positions p - window + 1 .. p (window 0: 0 .. p) of
+ * its own sequence; query head h reads KV head h / (q->heads / heads).
+ * Positions whose page is outside [0, n_pages) are not seen; a row that sees
+ * nothing gives zeros.  What a row does not see does not reach it, whatever
+ * its bytes.  Products are exact, sums and softmax in float32, probabilities
+ * carried to at least the output's precision.  out: any type (BFP_TILES:
+ * tile_quantize of the float32 result).  work: bfp_kv4_attn_work() bytes of
+ * device scratch, 16-byte aligned (NULL if that is 0); calls that may run at
+ * the same time need their own. */
+int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
+                   const bfp_rows *out, double scale, int window, void *work, size_t work_bytes,
+                   void *stream);
+/* Scratch bytes bfp_kv4_attn_d needs for these arguments (0: none, or
+ * arguments that it refuses). */
+size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
+                         const bfp_rows *out, int window);
+
 #ifdef __cplusplus
 }
 #endif

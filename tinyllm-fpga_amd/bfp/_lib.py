@@ -38,6 +38,26 @@ class StageDumpC(C.Structure):
     _fields_ = [("m", C.c_void_p * N_STAGES), ("e", C.c_void_p * N_STAGES)]
 
 
+class RowsC(C.Structure):
+    """struct bfp_rows."""
+    _fields_ = [("p", C.c_void_p), ("e", C.c_void_p), ("type", C.c_int), ("heads", C.c_int),
+                ("row_stride", C.c_longlong), ("head_stride", C.c_longlong)]
+
+
+class Kv4C(C.Structure):
+    """struct bfp_kv4."""
+    _fields_ = [("k", C.c_void_p), ("k_e", C.c_void_p), ("v", C.c_void_p), ("v_e", C.c_void_p),
+                ("n_pages", C.c_int), ("page", C.c_int), ("heads", C.c_int), ("hd", C.c_int)]
+
+
+class Kv4BatchC(C.Structure):
+    """struct bfp_kv4_batch."""
+    _fields_ = [("pages", C.c_void_p), ("start", C.c_void_p), ("len", C.c_void_p), ("n_seq", C.c_int),
+                ("n_rows", C.c_int), ("width", C.c_int), ("max_q", C.c_int), ("max_len", C.c_int)]
+
+
+_rows, _kv4, _kvb = C.POINTER(RowsC), C.POINTER(Kv4C), C.POINTER(Kv4BatchC)
+
 # name -> (restype, argtypes); the list of exported symbols is checked by the
 # CPU test suite against include/bfp.h.
 SIGNATURES = {
@@ -102,6 +122,13 @@ SIGNATURES = {
     "bfp_vocab_size": (i32, [vp]),
     "bfp_vocab_token": (i32, [vp, i32, C.POINTER(C.c_char_p), C.POINTER(sz)]),
     "bfp_vocab_decode": (i64, [vp, vp, i32, vp, sz]),
+    "bfp_rope_freqs": (i32, [i32, C.c_double, i32, C.c_double, i32, vp, C.POINTER(C.c_double)]),
+    "bfp_rope_table_d": (i32, [vp, i32, C.c_double, i64, i32, vp, vp]),
+    "bfp_rope_d": (i32, [_rows, i32, i32, vp, vp, i32, i32, i32, _rows, vp]),
+    "bfp_kv4_append_d": (i32, [_kv4, _kvb, _rows, _rows, _rows, _rows, vp, vp, i32, i32, i32, vp]),
+    "bfp_kv4_read_d": (i32, [_kv4, _kvb, _rows, _rows, vp]),
+    "bfp_kv4_attn_d": (i32, [_kv4, _kvb, _rows, _rows, C.c_double, i32, vp, sz, vp]),
+    "bfp_kv4_attn_work": (sz, [_kv4, _kvb, _rows, _rows, i32]),
     "bfp_embed_gather_d": (i32, [vp, vp, i32, i32, i32, vp, i32, vp, vp, vp]),
 }
 

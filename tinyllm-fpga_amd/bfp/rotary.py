@@ -1,0 +1,91 @@
+"""Rotary positions on device tensors, beside ``api.rope_fp`` (one 64-wide
+head, one position, float64): the angles of scaled contexts, and the
+rotation of rows of heads in either pairing.
+
+Tensors in and out stay on the device; every call is queued on the current
+stream of their device and can be captured into a graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import _rows
+from ._dev import _torch
+from ._lib import call
+
+SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3, "bands": 4}
+
+
+def rope_freqs(rot, base=10000.0, scaling="none", factor=1.0, orig_ctx=0):
+    """The rot/2 angles per position (float64, host) and the factor on cos
+    and sin.  scaling: how a context `factor` times as long as the trained
+    `orig_ctx` gets its angles --
+      "none"    base^(-2j/rot)
+      "linear"  divided by factor
+      "ntk"     base * factor^(rot/(rot-2))
+      "parts"   pairs that turn more than 32 times over orig_ctx stay, those
+                below one turn are divided, linear in the pair's index
+                between; cos and sin grow by 0.1 ln(factor) + 1
+      "bands"   above 4 turns stay, below 1 divided, linear in the turns"""
+    if scaling not in SCALINGS:
+        raise ValueError(f"scaling {scaling!r}: one of {', '.join(SCALINGS)}")
+    inv = np.empty(max(int(rot) // 2, 1), np.float64)
+    mscale = C.c_double()
+    call("bfp_rope_freqs", int(rot), float(base), SCALINGS[scaling], float(factor), int(orig_ctx),
+         inv.ctypes.data, C.byref(mscale))
+    return inv, mscale.value
+
+
+def rope_table(inv_freq, n_pos, mscale=1.0, first=0, out=None):
+    """(cos, sin) of positions first .. first + n_pos - 1: float32 (n_pos,
+    len(inv_freq), 2) on the current device (out: such a tensor to fill)."""
+    torch = _torch()
+    inv = np.ascontiguousarray(np.asarray(inv_freq, np.float64).reshape(-1))
+    shape = (int(n_pos), inv.size, 2)
+    if out is None:
+        if shape[0] < 0:
+            raise ValueError(f"n_pos={n_pos}")
+        out = torch.empty(shape, dtype=torch.float32, device="cuda")
+    elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or not out.is_cuda:
+        raise ValueError(f"out must be a contiguous float32 tensor {shape} on a GPU")
+    if shape[0]:
+        with _rows.on(out.device):
+            call("bfp_rope_table_d", inv.ctypes.data, inv.size, float(mscale), int(first), shape[0],
+                 out.data_ptr(), _rows.stream_of(out.device))
+    return out
+
+
+def check_table(table, device):
+    """n_pos and rot of a rope_table."""
+    if (table.dim() != 3 or table.shape[2] != 2 or table.dtype != _torch().float32 or not table.is_contiguous()
+            or table.device != device):
+        raise ValueError(f"the table must be rope_table's: contiguous float32 (positions, pairs, 2) on {device}")
+    return table.shape[0], 2 * table.shape[1]
+
+
+def rope(x, pos, table, interleaved=False, out=None, dtype=None):
+    """Rotate the first 2 * table.shape[1] values of every head of x (rows,
+    heads, hd) -- or of 16-bit tiles (m, e) -- by table[pos[row]], and copy
+    the rest.  Pairs are values (j, j + rot/2), as rope_fp has them, or with
+    interleaved (2j, 2j + 1).  A row whose position is not in the table gets
+    NaN there.  Returns `out` (may be x), or a new tensor of `dtype` (x's;
+    float32 for tiles)."""
+    torch = _torch()
+    device = _rows.device_of(x)
+    xr = _rows.rows(x, "x")
+    shape = _rows.shape_of(x)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype or (torch.float32 if isinstance(x, tuple) else x.dtype), device=device)
+    elif isinstance(out, tuple) or tuple(out.shape) != shape or (dtype is not None and out.dtype != dtype):
+        raise ValueError(f"out must be a tensor {shape}" + (f" of {dtype}" if dtype else ""))
+    yr = _rows.rows(out, "out", device)
+    n_pos, rot = check_table(table, device)
+    p = _rows.ints(pos, "pos", device, shape[0])
+    if shape[0] == 0:
+        return out
+    with _rows.on(device):
+        call("bfp_rope_d", C.byref(xr), shape[0], shape[2], p, table.data_ptr(), n_pos, rot,
+             1 if interleaved else 0, C.byref(yr), _rows.stream_of(device))
+    return out

@@ -1,0 +1,592 @@
+// Attention over the 4-bit paged cache.
+//
+// Per query row and head: out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale
+// q.k_j - m), one pass over the keys with the running maximum m and sum
+// (softmax in base 2, float32).  Both products run on the bfloat16 matrix
+// cores.  A cached value has two significant bits, so its bfloat16 is exact;
+// queries and probabilities that need more than bfloat16's eight are split
+// into terms of eight bits, and a row's terms are further columns of the same
+// matrix tile: a decode step has few rows to a KV head (the query heads that
+// share it), so the split costs no further matrix instruction.
+//
+// k_kv4_rows: a workgroup takes up to 16 columns (rows x terms) of one
+// sequence and KV head, its waves take 64 keys in turn.  With S^T = K Q^T the
+// keys are the matrix tile's rows and a lane's K operand is one tile of one
+// key, straight from memory through the decoding conversion.  S^T leaves the
+// probabilities in the layout in which O^T = V^T P^T takes them, with the keys
+// in the order (lane group, register, key of four), so they never move
+// between lanes.  V has to be turned over: its decoded tiles go through the
+// wave's own piece of LDS and come back with the transposing reads.
+#include <math.h>
+
+#include "bfp.h"
+#include "bfp_device.h"
+#include "bfp_f64.h"
+#include "bfp_internal.h"
+#include "bfp_kv4.h"
+#include "bfp_rows.h"
+
+namespace bfp {
+
+constexpr int KEYS = 64;             // keys a wave takes at a time
+// The running maximum is raised only when a score passes it by this many
+// powers of two: probabilities up to 2^8 are as exact as those up to 1, and
+// the sums are rescaled a few times in a whole context instead of whenever a
+// new maximum turns up.
+constexpr float M_SLACK = 8.0f;
+
+struct Kv4AttnArgs {
+  bfp_kv4 c;
+  bfp_kv4_batch b;
+  bfp_rows q, out;
+  int tiles, group, page_shift, window, splits;
+  float scale2;        // scale * log2(e)
+  float *part_o;       // [row][query head][split][hd], where splits > 1
+  float2 *part_ml;     // [row][query head][split]: m, sum
+};
+
+// Position p's visible keys are [lo, hi).
+__device__ __forceinline__ int key_hi(int p) { return p < 0 ? 0 : p + 1; }
+__device__ __forceinline__ int key_lo(int hi, int window) {
+  return window > 0 && hi > window ? hi - window : 0;
+}
+
+// x cut to bfloat16 toward zero: the rest is exact, and has the sign of x.
+__device__ __forceinline__ float cut_bf16(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+
+// Term t of x's split by cuts (three hold any float32).  An infinity or a
+// NaN is its own first term.
+__device__ __forceinline__ float cut_term(float x, int t) {
+  const bool good = fabsf(x) < INFINITY;
+  if (!good) return t == 0 ? (x != x ? NAN : x) : 0.0f;
+  for (int i = 0; i < t; ++i) x -= cut_bf16(x);
+  return cut_bf16(x);
+}
+
+// Term t of x's split by rounding.
+template <int T>
+__device__ __forceinline__ float round_term(float x, int t) {
+  if constexpr (T > 1) {
+#pragma unroll
+    for (int i = 1; i < T && i < 3; ++i) {
+      const float r = x - (float)(__bf16)x;
+      x = t >= i ? r : x;
+    }
+    if constexpr (T == 4) x = t == 3 ? 0.0f : x;
+  }
+  return x;
+}
+
+__device__ __forceinline__ bf16x8 pack8(const float (&v)[8]) {
+  bf16x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (__bf16)v[i];
+  return r;
+}
+
+template <int M>
+__device__ __forceinline__ float fpeer(float v) {
+  return __int_as_float(peer<M>(__float_as_int(v)));
+}
+
+// A sum over the T columns that hold the terms of a row (columns R apart).
+// The wider step first: the result is then the same in all of them.
+template <int T>
+__device__ __forceinline__ float term_sum(float v) {
+  if constexpr (T >= 2) v += fpeer<8>(v);
+  if constexpr (T >= 4) v += fpeer<4>(v);
+  return v;
+}
+
+__device__ __forceinline__ bool has_byte_255(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u;
+}
+// w with its bytes kept where keep has a bit (byte i: bit i).
+__device__ __forceinline__ uint32_t byte_mask(uint32_t keep) {
+  return (((keep & 1) | ((keep & 2) << 7) | ((keep & 4) << 14) | ((keep & 8) << 21)) * 255u);
+}
+
+// One 64-key tile of a wave's operands: lane (r = lane % 16, g = lane / 16)
+// holds keys 4r .. 4r+3 of head tiles g * C .. g * C + C - 1.
+template <int C>
+struct KvTile {
+  uint4 k[C][2], v[C][2];
+  uint32_t ke[C], ve[C];
+  bool ok;
+};
+
+__device__ __forceinline__ uint2 half_of(const uint4 (&w)[2], int j) {
+  return j == 0 ? make_uint2(w[0].x, w[0].y) : j == 1 ? make_uint2(w[0].z, w[0].w)
+         : j == 2 ? make_uint2(w[1].x, w[1].y) : make_uint2(w[1].z, w[1].w);
+}
+
+template <int C>
+__device__ __forceinline__ void load_tile(const Kv4AttnArgs &a, KvTile<C> &x, int id, int head, int key, int g) {
+  x.ok = id >= 0;
+  const long long o = kv4_tile(id < 0 ? 0 : id, a.c.heads, head, a.tiles, g * C, a.c.page, key & (a.c.page - 1));
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (g * C + c < a.tiles) {
+      const long long oc = o + (long long)c * a.c.page;
+      const uint4 *kp = (const uint4 *)(a.c.k + oc * KV4_TILE_BYTES);
+      const uint4 *vp = (const uint4 *)(a.c.v + oc * KV4_TILE_BYTES);
+      x.k[c][0] = kp[0];
+      x.k[c][1] = kp[1];
+      x.ke[c] = *(const uint32_t *)(a.c.k_e + oc);
+      x.v[c][0] = vp[0];
+      x.v[c][1] = vp[1];
+      x.ve[c] = *(const uint32_t *)(a.c.v_e + oc);
+    } else {
+      x.k[c][0] = x.k[c][1] = x.v[c][0] = x.v[c][1] = make_uint4(0, 0, 0, 0);
+      x.ke[c] = x.ve[c] = 0;
+    }
+  }
+}
+
+// LDS rows of 32 keys x hd bfloat16.  A row's bytes are an odd multiple of
+// 32: eight neighbouring rows' 32-byte pieces then lie in different banks,
+// for the writes (a tile of eight keys) and the transposing reads alike.
+__host__ __device__ inline int v_pitch(int tiles) { return 32 * (tiles | 1); }
+constexpr int V_ROWS = 32;
+// Floats of a wave's sums in LDS when the waves are joined: m and sum of 16
+// columns, then R rows of hd (and 4 more, for the banks).
+__host__ __device__ inline int join_floats(int R, int tiles) { return 32 + R * (16 * tiles + 4); }
+
+// Value o of a finished row: one of 16 neighbouring lanes with neighbouring o.
+__device__ __forceinline__ void out_store(const bfp_rows &r, long long o, float v) {
+  if (r.type != BFP_TILES) {
+    row_store(r, o, v);
+    return;
+  }
+  int e;
+  const int m = quantize16_lanes((double)v, e);
+  ((int16_t *)r.p)[o] = (int16_t)m;
+  if ((threadIdx.x & 15) == 0) r.e[o >> 4] = (int8_t)e;
+}
+
+// C: head tiles a lane group holds (hd <= 64 C); T: terms of a row (columns
+// R = 16 / T rows share); W: waves.
+template <int C, int T, int W>
+__global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
+  constexpr int R = 16 / T;
+  extern __shared__ __align__(16) char lds[];
+  const int seq = blockIdx.z, head = blockIdx.y;
+  const int rt = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+  const Kv4Span sp = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
+  const int G = a.group, rows = sp.n * G;   // rows of this KV head: (token, query head)
+  const int rr0 = rt * R;
+  if (rr0 >= rows) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int t = r / R;
+  const int tiles = a.tiles;
+
+  // this lane's column
+  const int rr = rr0 + r % R;
+  const bool mine = rr < rows;
+  const int i = mine ? rr / G : 0, qh = head * G + (mine ? rr % G : 0);
+  const int hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
+  // what all of them see, and any of them
+  const int last = (rr0 + R < rows ? rr0 + R : rows) - 1;
+  const int hi_min = key_hi(sp.at + rr0 / G), hi_max = key_hi(sp.at + last / G);
+  const int lo_min = key_lo(hi_min, a.window), lo_max = key_lo(hi_max, a.window);
+  const long long cap = (long long)a.b.width << a.page_shift;
+  const int end = hi_max < cap ? hi_max : (int)cap;
+  const int tile0 = lo_min / KEYS, n_tiles = end > lo_min ? (end + KEYS - 1) / KEYS - tile0 : 0;
+  const int per = (n_tiles + a.splits - 1) / a.splits;
+  const int first = tile0 + split * per;
+  const int stop = tile0 + (split + 1 < a.splits && (split + 1) * per < n_tiles ? (split + 1) * per : n_tiles);
+
+  // the column's query, term t
+  bf16x8 qf[C][2];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    float x[16];
+    if (mine && g * C + c < tiles) {
+      row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * (g * C + c), x);
+#pragma unroll
+      for (int d = 0; d < 16; ++d) x[d] = T == 1 ? x[d] : cut_term(x[d], t);
+    } else {
+#pragma unroll
+      for (int d = 0; d < 16; ++d) x[d] = 0.0f;
+    }
+    float y[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) y[d] = x[8 * h + d];
+      qf[c][h] = pack8(y);
+    }
+  }
+
+  float m = -INFINITY, sum = 0.0f;
+  f32x4 o[4 * C];
+#pragma unroll
+  for (int d = 0; d < 4 * C; ++d) o[d] = f32x4{0, 0, 0, 0};
+
+  const int pitch = v_pitch(tiles);
+  char *mylds = lds + w * V_ROWS * pitch;
+  char *vput = mylds + r * pitch + g * C * 32;                              // + 16 rows, + a tile
+  const char *vget = mylds + (g * 4 + (r >> 2)) * pitch + (r & 3) * 8;      // + 16 rows, + a tile
+  const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
+  auto page_of = [&](int tile) {
+    return tile < stop ? kv4_page(pages, a.b.width, a.c.n_pages, (tile * KEYS + 4 * r) >> a.page_shift) : -1;
+  };
+
+  KvTile<C> x;
+  int tile = first + w;
+  int id = page_of(tile);
+  if (tile < stop) load_tile(a, x, id, head, tile * KEYS + 4 * r, g);
+  id = page_of(tile + W);
+  for (; tile < stop; tile += W) {
+    KvTile<C> cur = x;
+    if (tile + W < stop) load_tile(a, x, id, head, (tile + W) * KEYS + 4 * r, g);
+    id = page_of(tile + 2 * W);
+    const int t0 = tile * KEYS;
+    const unsigned long long okmask = __ballot(cur.ok);
+    const bool inner = t0 >= lo_max && t0 + KEYS <= hi_min && okmask == ~0ull;
+    if (!inner) {
+      // keys that no row of this workgroup sees become zeros, whatever their bytes
+      uint32_t keep = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = t0 + 4 * r + j;
+        keep |= (cur.ok && key >= lo_min && key < end) ? 1u << j : 0u;
+      }
+      const uint32_t bytes = byte_mask(keep);
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        cur.ve[c] &= bytes;
+        const uint32_t k0 = keep & 1 ? ~0u : 0u, k1 = keep & 2 ? ~0u : 0u, k2 = keep & 4 ? ~0u : 0u, k3 = keep & 8 ? ~0u : 0u;
+        cur.v[c][0] = make_uint4(cur.v[c][0].x & k0, cur.v[c][0].y & k0, cur.v[c][0].z & k1, cur.v[c][0].w & k1);
+        cur.v[c][1] = make_uint4(cur.v[c][1].x & k2, cur.v[c][1].y & k2, cur.v[c][1].z & k3, cur.v[c][1].w & k3);
+      }
+    }
+
+    // scores: s[j][e] is key t0 + 16 g + 4 e + j of column r
+    f32x4 s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float sc = kv4_scale((cur.ke[c] >> (8 * j)) & 255u);
+        const uint2 words = half_of(cur.k[c], j);
+        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv4_decode8(words.x, sc), qf[c][0], s[j], 0, 0, 0);
+        s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv4_decode8(words.y, sc), qf[c][1], s[j], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] = term_sum<T>(s[j][e]) * a.scale2;
+    if (!inner) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool ok = (okmask >> (4 * g + e)) & 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int key = t0 + 16 * g + 4 * e + j;
+          s[j][e] = ok && key >= lo && key < hi ? s[j][e] : -INFINITY;
+        }
+      }
+    }
+
+    // running maximum; a NaN score does not move it and makes its row NaN below
+    float top = s[0][0];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = fmaxf(top, s[j][e]);
+    top = fmaxf(top, fpeer<16>(top));
+    top = fmaxf(top, fpeer<32>(top));
+    const bool raise = top > m + M_SLACK;
+    if (__any(raise)) {
+      const float mn = raise ? top : m;
+      const float f = raise ? exp2f(m - mn) : 1.0f;   // from -infinity: 0
+      m = mn;
+      sum *= f;
+#pragma unroll
+      for (int d = 0; d < 4 * C; ++d) o[d] *= f;
+    }
+    const float m0 = m == -INFINITY ? 0.0f : m;
+    float p[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[j][e] = __builtin_amdgcn_exp2f(s[j][e] - m0);
+        sum += p[j][e];
+      }
+
+    // a tile of V that holds a NaN counts as zeros in the product, so that it
+    // cannot reach a row that does not see it; the rows that do are set after
+    bool nan_v = false;
+#pragma unroll
+    for (int c = 0; c < C; ++c) nan_v |= has_byte_255(cur.ve[c]);
+    const bool any_nan = __any(nan_v);
+#pragma unroll
+    for (int jp = 0; jp < 2; ++jp) {
+      float pv[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pv[e] = round_term<T>(p[2 * jp][e], t);
+        pv[4 + e] = round_term<T>(p[2 * jp + 1][e], t);
+      }
+      const bf16x8 pb = pack8(pv);
+      bf16x8 seen;
+      if (any_nan) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          seen[e] = (__bf16)(s[2 * jp][e] == -INFINITY ? 0.0f : 1.0f);
+          seen[4 + e] = (__bf16)(s[2 * jp + 1][e] == -INFINITY ? 0.0f : 1.0f);
+        }
+      }
+      for (int pass = 0; pass < (any_nan ? 2 : 1); ++pass) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (g * C + c < tiles) {
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+              const int j = 2 * jp + jj;
+              uint32_t E = (cur.ve[c] >> (8 * j)) & 255u;
+              uint2 words = half_of(cur.v[c], j);
+              if (any_nan) {
+                const bool bad = E == KV4_NAN;
+                if (pass == 0) {
+                  words = bad ? make_uint2(0, 0) : words;
+                  E = bad ? 0u : E;
+                } else {   // 1 where the NaNs are
+                  words = bad ? make_uint2(0x22222222u, 0x22222222u) : make_uint2(0, 0);
+                  E = KV4_BIAS;
+                }
+              }
+              const float sc = kv4_scale(E);
+              bf16x8 *dst = (bf16x8 *)(vput + jj * 16 * pitch + c * 32);
+              dst[0] = kv4_decode8(words.x, sc);
+              dst[1] = kv4_decode8(words.y, sc);
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int d = 0; d < 4 * C; ++d) {
+          if (d < tiles) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef short s16x8 __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + d * 32));
+            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + 16 * pitch + d * 32));
+            const s16x8 vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+            const bf16x8 va = __builtin_bit_cast(bf16x8, vv);
+            if (pass == 0) {
+              o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[d], 0, 0, 0);
+            } else {
+              const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, seen, f32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[d][e] = n[e] > 0.0f ? NAN : o[d][e];
+            }
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+
+  // join the terms, then the waves
+  sum += fpeer<16>(sum);
+  sum += fpeer<32>(sum);
+  __syncthreads();
+  const int hd = 16 * tiles, stride = join_floats(R, tiles);
+  float *jw = (float *)lds + w * stride;
+  if (g == 0) {
+    jw[r] = m;
+    jw[16 + r] = sum;
+  }
+#pragma unroll
+  for (int d = 0; d < 4 * C; ++d) {
+    if (d < tiles) {
+      f32x4 v = o[d];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = term_sum<T>(v[e]);
+      if (r < R) *(f32x4 *)(jw + 32 + r * (hd + 4) + 16 * d + 4 * g) = v;
+    }
+  }
+  __syncthreads();
+  const float *jf = (const float *)lds;
+  // 16 lanes to a row's tile
+  for (int u = threadIdx.x >> 4; u < R * tiles; u += 4 * W) {
+    const int row = u / tiles, d = 16 * (u % tiles) + (threadIdx.x & 15);
+    if (rr0 + row >= rows) break;   // all 16 lanes
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < W; ++k) M = fmaxf(M, jf[k * stride + row]);
+    float L = 0.0f, acc = 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const float mk = jf[k * stride + row];
+      const float f = mk == -INFINITY ? 0.0f : exp2f(mk - M);
+      L += f * jf[k * stride + 16 + row];
+      acc += f * jf[k * stride + 32 + row * (hd + 4) + d];
+    }
+    const int ri = (rr0 + row) / G, rh = head * G + (rr0 + row) % G;
+    const long long tok = sp.row0 + ri;
+    if (a.splits > 1) {
+      const long long at = (tok * a.q.heads + rh) * a.splits + split;
+      if (d == 0) a.part_ml[at] = make_float2(M, L);
+      a.part_o[at * hd + d] = acc;
+    } else {
+      out_store(a.out, tok * a.out.row_stride + rh * a.out.head_stride + d, L == 0.0f ? 0.0f : acc / L);
+    }
+  }
+}
+
+// Joins the splits: a wave takes one row and query head.
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
+  const int seq = blockIdx.y;
+  const Kv4Span sp = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
+  const int u = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int i = u / a.q.heads, qh = u % a.q.heads;
+  if (i >= sp.n) return;
+  const long long tok = sp.row0 + i, at = (tok * a.q.heads + qh) * a.splits;
+  const int hd = 16 * a.tiles;
+  float M = -INFINITY, L = 0.0f;
+  for (int k = 0; k < a.splits; ++k) M = fmaxf(M, a.part_ml[at + k].x);
+  float acc[4] = {0, 0, 0, 0};
+  for (int k = 0; k < a.splits; ++k) {
+    const float2 ml = a.part_ml[at + k];
+    if (ml.x == -INFINITY) {   // saw nothing, or nothing but NaN scores
+      L += ml.y;
+      continue;
+    }
+    const float f = exp2f(ml.x - M);
+    L += f * ml.y;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+      if (64 * d + lane < hd) acc[d] += f * a.part_o[(at + k) * hd + 64 * d + lane];
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    if (64 * d + lane < hd)
+      out_store(a.out, tok * a.out.row_stride + qh * a.out.head_stride + 64 * d + lane, L == 0.0f ? 0.0f : acc[d] / L);
+}
+
+// ------------------------------------------------------------------- host
+struct Kv4Plan {
+  int terms, row_tiles, splits;
+  size_t work;
+};
+
+// The terms a row is carried in: one where queries, probabilities and results
+// are bfloat16 and the rows fill the tile's 16 columns anyway; two hold a
+// float16 or 16-bit-tile query and leave probabilities 2^-18 off; three
+// (of four places) hold float32 queries and results.
+static int terms_of(const bfp_rows &q, const bfp_rows &out, int rows) {
+  if (q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES) return 4;
+  return q.type == BFP_BF16 && out.type == BFP_BF16 && rows > 8 ? 1 : 2;
+}
+
+static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_rows &q, const bfp_rows &out, int window) {
+  Kv4Plan p{};
+  const int group = q.heads / c.heads;
+  const long long rows = (long long)b.max_q * group;
+  p.terms = terms_of(q, out, rows > 64 ? 64 : (int)rows);
+  const int R = 16 / p.terms;
+  p.row_tiles = (int)((rows + R - 1) / R);
+  const long long cap = (long long)b.width * c.page;
+  long long keys = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
+  if (window > 0 && keys > (long long)window + b.max_q) keys = (long long)window + b.max_q;
+  const long long tiles = (keys + KEYS - 1) / KEYS;
+  const long long groups = (long long)p.row_tiles * c.heads * b.n_seq;
+  long long s = groups > 0 ? 1024 / groups : 1;
+  if (s > tiles / 4) s = tiles / 4;
+  if (s > 128) s = 128;
+  p.splits = s < 1 ? 1 : (int)s;
+  if (p.splits > 1) {
+    const size_t cells = (size_t)b.n_rows * q.heads * p.splits;
+    p.work = cells * (16 * (c.hd / 16) * sizeof(float) + sizeof(float2));
+  }
+  return p;
+}
+
+static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
+                      const bfp_rows *out, int window) {
+  BFP_TRY(check_kv4(op, cache, batch));
+  if (!q || q->heads < cache->heads || q->heads % cache->heads || q->heads > 65536)
+    return set_err(BFP_EINVAL, "%s: q has %d heads, the cache %d", op, q ? q->heads : 0, cache->heads);
+  BFP_TRY(check_rows(op, "q", q, q->heads, cache->hd, true, batch->n_rows));
+  BFP_TRY(check_out(op, "out", out, q->heads, cache->hd, true, batch->n_rows));
+  if (!rows_aligned(*q, 8)) return set_err(BFP_EINVAL, "%s: q needs 16-byte alignment and strides in multiples of 8", op);
+  if (window < 0) return set_err(BFP_EINVAL, "%s: window=%d", op, window);
+  if ((long long)batch->max_q * (q->heads / cache->heads) > 0x3fffffffLL)
+    return set_err(BFP_EINVAL, "%s: max_q=%d rows of %d heads are too many", op, batch->max_q, q->heads);
+  return BFP_OK;
+}
+
+typedef void (*attn_fn)(Kv4AttnArgs);
+constexpr int ROWS_W = 4;
+template <int C>
+static attn_fn pick_rows(int terms) {
+  return terms == 1 ? k_kv4_rows<C, 1, ROWS_W> : terms == 2 ? k_kv4_rows<C, 2, ROWS_W> : k_kv4_rows<C, 4, ROWS_W>;
+}
+
+}  // namespace bfp
+
+using namespace bfp;
+
+extern "C" {
+
+size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
+                         const bfp_rows *out, int window) {
+  if (check_attn("kv4_attn_work", cache, batch, q, out, window)) return 0;
+  return plan_attn(*cache, *batch, *q, *out, window).work;
+}
+
+int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
+                   const bfp_rows *out, double scale, int window, void *work, size_t work_bytes,
+                   void *stream) {
+  const char *op = "kv4_attn";
+  BFP_TRY(check_attn(op, cache, batch, q, out, window));
+  if (!isfinite(scale)) return set_err(BFP_EINVAL, "%s: scale=%g", op, scale);
+  if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
+  const Kv4Plan p = plan_attn(*cache, *batch, *q, *out, window);
+  if (p.work && (!work || (uintptr_t)work % 16 || work_bytes < p.work))
+    return set_err(BFP_EINVAL, "%s: needs %zu bytes of 16-byte-aligned scratch, got %zu", op, p.work, work ? work_bytes : (size_t)0);
+  Kv4AttnArgs a{};
+  a.c = *cache;
+  a.b = *batch;
+  a.q = *q;
+  a.out = *out;
+  a.tiles = cache->hd / 16;
+  a.group = q->heads / cache->heads;
+  a.page_shift = __builtin_ctz((unsigned)cache->page);
+  a.window = window;
+  a.splits = p.splits;
+  a.scale2 = (float)(scale * 1.44269504088896340736);
+  if (p.work) {
+    const size_t cells = (size_t)batch->n_rows * q->heads * p.splits;
+    a.part_o = (float *)work;
+    a.part_ml = (float2 *)((float *)work + cells * 16 * a.tiles);
+  }
+  const long long blocks = (long long)p.row_tiles * p.splits;
+  if (blocks > 0x7fffffLL) return set_err(BFP_EINVAL, "%s: max_q=%d is too large for one call", op, batch->max_q);
+  const int C = (a.tiles + 3) / 4, R = 16 / p.terms;
+  attn_fn fn = C == 1 ? pick_rows<1>(p.terms) : C == 2 ? pick_rows<2>(p.terms) : C == 3 ? pick_rows<3>(p.terms) : pick_rows<4>(p.terms);
+  const int v_bytes = ROWS_W * V_ROWS * v_pitch(a.tiles), j_bytes = ROWS_W * join_floats(R, a.tiles) * 4;
+  const int lds = v_bytes > j_bytes ? v_bytes : j_bytes;
+  if (lds > 65536)   // the widest heads: one value for a kernel, whatever the call
+    HIP_TRY(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks, cache->heads, batch->n_seq), dim3(64 * ROWS_W), lds, (hipStream_t)stream, a);
+  BFP_TRY(launch_status(op));
+  if (p.splits > 1) {
+    const long long n = ((long long)batch->max_q * q->heads + 3) / 4;
+    hipLaunchKernelGGL(k_kv4_join, dim3((unsigned)n, batch->n_seq), dim3(256), 0, (hipStream_t)stream, a);
+    BFP_TRY(launch_status(op));
+  }
+  return BFP_OK;
+}
+
+}  // extern "C"

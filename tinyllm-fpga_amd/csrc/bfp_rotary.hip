@@ -1,0 +1,215 @@
+// Rotary positions beside rope_fp (rtl/vc707/host/gen_smollm_blockfp_full.py:
+// 250-258): the angles of scaled contexts, and the rotation of rows of heads
+// of any even width in either pairing.
+#include <math.h>
+
+#include "bfp.h"
+#include "bfp_internal.h"
+#include "bfp_rotary.h"
+#include "bfp_rows.h"
+
+namespace bfp {
+
+constexpr int ROPE_BS = 256;
+constexpr int ROPE_MAX_FREQ = 256;
+
+// The frequencies ride in the launch's arguments (2 KB): a call needs no
+// copy to the device and no buffer that outlives it.
+struct RopeFreqs {
+  double inv[ROPE_MAX_FREQ];
+};
+
+// (cos, sin) of one position and frequency a thread.
+__global__ __launch_bounds__(ROPE_BS) void k_rope_table(RopeFreqs f, FastDiv n_freq, double mscale,
+                                                        long long first, uint32_t n,
+                                                        float2 *__restrict__ table) {
+  const uint32_t u = blockIdx.x * ROPE_BS + threadIdx.x;
+  if (u >= n) return;
+  uint32_t j;
+  const uint32_t i = n_freq.div(u, j);
+  double s, c;
+  sincos((double)(first + i) * f.inv[j], &s, &c);
+  table[u] = make_float2((float)(c * mscale), (float)(s * mscale));
+}
+
+struct RopeArgs {
+  bfp_rows x, y;
+  const int32_t *pos;
+  const float2 *table;
+  int hd, n_pos, half, interleaved, row0;
+  FastDiv per_row, per_head;   // units of work of a row, of a head
+  uint32_t units;
+};
+
+// Every unit of a head is one pair, or one value past the rotated part:
+// rows of any width, stride and alignment.
+__global__ __launch_bounds__(ROPE_BS) void k_rope_pairs(RopeArgs a) {
+  const uint32_t u = blockIdx.x * ROPE_BS + threadIdx.x;
+  if (u >= a.units) return;
+  uint32_t rest, j;
+  const uint32_t t = a.row0 + a.per_row.div(u, rest);
+  const uint32_t h = a.per_head.div(rest, j);
+  const long long xo = t * a.x.row_stride + h * a.x.head_stride;
+  const long long yo = t * a.y.row_stride + h * a.y.head_stride;
+  if ((int)j >= a.half) {
+    const int d = (int)j + a.half;
+    row_store(a.y, yo + d, row_load(a.x, xo + d));
+    return;
+  }
+  const int p = a.pos[t];
+  const int da = a.interleaved ? 2 * j : j, db = a.interleaved ? 2 * j + 1 : j + a.half;
+  const bool in = (unsigned)p < (unsigned)a.n_pos;
+  const double2 cs = in ? rope_cs(a.table[(long long)p * a.half + j]) : make_double2(NAN, NAN);
+  double ya, yb;
+  rope_pair(row_load(a.x, xo + da), row_load(a.x, xo + db), cs, ya, yb);
+  row_store(a.y, yo + da, ya);
+  row_store(a.y, yo + db, yb);
+}
+
+// Units of 8 values in 16-byte accesses: 8 pairs (two groups of 8 values) of
+// the half layout, 4 of the interleaved one, or 8 values to copy.
+__global__ __launch_bounds__(ROPE_BS) void k_rope_wide(RopeArgs a) {
+  const uint32_t u = blockIdx.x * ROPE_BS + threadIdx.x;
+  if (u >= a.units) return;
+  uint32_t rest, j;
+  const uint32_t t = a.row0 + a.per_row.div(u, rest);
+  const uint32_t h = a.per_head.div(rest, j);
+  const long long xo = t * a.x.row_stride + h * a.x.head_stride;
+  const long long yo = t * a.y.row_stride + h * a.y.head_stride;
+  const int turned = a.interleaved ? a.half / 4 : a.half / 8;
+  if ((int)j >= turned) {
+    const int d = 2 * a.half + ((int)j - turned) * 8;
+    float v[8];
+    row_load_n(a.x, xo + d, v);
+    row_store_n(a.y, yo + d, v);
+    return;
+  }
+  const int p = a.pos[t];
+  const bool in = (unsigned)p < (unsigned)a.n_pos;
+  const float2 *cs = a.table + (in ? (long long)p * a.half : 0);
+  if (a.interleaved) {
+    float v[8];
+    row_load_n(a.x, xo + 8 * j, v);
+    double y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      rope_pair(v[2 * i], v[2 * i + 1], in ? rope_cs(cs[4 * j + i]) : make_double2(NAN, NAN), y[2 * i],
+                y[2 * i + 1]);
+    row_store_n(a.y, yo + 8 * j, y);
+  } else {
+    float va[8], vb[8];
+    row_load_n(a.x, xo + 8 * j, va);
+    row_load_n(a.x, xo + a.half + 8 * j, vb);
+    double ya[8], yb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      rope_pair(va[i], vb[i], in ? rope_cs(cs[8 * j + i]) : make_double2(NAN, NAN), ya[i], yb[i]);
+    row_store_n(a.y, yo + 8 * j, ya);
+    row_store_n(a.y, yo + a.half + 8 * j, yb);
+  }
+}
+
+}  // namespace bfp
+
+using namespace bfp;
+
+extern "C" {
+
+int bfp_rope_freqs(int rot, double base, int scaling, double factor, int orig_ctx,
+                   double *inv_freq, double *mscale) {
+  if (!inv_freq || !mscale) return set_err(BFP_EINVAL, "rope_freqs: null pointer");
+  if (rot < 2 || rot % 2 || rot > 2 * ROPE_MAX_FREQ)
+    return set_err(BFP_EINVAL, "rope_freqs: rot=%d must be even, 2..%d", rot, 2 * ROPE_MAX_FREQ);
+  if (!(base > 1.0) || !isfinite(base)) return set_err(BFP_EINVAL, "rope_freqs: base=%g", base);
+  if (scaling < BFP_ROPE_NONE || scaling > BFP_ROPE_BANDS)
+    return set_err(BFP_EINVAL, "rope_freqs: no such scaling (%d)", scaling);
+  if (scaling != BFP_ROPE_NONE && (!(factor >= 1.0) || !isfinite(factor)))
+    return set_err(BFP_EINVAL, "rope_freqs: factor=%g must be at least 1", factor);
+  if (scaling >= BFP_ROPE_PARTS && orig_ctx <= 0)
+    return set_err(BFP_EINVAL, "rope_freqs: orig_ctx=%d", orig_ctx);
+  if (scaling == BFP_ROPE_NTK && rot == 2)
+    return set_err(BFP_EINVAL, "rope_freqs: this scaling needs more than one pair");
+  const double turn = 2.0 * M_PI;
+  if (scaling == BFP_ROPE_NTK) base *= pow(factor, (double)rot / (double)(rot - 2));
+  // the pair (a real number) that turns `turns` times over orig_ctx
+  auto pair_of = [&](double turns) {
+    return rot * log((double)orig_ctx / (turns * turn)) / (2.0 * log(base));
+  };
+  double low = 0.0, high = 0.0;
+  if (scaling == BFP_ROPE_PARTS) {
+    low = fmax(floor(pair_of(32.0)), 0.0);
+    high = fmin(ceil(pair_of(1.0)), rot - 1.0);
+  }
+  for (int j = 0; j < rot / 2; ++j) {
+    const double w = pow(base, -(double)(2 * j) / (double)rot);
+    double keep = 1.0;   // the share of the unscaled frequency
+    if (scaling == BFP_ROPE_LINEAR) keep = 0.0;
+    if (scaling == BFP_ROPE_PARTS)
+      keep = 1.0 - fmin(fmax((j - low) / fmax(high - low, 0.001), 0.0), 1.0);
+    if (scaling == BFP_ROPE_BANDS)
+      keep = fmin(fmax(((double)orig_ctx * w / turn - 1.0) / (4.0 - 1.0), 0.0), 1.0);
+    inv_freq[j] = keep == 1.0 ? w : keep == 0.0 ? w / factor : w * keep + w / factor * (1.0 - keep);
+  }
+  *mscale = scaling == BFP_ROPE_PARTS ? 0.1 * log(factor) + 1.0 : 1.0;
+  return BFP_OK;
+}
+
+int bfp_rope_table_d(const double *inv_freq, int n_freq, double mscale, long long first, int n_pos,
+                     float *table, void *stream) {
+  if (!inv_freq || !table) return set_err(BFP_EINVAL, "rope_table: null pointer");
+  if (n_freq < 1 || n_freq > ROPE_MAX_FREQ)
+    return set_err(BFP_EINVAL, "rope_table: n_freq=%d must be in [1, %d]", n_freq, ROPE_MAX_FREQ);
+  if (n_pos < 0 || first < 0 || first + n_pos > (1LL << 31))
+    return set_err(BFP_EINVAL, "rope_table: first=%lld, n_pos=%d", first, n_pos);
+  if ((uintptr_t)table % 8) return set_err(BFP_EINVAL, "rope_table: table is not 8-byte aligned");
+  RopeFreqs f;
+  for (int j = 0; j < ROPE_MAX_FREQ; ++j) f.inv[j] = j < n_freq ? inv_freq[j] : 0.0;
+  // launches of fewer than 2^31 pairs
+  const int step = (int)(0x7fffff00LL / n_freq);
+  for (int i = 0; i < n_pos; i += step) {
+    const int rows = n_pos - i < step ? n_pos - i : step;
+    const uint32_t n = (uint32_t)rows * (uint32_t)n_freq;
+    hipLaunchKernelGGL(k_rope_table, dim3((n + ROPE_BS - 1) / ROPE_BS), dim3(ROPE_BS), 0,
+                       (hipStream_t)stream, f, FastDiv(n_freq), mscale, first + i, n,
+                       (float2 *)table + (long long)i * n_freq);
+    BFP_TRY(launch_status("rope_table"));
+    if (n_pos - i <= step) break;
+  }
+  return BFP_OK;
+}
+
+int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const float *table,
+               int n_pos, int rot, int interleaved, const bfp_rows *y, void *stream) {
+  if (n_rows < 0 || hd < 2 || hd > (1 << 20))
+    return set_err(BFP_EINVAL, "rope: n_rows=%d, hd=%d", n_rows, hd);
+  if (!x || x->heads < 1 || x->heads > (1 << 20))
+    return set_err(BFP_EINVAL, "rope: x %s", x ? "has no heads, or too many" : "is null");
+  BFP_TRY(check_rows("rope", "x", x, x->heads, hd, true, n_rows));
+  BFP_TRY(check_out("rope", "y", y, x->heads, hd, false, n_rows));
+  if (rot < 2 || rot % 2 || rot > hd) return set_err(BFP_EINVAL, "rope: rot=%d, hd=%d", rot, hd);
+  if (!pos || !table || n_pos < 1) return set_err(BFP_EINVAL, "rope: no positions or no table");
+  if ((uintptr_t)table % 8) return set_err(BFP_EINVAL, "rope: table is not 8-byte aligned");
+  if (n_rows == 0) return BFP_OK;
+  const int half = rot / 2;
+  // 16-byte accesses where the groups of 8 fall on them; else value by value
+  const bool wide = rows_aligned(*x, 8) && rows_aligned(*y, 8) && hd % 8 == 0 &&
+                    (interleaved ? rot % 8 == 0 : half % 8 == 0);
+  const int per_head = wide ? (interleaved ? rot / 8 : half / 8) + (hd - rot) / 8 : half + hd - rot;
+  const long long per_row = (long long)per_head * x->heads;
+  if (per_row > 0x3fffffffLL) return set_err(BFP_EINVAL, "rope: rows of %lld units", per_row);
+  RopeArgs a{*x, *y, pos, (const float2 *)table, hd, n_pos, half, interleaved ? 1 : 0, 0,
+             FastDiv((uint32_t)per_row), FastDiv((uint32_t)per_head), 0};
+  const int step = (int)(0x7fffff00LL / per_row);
+  for (int r = 0; r < n_rows;) {
+    const int rows = n_rows - r < step ? n_rows - r : step;
+    a.row0 = r;
+    a.units = (uint32_t)((long long)rows * per_row);
+    hipLaunchKernelGGL(wide ? k_rope_wide : k_rope_pairs, dim3((a.units + ROPE_BS - 1) / ROPE_BS),
+                       dim3(ROPE_BS), 0, (hipStream_t)stream, a);
+    BFP_TRY(launch_status("rope"));
+    r += rows;
+  }
+  return BFP_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,194 @@
+// Rows of values in one of the types of bfp_rows (include/bfp.h): host
+// checks, device loads and stores, and the division the kernels find their
+// row and head with.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "bfp.h"
+#include "bfp_internal.h"
+
+namespace bfp {
+
+// n / d for 0 <= n < 2^31 by a multiplication: sh = ceil(log2 d), mul =
+// ceil(2^(31+sh) / d) < 2^32 (2^sh < 2 d), and n mul / 2^(31+sh) exceeds n / d
+// by less than n / 2^(31+sh) <= 1/d, too little to reach the next whole
+// number.
+struct FastDiv {
+  uint32_t mul = 0, d = 1;
+  int sh = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div) {
+    while ((1ull << sh) < div) ++sh;
+    mul = (uint32_t)(((1ull << (31 + sh)) + div - 1) / div);
+  }
+  __host__ __device__ uint32_t div(uint32_t n) const {
+    return (uint32_t)(((uint64_t)n * mul) >> (31 + sh));
+  }
+  __host__ __device__ uint32_t div(uint32_t n, uint32_t &rem) const {
+    const uint32_t q = div(n);
+    rem = n - q * d;
+    return q;
+  }
+};
+
+// The checks every operator makes of a bfp_rows; what: its name in messages.
+inline int check_rows(const char *op, const char *what, const bfp_rows *r, int heads, int hd,
+                      bool tiles, long long n_rows) {
+  if (!r || !r->p) return set_err(BFP_EINVAL, "%s: %s is null", op, what);
+  if (r->type < BFP_F32 || r->type > BFP_TILES)
+    return set_err(BFP_EINVAL, "%s: %s has no such type (%d)", op, what, r->type);
+  if (r->type == BFP_TILES && (!tiles || !r->e))
+    return set_err(BFP_EINVAL, "%s: %s %s", op, what, tiles ? "has no exponents" : "cannot be tiles");
+  if (r->heads != heads)
+    return set_err(BFP_EINVAL, "%s: %s has %d heads, not %d", op, what, r->heads, heads);
+  if (r->row_stride < 0 || r->head_stride < 0)
+    return set_err(BFP_EINVAL, "%s: %s has a negative stride", op, what);
+  if (r->head_stride < hd && heads > 1)
+    return set_err(BFP_EINVAL, "%s: heads of %s overlap (stride %lld, hd %d)", op, what, r->head_stride, hd);
+  if (r->type == BFP_TILES && (hd % 16 || r->row_stride % 16 || r->head_stride % 16))
+    return set_err(BFP_EINVAL, "%s: tiles of %s need hd and strides in multiples of 16", op, what);
+  const int size = r->type == BFP_F32 ? 4 : 2;
+  if ((uintptr_t)r->p % size) return set_err(BFP_EINVAL, "%s: %s is not aligned to its type", op, what);
+  // offsets are 64-bit; the last one still has to fit
+  const long long last = n_rows > 0 ? n_rows - 1 : 0;
+  if (r->row_stride > 0 && last > (1LL << 60) / r->row_stride)
+    return set_err(BFP_EINVAL, "%s: %s is too large", op, what);
+  return BFP_OK;
+}
+
+// The same for rows that are written: no two of them may share a value.
+inline int check_out(const char *op, const char *what, const bfp_rows *r, int heads, int hd,
+                     bool tiles, long long n_rows) {
+  BFP_TRY(check_rows(op, what, r, heads, hd, tiles, n_rows));
+  if (r->row_stride < hd && n_rows > 1)
+    return set_err(BFP_EINVAL, "%s: rows of %s overlap (stride %lld, hd %d)", op, what, r->row_stride, hd);
+  return BFP_OK;
+}
+
+// Whether groups of n values (n values a multiple of 16 bytes) that start at
+// multiples of n in a head can be moved with 16-byte accesses.
+inline bool rows_aligned(const bfp_rows &r, int n) {
+  return (uintptr_t)r.p % 16 == 0 && r.row_stride % n == 0 && r.head_stride % n == 0;
+}
+
+__device__ __forceinline__ float bf16_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
+// Round to nearest even; NaN stays NaN.
+__device__ __forceinline__ uint16_t f32_to_bf16(float f) {
+  const __bf16 b = (__bf16)f;
+  return __builtin_bit_cast(uint16_t, b);
+}
+__device__ __forceinline__ float f16_to_f32(uint32_t b) {
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+}
+__device__ __forceinline__ uint16_t f32_to_f16(float f) {
+  const _Float16 h = (_Float16)f;
+  return __builtin_bit_cast(uint16_t, h);
+}
+// float64 to 16 bits with one rounding: float32 first, toward zero with the
+// lost bits gathered in the last one (so that no value moves onto a point
+// halfway between two 16-bit numbers), then to nearest.
+__device__ __forceinline__ float f64_to_f32_sticky(double d) {
+  const float f = (float)d;
+  const double back = (double)f;
+  uint32_t b = __float_as_uint(f);
+  if (fabs(back) > fabs(d)) --b;      // also from infinity to the largest float
+  if (back != d && d == d) b |= 1u;
+  return __uint_as_float(b);
+}
+
+// A tile's values are m 2^(e-15): exact in float32 (|m| <= 2^15, e >= -128).
+__device__ __forceinline__ float tile_value(int m, int e) { return ldexpf((float)m, e - 15); }
+
+// One value.
+__device__ __forceinline__ float row_load(const bfp_rows &r, long long o) {
+  switch (r.type) {
+    case BFP_F32: return ((const float *)r.p)[o];
+    case BFP_BF16: return bf16_to_f32(((const uint16_t *)r.p)[o]);
+    case BFP_F16: return f16_to_f32(((const uint16_t *)r.p)[o]);
+    default: return tile_value(((const int16_t *)r.p)[o], r.e[o >> 4]);
+  }
+}
+
+// N values (8 or 16) from a 16-byte-aligned offset; all lie in one tile.
+template <int N>
+__device__ __forceinline__ void row_load_n(const bfp_rows &r, long long o, float (&v)[N]) {
+  static_assert(N == 8 || N == 16, "");
+  if (r.type == BFP_F32) {
+    const float4 *p = (const float4 *)((const float *)r.p + o);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 x = p[i];
+      v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+    }
+    return;
+  }
+  const uint4 *p = (const uint4 *)((const uint16_t *)r.p + o);
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    const uint4 x = p[i];
+    w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+  }
+  if (r.type == BFP_BF16) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else if (r.type == BFP_F16) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      v[2 * i] = f16_to_f32(w[i] & 0xffffu);
+      v[2 * i + 1] = f16_to_f32(w[i] >> 16);
+    }
+  } else {
+    const int e = r.e[o >> 4];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      v[2 * i] = tile_value((int16_t)(w[i] & 0xffffu), e);
+      v[2 * i + 1] = tile_value((int16_t)(w[i] >> 16), e);
+    }
+  }
+}
+
+// One value out (never tiles).
+__device__ __forceinline__ void row_store(const bfp_rows &r, long long o, float v) {
+  switch (r.type) {
+    case BFP_F32: ((float *)r.p)[o] = v; break;
+    case BFP_BF16: ((uint16_t *)r.p)[o] = f32_to_bf16(v); break;
+    default: ((uint16_t *)r.p)[o] = f32_to_f16(v); break;
+  }
+}
+__device__ __forceinline__ void row_store(const bfp_rows &r, long long o, double v) {
+  row_store(r, o, r.type == BFP_F32 ? (float)v : f64_to_f32_sticky(v));
+}
+
+// N values out to a 16-byte-aligned offset.
+template <int N, typename F>
+__device__ __forceinline__ void row_store_n(const bfp_rows &r, long long o, const F (&v)[N]) {
+  static_assert(N == 8 || N == 16, "");
+  if (r.type == BFP_F32) {
+    float4 *p = (float4 *)((float *)r.p + o);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      p[i] = make_float4((float)v[4 * i], (float)v[4 * i + 1], (float)v[4 * i + 2], (float)v[4 * i + 3]);
+    return;
+  }
+  uint32_t w[N / 2];
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) {
+    float a, b;
+    if constexpr (sizeof(F) == 8)
+      a = f64_to_f32_sticky(v[2 * i]), b = f64_to_f32_sticky(v[2 * i + 1]);
+    else
+      a = v[2 * i], b = v[2 * i + 1];
+    w[i] = r.type == BFP_BF16 ? (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16)
+                              : (uint32_t)f32_to_f16(a) | ((uint32_t)f32_to_f16(b) << 16);
+  }
+  uint4 *p = (uint4 *)((uint16_t *)r.p + o);
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) p[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+
+}  // namespace bfp
