@@ -16,12 +16,14 @@ from __future__ import annotations
 import ctypes as C
 import math
 
+import torch
+
 from . import _rows
-from ._dev import _torch
-from ._lib import Kv4BatchC, Kv4C, call, lib
+from ._lib import Kv4BatchC, Kv4C, lib
 from .rotary import check_table
 
 TILE = 16
+_append, _read, _attend = (_rows.Entry(f"bfp_kv4_{name}_d") for name in ("append", "read", "attn"))
 
 
 class Batch:
@@ -38,7 +40,6 @@ class Batch:
         if pages.dim() != 2 or pages.shape[1] < 1:
             raise ValueError(f"pages has shape {tuple(pages.shape)}, not (sequences, width)")
         n = pages.shape[0]
-        torch = _torch()
         for t, what, shape in ((pages, "pages", tuple(pages.shape)), (start, "start", (n + 1,)), (lens, "lens", (n,))):
             if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != pages.device \
                     or not t.is_cuda:
@@ -48,10 +49,17 @@ class Batch:
         self.pages, self.start, self.lens = pages, start, lens
         self.max_q, self.max_len = int(max_q), int(max_len)
         self.device = pages.device
+        self._made = (-1, None)
 
     def _c(self, n_rows):
-        return Kv4BatchC(self.pages.data_ptr(), self.start.data_ptr(), self.lens.data_ptr(), self.pages.shape[0],
-                         n_rows, self.pages.shape[1], self.max_q, self.max_len)
+        """The struct for row arrays of n_rows (this object keeps the tensors
+        it points to)."""
+        n, c = self._made
+        if n != n_rows:
+            c = Kv4BatchC(self.pages.data_ptr(), self.start.data_ptr(), self.lens.data_ptr(), self.pages.shape[0],
+                          n_rows, self.pages.shape[1], self.max_q, self.max_len)
+            self._made = (n_rows, c)
+        return C.byref(c)
 
 
 class Fp4Cache:
@@ -60,7 +68,6 @@ class Fp4Cache:
     (Batch.pages)."""
 
     def __init__(self, n_pages, page, heads, hd, device=None):
-        torch = _torch()
         if n_pages < 1 or heads < 1 or hd < TILE or hd % TILE:
             raise ValueError(f"n_pages={n_pages}, heads={heads}, hd={hd} (a multiple of {TILE})")
         device = torch.device("cuda" if device is None else device)
@@ -77,7 +84,6 @@ class Fp4Cache:
         return self
 
     def _set(self, k, k_exp, v, v_exp):
-        torch = _torch()
         if k.dim() != 5 or k.shape[4] != TILE // 2:
             raise ValueError(f"k has shape {tuple(k.shape)}, not (n_pages, heads, hd/16, page, 8)")
         for t, what, shape in ((k, "k", k.shape), (v, "v", k.shape), (k_exp, "k_exp", k.shape[:4]),
@@ -91,14 +97,18 @@ class Fp4Cache:
         self.k, self.k_exp, self.v, self.v_exp = k, k_exp, v, v_exp
         self.n_pages, self.heads, self.hd, self.page = n_pages, heads, tiles * TILE, page
         self.device = k.device
-        self._c = Kv4C(k.data_ptr(), k_exp.data_ptr(), v.data_ptr(), v_exp.data_ptr(), n_pages, page, heads, self.hd)
+        self._scale = 1.0 / math.sqrt(self.hd)
+        self._made = Kv4C(k.data_ptr(), k_exp.data_ptr(), v.data_ptr(), v_exp.data_ptr(), n_pages, page, heads, self.hd)
+        self._c = C.byref(self._made)
 
-    def _check(self, batch, shape, what, heads=None):
+    def _values(self, batch, x, what):
+        """x's values, checked against the batch and the head width."""
         if batch.device != self.device:
             raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
-        want = (self.heads if heads is None else heads, self.hd)
-        if len(shape) != 3 or shape[1:] != want:
-            raise ValueError(f"{what} has shape {shape}, not (rows, {want[0]}, {want[1]})")
+        t = _rows.values_of(x, what)
+        if t.shape[2] != self.hd:
+            raise ValueError(f"{what} has shape {tuple(t.shape)}, not (rows, heads, {self.hd})")
+        return t
 
     def append(self, batch, k, v, table=None, interleaved=False, pos=None, q=None, q_out=None):
         """Write the batch's new k and v (rows, heads, hd) into their slots,
@@ -109,35 +119,35 @@ class Fp4Cache:
         every sequence are undefined.  A row whose position is negative, or
         whose page is not one of the cache's, writes nothing, and its
         rotated query is zero."""
-        kr, vr = _rows.rows(k, "k", self.device), _rows.rows(v, "v", self.device)
-        shape = _rows.shape_of(k)
-        self._check(batch, shape, "k")
-        if _rows.shape_of(v) != shape:
-            raise ValueError(f"k {shape} and v {_rows.shape_of(v)} differ")
-        n = shape[0]
-        qr = qo = None
+        dev = self.device
+        kt, vt = self._values(batch, k, "k"), self._values(batch, v, "v")
+        n = kt.shape[0]
+        if kt.shape[1] != self.heads or vt.shape != kt.shape:
+            raise ValueError(f"k {tuple(kt.shape)} and v {tuple(vt.shape)} must both be (rows, {self.heads}, {self.hd})")
+        kr, vr = _rows.rows(k, "k", dev), _rows.rows(v, "v", dev)
+        qb = ob = None
         if q is not None:
-            qr = _rows.rows(q, "q", self.device)
-            qs = _rows.shape_of(q)
-            if qs[0] != n or qs[2] != self.hd:
-                raise ValueError(f"q has shape {qs}, not ({n}, heads, {self.hd})")
+            qt = self._values(batch, q, "q")
+            if qt.shape[0] != n:
+                raise ValueError(f"q has {qt.shape[0]} rows, k {n}")
+            qr = _rows.rows(q, "q", dev)
             if q_out is None:
-                torch = _torch()
-                q_out = torch.empty(qs, dtype=torch.float32 if isinstance(q, tuple) else q.dtype, device=self.device)
-            elif _rows.shape_of(q_out) != qs:
-                raise ValueError(f"q_out has shape {_rows.shape_of(q_out)}, not {qs}")
-            qo = _rows.rows(q_out, "q_out", self.device)
+                q_out, qo = _rows.new(q, qt, None)
+            elif type(q_out) is tuple or q_out.shape != qt.shape:
+                raise ValueError(f"q_out must be a tensor {tuple(qt.shape)}")
+            else:
+                qo = _rows.rows(q_out, "q_out", dev)
+            qb, ob = C.byref(qr), C.byref(qo)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        n_pos, rot = check_table(table, self.device) if table is not None else (0, 0)
-        p = _rows.ints(pos, "pos", self.device, n) if pos is not None else None
-        if n == 0:
-            return q_out
-        with _rows.on(self.device):
-            call("bfp_kv4_append_d", C.byref(self._c), C.byref(batch._c(n)), C.byref(kr), C.byref(vr),
-                 C.byref(qr) if qr is not None else None, C.byref(qo) if qo is not None else None, p,
-                 table.data_ptr() if table is not None else None, n_pos, rot, 1 if interleaved else 0,
-                 _rows.stream_of(self.device))
+        tp, n_pos, rot = None, 0, 0
+        if table is not None:
+            n_pos, rot = check_table(table, dev)
+            tp = table.data_ptr()
+        p = _rows.ints(pos, "pos", dev, n) if pos is not None else None
+        if n:
+            _append(dev, self._c, batch._c(n), C.byref(kr), C.byref(vr), qb, ob, p, tp, n_pos, rot,
+                    1 if interleaved else 0)
         return q_out
 
     def read(self, batch, n_rows=None, dtype=None, k=None, v=None):
@@ -146,23 +156,24 @@ class Fp4Cache:
         (float32), whose rows outside every sequence are undefined, or into
         k and v (either may be left out).  A row without a slot gives
         zeros."""
-        torch = _torch()
         if k is None and v is None:
             if n_rows is None:
                 raise ValueError("read needs n_rows, or tensors to read into")
-            k, v = torch.empty(2, int(n_rows), self.heads, self.hd, dtype=dtype or torch.float32, device=self.device)
-        n = (k if k is not None else v).shape[0]
-        rs = []
-        for t, what in ((k, "k"), (v, "v")):
-            rs.append(None if t is None else _rows.rows(t, what, self.device))
-            if t is not None:
-                self._check(batch, _rows.shape_of(t), what)
-                if t.shape[0] != n:
-                    raise ValueError(f"k has {n} rows, v {t.shape[0]}")
+            shape = (int(n_rows), self.heads, self.hd)
+            k = torch.empty(shape, dtype=torch.float32 if dtype is None else dtype, device=self.device)
+            v = torch.empty_like(k)
+        n, rs = None, []
+        for x, what in ((k, "k"), (v, "v")):
+            if x is None:
+                rs.append(None)
+                continue
+            t = self._values(batch, x, what)
+            if t.shape[1] != self.heads or n not in (None, t.shape[0]):
+                raise ValueError(f"{what} has shape {tuple(t.shape)}, not ({'rows' if n is None else n}, {self.heads}, {self.hd})")
+            n = t.shape[0]
+            rs.append(C.byref(_rows.rows(x, what, self.device)))
         if n:
-            with _rows.on(self.device):
-                call("bfp_kv4_read_d", C.byref(self._c), C.byref(batch._c(n)),
-                     *(None if r is None else C.byref(r) for r in rs), _rows.stream_of(self.device))
+            _read(self.device, self._c, batch._c(n), *rs)
         return k, v
 
     def attend(self, batch, q, scale=None, window=0, out=None, dtype=None, work=None):
@@ -174,39 +185,39 @@ class Fp4Cache:
         tiles) whose rows outside every sequence are undefined.  A row that
         sees nothing is zero.  work: uint8 scratch of attend_work() bytes
         (allocated per call otherwise)."""
-        torch = _torch()
-        qr = _rows.rows(q, "q", self.device)
-        shape = _rows.shape_of(q)
-        self._check(batch, shape, "q", shape[1])
-        if shape[1] % self.heads:
-            raise ValueError(f"{shape[1]} query heads for {self.heads} KV heads")
-        if out is None:
-            out = torch.empty(shape, dtype=dtype or (torch.float32 if isinstance(q, tuple) else q.dtype),
-                              device=self.device)
-        elif _rows.shape_of(out) != shape:
-            raise ValueError(f"out has shape {_rows.shape_of(out)}, not {shape}")
-        orow = _rows.rows(out, "out", self.device)
-        if shape[0] == 0:
+        dev = self.device
+        t, qr, out, orow = self._attend_rows(batch, q, out, dtype)
+        n = t.shape[0]
+        if n == 0:
             return out
-        b = batch._c(shape[0])
-        with _rows.on(self.device):
-            if work is None:
-                n = lib().bfp_kv4_attn_work(C.byref(self._c), C.byref(b), C.byref(qr), C.byref(orow), int(window))
-                work = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
-            elif work.device != self.device or not work.is_contiguous():
-                raise ValueError(f"work must be a contiguous tensor on {self.device}")
-            call("bfp_kv4_attn_d", C.byref(self._c), C.byref(b), C.byref(qr), C.byref(orow),
-                 1.0 / math.sqrt(self.hd) if scale is None else float(scale), int(window),
-                 work.data_ptr() if work is not None else None,
-                 work.numel() * work.element_size() if work is not None else 0, _rows.stream_of(self.device))
+        b, qb, ob, window = batch._c(n), C.byref(qr), C.byref(orow), int(window)
+        if work is None:
+            size = lib().bfp_kv4_attn_work(self._c, b, qb, ob, window)
+            if size:
+                work = torch.empty(size, dtype=torch.uint8, device=dev)
+        elif work.device != dev or not work.is_contiguous():
+            raise ValueError(f"work must be a contiguous tensor on {dev}")
+        else:
+            size = work.numel() * work.element_size()
+        _attend(dev, self._c, b, qb, ob, self._scale if scale is None else float(scale), window,
+                work.data_ptr() if work is not None else None, size)
         return out
+
+    def _attend_rows(self, batch, q, out, dtype):
+        t = self._values(batch, q, "q")
+        heads = t.shape[1]
+        if heads % self.heads or not heads:
+            raise ValueError(f"{heads} query heads for {self.heads} KV heads")
+        qr = _rows.rows(q, "q", self.device)
+        if out is None:
+            out, orow = _rows.new(q, t, dtype)
+        else:
+            if self._values(batch, out, "out").shape != t.shape:
+                raise ValueError(f"out must be {tuple(t.shape)}")
+            orow = _rows.rows(out, "out", self.device)
+        return t, qr, out, orow
 
     def attend_work(self, batch, q, out=None, dtype=None, window=0):
         """Scratch bytes attend() needs for such a call."""
-        torch = _torch()
-        qr = _rows.rows(q, "q", self.device)
-        orow = _rows.rows(out if out is not None else torch.empty(
-            _rows.shape_of(q), dtype=dtype or (torch.float32 if isinstance(q, tuple) else q.dtype),
-            device=self.device), "out", self.device)
-        return lib().bfp_kv4_attn_work(C.byref(self._c), C.byref(batch._c(_rows.shape_of(q)[0])), C.byref(qr),
-                                       C.byref(orow), int(window))
+        t, qr, out, orow = self._attend_rows(batch, q, out, dtype)
+        return lib().bfp_kv4_attn_work(self._c, batch._c(t.shape[0]), C.byref(qr), C.byref(orow), int(window))

@@ -10,11 +10,12 @@ from __future__ import annotations
 import ctypes as C
 
 import numpy as np
+import torch
 
 from . import _rows
-from ._dev import _torch
 from ._lib import call
 
+_table, _rope = _rows.Entry("bfp_rope_table_d"), _rows.Entry("bfp_rope_d")
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3, "bands": 4}
 
 
@@ -41,8 +42,9 @@ def rope_freqs(rot, base=10000.0, scaling="none", factor=1.0, orig_ctx=0):
 def rope_table(inv_freq, n_pos, mscale=1.0, first=0, out=None):
     """(cos, sin) of positions first .. first + n_pos - 1: float32 (n_pos,
     len(inv_freq), 2) on the current device (out: such a tensor to fill)."""
-    torch = _torch()
-    inv = np.ascontiguousarray(np.asarray(inv_freq, np.float64).reshape(-1))
+    inv = inv_freq
+    if type(inv) is not np.ndarray or inv.dtype != np.float64 or inv.ndim != 1 or not inv.flags.c_contiguous:
+        inv = np.ascontiguousarray(np.asarray(inv_freq, np.float64).reshape(-1))
     shape = (int(n_pos), inv.size, 2)
     if out is None:
         if shape[0] < 0:
@@ -51,18 +53,17 @@ def rope_table(inv_freq, n_pos, mscale=1.0, first=0, out=None):
     elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or not out.is_cuda:
         raise ValueError(f"out must be a contiguous float32 tensor {shape} on a GPU")
     if shape[0]:
-        with _rows.on(out.device):
-            call("bfp_rope_table_d", inv.ctypes.data, inv.size, float(mscale), int(first), shape[0],
-                 out.data_ptr(), _rows.stream_of(out.device))
+        _table(out.device, inv.ctypes.data, inv.size, float(mscale), int(first), shape[0], out.data_ptr())
     return out
 
 
 def check_table(table, device):
     """n_pos and rot of a rope_table."""
-    if (table.dim() != 3 or table.shape[2] != 2 or table.dtype != _torch().float32 or not table.is_contiguous()
-            or table.device != device):
+    shape = table.shape
+    if len(shape) != 3 or shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous() \
+            or table.device != device:
         raise ValueError(f"the table must be rope_table's: contiguous float32 (positions, pairs, 2) on {device}")
-    return table.shape[0], 2 * table.shape[1]
+    return shape[0], 2 * shape[1]
 
 
 def rope(x, pos, table, interleaved=False, out=None, dtype=None):
@@ -72,20 +73,18 @@ def rope(x, pos, table, interleaved=False, out=None, dtype=None):
     interleaved (2j, 2j + 1).  A row whose position is not in the table gets
     NaN there.  Returns `out` (may be x), or a new tensor of `dtype` (x's;
     float32 for tiles)."""
-    torch = _torch()
-    device = _rows.device_of(x)
-    xr = _rows.rows(x, "x")
-    shape = _rows.shape_of(x)
+    t = _rows.values_of(x, "x")
+    device = _rows.gpu_of(t, "x")
+    xr = _rows.rows(x, "x", device)
+    n, _, hd = t.shape
     if out is None:
-        out = torch.empty(shape, dtype=dtype or (torch.float32 if isinstance(x, tuple) else x.dtype), device=device)
-    elif isinstance(out, tuple) or tuple(out.shape) != shape or (dtype is not None and out.dtype != dtype):
-        raise ValueError(f"out must be a tensor {shape}" + (f" of {dtype}" if dtype else ""))
-    yr = _rows.rows(out, "out", device)
+        out, yr = _rows.new(x, t, dtype)
+    elif type(out) is tuple or out.shape != t.shape or (dtype is not None and out.dtype != dtype):
+        raise ValueError(f"out must be a tensor {tuple(t.shape)}" + (f" of {dtype}" if dtype else ""))
+    else:
+        yr = _rows.rows(out, "out", device)
     n_pos, rot = check_table(table, device)
-    p = _rows.ints(pos, "pos", device, shape[0])
-    if shape[0] == 0:
-        return out
-    with _rows.on(device):
-        call("bfp_rope_d", C.byref(xr), shape[0], shape[2], p, table.data_ptr(), n_pos, rot,
-             1 if interleaved else 0, C.byref(yr), _rows.stream_of(device))
+    p = _rows.ints(pos, "pos", device, n)
+    if n:
+        _rope(device, C.byref(xr), n, hd, p, table.data_ptr(), n_pos, rot, 1 if interleaved else 0, C.byref(yr))
     return out
