@@ -35,6 +35,9 @@ constexpr int KEYS = 64;             // keys a wave takes at a time
 // new maximum turns up.
 constexpr float M_SLACK = 8.0f;
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
 struct Kv4AttnArgs {
   bfp_kv4 c;
   bfp_kv4_batch b;
@@ -375,13 +378,9 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
 #pragma unroll
         for (int d = 0; d < 4 * C; ++d) {
           if (d < tiles) {
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            typedef short s16x8 __attribute__((ext_vector_type(8)));
-            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
             const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + d * 32));
             const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + 16 * pitch + d * 32));
-            const s16x8 vv = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-            const bf16x8 va = __builtin_bit_cast(bf16x8, vv);
+            const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
             if (pass == 0) {
               o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[d], 0, 0, 0);
             } else {
@@ -444,6 +443,291 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
   }
 }
 
+// ------------------------------------------------------------- many rows
+// k_kv4_prompt: a workgroup takes 32 rows a wave of one sequence and KV head
+// (a row is a token and one of the query heads that share the KV head), all
+// waves the same 64 keys.  Each key tile is decoded once into LDS as
+// bfloat16, two buffers deep: the next tile's bytes are on their way while
+// this one is multiplied.  The matrix tiles are 32 x 32: an operand read
+// from LDS (1 KB) then feeds 16384 products, so the waves together ask for
+// what LDS delivers only when the matrix cores run without a pause.  As in
+// k_kv4_rows, keys are the rows of S^T, and the probabilities stay in place.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// K rows: read 16 bytes a lane, 32 rows at a time; 16 bytes past the row put
+// eight neighbouring rows in different banks.  V rows: read by transposing
+// loads of 4 rows x 64 bytes, which an odd multiple of 64 bytes spreads.
+__host__ __device__ inline int pk_pitch(int tiles) { return 32 * tiles + 16; }
+__host__ __device__ inline int pv_pitch(int tiles) { return 64 * (((tiles + 1) / 2) | 1); }
+// A buffer: K, V, and V's exponent bytes (key, 16 tiles).
+__host__ __device__ inline int prompt_buffer(int tiles) { return KEYS * (pk_pitch(tiles) + pv_pitch(tiles) + 16); }
+constexpr int OUT_PITCH = 36;   // floats: 32 values of a row, on their way out
+
+// DT: 32-wide pieces of the head (hd <= 32 DT); T: terms; W: waves.
+template <int DT, int T, int W>
+__global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs a) {
+  constexpr int ROWS = 32 * W, UNITS = (4 * DT + W - 1) / W;
+  extern __shared__ __align__(16) char lds[];
+  // of tile t, at t % 3: set while it is decoded, read a barrier later, cleared
+  // another one later, two barriers before it is set again
+  __shared__ int nan_tiles[3];
+  const int seq = blockIdx.z, head = blockIdx.y;
+  // the last rows see the most keys: first
+  const int rt = (gridDim.x - 1 - blockIdx.x) / a.splits, split = (gridDim.x - 1 - blockIdx.x) % a.splits;
+  const Kv4Span sp = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
+  const int G = a.group, rows = sp.n * G;
+  if (rt >= (rows + ROWS - 1) / ROWS) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+  const int tiles = a.tiles;
+  const int wg0 = rt * ROWS, rr0 = wg0 + 32 * w, rr = rr0 + n;
+  const bool mine = rr < rows;
+  const int i = mine ? rr / G : 0, qh = head * G + (mine ? rr % G : 0);
+  const int hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
+  // what this wave's rows all see, and any of the workgroup's
+  const int wfirst = rr0 < rows ? rr0 : rows - 1, wlast = (rr0 + 32 < rows ? rr0 + 32 : rows) - 1;
+  const int hi_min = key_hi(sp.at + wfirst / G), hi_max = rr0 < rows ? key_hi(sp.at + wlast / G) : 0;
+  const int lo_min = key_lo(hi_min, a.window), lo_max = key_lo(hi_max, a.window);
+  const int glast = (wg0 + ROWS < rows ? wg0 + ROWS : rows) - 1;
+  const int begin = key_lo(key_hi(sp.at + wg0 / G), a.window);
+  const int top_hi = key_hi(sp.at + glast / G);
+  const long long cap = (long long)a.b.width << a.page_shift;
+  const int end = top_hi < cap ? top_hi : (int)cap;
+  const int tile0 = begin / KEYS, n_tiles = end > begin ? (end + KEYS - 1) / KEYS - tile0 : 0;
+  const int per = (n_tiles + a.splits - 1) / a.splits;
+  const int first = tile0 + split * per;
+  const int stop = tile0 + (split + 1 < a.splits && (split + 1) * per < n_tiles ? (split + 1) * per : n_tiles);
+
+  bf16x8 qf[T][2 * DT];
+#pragma unroll
+  for (int c = 0; c < 2 * DT; ++c) {
+    float x[8];
+    if (mine && c < tiles) {
+      row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * c + 8 * h, x);
+    } else {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) x[d] = 0.0f;
+    }
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      float y[8];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) y[d] = T == 1 ? x[d] : cut_term(x[d], t);
+      qf[t][c] = pack8(y);
+    }
+  }
+
+  float m = -INFINITY, sum = 0.0f;
+  f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+
+  const int kp = pk_pitch(tiles), vp = pv_pitch(tiles), buffer = prompt_buffer(tiles);
+  const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
+  // a wave brings in tiles of 64 keys, a key a lane
+  uint2 raw[UNITS];
+  uint32_t rawe[UNITS];
+  unsigned long long okmask = 0, next_ok = 0;
+  auto page_of = [&](int tile) {
+    const int key = tile * KEYS + lane;
+    return tile < stop && key >= begin && key < end ? kv4_page(pages, a.b.width, a.c.n_pages, key >> a.page_shift) : -1;
+  };
+  auto fetch = [&](int tile, int id) {
+    next_ok = __ballot(id >= 0);
+    const long long at = kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + lane) & (a.c.page - 1));
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int x = w + u * W;
+      if (x < 2 * tiles) {
+        const bool is_v = x >= tiles;
+        const long long o8 = at + (long long)(is_v ? x - tiles : x) * a.c.page;
+        raw[u] = id >= 0 ? *(const uint2 *)((is_v ? a.c.v : a.c.k) + o8 * KV4_TILE_BYTES) : make_uint2(0, 0);
+        rawe[u] = id >= 0 ? (is_v ? a.c.v_e : a.c.k_e)[o8] : 0u;
+      }
+    }
+  };
+  auto decode = [&](int tile) {
+    char *b = lds + ((tile - first) & 1) * buffer;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int x = w + u * W;
+      if (x < 2 * tiles) {
+        const bool is_v = x >= tiles;
+        const int ht = is_v ? x - tiles : x;
+        uint2 words = raw[u];
+        uint32_t E = rawe[u];
+        if (is_v) {
+          // NaN tiles count as zeros in the product; the rows that see them are set after
+          ((uint8_t *)b)[KEYS * (kp + vp) + lane * 16 + ht] = (uint8_t)E;
+          if (E == KV4_NAN) {
+            words = make_uint2(0, 0);
+            E = 0;
+            nan_tiles[(tile - first) % 3] = 1;
+          }
+        }
+        const float sc = kv4_scale(E);
+        bf16x8 *dst = (bf16x8 *)(b + (is_v ? KEYS * kp + lane * vp : lane * kp) + 32 * ht);
+        dst[0] = kv4_decode8(words.x, sc);
+        dst[1] = kv4_decode8(words.y, sc);
+      }
+    }
+  };
+
+  if (threadIdx.x < 3) nan_tiles[threadIdx.x] = 0;
+  __syncthreads();
+  int id = page_of(first);
+  if (first < stop) {
+    fetch(first, id);
+    decode(first);
+    okmask = next_ok;
+  }
+  id = page_of(first + 1);
+  __syncthreads();
+  for (int tile = first; tile < stop; ++tile) {
+    const bool more = tile + 1 < stop;
+    if (more) fetch(tile + 1, id);
+    id = page_of(tile + 2);
+    if (threadIdx.x == 0) nan_tiles[(tile - first + 2) % 3] = 0;
+    const char *kb = lds + ((tile - first) & 1) * buffer, *vb = kb + KEYS * kp;
+    const int t0 = tile * KEYS;
+    if (t0 < hi_max && t0 + KEYS > lo_min) {
+      // scores: s[u][e] is key t0 + 32 u + 8 (e / 4) + 4 h + e % 4 of row n
+      f32x16 s[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2 * DT; ++c) {
+          if (c < tiles) {
+            const bf16x8 kf = *(const bf16x8 *)(kb + (32 * u + n) * kp + 32 * c + 16 * h);
+#pragma unroll
+            for (int t = 0; t < T; ++t) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[t][c], s[u], 0, 0, 0);
+          }
+        }
+      }
+      const bool inner = t0 >= lo_max && t0 + KEYS <= hi_min && okmask == ~0ull;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] *= a.scale2;
+      if (!inner) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int k = 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
+            s[u][e] = ((okmask >> k) & 1) && t0 + k >= lo && t0 + k < hi ? s[u][e] : -INFINITY;
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
+      top = fmaxf(top, fpeer<32>(top));
+      const bool raise = top > m + M_SLACK;
+      if (__any(raise)) {
+        const float mn = raise ? top : m;
+        const float f = raise ? exp2f(m - mn) : 1.0f;
+        m = mn;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= f;
+      }
+      const float m0 = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(s[u][e] - m0);
+          sum += p[e];
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          bf16x8 pb[T];
+#pragma unroll
+          for (int t = 0; t < T; ++t) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              pb[t][e] = (__bf16)p[8 * half + e];
+              if (t + 1 < T) p[8 * half + e] -= (float)pb[t][e];
+            }
+          }
+          const char *vr = vb + (32 * u + 16 * half + 4 * h + ((lane & 15) >> 2)) * vp + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            if (2 * d < tiles) {
+              const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 64 * d));
+              const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 8 * vp + 64 * d));
+              const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+              for (int t = 0; t < T; ++t) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[t], o[d], 0, 0, 0);
+            }
+          }
+        }
+      }
+      if (nan_tiles[(tile - first) % 3]) {
+        const uint8_t *ve = (const uint8_t *)vb + KEYS * vp;
+#pragma unroll
+        for (int c = 0; c < 2 * DT; ++c) {
+          if (c < tiles) {
+            bool hit = false;
+            for (int k = 0; k < KEYS; ++k) hit |= ve[16 * k + c] == KV4_NAN && t0 + k >= lo && t0 + k < hi;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[c >> 1][8 * (c & 1) + e] = hit ? NAN : o[c >> 1][8 * (c & 1) + e];
+          }
+        }
+      }
+    }
+    if (more) {   // into the other buffer: its last readers passed the last barrier
+      decode(tile + 1);
+      okmask = next_ok;
+    }
+    __syncthreads();
+  }
+
+  // results: 32 values of the wave's rows at a time through LDS, 16 lanes to a tile
+  sum += fpeer<32>(sum);
+  float *ow = (float *)lds + w * 32 * OUT_PITCH, *ml = (float *)lds + W * 32 * OUT_PITCH + w * 64;
+  if (h == 0) {
+    ml[n] = m;
+    ml[32 + n] = sum;
+  }
+  const int hd = 16 * tiles;
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    if (2 * d >= tiles) break;
+    const f32x16 v = o[d];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      *(f32x4 *)(ow + n * OUT_PITCH + 8 * b + 4 * h) = f32x4{v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    for (int k = lane >> 4; k < 64; k += 4) {
+      const int row = k >> 1, dim = 32 * d + 16 * (k & 1) + (lane & 15);
+      if (rr0 + row >= rows) break;
+      if (dim >= hd) continue;   // all 16 lanes
+      const int ri = (rr0 + row) / G, rh = head * G + (rr0 + row) % G;
+      const long long tok = sp.row0 + ri;
+      const float L = ml[32 + row], acc = ow[row * OUT_PITCH + dim - 32 * d];
+      if (a.splits > 1) {
+        const long long at = (tok * a.q.heads + rh) * a.splits + split;
+        if (dim == 0) a.part_ml[at] = make_float2(ml[row], L);
+        a.part_o[at * hd + dim] = acc;
+      } else {
+        out_store(a.out, tok * a.out.row_stride + rh * a.out.head_stride + dim, L == 0.0f ? 0.0f : acc / L);
+      }
+    }
+  }
+}
+
 // Joins the splits: a wave takes one row and query head.
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
   const int seq = blockIdx.y;
@@ -476,7 +760,8 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
 
 // ------------------------------------------------------------------- host
 struct Kv4Plan {
-  int terms, row_tiles, splits;
+  bool prompt;       // k_kv4_prompt, else k_kv4_rows
+  int terms, waves, row_tiles, splits;
   size_t work;
 };
 
@@ -491,23 +776,32 @@ static int terms_of(const bfp_rows &q, const bfp_rows &out, int rows) {
 
 static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_rows &q, const bfp_rows &out, int window) {
   Kv4Plan p{};
-  const int group = q.heads / c.heads;
+  const int group = q.heads / c.heads, tiles = c.hd / 16;
   const long long rows = (long long)b.max_q * group;
-  p.terms = terms_of(q, out, rows > 64 ? 64 : (int)rows);
-  const int R = 16 / p.terms;
-  p.row_tiles = (int)((rows + R - 1) / R);
   const long long cap = (long long)b.width * c.page;
   long long keys = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
   if (window > 0 && keys > (long long)window + b.max_q) keys = (long long)window + b.max_q;
-  const long long tiles = (keys + KEYS - 1) / KEYS;
+  const long long key_tiles = (keys + KEYS - 1) / KEYS;
+  p.prompt = rows > 64;
+  if (p.prompt) {
+    const bool wide = q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES;
+    p.terms = wide ? 3 : (q.type == BFP_BF16 && out.type == BFP_BF16 ? 1 : 2);
+    p.waves = tiles <= 8 && p.terms < 3 ? 8 : 4;
+    p.row_tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
+  } else {
+    p.terms = terms_of(q, out, (int)rows);
+    p.waves = 4;
+    const int R = 16 / p.terms;
+    p.row_tiles = (int)((rows + R - 1) / R);
+  }
   const long long groups = (long long)p.row_tiles * c.heads * b.n_seq;
-  long long s = groups > 0 ? 1024 / groups : 1;
-  if (s > tiles / 4) s = tiles / 4;
+  long long s = groups > 0 ? (p.prompt ? 512 : 1024) / groups : 1;
+  if (s > key_tiles / 4) s = key_tiles / 4;
   if (s > 128) s = 128;
   p.splits = s < 1 ? 1 : (int)s;
   if (p.splits > 1) {
     const size_t cells = (size_t)b.n_rows * q.heads * p.splits;
-    p.work = cells * (16 * (c.hd / 16) * sizeof(float) + sizeof(float2));
+    p.work = cells * (16 * tiles * sizeof(float) + sizeof(float2));
   }
   return p;
 }
@@ -527,10 +821,13 @@ static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch 
 }
 
 typedef void (*attn_fn)(Kv4AttnArgs);
-constexpr int ROWS_W = 4;
 template <int C>
 static attn_fn pick_rows(int terms) {
-  return terms == 1 ? k_kv4_rows<C, 1, ROWS_W> : terms == 2 ? k_kv4_rows<C, 2, ROWS_W> : k_kv4_rows<C, 4, ROWS_W>;
+  return terms == 1 ? k_kv4_rows<C, 1, 4> : terms == 2 ? k_kv4_rows<C, 2, 4> : k_kv4_rows<C, 4, 4>;
+}
+template <int DT, int W2>
+static attn_fn pick_prompt(int terms) {
+  return terms == 1 ? k_kv4_prompt<DT, 1, W2> : terms == 2 ? k_kv4_prompt<DT, 2, W2> : k_kv4_prompt<DT, 3, 4>;
 }
 
 }  // namespace bfp
@@ -573,13 +870,22 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   }
   const long long blocks = (long long)p.row_tiles * p.splits;
   if (blocks > 0x7fffffLL) return set_err(BFP_EINVAL, "%s: max_q=%d is too large for one call", op, batch->max_q);
-  const int C = (a.tiles + 3) / 4, R = 16 / p.terms;
-  attn_fn fn = C == 1 ? pick_rows<1>(p.terms) : C == 2 ? pick_rows<2>(p.terms) : C == 3 ? pick_rows<3>(p.terms) : pick_rows<4>(p.terms);
-  const int v_bytes = ROWS_W * V_ROWS * v_pitch(a.tiles), j_bytes = ROWS_W * join_floats(R, a.tiles) * 4;
-  const int lds = v_bytes > j_bytes ? v_bytes : j_bytes;
-  if (lds > 65536)   // the widest heads: one value for a kernel, whatever the call
-    HIP_TRY(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024));
-  hipLaunchKernelGGL(fn, dim3((unsigned)blocks, cache->heads, batch->n_seq), dim3(64 * ROWS_W), lds, (hipStream_t)stream, a);
+  attn_fn fn;
+  int lds;
+  if (p.prompt) {
+    fn = a.tiles <= 4 ? pick_prompt<2, 8>(p.terms) : a.tiles <= 6 ? pick_prompt<3, 8>(p.terms)
+         : a.tiles <= 8 ? pick_prompt<4, 8>(p.terms) : a.tiles <= 12 ? pick_prompt<6, 4>(p.terms) : pick_prompt<8, 4>(p.terms);
+    const int in = 2 * prompt_buffer(a.tiles), res = p.waves * (32 * OUT_PITCH + 64) * 4;
+    lds = in > res ? in : res;
+  } else {
+    const int C = (a.tiles + 3) / 4, R = 16 / p.terms;
+    fn = C == 1 ? pick_rows<1>(p.terms) : C == 2 ? pick_rows<2>(p.terms) : C == 3 ? pick_rows<3>(p.terms) : pick_rows<4>(p.terms);
+    const int in = p.waves * V_ROWS * v_pitch(a.tiles), res = p.waves * join_floats(R, a.tiles) * 4;
+    lds = in > res ? in : res;
+  }
+  if (lds > 65536)   // one limit for a kernel, whatever the call
+    HIP_TRY(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 159 * 1024));
+  hipLaunchKernelGGL(fn, dim3((unsigned)blocks, cache->heads, batch->n_seq), dim3(64 * p.waves), lds, (hipStream_t)stream, a);
   BFP_TRY(launch_status(op));
   if (p.splits > 1) {
     const long long n = ((long long)batch->max_q * q->heads + 3) / 4;
