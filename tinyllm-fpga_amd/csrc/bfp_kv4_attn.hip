@@ -35,6 +35,7 @@ constexpr int KEYS = 64;             // keys a wave takes at a time
 // new maximum turns up.
 constexpr float M_SLACK = 8.0f;
 
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
@@ -43,7 +44,9 @@ struct Kv4AttnArgs {
   bfp_kv4_batch b;
   bfp_rows q, out;
   int tiles, group, page_shift, window, splits;
-  float scale2;        // scale * log2(e)
+  float scale2;        // |scale| * log2(e), kept above 0; the queries take the sign
+  float slack;         // M_SLACK in scores: M_SLACK / scale2
+  float q_sign;
   float *part_o;       // [row][query head][split][hd], where splits > 1
   float2 *part_ml;     // [row][query head][split]: m, sum
 };
@@ -209,7 +212,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
     if (mine && g * C + c < tiles) {
       row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * (g * C + c), x);
 #pragma unroll
-      for (int d = 0; d < 16; ++d) x[d] = T == 1 ? x[d] : cut_term(x[d], t);
+      for (int d = 0; d < 16; ++d) x[d] = (T == 1 ? x[d] : cut_term(x[d], t)) * a.q_sign;
     } else {
 #pragma unroll
       for (int d = 0; d < 16; ++d) x[d] = 0.0f;
@@ -283,7 +286,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[j][e] = term_sum<T>(s[j][e]) * a.scale2;
+      for (int e = 0; e < 4; ++e) s[j][e] = term_sum<T>(s[j][e]);
     if (!inner) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int key = t0 + 16 * g + 4 * e + j;
-          s[j][e] = ok && key >= lo && key < hi ? s[j][e] : -INFINITY;
+          s[j][e] = ok & (key >= lo) & (key < hi) ? s[j][e] : -INFINITY;
         }
       }
     }
@@ -304,22 +307,22 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
       for (int e = 0; e < 4; ++e) top = fmaxf(top, s[j][e]);
     top = fmaxf(top, fpeer<16>(top));
     top = fmaxf(top, fpeer<32>(top));
-    const bool raise = top > m + M_SLACK;
+    const bool raise = top > m + a.slack;
     if (__any(raise)) {
       const float mn = raise ? top : m;
-      const float f = raise ? exp2f(m - mn) : 1.0f;   // from -infinity: 0
+      const float f = raise ? exp2f((m - mn) * a.scale2) : 1.0f;   // from -infinity: 0
       m = mn;
       sum *= f;
 #pragma unroll
       for (int d = 0; d < 4 * C; ++d) o[d] *= f;
     }
-    const float m0 = m == -INFINITY ? 0.0f : m;
+    const float m0 = m == -INFINITY ? 0.0f : -m * a.scale2;
     float p[4][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        p[j][e] = __builtin_amdgcn_exp2f(s[j][e] - m0);
+        p[j][e] = __builtin_amdgcn_exp2f(fmaf(s[j][e], a.scale2, m0));
         sum += p[j][e];
       }
 
@@ -402,7 +405,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
   const int hd = 16 * tiles, stride = join_floats(R, tiles);
   float *jw = (float *)lds + w * stride;
   if (g == 0) {
-    jw[r] = m;
+    jw[r] = m * a.scale2;   // base-2 logarithm from here on
     jw[16 + r] = sum;
   }
 #pragma unroll
@@ -457,16 +460,23 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // K rows: read 16 bytes a lane, 32 rows at a time; 16 bytes past the row put
 // eight neighbouring rows in different banks.  V rows: read by transposing
 // loads of 4 rows x 64 bytes, which an odd multiple of 64 bytes spreads.
-__host__ __device__ inline int pk_pitch(int tiles) { return 32 * tiles + 16; }
-__host__ __device__ inline int pv_pitch(int tiles) { return 64 * (((tiles + 1) / 2) | 1); }
+constexpr int pk_pitch(int tb) { return 32 * tb + 16; }
+constexpr int pv_pitch(int tb) { return 64 * ((tb / 2) | 1); }
 // A buffer: K, V, and V's exponent bytes (key, 16 tiles).
-__host__ __device__ inline int prompt_buffer(int tiles) { return KEYS * (pk_pitch(tiles) + pv_pitch(tiles) + 16); }
+constexpr int prompt_buffer(int tb) { return KEYS * (pk_pitch(tb) + pv_pitch(tb) + 16); }
 constexpr int OUT_PITCH = 36;   // floats: 32 values of a row, on their way out
+constexpr int prompt_lds(int tb, int waves) {
+  const int in = 2 * prompt_buffer(tb), out = waves * (32 * OUT_PITCH + 64) * 4;
+  return in > out ? in : out;
+}
 
-// DT: 32-wide pieces of the head (hd <= 32 DT); T: terms; W: waves.
-template <int DT, int T, int W>
+// TB: tiles of the head the loops are built for (even; a narrower head's
+// missing tiles are zeros in K, and columns of V whose results nobody
+// takes); T: terms; W: waves.
+template <int TB, int T, int W>
 __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs a) {
-  constexpr int ROWS = 32 * W, UNITS = (4 * DT + W - 1) / W;
+  constexpr int ROWS = 32 * W, DT = TB / 2, UNITS = (TB + W - 1) / W;
+  constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), BUFFER = prompt_buffer(TB);
   extern __shared__ __align__(16) char lds[];
   // of tile t, at t % 3: set while it is decoded, read a barrier later, cleared
   // another one later, two barriers before it is set again
@@ -477,7 +487,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   const Kv4Span sp = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
   const int G = a.group, rows = sp.n * G;
   if (rt >= (rows + ROWS - 1) / ROWS) return;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, h = lane >> 5;
   const int tiles = a.tiles;
   const int wg0 = rt * ROWS, rr0 = wg0 + 32 * w, rr = rr0 + n;
   const bool mine = rr < rows;
@@ -497,9 +507,9 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   const int first = tile0 + split * per;
   const int stop = tile0 + (split + 1 < a.splits && (split + 1) * per < n_tiles ? (split + 1) * per : n_tiles);
 
-  bf16x8 qf[T][2 * DT];
+  bf16x8 qf[T][TB];
 #pragma unroll
-  for (int c = 0; c < 2 * DT; ++c) {
+  for (int c = 0; c < TB; ++c) {
     float x[8];
     if (mine && c < tiles) {
       row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * c + 8 * h, x);
@@ -511,7 +521,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
     for (int t = 0; t < T; ++t) {
       float y[8];
 #pragma unroll
-      for (int d = 0; d < 8; ++d) y[d] = T == 1 ? x[d] : cut_term(x[d], t);
+      for (int d = 0; d < 8; ++d) y[d] = (T == 1 ? x[d] : cut_term(x[d], t)) * a.q_sign;
       qf[t][c] = pack8(y);
     }
   }
@@ -523,11 +533,10 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
-  const int kp = pk_pitch(tiles), vp = pv_pitch(tiles), buffer = prompt_buffer(tiles);
   const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
-  // a wave brings in tiles of 64 keys, a key a lane
-  uint2 raw[UNITS];
-  uint32_t rawe[UNITS];
+  // wave w brings in head tiles w, w + W, ... of K and V, a key a lane
+  uint2 rk[UNITS], rv[UNITS];
+  uint32_t rke[UNITS], rve[UNITS];
   unsigned long long okmask = 0, next_ok = 0;
   auto page_of = [&](int tile) {
     const int key = tile * KEYS + lane;
@@ -538,38 +547,36 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
     const long long at = kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + lane) & (a.c.page - 1));
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int x = w + u * W;
-      if (x < 2 * tiles) {
-        const bool is_v = x >= tiles;
-        const long long o8 = at + (long long)(is_v ? x - tiles : x) * a.c.page;
-        raw[u] = id >= 0 ? *(const uint2 *)((is_v ? a.c.v : a.c.k) + o8 * KV4_TILE_BYTES) : make_uint2(0, 0);
-        rawe[u] = id >= 0 ? (is_v ? a.c.v_e : a.c.k_e)[o8] : 0u;
+      const int t = w + u * W;
+      rk[u] = rv[u] = make_uint2(0, 0);
+      rke[u] = rve[u] = 0;
+      if (t < tiles && id >= 0) {
+        const long long o8 = at + (long long)t * a.c.page;
+        rk[u] = *(const uint2 *)(a.c.k + o8 * KV4_TILE_BYTES);
+        rv[u] = *(const uint2 *)(a.c.v + o8 * KV4_TILE_BYTES);
+        rke[u] = a.c.k_e[o8];
+        rve[u] = a.c.v_e[o8];
       }
     }
   };
   auto decode = [&](int tile) {
-    char *b = lds + ((tile - first) & 1) * buffer;
+    char *b = lds + ((tile - first) & 1) * BUFFER;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-      const int x = w + u * W;
-      if (x < 2 * tiles) {
-        const bool is_v = x >= tiles;
-        const int ht = is_v ? x - tiles : x;
-        uint2 words = raw[u];
-        uint32_t E = rawe[u];
-        if (is_v) {
-          // NaN tiles count as zeros in the product; the rows that see them are set after
-          ((uint8_t *)b)[KEYS * (kp + vp) + lane * 16 + ht] = (uint8_t)E;
-          if (E == KV4_NAN) {
-            words = make_uint2(0, 0);
-            E = 0;
-            nan_tiles[(tile - first) % 3] = 1;
-          }
-        }
-        const float sc = kv4_scale(E);
-        bf16x8 *dst = (bf16x8 *)(b + (is_v ? KEYS * kp + lane * vp : lane * kp) + 32 * ht);
-        dst[0] = kv4_decode8(words.x, sc);
-        dst[1] = kv4_decode8(words.y, sc);
+      const int t = w + u * W;
+      if (t < TB) {   // tiles the head does not have: zeros
+        const float ks = kv4_scale(rke[u]);
+        bf16x8 *kd = (bf16x8 *)(b + lane * KP + 32 * t);
+        kd[0] = kv4_decode8(rk[u].x, ks);
+        kd[1] = kv4_decode8(rk[u].y, ks);
+        // NaN tiles of V count as zeros in the product; the rows that see them are set after
+        const bool bad = rve[u] == KV4_NAN;
+        ((uint8_t *)b)[KEYS * (KP + VP) + lane * 16 + t] = (uint8_t)rve[u];
+        if (bad) nan_tiles[(tile - first) % 3] = 1;
+        const float vs = kv4_scale(bad ? 0u : rve[u]);
+        bf16x8 *vd = (bf16x8 *)(b + KEYS * KP + lane * VP + 32 * t);
+        vd[0] = kv4_decode8(bad ? 0u : rv[u].x, vs);
+        vd[1] = kv4_decode8(bad ? 0u : rv[u].y, vs);
       }
     }
   };
@@ -589,7 +596,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
     if (more) fetch(tile + 1, id);
     id = page_of(tile + 2);
     if (threadIdx.x == 0) nan_tiles[(tile - first + 2) % 3] = 0;
-    const char *kb = lds + ((tile - first) & 1) * buffer, *vb = kb + KEYS * kp;
+    const char *kb = lds + ((tile - first) & 1) * BUFFER, *vb = kb + KEYS * KP;
     const int t0 = tile * KEYS;
     if (t0 < hi_max && t0 + KEYS > lo_min) {
       // scores: s[u][e] is key t0 + 32 u + 8 (e / 4) + 4 h + e % 4 of row n
@@ -599,26 +606,21 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 2 * DT; ++c) {
-          if (c < tiles) {
-            const bf16x8 kf = *(const bf16x8 *)(kb + (32 * u + n) * kp + 32 * c + 16 * h);
+        for (int c = 0; c < TB; ++c) {
+          const bf16x8 kf = *(const bf16x8 *)(kb + (32 * u + n) * KP + 32 * c + 16 * h);
 #pragma unroll
-            for (int t = 0; t < T; ++t) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[t][c], s[u], 0, 0, 0);
-          }
+          for (int t = 0; t < T; ++t) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[t][c], s[u], 0, 0, 0);
         }
       }
       const bool inner = t0 >= lo_max && t0 + KEYS <= hi_min && okmask == ~0ull;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[u][e] *= a.scale2;
       if (!inner) {
+        const uint32_t ok_h[2] = {(uint32_t)okmask >> (4 * h), (uint32_t)(okmask >> 32) >> (4 * h)};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int k = 32 * u + 8 * (e >> 2) + 4 * h + (e & 3);
-            s[u][e] = ((okmask >> k) & 1) && t0 + k >= lo && t0 + k < hi ? s[u][e] : -INFINITY;
+            const int k = 8 * (e >> 2) + (e & 3), key = t0 + 32 * u + 4 * h + k;
+            s[u][e] = (((ok_h[u] >> k) & 1) != 0) & (key >= lo) & (key < hi) ? s[u][e] : -INFINITY;
           }
       }
       float top = s[0][0];
@@ -627,10 +629,10 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
       top = fmaxf(top, fpeer<32>(top));
-      const bool raise = top > m + M_SLACK;
+      const bool raise = top > m + a.slack;
       if (__any(raise)) {
         const float mn = raise ? top : m;
-        const float f = raise ? exp2f(m - mn) : 1.0f;
+        const float f = raise ? exp2f((m - mn) * a.scale2) : 1.0f;
         m = mn;
         sum *= f;
 #pragma unroll
@@ -638,49 +640,55 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[d][e] *= f;
       }
-      const float m0 = m == -INFINITY ? 0.0f : m;
+      const float m0 = m == -INFINITY ? 0.0f : -m * a.scale2;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float p[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          p[e] = __builtin_amdgcn_exp2f(s[u][e] - m0);
-          sum += p[e];
-        }
+        for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], a.scale2, m0));
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           bf16x8 pb[T];
+          if constexpr (T == 1) {
+            // the sum takes the probabilities as the product takes them
 #pragma unroll
-          for (int t = 0; t < T; ++t) {
+            for (int e = 0; e < 8; e += 2) {
+              const bf16x2 two = {(__bf16)p[8 * half + e], (__bf16)p[8 * half + e + 1]};
+              pb[0][e] = two[0];
+              pb[0][e + 1] = two[1];
+              sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, two), s16x2{0x3f80, 0x3f80}, sum, false);
+            }
+          } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              pb[t][e] = (__bf16)p[8 * half + e];
-              if (t + 1 < T) p[8 * half + e] -= (float)pb[t][e];
+            for (int e = 0; e < 8; ++e) sum += p[8 * half + e];
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                pb[t][e] = (__bf16)p[8 * half + e];
+                if (t + 1 < T) p[8 * half + e] -= (float)pb[t][e];
+              }
             }
           }
-          const char *vr = vb + (32 * u + 16 * half + 4 * h + ((lane & 15) >> 2)) * vp + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+          const char *vr = vb + (32 * u + 16 * half + 4 * h + ((lane & 15) >> 2)) * VP + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            if (2 * d < tiles) {
-              const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 64 * d));
-              const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 8 * vp + 64 * d));
-              const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 64 * d));
+            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 8 * VP + 64 * d));
+            const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-              for (int t = 0; t < T; ++t) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[t], o[d], 0, 0, 0);
-            }
+            for (int t = 0; t < T; ++t) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[t], o[d], 0, 0, 0);
           }
         }
       }
       if (nan_tiles[(tile - first) % 3]) {
-        const uint8_t *ve = (const uint8_t *)vb + KEYS * vp;
+        const uint8_t *ve = (const uint8_t *)vb + KEYS * VP;
 #pragma unroll
-        for (int c = 0; c < 2 * DT; ++c) {
-          if (c < tiles) {
-            bool hit = false;
-            for (int k = 0; k < KEYS; ++k) hit |= ve[16 * k + c] == KV4_NAN && t0 + k >= lo && t0 + k < hi;
+        for (int c = 0; c < TB; ++c) {
+          bool hit = false;
+          for (int k = 0; k < KEYS; ++k) hit |= (ve[16 * k + c] == KV4_NAN) & (t0 + k >= lo) & (t0 + k < hi);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[c >> 1][8 * (c & 1) + e] = hit ? NAN : o[c >> 1][8 * (c & 1) + e];
-          }
+          for (int e = 0; e < 8; ++e) o[c >> 1][8 * (c & 1) + e] = hit ? NAN : o[c >> 1][8 * (c & 1) + e];
         }
       }
     }
@@ -695,7 +703,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   sum += fpeer<32>(sum);
   float *ow = (float *)lds + w * 32 * OUT_PITCH, *ml = (float *)lds + W * 32 * OUT_PITCH + w * 64;
   if (h == 0) {
-    ml[n] = m;
+    ml[n] = m * a.scale2;
     ml[32 + n] = sum;
   }
   const int hd = 16 * tiles;
@@ -710,6 +718,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       *(f32x4 *)(ow + n * OUT_PITCH + 8 * b + 4 * h) = f32x4{v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
     __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
     for (int k = lane >> 4; k < 64; k += 4) {
       const int row = k >> 1, dim = 32 * d + 16 * (k & 1) + (lane & 15);
       if (rr0 + row >= rows) break;
@@ -825,9 +834,9 @@ template <int C>
 static attn_fn pick_rows(int terms) {
   return terms == 1 ? k_kv4_rows<C, 1, 4> : terms == 2 ? k_kv4_rows<C, 2, 4> : k_kv4_rows<C, 4, 4>;
 }
-template <int DT, int W2>
+template <int TB, int W>
 static attn_fn pick_prompt(int terms) {
-  return terms == 1 ? k_kv4_prompt<DT, 1, W2> : terms == 2 ? k_kv4_prompt<DT, 2, W2> : k_kv4_prompt<DT, 3, 4>;
+  return terms == 1 ? k_kv4_prompt<TB, 1, W> : terms == 2 ? k_kv4_prompt<TB, 2, W> : k_kv4_prompt<TB, 3, 4>;
 }
 
 }  // namespace bfp
@@ -862,7 +871,10 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   a.page_shift = __builtin_ctz((unsigned)cache->page);
   a.window = window;
   a.splits = p.splits;
-  a.scale2 = (float)(scale * 1.44269504088896340736);
+  // a scale of zero (all scores alike) is taken as one that leaves nothing of them
+  a.scale2 = fmaxf((float)(fabs(scale) * 1.44269504088896340736), 0x1p-100f);
+  a.slack = M_SLACK / a.scale2;
+  a.q_sign = scale < 0 ? -1.0f : 1.0f;
   if (p.work) {
     const size_t cells = (size_t)batch->n_rows * q->heads * p.splits;
     a.part_o = (float *)work;
@@ -873,10 +885,10 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   attn_fn fn;
   int lds;
   if (p.prompt) {
-    fn = a.tiles <= 4 ? pick_prompt<2, 8>(p.terms) : a.tiles <= 6 ? pick_prompt<3, 8>(p.terms)
-         : a.tiles <= 8 ? pick_prompt<4, 8>(p.terms) : a.tiles <= 12 ? pick_prompt<6, 4>(p.terms) : pick_prompt<8, 4>(p.terms);
-    const int in = 2 * prompt_buffer(a.tiles), res = p.waves * (32 * OUT_PITCH + 64) * 4;
-    lds = in > res ? in : res;
+    const int tb = a.tiles <= 2 ? 2 : a.tiles <= 4 ? 4 : a.tiles <= 6 ? 6 : a.tiles <= 8 ? 8 : a.tiles <= 12 ? 12 : 16;
+    fn = tb == 2 ? pick_prompt<2, 8>(p.terms) : tb == 4 ? pick_prompt<4, 8>(p.terms) : tb == 6 ? pick_prompt<6, 8>(p.terms)
+         : tb == 8 ? pick_prompt<8, 8>(p.terms) : tb == 12 ? pick_prompt<12, 4>(p.terms) : pick_prompt<16, 4>(p.terms);
+    lds = prompt_lds(tb, p.waves);
   } else {
     const int C = (a.tiles + 3) / 4, R = 16 / p.terms;
     fn = C == 1 ? pick_rows<1>(p.terms) : C == 2 ? pick_rows<2>(p.terms) : C == 3 ? pick_rows<3>(p.terms) : pick_rows<4>(p.terms);
