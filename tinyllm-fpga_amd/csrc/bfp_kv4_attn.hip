@@ -462,11 +462,15 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // loads of 4 rows x 64 bytes, which an odd multiple of 64 bytes spreads.
 constexpr int pk_pitch(int tb) { return 32 * tb + 16; }
 constexpr int pv_pitch(int tb) { return 64 * ((tb / 2) | 1); }
-// A buffer: K, V, and V's exponent bytes (key, 16 tiles).
-constexpr int prompt_buffer(int tb) { return KEYS * (pk_pitch(tb) + pv_pitch(tb) + 16); }
+// A tile of K, and of V with its exponent bytes (key, 16 tiles).
+constexpr int k_bytes(int tb) { return KEYS * pk_pitch(tb); }
+constexpr int v_bytes(int tb) { return KEYS * (pv_pitch(tb) + 16); }
+// Tiles of V held: with three, one barrier a tile is enough; the widest heads
+// leave room for two, and take a second barrier.
+constexpr int v_buffers(int tb) { return tb <= 12 ? 3 : 2; }
 constexpr int OUT_PITCH = 36;   // floats: 32 values of a row, on their way out
 constexpr int prompt_lds(int tb, int waves) {
-  const int in = 2 * prompt_buffer(tb), out = waves * (32 * OUT_PITCH + 64) * 4;
+  const int in = 2 * k_bytes(tb) + v_buffers(tb) * v_bytes(tb), out = waves * (32 * OUT_PITCH + 64) * 4;
   return in > out ? in : out;
 }
 
@@ -476,11 +480,9 @@ constexpr int prompt_lds(int tb, int waves) {
 template <int TB, int T, int W>
 __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs a) {
   constexpr int ROWS = 32 * W, DT = TB / 2, UNITS = (TB + W - 1) / W;
-  constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), BUFFER = prompt_buffer(TB);
+  constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), NV = v_buffers(TB);
   extern __shared__ __align__(16) char lds[];
-  // of tile t, at t % 3: set while it is decoded, read a barrier later, cleared
-  // another one later, two barriers before it is set again
-  __shared__ int nan_tiles[3];
+  __shared__ int nan_tiles[4];
   const int seq = blockIdx.z, head = blockIdx.y;
   // the last rows see the most keys: first
   const int rt = (gridDim.x - 1 - blockIdx.x) / a.splits, split = (gridDim.x - 1 - blockIdx.x) % a.splits;
@@ -537,98 +539,108 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   // wave w brings in head tiles w, w + W, ... of K and V, a key a lane
   uint2 rk[UNITS], rv[UNITS];
   uint32_t rke[UNITS], rve[UNITS];
-  unsigned long long okmask = 0, next_ok = 0;
+  bool there = false;
   auto page_of = [&](int tile) {
     const int key = tile * KEYS + lane;
     return tile < stop && key >= begin && key < end ? kv4_page(pages, a.b.width, a.c.n_pages, key >> a.page_shift) : -1;
   };
+  // a key without a page reads the first one's bytes; they are not used
   auto fetch = [&](int tile, int id) {
-    next_ok = __ballot(id >= 0);
-    const long long at = kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + lane) & (a.c.page - 1));
+    there = id >= 0;
+    const long long at = kv4_tile(there ? id : 0, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + lane) & (a.c.page - 1));
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int t = w + u * W;
-      rk[u] = rv[u] = make_uint2(0, 0);
-      rke[u] = rve[u] = 0;
-      if (t < tiles && id >= 0) {
-        const long long o8 = at + (long long)t * a.c.page;
-        rk[u] = *(const uint2 *)(a.c.k + o8 * KV4_TILE_BYTES);
-        rv[u] = *(const uint2 *)(a.c.v + o8 * KV4_TILE_BYTES);
-        rke[u] = a.c.k_e[o8];
-        rve[u] = a.c.v_e[o8];
-      }
+      const long long o8 = at + (long long)(t < tiles ? t : tiles - 1) * a.c.page;
+      rk[u] = *(const uint2 *)(a.c.k + o8 * KV4_TILE_BYTES);
+      rv[u] = *(const uint2 *)(a.c.v + o8 * KV4_TILE_BYTES);
+      rke[u] = a.c.k_e[o8];
+      rve[u] = a.c.v_e[o8];
     }
   };
-  auto decode = [&](int tile) {
-    char *b = lds + ((tile - first) & 1) * BUFFER;
+  char *const k_lds = lds, *const v_lds = lds + 2 * k_bytes(TB);
+  auto decode = [&](int t1) {   // tile first + t1
+    char *kb = k_lds + (t1 & 1) * k_bytes(TB) + lane * KP, *vt = v_lds + t1 % NV * v_bytes(TB), *vb = vt + lane * VP;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int t = w + u * W;
-      if (t < TB) {   // tiles the head does not have: zeros
-        const float ks = kv4_scale(rke[u]);
-        bf16x8 *kd = (bf16x8 *)(b + lane * KP + 32 * t);
-        kd[0] = kv4_decode8(rk[u].x, ks);
-        kd[1] = kv4_decode8(rk[u].y, ks);
-        // NaN tiles of V count as zeros in the product; the rows that see them are set after
-        const bool bad = rve[u] == KV4_NAN;
-        ((uint8_t *)b)[KEYS * (KP + VP) + lane * 16 + t] = (uint8_t)rve[u];
-        if (bad) nan_tiles[(tile - first) % 3] = 1;
-        const float vs = kv4_scale(bad ? 0u : rve[u]);
-        bf16x8 *vd = (bf16x8 *)(b + KEYS * KP + lane * VP + 32 * t);
-        vd[0] = kv4_decode8(bad ? 0u : rv[u].x, vs);
-        vd[1] = kv4_decode8(bad ? 0u : rv[u].y, vs);
-      }
+      if (UNITS * W > TB && t >= TB) break;
+      const bool ok = there && t < tiles;   // zeros for what the head or the cache does not have
+      const float ks = kv4_scale(rke[u]);
+      bf16x8 *kd = (bf16x8 *)(kb + 32 * t);
+      kd[0] = kv4_decode8(t < tiles ? rk[u].x : 0u, ks);
+      kd[1] = kv4_decode8(t < tiles ? rk[u].y : 0u, ks);
+      // NaN tiles of V count as zeros in the product; the rows that see them are set after
+      const uint32_t E = ok ? rve[u] : 0u;
+      const bool take = ok && E != KV4_NAN;
+      vt[KEYS * VP + lane * 16 + t] = (char)E;
+      if (E == KV4_NAN) nan_tiles[t1 & 3] = 1;
+      const float vs = kv4_scale(take ? E : 0u);
+      bf16x8 *vd = (bf16x8 *)(vb + 32 * t);
+      vd[0] = kv4_decode8(take ? rv[u].x : 0u, vs);
+      vd[1] = kv4_decode8(take ? rv[u].y : 0u, vs);
     }
+  };
+  // scores of half a tile (32 keys), before any mask: s[e] is key 8 (e / 4) + 4 h + e % 4 of row n
+  auto scores = [&](int t1, int u) {
+    const char *kr = k_lds + (t1 & 1) * k_bytes(TB) + (32 * u + n) * KP + 16 * h;
+    f32x16 s;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < TB; ++c) {
+      const bf16x8 kf = *(const bf16x8 *)(kr + 32 * c);
+#pragma unroll
+      for (int t = 0; t < T; ++t) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[t][c], s, 0, 0, 0);
+    }
+    return s;
+  };
+  auto mask = [&](f32x16 &s, int tile, int u, unsigned long long ok) {
+    const int t0 = tile * KEYS;
+    if (t0 >= lo_max && t0 + KEYS <= hi_min && ok == ~0ull) return;
+    asm volatile("");   // a branch past the selects, not selects every time
+    const uint32_t okh = (uint32_t)(ok >> (32 * u)) >> (4 * h);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int k = 8 * (e >> 2) + (e & 3), key = t0 + 32 * u + 4 * h + k;
+      s[e] = (((okh >> k) & 1) != 0) & (key >= lo) & (key < hi) ? s[e] : -INFINITY;
+    }
+  };
+  auto top_of = [&](const f32x16 &s) {
+    float top = s[0];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
+    return fmaxf(top, fpeer<32>(top));
   };
 
-  if (threadIdx.x < 3) nan_tiles[threadIdx.x] = 0;
+  // Steps of 32 keys.  A step takes the scores of its keys from the step
+  // before it and multiplies the next step's (matrix cores) while it
+  // exponentiates its own (vector units); then its probabilities and V.
+  // A tile's bytes arrive and are decoded a tile ahead: barrier t lies
+  // between the steps of tile t, decoding tile t + 1 before it.  So K of
+  // tile t is read between barriers t - 1 and t and written between t - 2 and
+  // t - 1, V is read between t - 1 and t + 1.  nan_tiles[t % 4] is cleared before
+  // barrier t - 2, set between t - 2 and t - 1, read between t and t + 1.
+  if (threadIdx.x < 4) nan_tiles[threadIdx.x] = 0;
   __syncthreads();
   int id = page_of(first);
-  if (first < stop) {
-    fetch(first, id);
-    decode(first);
-    okmask = next_ok;
-  }
+  fetch(first, id);
+  unsigned long long ok = __ballot(there);
+  decode(0);
   id = page_of(first + 1);
   __syncthreads();
+  f32x16 s = scores(0, 0);
+  mask(s, first, 0, ok);
+  float top = top_of(s);
   for (int tile = first; tile < stop; ++tile) {
-    const bool more = tile + 1 < stop;
-    if (more) fetch(tile + 1, id);
+    const int t1 = tile - first;
+    fetch(tile + 1, id);
+    const unsigned long long ok_next = __ballot(there);
     id = page_of(tile + 2);
-    if (threadIdx.x == 0) nan_tiles[(tile - first + 2) % 3] = 0;
-    const char *kb = lds + ((tile - first) & 1) * BUFFER, *vb = kb + KEYS * KP;
-    const int t0 = tile * KEYS;
-    if (t0 < hi_max && t0 + KEYS > lo_min) {
-      // scores: s[u][e] is key t0 + 32 u + 8 (e / 4) + 4 h + e % 4 of row n
-      f32x16 s[2];
+    if (threadIdx.x == 0) nan_tiles[(t1 + 2) & 3] = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < TB; ++c) {
-          const bf16x8 kf = *(const bf16x8 *)(kb + (32 * u + n) * KP + 32 * c + 16 * h);
-#pragma unroll
-          for (int t = 0; t < T; ++t) s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[t][c], s[u], 0, 0, 0);
-        }
-      }
-      const bool inner = t0 >= lo_max && t0 + KEYS <= hi_min && okmask == ~0ull;
-      if (!inner) {
-        const uint32_t ok_h[2] = {(uint32_t)okmask >> (4 * h), (uint32_t)(okmask >> 32) >> (4 * h)};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int k = 8 * (e >> 2) + (e & 3), key = t0 + 32 * u + 4 * h + k;
-            s[u][e] = (((ok_h[u] >> k) & 1) != 0) & (key >= lo) & (key < hi) ? s[u][e] : -INFINITY;
-          }
-      }
-      float top = s[0][0];
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
-      top = fmaxf(top, fpeer<32>(top));
+    for (int u = 0; u < 2; ++u) {
+      if (u == 1) __syncthreads();
       const bool raise = top > m + a.slack;
       if (__any(raise)) {
         const float mn = raise ? top : m;
@@ -641,63 +653,72 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
           for (int e = 0; e < 16; ++e) o[d][e] *= f;
       }
       const float m0 = m == -INFINITY ? 0.0f : -m * a.scale2;
+      f32x16 sn = u == 0 ? scores(t1, 1) : scores(t1 + 1, 0);
+      float p[16];
+      bf16x8 pb[2][T];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float p[16];
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[u][e], a.scale2, m0));
+        for (int e = 8 * half; e < 8 * half + 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, m0));
+        if constexpr (T == 1) {
+          // the sum takes the probabilities as the product takes them
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          bf16x8 pb[T];
-          if constexpr (T == 1) {
-            // the sum takes the probabilities as the product takes them
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const bf16x2 two = {(__bf16)p[8 * half + e], (__bf16)p[8 * half + e + 1]};
-              pb[0][e] = two[0];
-              pb[0][e + 1] = two[1];
-              sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, two), s16x2{0x3f80, 0x3f80}, sum, false);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum += p[8 * half + e];
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                pb[t][e] = (__bf16)p[8 * half + e];
-                if (t + 1 < T) p[8 * half + e] -= (float)pb[t][e];
-              }
-            }
+          for (int e = 0; e < 8; e += 2) {
+            const bf16x2 two = {(__bf16)p[8 * half + e], (__bf16)p[8 * half + e + 1]};
+            pb[half][0][e] = two[0];
+            pb[half][0][e + 1] = two[1];
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, two), s16x2{0x3f80, 0x3f80}, sum, false);
           }
-          const char *vr = vb + (32 * u + 16 * half + 4 * h + ((lane & 15) >> 2)) * VP + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+        } else {
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 64 * d));
-            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 8 * VP + 64 * d));
-            const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+          for (int e = 0; e < 8; ++e) sum += p[8 * half + e];
 #pragma unroll
-            for (int t = 0; t < T; ++t) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[t], o[d], 0, 0, 0);
+          for (int t = 0; t < T; ++t) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              pb[half][t][e] = (__bf16)p[8 * half + e];
+              if (t + 1 < T) p[8 * half + e] -= (float)pb[half][t][e];
+            }
           }
         }
       }
-      if (nan_tiles[(tile - first) % 3]) {
-        const uint8_t *ve = (const uint8_t *)vb + KEYS * VP;
+      const char *vr = v_lds + t1 % NV * v_bytes(TB) + (32 * u + 4 * h + ((lane & 15) >> 2)) * VP + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
 #pragma unroll
-        for (int c = 0; c < TB; ++c) {
-          bool hit = false;
-          for (int k = 0; k < KEYS; ++k) hit |= (ve[16 * k + c] == KV4_NAN) & (t0 + k >= lo) & (t0 + k < hi);
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[c >> 1][8 * (c & 1) + e] = hit ? NAN : o[c >> 1][8 * (c & 1) + e];
+        for (int d = 0; d < DT; ++d) {
+          const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + 16 * half * VP + 64 * d));
+          const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vr + (16 * half + 8) * VP + 64 * d));
+          const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int t = 0; t < T; ++t) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[half][t], o[d], 0, 0, 0);
         }
       }
+      if (u == 0) {
+        decode(t1 + 1);
+        mask(sn, tile, 1, ok);
+      } else {
+        mask(sn, tile + 1, 0, ok_next);
+      }
+      s = sn;
+      top = top_of(s);
     }
-    if (more) {   // into the other buffer: its last readers passed the last barrier
-      decode(tile + 1);
-      okmask = next_ok;
+    ok = ok_next;
+    if (nan_tiles[t1 & 3]) {
+      const uint8_t *ve = (const uint8_t *)v_lds + t1 % NV * v_bytes(TB) + KEYS * VP;
+      const int t0 = tile * KEYS;
+#pragma unroll
+      for (int c = 0; c < TB; ++c) {
+        bool hit = false;
+#pragma unroll 1
+        for (int k = 0; k < KEYS; ++k) hit |= (ve[16 * k + c] == KV4_NAN) & (t0 + k >= lo) & (t0 + k < hi);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[c >> 1][8 * (c & 1) + e] = hit ? NAN : o[c >> 1][8 * (c & 1) + e];
+      }
     }
-    __syncthreads();
+    if constexpr (NV == 2) __syncthreads();   // before V of tile t - 1 gives way to t + 1
   }
+  __syncthreads();
 
   // results: 32 values of the wave's rows at a time through LDS, 16 lanes to a tile
   sum += fpeer<32>(sum);
