@@ -43,7 +43,8 @@ struct Kv4AttnArgs {
   bfp_kv4 c;
   bfp_kv4_batch b;
   bfp_rows q, out;
-  int tiles, group, page_shift, window, splits;
+  int tiles, group, page_shift, window, splits, row_tiles;
+  FastDiv by_seq, by_head, by_split;   // k_kv4_prompt's workgroups
   float scale2;        // |scale| * log2(e), kept above 0; the queries take the sign
   float slack;         // M_SLACK in scores: M_SLACK / scale2
   float q_sign;
@@ -483,9 +484,15 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), NV = v_buffers(TB);
   extern __shared__ __align__(16) char lds[];
   __shared__ int nan_tiles[4];
-  const int seq = blockIdx.z, head = blockIdx.y;
-  // the last rows see the most keys: first
-  const int rt = (gridDim.x - 1 - blockIdx.x) / a.splits, split = (gridDim.x - 1 - blockIdx.x) % a.splits;
+  // One sequence after the other, its last rows, which see the most keys,
+  // first.  Neighbouring workgroups take different KV heads and the same rows:
+  // workgroups go to the XCDs and their shader engines in turn, whether one
+  // is ready sooner or not, so neighbours should take equally long.
+  uint32_t u, h1, s1;
+  const int seq = (int)a.by_seq.div(blockIdx.x, u);
+  u = a.by_head.div(u, h1);
+  u = a.by_split.div(u, s1);
+  const int head = (int)h1, split = (int)s1, rt = a.row_tiles - 1 - (int)u;
   const Kv4Span sp = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
   const int G = a.group, rows = sp.n * G;
   if (rt >= (rows + ROWS - 1) / ROWS) return;
@@ -901,7 +908,14 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
     a.part_o = (float *)work;
     a.part_ml = (float2 *)((float *)work + cells * 16 * a.tiles);
   }
-  const long long blocks = (long long)p.row_tiles * p.splits;
+  a.row_tiles = p.row_tiles;
+  a.by_head = FastDiv(cache->heads);
+  a.by_split = FastDiv(p.splits);
+  long long blocks = (long long)p.row_tiles * p.splits * (p.prompt ? cache->heads : 1);
+  if (blocks <= 0x7fffffLL && p.prompt) {
+    a.by_seq = FastDiv((uint32_t)blocks);
+    blocks *= batch->n_seq;
+  }
   if (blocks > 0x7fffffLL) return set_err(BFP_EINVAL, "%s: max_q=%d is too large for one call", op, batch->max_q);
   attn_fn fn;
   int lds;
@@ -918,7 +932,7 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   }
   if (lds > 65536)   // one limit for a kernel, whatever the call
     HIP_TRY(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 159 * 1024));
-  hipLaunchKernelGGL(fn, dim3((unsigned)blocks, cache->heads, batch->n_seq), dim3(64 * p.waves), lds, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(fn, p.prompt ? dim3((unsigned)blocks) : dim3((unsigned)blocks, cache->heads, batch->n_seq), dim3(64 * p.waves), lds, (hipStream_t)stream, a);
   BFP_TRY(launch_status(op));
   if (p.splits > 1) {
     const long long n = ((long long)batch->max_q * q->heads + 3) / 4;
