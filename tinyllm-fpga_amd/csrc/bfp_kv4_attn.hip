@@ -115,13 +115,13 @@ __device__ __forceinline__ uint32_t byte_mask(uint32_t keep) {
   return (((keep & 1) | ((keep & 2) << 7) | ((keep & 4) << 14) | ((keep & 8) << 21)) * 255u);
 }
 
-// One 64-key tile of a wave's operands: lane (r = lane % 16, g = lane / 16)
-// holds keys 4r .. 4r+3 of head tiles g * C .. g * C + C - 1.
+// A wave's side (K or V) of one 64-key tile: lane (r = lane % 16, g = lane /
+// 16) holds keys 4r .. 4r+3 of head tiles g * C .. g * C + C - 1, four keys' exponents a
+// word.
 template <int C>
-struct KvTile {
-  uint4 k[C][2], v[C][2];
-  uint32_t ke[C], ve[C];
-  bool ok;
+struct KvSide {
+  uint4 w[C][2];
+  uint32_t e[C];
 };
 
 __device__ __forceinline__ uint2 half_of(const uint4 (&w)[2], int j) {
@@ -129,33 +129,33 @@ __device__ __forceinline__ uint2 half_of(const uint4 (&w)[2], int j) {
          : j == 2 ? make_uint2(w[1].x, w[1].y) : make_uint2(w[1].z, w[1].w);
 }
 
+// Head tiles that do not exist are read as the last one; keys without a page
+// as the first page's.
 template <int C>
-__device__ __forceinline__ void load_tile(const Kv4AttnArgs &a, KvTile<C> &x, int id, int head, int key, int g) {
-  x.ok = id >= 0;
-  const long long o = kv4_tile(id < 0 ? 0 : id, a.c.heads, head, a.tiles, g * C, a.c.page, key & (a.c.page - 1));
+__device__ __forceinline__ void load_side(KvSide<C> &x, const uint8_t *data, const uint8_t *exps, long long o,
+                                          int page, int t, int tiles) {
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    if (g * C + c < a.tiles) {
-      const long long oc = o + (long long)c * a.c.page;
-      const uint4 *kp = (const uint4 *)(a.c.k + oc * KV4_TILE_BYTES);
-      const uint4 *vp = (const uint4 *)(a.c.v + oc * KV4_TILE_BYTES);
-      x.k[c][0] = kp[0];
-      x.k[c][1] = kp[1];
-      x.ke[c] = *(const uint32_t *)(a.c.k_e + oc);
-      x.v[c][0] = vp[0];
-      x.v[c][1] = vp[1];
-      x.ve[c] = *(const uint32_t *)(a.c.v_e + oc);
-    } else {
-      x.k[c][0] = x.k[c][1] = x.v[c][0] = x.v[c][1] = make_uint4(0, 0, 0, 0);
-      x.ke[c] = x.ve[c] = 0;
-    }
+    const long long oc = o + (long long)(t + c < tiles ? t + c : tiles - 1) * page;
+    const uint4 *p = (const uint4 *)(data + oc * KV4_TILE_BYTES);
+    x.w[c][0] = p[0];
+    x.w[c][1] = p[1];
+    x.e[c] = *(const uint32_t *)(exps + oc);
   }
 }
 
+// The exponent byte of key j as the conversions take it: they look at the
+// exponent field only, whatever lies beside it.
+__device__ __forceinline__ float scale_of(uint32_t e, int j) {
+  return __uint_as_float(j == 0 ? e << 23 : j == 1 ? e << 15 : j == 2 ? e << 7 : e >> 1);
+}
+
 // LDS rows of 32 keys x hd bfloat16.  A row's bytes are an odd multiple of
-// 32: eight neighbouring rows' 32-byte pieces then lie in different banks,
-// for the writes (a tile of eight keys) and the transposing reads alike.
-__host__ __device__ inline int v_pitch(int tiles) { return 32 * (tiles | 1); }
+// 32, so that the 32-byte pieces of neighbouring rows, which the transposing
+// reads take, lie in different banks; the two 16-byte halves of every piece
+// change places in each second group of four rows, so that eight lanes'
+// writes do too (without that they took twice as long).
+constexpr int v_pitch(int C) { return 32 * (4 * C | 1); }
 constexpr int V_ROWS = 32;
 // Floats of a wave's sums in LDS when the waves are joined: m and sum of 16
 // columns, then R rows of hd (and 4 more, for the banks).
@@ -176,7 +176,7 @@ __device__ __forceinline__ void out_store(const bfp_rows &r, long long o, float 
 // C: head tiles a lane group holds (hd <= 64 C); T: terms of a row (columns
 // R = 16 / T rows share); W: waves.
 template <int C, int T, int W>
-__global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * W, C == 1 ? 4 : C == 2 ? 2 : 1) void k_kv4_rows(Kv4AttnArgs a) {
   constexpr int R = 16 / T;
   extern __shared__ __align__(16) char lds[];
   const int seq = blockIdx.z, head = blockIdx.y;
@@ -232,63 +232,58 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
 #pragma unroll
   for (int d = 0; d < 4 * C; ++d) o[d] = f32x4{0, 0, 0, 0};
 
-  const int pitch = v_pitch(tiles);
-  char *mylds = lds + w * V_ROWS * pitch;
-  char *vput = mylds + r * pitch + g * C * 32;                              // + 16 rows, + a tile
-  const char *vget = mylds + (g * 4 + (r >> 2)) * pitch + (r & 3) * 8;      // + 16 rows, + a tile
+  constexpr int PITCH = v_pitch(C);
+  char *mylds = lds + w * V_ROWS * PITCH;
+  const int swap = (r >> 2) & 1;
+  char *vput0 = mylds + r * PITCH + g * C * 32 + 16 * swap, *vput1 = vput0 + 16 - 32 * swap;   // + 16 rows, + a tile
+  const char *vget = mylds + (g * 4 + (r >> 2)) * PITCH + (((r & 3) ^ (2 * (g & 1))) * 8);        // + 16 rows, + a tile
   const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
   auto page_of = [&](int tile) {
     return tile < stop ? kv4_page(pages, a.b.width, a.c.n_pages, (tile * KEYS + 4 * r) >> a.page_shift) : -1;
   };
+  auto offset_of = [&](int tile, int id) {
+    return kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + 4 * r) & (a.c.page - 1));
+  };
 
-  KvTile<C> x;
+  // K of the next tile is asked for when this one's scores are done, V when
+  // this one's has gone to LDS: no second set of registers
+  KvSide<C> k, v;
   int tile = first + w;
   int id = page_of(tile);
-  if (tile < stop) load_tile(a, x, id, head, tile * KEYS + 4 * r, g);
-  id = page_of(tile + W);
+  long long at = offset_of(tile, id);
+  load_side(k, a.c.k, a.c.k_e, at, a.c.page, g * C, tiles);
+  load_side(v, a.c.v, a.c.v_e, at, a.c.page, g * C, tiles);
   for (; tile < stop; tile += W) {
-    KvTile<C> cur = x;
-    if (tile + W < stop) load_tile(a, x, id, head, (tile + W) * KEYS + 4 * r, g);
-    id = page_of(tile + 2 * W);
     const int t0 = tile * KEYS;
-    const unsigned long long okmask = __ballot(cur.ok);
+    const int next_id = page_of(tile + W);
+    const bool have = id >= 0;
+    const unsigned long long okmask = __ballot(have);
     const bool inner = t0 >= lo_max && t0 + KEYS <= hi_min && okmask == ~0ull;
-    if (!inner) {
-      // keys that no row of this workgroup sees become zeros, whatever their bytes
-      uint32_t keep = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = t0 + 4 * r + j;
-        keep |= (cur.ok && key >= lo_min && key < end) ? 1u << j : 0u;
-      }
-      const uint32_t bytes = byte_mask(keep);
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        cur.ve[c] &= bytes;
-        const uint32_t k0 = keep & 1 ? ~0u : 0u, k1 = keep & 2 ? ~0u : 0u, k2 = keep & 4 ? ~0u : 0u, k3 = keep & 8 ? ~0u : 0u;
-        cur.v[c][0] = make_uint4(cur.v[c][0].x & k0, cur.v[c][0].y & k0, cur.v[c][0].z & k1, cur.v[c][0].w & k1);
-        cur.v[c][1] = make_uint4(cur.v[c][1].x & k2, cur.v[c][1].y & k2, cur.v[c][1].z & k3, cur.v[c][1].w & k3);
-      }
-    }
 
     // scores: s[j][e] is key t0 + 16 g + 4 e + j of column r
     f32x4 s[4];
+#pragma unroll
+    for (int c = 0; c < C; ++c)   // a head tile that does not exist: its bytes must not make a NaN of 0 times them
+      if (g * C + c >= tiles) k.e[c] = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       s[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const float sc = kv4_scale((cur.ke[c] >> (8 * j)) & 255u);
-        const uint2 words = half_of(cur.k[c], j);
+        const float sc = scale_of(k.e[c], j);
+        const uint2 words = half_of(k.w[c], j);
         s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv4_decode8(words.x, sc), qf[c][0], s[j], 0, 0, 0);
         s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv4_decode8(words.y, sc), qf[c][1], s[j], 0, 0, 0);
       }
     }
+    at = offset_of(tile + W, next_id);   // past the end: the first page, not used
+    load_side(k, a.c.k, a.c.k_e, at, a.c.page, g * C, tiles);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[j][e] = term_sum<T>(s[j][e]);
     if (!inner) {
+      asm volatile("");   // a branch past all this, not selects every time
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const bool ok = (okmask >> (4 * g + e)) & 1;
@@ -297,6 +292,21 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
           const int key = t0 + 16 * g + 4 * e + j;
           s[j][e] = ok & (key >= lo) & (key < hi) ? s[j][e] : -INFINITY;
         }
+      }
+      // values that no row of this workgroup sees become zeros, whatever their bytes
+      uint32_t keep = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = t0 + 4 * r + j;
+        keep |= (have & (key >= lo_min) & (key < end)) ? 1u << j : 0u;
+      }
+      const uint32_t bytes = byte_mask(keep);
+      const uint32_t k0 = keep & 1 ? ~0u : 0u, k1 = keep & 2 ? ~0u : 0u, k2 = keep & 4 ? ~0u : 0u, k3 = keep & 8 ? ~0u : 0u;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        v.e[c] &= bytes;
+        v.w[c][0] = make_uint4(v.w[c][0].x & k0, v.w[c][0].y & k0, v.w[c][0].z & k1, v.w[c][0].w & k1);
+        v.w[c][1] = make_uint4(v.w[c][1].x & k2, v.w[c][1].y & k2, v.w[c][1].z & k3, v.w[c][1].w & k3);
       }
     }
 
@@ -318,85 +328,86 @@ __global__ __launch_bounds__(64 * W) void k_kv4_rows(Kv4AttnArgs a) {
       for (int d = 0; d < 4 * C; ++d) o[d] *= f;
     }
     const float m0 = m == -INFINITY ? 0.0f : -m * a.scale2;
-    float p[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[j][e] = __builtin_amdgcn_exp2f(fmaf(s[j][e], a.scale2, m0));
-        sum += p[j][e];
-      }
-
-    // a tile of V that holds a NaN counts as zeros in the product, so that it
-    // cannot reach a row that does not see it; the rows that do are set after
-    bool nan_v = false;
-#pragma unroll
-    for (int c = 0; c < C; ++c) nan_v |= has_byte_255(cur.ve[c]);
-    const bool any_nan = __any(nan_v);
+    bf16x8 pb[2];
 #pragma unroll
     for (int jp = 0; jp < 2; ++jp) {
       float pv[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pv[e] = round_term<T>(p[2 * jp][e], t);
-        pv[4 + e] = round_term<T>(p[2 * jp + 1][e], t);
-      }
-      const bf16x8 pb = pack8(pv);
-      bf16x8 seen;
-      if (any_nan) {
+      for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          seen[e] = (__bf16)(s[2 * jp][e] == -INFINITY ? 0.0f : 1.0f);
-          seen[4 + e] = (__bf16)(s[2 * jp + 1][e] == -INFINITY ? 0.0f : 1.0f);
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[2 * jp + jj][e], a.scale2, m0));
+          sum += p;
+          pv[4 * jj + e] = round_term<T>(p, t);
         }
-      }
-      for (int pass = 0; pass < (any_nan ? 2 : 1); ++pass) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      pb[jp] = pack8(pv);
+    }
+
+    // A tile of V that holds a NaN counts as zeros in the product, so that it
+    // cannot reach a row that does not see it; the rows that do are set below.
+    uint32_t bad = 0;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          if (g * C + c < tiles) {
+    for (int c = 0; c < C; ++c) bad |= has_byte_255(v.e[c]) && g * C + c < tiles ? 1u << c : 0u;
+    const bool any_nan = __any(bad);
+    uint32_t ve[C];
+    if (any_nan) {
 #pragma unroll
-            for (int jj = 0; jj < 2; ++jj) {
-              const int j = 2 * jp + jj;
-              uint32_t E = (cur.ve[c] >> (8 * j)) & 255u;
-              uint2 words = half_of(cur.v[c], j);
-              if (any_nan) {
-                const bool bad = E == KV4_NAN;
-                if (pass == 0) {
-                  words = bad ? make_uint2(0, 0) : words;
-                  E = bad ? 0u : E;
-                } else {   // 1 where the NaNs are
-                  words = bad ? make_uint2(0x22222222u, 0x22222222u) : make_uint2(0, 0);
-                  E = KV4_BIAS;
-                }
-              }
-              const float sc = kv4_scale(E);
-              bf16x8 *dst = (bf16x8 *)(vput + jj * 16 * pitch + c * 32);
-              dst[0] = kv4_decode8(words.x, sc);
-              dst[1] = kv4_decode8(words.y, sc);
-            }
-          }
+      for (int c = 0; c < C; ++c) {
+        ve[c] = v.e[c];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (((ve[c] >> (8 * j)) & 255u) != KV4_NAN) continue;
+          v.e[c] &= ~(255u << (8 * j));
+          (j & 1 ? v.w[c][j >> 1].z : v.w[c][j >> 1].x) = 0;
+          (j & 1 ? v.w[c][j >> 1].w : v.w[c][j >> 1].y) = 0;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int d = 0; d < 4 * C; ++d) {
-          if (d < tiles) {
-            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + d * 32));
-            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + 16 * pitch + d * 32));
-            const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-            if (pass == 0) {
-              o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[d], 0, 0, 0);
-            } else {
-              const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, seen, f32x4{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[d][e] = n[e] > 0.0f ? NAN : o[d][e];
-            }
-          }
-        }
-        __builtin_amdgcn_wave_barrier();
       }
     }
+#pragma unroll
+    for (int jp = 0; jp < 2; ++jp) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const float sc = scale_of(v.e[c], 2 * jp + jj);
+          const uint2 words = half_of(v.w[c], 2 * jp + jj);
+          *(bf16x8 *)(vput0 + jj * 16 * PITCH + c * 32) = kv4_decode8(words.x, sc);
+          *(bf16x8 *)(vput1 + jj * 16 * PITCH + c * 32) = kv4_decode8(words.y, sc);
+        }
+      }
+      if (jp == 1) load_side(v, a.c.v, a.c.v_e, at, a.c.page, g * C, tiles);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int d = 0; d < 4 * C; ++d) {
+        const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + d * 32));
+        const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(vget + 16 * PITCH + d * 32));
+        const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb[jp], o[d], 0, 0, 0);
+      }
+    }
+    if (any_nan) {
+      uint8_t *le = (uint8_t *)mylds;   // exponents, (key, 16 tiles)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) le[(4 * r + j) * 16 + g * C + c] = (uint8_t)(ve[c] >> (8 * j));
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int d = 0; d < 4 * C; ++d) {
+        bool hit = false;
+#pragma unroll 1
+        for (int key = 0; key < KEYS; ++key) hit |= (le[16 * key + d] == KV4_NAN) & (t0 + key >= lo) & (t0 + key < hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][e] = hit ? NAN : o[d][e];
+      }
+    }
+    id = next_id;
   }
 
   // join the terms, then the waves
@@ -568,6 +579,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   char *const k_lds = lds, *const v_lds = lds + 2 * k_bytes(TB);
   auto decode = [&](int t1) {   // tile first + t1
     char *kb = k_lds + (t1 & 1) * k_bytes(TB) + lane * KP, *vt = v_lds + t1 % NV * v_bytes(TB), *vb = vt + lane * VP;
+    const int sw = (lane >> 1) & 3;   // 16-byte pieces of each 64 change places, for the writes' banks
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int t = w + u * W;
@@ -583,9 +595,8 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       vt[KEYS * VP + lane * 16 + t] = (char)E;
       if (E == KV4_NAN) nan_tiles[t1 & 3] = 1;
       const float vs = kv4_scale(take ? E : 0u);
-      bf16x8 *vd = (bf16x8 *)(vb + 32 * t);
-      vd[0] = kv4_decode8(take ? rv[u].x : 0u, vs);
-      vd[1] = kv4_decode8(take ? rv[u].y : 0u, vs);
+      *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1)) ^ sw)) = kv4_decode8(take ? rv[u].x : 0u, vs);
+      *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1) + 1) ^ sw)) = kv4_decode8(take ? rv[u].y : 0u, vs);
     }
   };
   // scores of half a tile (32 keys), before any mask: s[e] is key 8 (e / 4) + 4 h + e % 4 of row n
@@ -619,6 +630,9 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
     for (int e = 0; e < 16; ++e) top = fmaxf(top, s[e]);
     return fmaxf(top, fpeer<32>(top));
   };
+
+  const int vrow = 4 * h + ((lane & 15) >> 2);   // of 8: the rows and columns this lane reads V from
+  const int vcol = 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ (vrow >> 1)) + 8 * (lane & 1);
 
   // Steps of 32 keys.  A step takes the scores of its keys from the step
   // before it and multiplies the next step's (matrix cores) while it
@@ -689,7 +703,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
           }
         }
       }
-      const char *vr = v_lds + t1 % NV * v_bytes(TB) + (32 * u + 4 * h + ((lane & 15) >> 2)) * VP + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      const char *vr = v_lds + t1 % NV * v_bytes(TB) + (32 * u + vrow) * VP + vcol;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
@@ -774,20 +788,31 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4AttnArgs a) {
   if (i >= sp.n) return;
   const long long tok = sp.row0 + i, at = (tok * a.q.heads + qh) * a.splits;
   const int hd = 16 * a.tiles;
-  float M = -INFINITY, L = 0.0f;
-  for (int k = 0; k < a.splits; ++k) M = fmaxf(M, a.part_ml[at + k].x);
+  // lane k holds split k's maximum and sum (at most 64 splits)
+  const float2 ml = lane < a.splits ? a.part_ml[at + lane] : make_float2(-INFINITY, 0.0f);
+  float M = ml.x;
+  M = fmaxf(M, fpeer<32>(M));
+  M = fmaxf(M, fpeer<16>(M));
+  M = fmaxf(M, fpeer<8>(M));
+  M = fmaxf(M, fpeer<4>(M));
+  M = fmaxf(M, fpeer<2>(M));
+  M = fmaxf(M, fpeer<1>(M));
+  // a split that saw nothing (or NaN scores alone, whose sum is NaN): factor 0
+  const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+  float L = f * ml.y;
+  L += fpeer<32>(L);
+  L += fpeer<16>(L);
+  L += fpeer<8>(L);
+  L += fpeer<4>(L);
+  L += fpeer<2>(L);
+  L += fpeer<1>(L);
   float acc[4] = {0, 0, 0, 0};
+#pragma unroll 8
   for (int k = 0; k < a.splits; ++k) {
-    const float2 ml = a.part_ml[at + k];
-    if (ml.x == -INFINITY) {   // saw nothing, or nothing but NaN scores
-      L += ml.y;
-      continue;
-    }
-    const float f = exp2f(ml.x - M);
-    L += f * ml.y;
+    const float fk = __shfl(f, k, 64);
 #pragma unroll
     for (int d = 0; d < 4; ++d)
-      if (64 * d + lane < hd) acc[d] += f * a.part_o[(at + k) * hd + 64 * d + lane];
+      if (64 * d + lane < hd) acc[d] += fk * a.part_o[(at + k) * hd + 64 * d + lane];
   }
 #pragma unroll
   for (int d = 0; d < 4; ++d)
@@ -834,7 +859,7 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   const long long groups = (long long)p.row_tiles * c.heads * b.n_seq;
   long long s = groups > 0 ? (p.prompt ? 512 : 1024) / groups : 1;
   if (s > key_tiles / 4) s = key_tiles / 4;
-  if (s > 128) s = 128;
+  if (s > 64) s = 64;   // a lane of k_kv4_join each
   p.splits = s < 1 ? 1 : (int)s;
   if (p.splits > 1) {
     const size_t cells = (size_t)b.n_rows * q.heads * p.splits;
@@ -927,7 +952,7 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   } else {
     const int C = (a.tiles + 3) / 4, R = 16 / p.terms;
     fn = C == 1 ? pick_rows<1>(p.terms) : C == 2 ? pick_rows<2>(p.terms) : C == 3 ? pick_rows<3>(p.terms) : pick_rows<4>(p.terms);
-    const int in = p.waves * V_ROWS * v_pitch(a.tiles), res = p.waves * join_floats(R, a.tiles) * 4;
+    const int in = p.waves * V_ROWS * v_pitch(C), res = p.waves * join_floats(R, a.tiles) * 4;
     lds = in > res ? in : res;
   }
   if (lds > 65536)   // one limit for a kernel, whatever the call
