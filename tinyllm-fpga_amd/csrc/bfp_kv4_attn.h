@@ -1,0 +1,179 @@
+// What the kernels of the attention over the 4-bit cache share: their
+// arguments, masks, the terms values are split into, and how work is placed.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <math.h>
+
+#include "bfp.h"
+#include "bfp_device.h"
+#include "bfp_f64.h"
+#include "bfp_internal.h"
+#include "bfp_kv4.h"
+#include "bfp_rows.h"
+
+namespace bfp {
+
+constexpr int KEYS = 64;             // keys a wave takes at a time
+// The running maximum is raised only when a score passes it by this many
+// powers of two: probabilities up to 2^8 are as exact as those up to 1, and
+// the sums are rescaled a few times in a whole context instead of whenever a
+// new maximum turns up.
+constexpr float M_SLACK = 8.0f;
+
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+struct Kv4AttnArgs {
+  bfp_kv4 c;
+  bfp_kv4_batch b;
+  bfp_rows q, out;
+  int tiles, group, page_shift, window, row_tiles;
+  int splits, chunk;   // k_kv4_prompt: pieces of the keys, and their length in tiles
+  int stream;          // k_kv4_rows: workgroups that share all tiles (0: one takes all keys of its rows)
+  FastDiv by_seq, by_head, by_split;
+  // A workgroup's piece: one sequence after the other, its last rows, which
+  // see the most keys, first.  Neighbouring workgroups take different KV heads
+  // of the same rows and keys: workgroups go to the XCDs and their shader
+  // engines in turn, whether one is ready sooner or not, so neighbours should
+  // take equally long.
+  __device__ void place(int &seq, int &head, int &split, int &rt) const {
+    uint32_t u, h, s;
+    seq = (int)by_seq.div(blockIdx.x, u);
+    u = by_head.div(u, h);
+    rt = row_tiles - 1 - (int)by_split.div(u, s);
+    split = (int)s;
+    head = (int)h + split % c.heads;
+    head = head < c.heads ? head : head - c.heads;
+  }
+  float scale2;        // |scale| * log2(e), kept above 0; the queries take the sign
+  float slack;         // M_SLACK in scores: M_SLACK / scale2
+  float q_sign;
+  // unfinished rows: the sums, and (maximum, sum of probabilities)
+  float *part_o;       // k_kv4_prompt [row][query head][split][hd]; k_kv4_rows [slot][R][hd]
+  float2 *part_ml;     // without [hd]
+};
+
+// Position p's visible keys are [lo, hi).
+__device__ __forceinline__ int key_hi(int p) { return p < 0 ? 0 : p + 1; }
+__device__ __forceinline__ int key_lo(int hi, int window) {
+  return window > 0 && hi > window ? hi - window : 0;
+}
+
+// The tiles of split `split` out of a row tile's n: chunks as long as the
+// longest sequence's splits are, so that workgroups take equally long
+// whatever the lengths; the last split takes what is left, where a sequence
+// is longer than the batch says.
+struct KeyPart {
+  int first, stop;
+};
+__device__ __forceinline__ KeyPart key_part(int n, int split, int splits, int chunk) {
+  const long long a = (long long)split * chunk, b = a + chunk;
+  KeyPart p;
+  p.first = a < n ? (int)a : n;
+  p.stop = split + 1 == splits || b > n ? n : (int)b;
+  return p;
+}
+
+// x cut to bfloat16 toward zero: the rest is exact, and has the sign of x.
+__device__ __forceinline__ float cut_bf16(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+
+// Term t of x's split by cuts (three hold any float32).  An infinity or a
+// NaN is its own first term.
+__device__ __forceinline__ float cut_term(float x, int t) {
+  const bool good = fabsf(x) < INFINITY;
+  if (!good) return t == 0 ? (x != x ? NAN : x) : 0.0f;
+  for (int i = 0; i < t; ++i) x -= cut_bf16(x);
+  return cut_bf16(x);
+}
+
+// Term t of x's split by rounding.
+template <int T>
+__device__ __forceinline__ float round_term(float x, int t) {
+  if constexpr (T > 1) {
+#pragma unroll
+    for (int i = 1; i < T && i < 3; ++i) {
+      const float r = x - (float)(__bf16)x;
+      x = t >= i ? r : x;
+    }
+    if constexpr (T == 4) x = t == 3 ? 0.0f : x;
+  }
+  return x;
+}
+
+__device__ __forceinline__ bf16x8 pack8(const float (&v)[8]) {
+  bf16x8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = (__bf16)v[i];
+  return r;
+}
+
+template <int M>
+__device__ __forceinline__ float fpeer(float v) {
+  return __int_as_float(peer<M>(__float_as_int(v)));
+}
+
+// A sum over the T columns that hold the terms of a row (columns R apart).
+// The wider step first: the result is then the same in all of them.
+template <int T>
+__device__ __forceinline__ float term_sum(float v) {
+  if constexpr (T >= 2) v += fpeer<8>(v);
+  if constexpr (T >= 4) v += fpeer<4>(v);
+  return v;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, fpeer<32>(v));
+  v = fmaxf(v, fpeer<16>(v));
+  v = fmaxf(v, fpeer<8>(v));
+  v = fmaxf(v, fpeer<4>(v));
+  v = fmaxf(v, fpeer<2>(v));
+  return fmaxf(v, fpeer<1>(v));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += fpeer<32>(v);
+  v += fpeer<16>(v);
+  v += fpeer<8>(v);
+  v += fpeer<4>(v);
+  v += fpeer<2>(v);
+  return v + fpeer<1>(v);
+}
+
+__device__ __forceinline__ bool has_byte_255(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u;
+}
+// w with its bytes kept where keep has a bit (byte i: bit i).
+__device__ __forceinline__ uint32_t byte_mask(uint32_t keep) {
+  return (((keep & 1) | ((keep & 2) << 7) | ((keep & 4) << 14) | ((keep & 8) << 21)) * 255u);
+}
+
+// Value o of a finished row: one of 16 neighbouring lanes with neighbouring o.
+__device__ __forceinline__ void out_store(const bfp_rows &r, long long o, float v) {
+  if (r.type != BFP_TILES) {
+    row_store(r, o, v);
+    return;
+  }
+  int e;
+  const int m = quantize16_lanes((double)v, e);
+  ((int16_t *)r.p)[o] = (int16_t)m;
+  if ((threadIdx.x & 15) == 0) r.e[o >> 4] = (int8_t)e;
+}
+
+typedef void (*attn_fn)(Kv4AttnArgs);
+// The kernel for heads of `tiles` tiles (k_kv4_rows: with 4 waves, or the 16
+// or 8 that rows_waves says) and its dynamic LDS.
+struct AttnKernel {
+  attn_fn fn;
+  int lds;
+};
+AttnKernel rows_kernel(int tiles, int terms, int waves);
+AttnKernel prompt_kernel(int tiles, int terms);
+inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
+inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }
+// Queues the kernels that finish what the others left in pieces.
+void launch_join_rows(const Kv4AttnArgs &a, int terms, hipStream_t s);
+void launch_join_prompt(const Kv4AttnArgs &a, hipStream_t s);
+
+}  // namespace bfp
