@@ -52,6 +52,7 @@ struct Kv4AttnArgs {
   // unfinished rows: the sums, and (maximum, sum of probabilities)
   float *part_o;       // k_kv4_prompt [row][query head][split][hd]; k_kv4_rows [slot][R][hd]
   float2 *part_ml;     // without [hd]
+  unsigned long long *there, number;   // k_kv4_rows: which slots are filled, and this call's number
 };
 
 // Position p's visible keys are [lo, hi).
@@ -89,25 +90,40 @@ __device__ __forceinline__ float cut_term(float x, int t) {
   return cut_bf16(x);
 }
 
-// Term t of x's split by rounding.
-template <int T>
-__device__ __forceinline__ float round_term(float x, int t) {
-  if constexpr (T > 1) {
-#pragma unroll
-    for (int i = 1; i < T && i < 3; ++i) {
-      const float r = x - (float)(__bf16)x;
-      x = t >= i ? r : x;
-    }
-    if constexpr (T == 4) x = t == 3 ? 0.0f : x;
-  }
-  return x;
-}
-
 __device__ __forceinline__ bf16x8 pack8(const float (&v)[8]) {
   bf16x8 r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = (__bf16)v[i];
   return r;
+}
+
+// Term t of eight probabilities.  Two terms: the first cut, the second
+// rounded (2^-16 of the value at most).  Three (of four places): all cut,
+// which holds a float32 exactly; what the fourth place gets is not used.
+template <int T>
+__device__ __forceinline__ bf16x8 pack_terms(float (&p)[8], int t) {
+  if constexpr (T == 1) {
+    return pack8(p);
+  } else if constexpr (T == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = cut_bf16(p[i]), rest = p[i] - c;
+      p[i] = t == 0 ? c : rest;
+    }
+    return pack8(p);
+  } else {
+    const uint32_t m1 = t >= 1 ? 0xffff0000u : 0u, m2 = t >= 2 ? 0xffff0000u : 0u;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] -= __uint_as_float(__float_as_uint(p[i]) & m1);
+      p[i] -= __uint_as_float(__float_as_uint(p[i]) & m2);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)   // the upper halves of two
+      w[i] = __builtin_amdgcn_perm(__float_as_uint(p[2 * i + 1]), __float_as_uint(p[2 * i]), 0x07060302u);
+    return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+  }
 }
 
 template <int M>
@@ -124,21 +140,26 @@ __device__ __forceinline__ float term_sum(float v) {
   return v;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, fpeer<32>(v));
-  v = fmaxf(v, fpeer<16>(v));
+// Over 16 neighbouring lanes, and over the wave.
+__device__ __forceinline__ float max16(float v) {
   v = fmaxf(v, fpeer<8>(v));
   v = fmaxf(v, fpeer<4>(v));
   v = fmaxf(v, fpeer<2>(v));
   return fmaxf(v, fpeer<1>(v));
 }
-__device__ __forceinline__ float wave_sum(float v) {
-  v += fpeer<32>(v);
-  v += fpeer<16>(v);
+__device__ __forceinline__ float sum16(float v) {
   v += fpeer<8>(v);
   v += fpeer<4>(v);
   v += fpeer<2>(v);
   return v + fpeer<1>(v);
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, fpeer<32>(v));
+  return max16(fmaxf(v, fpeer<16>(v)));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v += fpeer<32>(v);
+  return sum16(v + fpeer<16>(v));
 }
 
 __device__ __forceinline__ bool has_byte_255(uint32_t w) {
@@ -161,6 +182,11 @@ __device__ __forceinline__ void out_store(const bfp_rows &r, long long o, float 
   if ((threadIdx.x & 15) == 0) r.e[o >> 4] = (int8_t)e;
 }
 
+// What a row tile of k_kv4_rows costs beside its tiles (the queries, the first
+// loads, the results: about 4 us), in tiles of the list that hold nothing:
+// pieces of many short sequences hold fewer tiles.
+constexpr int ROWS_EXTRA = 4;
+
 typedef void (*attn_fn)(Kv4AttnArgs);
 // The kernel for heads of `tiles` tiles (k_kv4_rows: with 4 waves, or the 16
 // or 8 that rows_waves says) and its dynamic LDS.
@@ -172,8 +198,7 @@ AttnKernel rows_kernel(int tiles, int terms, int waves);
 AttnKernel prompt_kernel(int tiles, int terms);
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }
-// Queues the kernels that finish what the others left in pieces.
-void launch_join_rows(const Kv4AttnArgs &a, int terms, hipStream_t s);
+// Queues the kernel that joins what k_kv4_prompt left in pieces.
 void launch_join_prompt(const Kv4AttnArgs &a, hipStream_t s);
 
 }  // namespace bfp

@@ -11,6 +11,9 @@
 // prompts multiply term by term.
 #include "bfp_kv4_attn.h"
 
+#include <atomic>
+#include <chrono>
+
 namespace bfp {
 
 struct Kv4Plan {
@@ -63,18 +66,29 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
     // Short contexts: one workgroup takes a row tile's keys, four tiles a wave
     // at most, and there is nothing to join.  Otherwise as many workgroups as
     // run at once share all keys equally.
-    if (key_tiles > 4 * p.waves || p.waves == 4) {
+    if (key_tiles > 4 * p.waves) {
       p.waves = 4;
-      if (b.n_seq <= 256 && groups * cap_tiles < 0x7fffffffLL) {
-        const long long most = (groups * key_tiles + 3) / 4, slots = tiles <= 4 ? 1024 : tiles <= 8 ? 512 : 256;
+      if (b.n_seq <= 256 && groups * (cap_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
+        const long long most = groups * (key_tiles + ROWS_EXTRA) / 4 + 1, slots = tiles <= 4 ? 768 : tiles <= 8 ? 512 : 256;
         p.stream = (int)(most < slots ? most : slots);
         if (p.stream < 1) p.stream = 1;
         p.cells = 2 * (size_t)p.stream * R;
       }
     }
   }
-  p.work = p.cells * (16 * tiles * sizeof(float) + sizeof(float2));
+  p.work = p.cells * (16 * tiles * sizeof(float) + sizeof(float2)) + 2 * p.stream * sizeof(unsigned long long);
   return p;
+}
+
+// A number no other call has: what k_kv4_rows knows its flags in the
+// workspace by, whatever the workspace held before.
+static unsigned long long call_number() {
+  static std::atomic<unsigned long long> next{[] {
+    const unsigned long long t = (unsigned long long)std::chrono::steady_clock::now().time_since_epoch().count();
+    return (t ^ (unsigned long long)(uintptr_t)&next) * 0x9E3779B97F4A7C15ull;
+  }()};
+  const unsigned long long n = next.fetch_add(1, std::memory_order_relaxed);
+  return n ? n : next.fetch_add(1, std::memory_order_relaxed);   // 0 is no call's
 }
 
 static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
@@ -132,6 +146,8 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   if (p.work) {
     a.part_o = (float *)work;
     a.part_ml = (float2 *)((float *)work + p.cells * 16 * a.tiles);
+    a.there = (unsigned long long *)(a.part_ml + p.cells);
+    a.number = call_number();
   }
   a.row_tiles = p.row_tiles;
   a.by_head = FastDiv(cache->heads);
@@ -145,12 +161,8 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
     HIP_TRY(hipFuncSetAttribute((const void *)k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024));
   hipLaunchKernelGGL(k.fn, dim3((unsigned)blocks), dim3(64 * p.waves), k.lds, (hipStream_t)stream, a);
   BFP_TRY(launch_status(op));
-  if (p.stream)
-    launch_join_rows(a, p.terms, (hipStream_t)stream);
-  else if (p.splits > 1)
-    launch_join_prompt(a, (hipStream_t)stream);
-  else
-    return BFP_OK;
+  if (p.splits == 1) return BFP_OK;
+  launch_join_prompt(a, (hipStream_t)stream);
   return launch_status(op);
 }
 

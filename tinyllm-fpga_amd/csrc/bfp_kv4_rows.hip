@@ -64,12 +64,15 @@ __host__ __device__ inline int join_floats(int R, int tiles) { return 32 + R * (
 // the other, each of those its keys in order -- and every workgroup takes an
 // equally long piece of it, whatever the sequences' lengths.  A piece may end
 // in the middle of a row tile's keys: then the sums of the row tile's parts go
-// to slots of the workspace, and k_kv4_join_rows puts them together.
+// to slots of the workspace, and the workgroup that finishes the last of them
+// joins them, always in the order of the keys.
 constexpr int STREAM_SEQS = 256;   // sequences of such a batch: one a thread
+constexpr int MAX_PARTS = 128;     // of a row tile: their factors are held in LDS
 struct RowsSeq {
   int row0, n, at;     // Kv4Span
   int tile0, tiles;    // the keys that any of its rows sees, in tiles (at least one: somebody writes the zeros)
   int groups;          // row tiles x KV heads
+  __device__ uint32_t span() const { return (uint32_t)tiles + ROWS_EXTRA; }
 };
 __device__ __forceinline__ RowsSeq rows_seq(const Kv4AttnArgs &a, int R, int b) {
   const Kv4Span sp = kv4_span(a.b.start[b], a.b.start[b + 1], a.b.len[b], a.b.n_rows, a.b.max_q);
@@ -87,14 +90,16 @@ __device__ __forceinline__ RowsSeq rows_seq(const Kv4AttnArgs &a, int R, int b) 
 // all; each workgroup takes `piece` of them.  256 threads.
 struct Stream {
   uint32_t before[STREAM_SEQS + 1];
-  uint32_t wave[4];
+  uint32_t wave[4], longest[4];
+  int last;
 };
 __device__ __forceinline__ uint32_t stream_plan(const Kv4AttnArgs &a, int R, Stream &st) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  uint32_t n = 0;
+  uint32_t n = 0, most = 0;
   if (t < a.b.n_seq) {
     const RowsSeq s = rows_seq(a, R, t);
-    n = (uint32_t)s.groups * (uint32_t)s.tiles;
+    n = (uint32_t)s.groups * s.span();
+    most = (uint32_t)s.tiles;
   }
   uint32_t up = n;   // inclusive sums over the wave
 #pragma unroll
@@ -103,6 +108,12 @@ __device__ __forceinline__ uint32_t stream_plan(const Kv4AttnArgs &a, int R, Str
     up += lane >= d ? x : 0;
   }
   if (lane == 63) st.wave[w] = up;
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) {
+    const uint32_t x = __shfl_xor(most, d, 64);
+    most = x > most ? x : most;
+  }
+  if (lane == 0) st.longest[w] = most;
   __syncthreads();
   uint32_t base = 0;
 #pragma unroll
@@ -110,14 +121,69 @@ __device__ __forceinline__ uint32_t stream_plan(const Kv4AttnArgs &a, int R, Str
   if (t < a.b.n_seq) st.before[t + 1] = base + up;
   if (t == 0) st.before[0] = 0;
   __syncthreads();
-  const uint32_t all = st.before[a.b.n_seq], piece = (all + a.stream - 1) / a.stream;
-  return (piece + 3) / 4 * 4;   // a tile for each of four waves
+  most = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) most = st.longest[k] > most ? st.longest[k] : most;
+  const uint32_t all = st.before[a.b.n_seq], share = (all + a.stream - 1) / a.stream;
+  // m tiles in pieces of at least m / (MAX_PARTS - 2): at most MAX_PARTS of them, wherever they begin
+  const uint32_t least = (most + MAX_PARTS - 3) / (MAX_PARTS - 2);
+  return ((share > least ? share : least) + 3) / 4 * 4;   // a tile for each of four waves
+}
+
+// What workgroups hand each other goes past the XCDs' L2 caches, store by
+// store and load by load (device-scope accesses): a store is done when the
+// wait for it is over, so a workgroup's arrival after that wait and a barrier
+// says that its sums are there.  A device-scope fence instead would write back
+// and drop all of an L2 each time: 55 us for a call that takes 13 this way.
+__device__ __forceinline__ void put(float *p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put(float2 *p, float2 v) {
+  __hip_atomic_store((unsigned long long *)p, ((unsigned long long)__float_as_uint(v.y) << 32) | __float_as_uint(v.x),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get(const float *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get(const float2 *p) {
+  const unsigned long long u = __hip_atomic_load((const unsigned long long *)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32)));
+}
+__device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Wave 0: this part (number `mine` of a row tile's) is there; true for the
+// wave that finds all parts there, which is at least the last one's.  A part
+// is there if its flag holds the call's number (64 bits, from a random
+// start), so the workspace needs no clearing; whoever joins the parts takes
+// the flags away, so a replayed graph finds none.  Two workgroups may both
+// find all parts: they write the same results.
+__device__ __forceinline__ uint32_t part_slot(uint32_t p0, uint32_t k) { return 2 * (p0 + k) + (k == 0 ? 1 : 0); }
+__device__ __forceinline__ bool arrive(unsigned long long *there, unsigned long long number, uint32_t p0, uint32_t mine,
+                                       uint32_t parts) {
+  const uint32_t lane = threadIdx.x & 63;
+  if (lane == 0)
+    __hip_atomic_store(there + part_slot(p0, mine), number, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  stores_done();
+  bool all = true;
+#pragma unroll
+  for (uint32_t k = 0; k < MAX_PARTS; k += 64)
+    if (k + lane < parts)
+      all &= __hip_atomic_load(there + part_slot(p0, k + lane), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == number;
+  if (!__all(all)) return false;
+#pragma unroll
+  for (uint32_t k = 0; k < MAX_PARTS; k += 64)
+    if (k + lane < parts)
+      __hip_atomic_store(there + part_slot(p0, k + lane), 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return true;
 }
 
 // C: head tiles a lane group holds (hd <= 64 C); T: terms of a row (columns
 // R = 16 / T rows share); W: waves.
+template <int C, int R>
+__device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, int head, int rr0, uint32_t p0, int parts);
+
 template <int C, int T, int W>
-__global__ __launch_bounds__(64 * W, W > 8 || C == 1 ? 4 : W > 4 || C == 2 ? 2 : 1) void k_kv4_rows(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 2 : 1) void k_kv4_rows(Kv4AttnArgs a) {
   constexpr int R = 16 / T;
   extern __shared__ __align__(16) char lds[];
   __shared__ Stream st;
@@ -141,20 +207,44 @@ __global__ __launch_bounds__(64 * W, W > 8 || C == 1 ? 4 : W > 4 || C == 2 ? 2 :
   const int t = r / R;
   const int tiles = a.tiles;
   // one round takes keys of one row tile and KV head
-  for (bool begun = false; x < x_stop; begun = true) {
+  bool begun = false;
+  while (x < x_stop) {
+    const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
+    auto offset_of = [&](int tile, int id) {
+      return kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + 4 * r) & (a.c.page - 1));
+    };
+    // Without a window a wave's first tile is known before the lengths are:
+    // its page number and its bytes are on their way while those arrive.
+    KvSide<C> k, v;
+    int id = -1;
+    long long at = 0;
+    const bool early = !(W == 4 && a.stream) && a.window == 0;
+    if (early) {
+      id = kv4_page(pages, a.b.width, a.c.n_pages, (w * KEYS + 4 * r) >> a.page_shift);
+      at = offset_of(w, id);
+      load_side(k, a.c.k, a.c.k_e, at, a.c.page, g * C, tiles);
+      load_side(v, a.c.v, a.c.v_e, at, a.c.page, g * C, tiles);
+    }
     const RowsSeq sp = rows_seq(a, R, seq);
     int from = 0, upto = sp.tiles, slot = -1;
+    uint32_t begin = 0;
     if (W == 4 && a.stream) {
-      const uint32_t y = x - st.before[seq], group = y / (uint32_t)sp.tiles;
-      from = (int)(y - group * (uint32_t)sp.tiles);
-      const uint32_t left = x_stop - x, whole = (uint32_t)(sp.tiles - from);
-      upto = from + (int)(left < whole ? left : whole);
+      const uint32_t y = x - st.before[seq], group = y / sp.span(), off = y - group * sp.span();
+      const uint32_t left = x_stop - x, whole = sp.span() - off, take = left < whole ? left : whole;
+      begin = x - off;
+      x += take;
+      from = (int)off;
+      if (from >= sp.tiles) {   // nothing but the end of its span
+        while (x < x_stop && x == st.before[seq + 1]) ++seq;
+        continue;
+      }
+      upto = from + (int)take < sp.tiles ? from + (int)take : sp.tiles;
       // the first part of a row tile's keys goes to the workgroup's second slot, any other to its first
       if (from > 0 || upto < sp.tiles) slot = 2 * blockIdx.x + (from == 0 ? 1 : 0);
       head = (int)(group % (uint32_t)a.c.heads);
       rt = (int)(group / (uint32_t)a.c.heads);
-      x += (uint32_t)(upto - from);
       if (begun) __syncthreads();   // the last round's sums have been read
+      begun = true;
     } else {
       x = x_stop;
     }
@@ -209,22 +299,19 @@ __global__ __launch_bounds__(64 * W, W > 8 || C == 1 ? 4 : W > 4 || C == 2 ? 2 :
     const int swap = (r >> 2) & 1;
     char *vput0 = mylds + r * PITCH + g * C * 32 + 16 * swap, *vput1 = vput0 + 16 - 32 * swap;   // + 16 rows, + a tile
     const char *vget = mylds + (g * 4 + (r >> 2)) * PITCH + (((r & 3) ^ (2 * (g & 1))) * 8);        // + 16 rows, + a tile
-    const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
     auto page_of = [&](int tile) {
       return tile < stop ? kv4_page(pages, a.b.width, a.c.n_pages, (tile * KEYS + 4 * r) >> a.page_shift) : -1;
-    };
-    auto offset_of = [&](int tile, int id) {
-      return kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + 4 * r) & (a.c.page - 1));
     };
 
     // K of the next tile is asked for when this one's scores are done, V when
     // this one's has gone to LDS: no second set of registers
-    KvSide<C> k, v;
     int tile = first + w;
-    int id = page_of(tile);
-    long long at = offset_of(tile, id);
-    load_side(k, a.c.k, a.c.k_e, at, a.c.page, g * C, tiles);
-    load_side(v, a.c.v, a.c.v_e, at, a.c.page, g * C, tiles);
+    if (!early) {
+      id = page_of(tile);
+      at = offset_of(tile, id);
+      load_side(k, a.c.k, a.c.k_e, at, a.c.page, g * C, tiles);
+      load_side(v, a.c.v, a.c.v_e, at, a.c.page, g * C, tiles);
+    }
     for (; tile < stop; tile += W) {
       const int t0 = tile * KEYS;
       const int next_id = page_of(tile + W);
@@ -310,9 +397,9 @@ __global__ __launch_bounds__(64 * W, W > 8 || C == 1 ? 4 : W > 4 || C == 2 ? 2 :
           for (int e = 0; e < 4; ++e) {
             const float p = __builtin_amdgcn_exp2f(fmaf(s[2 * jp + jj][e], a.scale2, m0));
             sum += p;
-            pv[4 * jj + e] = round_term<T>(p, t);
+            pv[4 * jj + e] = p;
           }
-        pb[jp] = pack8(pv);
+        pb[jp] = pack_terms<T>(pv, t);
       }
 
       // A tile of V that holds a NaN counts as zeros in the product, so that it
@@ -397,86 +484,114 @@ __global__ __launch_bounds__(64 * W, W > 8 || C == 1 ? 4 : W > 4 || C == 2 ? 2 :
       if (d < tiles) {
         f32x4 v = o[d];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = term_sum<T>(v[e]);
+        for (int e = 0; e < 4; ++e) v[e] = term_sum<T>(T == 4 && t == 3 ? 0.0f : v[e]);
         if (r < R) *(f32x4 *)(jw + 32 + r * (hd + 4) + 16 * d + 4 * g) = v;
       }
     }
     __syncthreads();
     const float *jf = (const float *)lds;
-    // 16 lanes to a row's tile
+    // 16 lanes to a row's tile; lane k of them works out wave k's factor
+    const int l16 = threadIdx.x & 15;
     for (int u = threadIdx.x >> 4; u < R * tiles; u += 4 * W) {
-      const int row = u / tiles, d = 16 * (u % tiles) + (threadIdx.x & 15);
+      const int row = u / tiles, d = 16 * (u % tiles) + l16;
       if (rr0 + row >= rows) break;   // all 16 lanes
-      float M = -INFINITY;
+      const float mk = l16 < W ? jf[l16 * stride + row] : -INFINITY, M = max16(mk);
+      const float f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
+      const float L = sum16(l16 < W ? f * jf[l16 * stride + 16 + row] : 0.0f);
+      float acc = 0.0f;
 #pragma unroll
-      for (int k = 0; k < W; ++k) M = fmaxf(M, jf[k * stride + row]);
-      float L = 0.0f, acc = 0.0f;
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        const float mk = jf[k * stride + row];
-        const float f = mk == -INFINITY ? 0.0f : exp2f(mk - M);
-        L += f * jf[k * stride + 16 + row];
-        acc += f * jf[k * stride + 32 + row * (hd + 4) + d];
-      }
+      for (int k = 0; k < W; ++k)
+        acc += __shfl(f, (lane & 48) + k, 64) * jf[k * stride + 32 + row * (hd + 4) + d];
       const int ri = (rr0 + row) / G, rh = head * G + (rr0 + row) % G;
       const long long tok = sp.row0 + ri;
       if (slot >= 0) {
-        if (d == 0) a.part_ml[slot * R + row] = make_float2(M, L);
-        a.part_o[((long long)slot * R + row) * hd + d] = acc;
+        if (d == 0) put(a.part_ml + slot * R + row, make_float2(M, L));
+        put(a.part_o + ((long long)slot * R + row) * hd + d, acc);
       } else {
         out_store(a.out, tok * a.out.row_stride + rh * a.out.head_stride + d, L == 0.0f ? 0.0f : acc / L);
       }
     }
     if (!(W == 4 && a.stream)) return;
+    if (slot >= 0) {
+      // the row tile's parts are the pieces from p0 on
+      const uint32_t p0 = begin / piece, parts = (begin + sp.tiles - 1) / piece - p0 + 1;
+      stores_done();
+      __syncthreads();
+      if (w == 0) {
+        const bool all = arrive(a.there, a.number, p0, blockIdx.x - p0, parts);
+        if (lane == 0) st.last = all;
+      }
+      __syncthreads();
+      if (st.last) join_parts<C, R>(a, lds, sp, head, rr0, p0, (int)parts);
+    }
     while (x < x_stop && x == st.before[seq + 1]) ++seq;   // and past sequences without rows
   }
 }
 
-// Joins the parts of a row that several workgroups left: a wave takes one row
-// and query head.
-__global__ __launch_bounds__(256) void k_kv4_join_rows(Kv4AttnArgs a, int R) {
-  __shared__ Stream st;
-  const uint32_t piece = stream_plan(a, R, st);
-  const int seq = blockIdx.y;
-  const RowsSeq sp = rows_seq(a, R, seq);
-  const int u = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int i = u / a.q.heads, qh = u % a.q.heads;
-  if (i >= sp.n) return;
-  const int G = a.group, rr = i * G + qh % G, row = rr % R;
-  const uint32_t begin = st.before[seq] + (uint32_t)(rr / R * a.c.heads + qh / G) * (uint32_t)sp.tiles;
-  const uint32_t p0 = begin / piece, parts = (begin + sp.tiles - 1) / piece - p0 + 1;
-  if (parts == 1) return;   // written where it was made
-  auto slot = [&](uint32_t k) { return (long long)(2 * (p0 + k) + (k == 0 ? 1 : 0)) * R + row; };
-  const int hd = 16 * a.tiles;
-  float M = -INFINITY;
-  for (uint32_t k = lane; k < parts; k += 64) M = fmaxf(M, a.part_ml[slot(k)].x);
-  M = wave_max(M);
-  float L = 0.0f, acc[4] = {0, 0, 0, 0};
-  for (uint32_t k0 = 0; k0 < parts; k0 += 64) {
-    const float2 ml = k0 + lane < parts ? a.part_ml[slot(k0 + lane)] : make_float2(-INFINITY, 0.0f);
-    // a part that saw nothing (or NaN scores alone, whose sum is NaN): factor 0
-    const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-    L += f * ml.y;
-    const int n = parts - k0 < 64 ? (int)(parts - k0) : 64;
-    for (int k = 0; k < n; ++k) {
-      const float fk = __shfl(f, k, 64);
-      const float *o = a.part_o + slot(k0 + k) * hd;
+// A row tile's rows from the parts of their keys.  All of a workgroup of four
+// waves: the parts' factors first, then every wave takes each fourth part, a
+// lane the same values of all of them.
+template <int C, int R>
+__device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, int head, int rr0, uint32_t p0, int parts) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, G = a.group, hd = 16 * a.tiles;
+  const int left = sp.n * G - rr0, rows = left < R ? left : R;
+  float *factor = (float *)lds, *total = factor + MAX_PARTS * R, *sums = total + R;   // [part][R], [R], [4][256]
+  auto slot = [&](int k) { return (long long)part_slot(p0, (uint32_t)k) * R; };
+  for (int row = w; row < rows; row += 4) {
+    float2 ml[MAX_PARTS / 64];
+    float M = -INFINITY, L = 0.0f;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-        if (64 * d + lane < hd) acc[d] += fk * o[64 * d + lane];
+    for (int k = 0; k < MAX_PARTS / 64; ++k) {
+      ml[k] = 64 * k + lane < parts ? get(a.part_ml + slot(64 * k + lane) + row) : make_float2(-INFINITY, 0.0f);
+      M = fmaxf(M, ml[k].x);
     }
-  }
-  L = wave_sum(L);
-  const long long at = (long long)(sp.row0 + i) * a.out.row_stride + qh * a.out.head_stride;
+    M = wave_max(M);
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
-    if (64 * d + lane < hd) out_store(a.out, at + 64 * d + lane, L == 0.0f ? 0.0f : acc[d] / L);
+    for (int k = 0; k < MAX_PARTS / 64; ++k) {
+      // a part that saw nothing (or NaN scores alone, whose sum is NaN): factor 0
+      const float f = ml[k].x == -INFINITY ? 0.0f : exp2f(ml[k].x - M);
+      L += f * ml[k].y;
+      if (64 * k + lane < parts) factor[(64 * k + lane) * R + row] = f;
+    }
+    L = wave_sum(L);
+    if (lane == 0) total[row] = L;
+  }
+  __syncthreads();
+  const int values = rows * hd;   // of a part, row after row: multiples of 16
+  for (int v0 = 0; v0 < values; v0 += 256) {
+    float acc[4] = {0, 0, 0, 0};
+    int at[4], row[4];   // past the last value: the last one, not taken
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      at[e] = v0 + 64 * e + lane < values ? v0 + 64 * e + lane : values - 1;
+      row[e] = at[e] / hd;
+    }
+#pragma unroll 4
+    for (int k = w; k < parts; k += 4) {
+      const float *o = a.part_o + slot(k) * hd;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += factor[k * R + row[e]] * get(o + at[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[w * 256 + 64 * e + lane] = acc[e];
+    __syncthreads();
+    const int v = v0 + threadIdx.x;
+    if (v < values) {   // whole groups of 16 lanes
+      const int r = v / hd, rr = rr0 + r;
+      const float L = total[r], acc4 = (sums[threadIdx.x] + sums[256 + threadIdx.x]) + (sums[512 + threadIdx.x] + sums[768 + threadIdx.x]);
+      out_store(a.out, (long long)(sp.row0 + rr / G) * a.out.row_stride + (head * G + rr % G) * a.out.head_stride + v % hd,
+                L == 0.0f ? 0.0f : acc4 / L);
+    }
+    __syncthreads();
+  }
 }
 
 template <int C, int W>
 static AttnKernel pick(int tiles, int terms) {
-  const int R = 16 / terms, in = W * V_ROWS * v_pitch(C), out = W * join_floats(R, tiles) * 4;
-  return {terms == 1 ? k_kv4_rows<C, 1, W> : terms == 2 ? k_kv4_rows<C, 2, W> : k_kv4_rows<C, 4, W>, in > out ? in : out};
+  const int R = 16 / terms;
+  int lds = W * V_ROWS * v_pitch(C);
+  for (int n : {W * join_floats(R, tiles) * 4, (MAX_PARTS * R + R + 1024) * 4}) lds = n > lds ? n : lds;
+  return {terms == 1 ? k_kv4_rows<C, 1, W> : terms == 2 ? k_kv4_rows<C, 2, W> : k_kv4_rows<C, 4, W>, lds};
 }
 
 AttnKernel rows_kernel(int tiles, int terms, int waves) {
@@ -484,11 +599,6 @@ AttnKernel rows_kernel(int tiles, int terms, int waves) {
   if (C == 1) return waves == 4 ? pick<1, 4>(tiles, terms) : pick<1, 16>(tiles, terms);
   if (C == 2) return waves == 4 ? pick<2, 4>(tiles, terms) : pick<2, 8>(tiles, terms);
   return C == 3 ? pick<3, 4>(tiles, terms) : pick<4, 4>(tiles, terms);
-}
-
-void launch_join_rows(const Kv4AttnArgs &a, int terms, hipStream_t s) {
-  const long long n = ((long long)a.b.max_q * a.q.heads + 3) / 4;
-  hipLaunchKernelGGL(k_kv4_join_rows, dim3((unsigned)n, a.b.n_seq), dim3(256), 0, s, a, 16 / terms);
 }
 
 }  // namespace bfp
