@@ -159,9 +159,13 @@ class Fp4Cache:
         if k is None and v is None:
             if n_rows is None:
                 raise ValueError("read needs n_rows, or tensors to read into")
-            shape = (int(n_rows), self.heads, self.hd)
-            k = torch.empty(shape, dtype=torch.float32 if dtype is None else dtype, device=self.device)
-            v = torch.empty_like(k)
+            k, kr = _rows.empty(int(n_rows), self.heads, self.hd, dtype, self.device)
+            v, vr = _rows.empty(int(n_rows), self.heads, self.hd, dtype, self.device)
+            if batch.device != self.device:
+                raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+            if n_rows:
+                _read(self.device, self._c, batch._c(int(n_rows)), C.byref(kr), C.byref(vr))
+            return k, v
         n, rs = None, []
         for x, what in ((k, "k"), (v, "v")):
             if x is None:

@@ -32,11 +32,18 @@ def rope_freqs(rot, base=10000.0, scaling="none", factor=1.0, orig_ctx=0):
       "bands"   above 4 turns stay, below 1 divided, linear in the turns"""
     if scaling not in SCALINGS:
         raise ValueError(f"scaling {scaling!r}: one of {', '.join(SCALINGS)}")
-    inv = np.empty(max(int(rot) // 2, 1), np.float64)
-    mscale = C.c_double()
-    call("bfp_rope_freqs", int(rot), float(base), SCALINGS[scaling], float(factor), int(orig_ctx),
-         inv.ctypes.data, C.byref(mscale))
-    return inv, mscale.value
+    n = max(int(rot) // 2, 1)
+    inv, mscale = (C.c_double * n)(), C.c_double()
+    call("bfp_rope_freqs", int(rot), float(base), SCALINGS[scaling], float(factor), int(orig_ctx), inv,
+         C.byref(mscale))
+    return np.frombuffer(inv, np.float64), mscale.value
+
+
+def _address(a):
+    try:   # a third of the time a.ctypes.data takes
+        return C.addressof(C.c_char.from_buffer(a))
+    except (TypeError, ValueError, BufferError):   # not writable, or empty
+        return a.ctypes.data
 
 
 def rope_table(inv_freq, n_pos, mscale=1.0, first=0, out=None):
@@ -53,7 +60,7 @@ def rope_table(inv_freq, n_pos, mscale=1.0, first=0, out=None):
     elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or not out.is_cuda:
         raise ValueError(f"out must be a contiguous float32 tensor {shape} on a GPU")
     if shape[0]:
-        _table(out.device, inv.ctypes.data, inv.size, float(mscale), int(first), shape[0], out.data_ptr())
+        _table(out.device, _address(inv), inv.size, float(mscale), int(first), shape[0], out.data_ptr())
     return out
 
 

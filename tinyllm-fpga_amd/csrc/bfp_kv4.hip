@@ -58,7 +58,12 @@ struct Kv4AppendArgs {
   bfp_rows k, v, q, q_out;
   const int32_t *pos;
   const float2 *table;
-  int n_pos, half, interleaved, hq;
+  int n_pos, half, interleaved;
+  // workgroups [0, q_blocks) of a sequence turn queries, the others append
+  RopeShape shape;
+  FastDiv q_row, q_head;   // q's units of a row, of N heads
+  int q_blocks;
+  uint32_t q_units;
   Kv4Units units;
   FastDiv tiles;   // of a head
   uint32_t n_units;
@@ -119,38 +124,58 @@ __device__ __forceinline__ void load_turned(const bfp_rows &r, long long o, int 
   }
 }
 
-// Bound by the bytes of k, v and q in and of q and the tiles out.
+// Zeros where rope_unit or rope_wide_unit would write.
+template <int N>
+__device__ __forceinline__ void zero_unit(const RopeShape &s, const bfp_rows &y, long long t, int h0, int j) {
+  const bool turn = j < s.turned;
+  const int w = N ? 8 : 1, da = !turn ? 2 * s.half + (j - s.turned) * w : s.interleaved ? (N ? 8 : 2) * j : w * j;
+  const int values = N ? 8 : turn && s.interleaved ? 2 : 1;
+  for (int h = h0; h < y.heads && h < h0 + (N ? N : 1); ++h) {
+    const long long yo = t * y.row_stride + h * y.head_stride + da;
+    for (int i = 0; i < values; ++i) {
+      row_store(y, yo + i, 0.0f);
+      if (turn && !s.interleaved) row_store(y, yo + s.half + i, 0.0f);
+    }
+  }
+}
+
+// N: heads of q a thread turns (0: value by value).  Bound by the bytes of k,
+// v and q in and of q and the tiles out.
+template <int N>
 __global__ __launch_bounds__(KV4_BS) void k_kv4_append(Kv4AppendArgs a) {
   const int seq = blockIdx.y;
-  const uint32_t u = blockIdx.x * KV4_BS + threadIdx.x;
-  if (u >= a.n_units) return;
+  const bool is_q = (int)blockIdx.x < a.q_blocks;
+  const uint32_t u = (blockIdx.x - (is_q ? 0 : a.q_blocks)) * KV4_BS + threadIdx.x;
+  if (u >= (is_q ? a.q_units : a.n_units)) return;
   const Kv4Span s = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
   int i;
   uint32_t col, tile;
-  a.units.of(u, i, col);
+  if (is_q)
+    i = (int)a.q_row.div(u, col);
+  else
+    a.units.of(u, i, col);
   if (i >= s.n) return;
-  int head = (int)a.tiles.div(col, tile);
-  const int tiles = (int)a.tiles.d;
   const long long t = s.row0 + i;
   const int at = s.at + i;
   const int id = at < 0 ? -1 : kv4_page(a.b.pages + (long long)seq * a.b.width, a.b.width, a.c.n_pages, at / a.c.page);
   const int p = a.pos ? a.pos[t] : at;
   const bool known = (unsigned)p < (unsigned)a.n_pos;
   const float2 *cs = a.table + (known ? (long long)p * a.half : 0);
-  const int d0 = 16 * (int)tile;
-  if (head < a.hq) {
-    double y[16];
+  if (is_q) {
+    uint32_t j;
+    const int h = (int)a.q_head.div(col, j);
     if (id < 0) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) y[j] = 0.0;
+      zero_unit<N>(a.shape, a.q_out, t, h * (N ? N : 1), (int)j);
+    } else if constexpr (N == 0) {
+      rope_unit(a.shape, a.q, a.q_out, t, h, (int)j, known ? cs : nullptr);
     } else {
-      load_turned(a.q, t * a.q.row_stride + head * a.q.head_stride, d0, cs, a.half, a.interleaved, known, y);
+      rope_wide_unit<N>(a.shape, a.q, a.q_out, t, h * N, a.q.heads, (int)j, known ? cs : nullptr);
     }
-    row_store_n(a.q_out, t * a.q_out.row_stride + head * a.q_out.head_stride + d0, y);
     return;
   }
-  head -= a.hq;
   if (id < 0) return;
+  int head = (int)a.tiles.div(col, tile);
+  const int d0 = 16 * (int)tile;
   const bool is_v = head >= a.c.heads;
   if (is_v) head -= a.c.heads;
   float x[16];
@@ -164,7 +189,7 @@ __global__ __launch_bounds__(KV4_BS) void k_kv4_append(Kv4AppendArgs a) {
   }
   uint32_t E;
   const uint2 w = kv4_encode(x, E);
-  const long long o = kv4_tile(id, a.c.heads, head, tiles, (int)tile, a.c.page, at & (a.c.page - 1));
+  const long long o = kv4_tile(id, a.c.heads, head, (int)a.tiles.d, (int)tile, a.c.page, at & (a.c.page - 1));
   *(uint2 *)((is_v ? a.c.v : a.c.k) + o * KV4_TILE_BYTES) = w;
   (is_v ? a.c.v_e : a.c.k_e)[o] = (uint8_t)E;
 }
@@ -261,14 +286,29 @@ int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp
   a.b = *batch;
   a.k = *k;
   a.v = *v;
-  if (q) a.q = *q, a.q_out = *q_out, a.hq = q->heads;
   a.pos = pos;
   a.table = (const float2 *)table;
   a.n_pos = table ? n_pos : 0;
   a.half = table ? rot / 2 : 0;
   a.interleaved = interleaved ? 1 : 0;
-  BFP_TRY(plan_units(op, a.c, a.b, a.hq + 2 * a.c.heads, a.units, a.tiles, a.n_units));
-  hipLaunchKernelGGL(k_kv4_append, dim3((a.n_units + KV4_BS - 1) / KV4_BS, batch->n_seq), dim3(KV4_BS), 0,
+  BFP_TRY(plan_units(op, a.c, a.b, 2 * a.c.heads, a.units, a.tiles, a.n_units));
+  int n = 1;
+  if (q) {
+    a.q = *q, a.q_out = *q_out;
+    a.shape = rope_shape(*q, *q_out, hd, 2 * a.half, interleaved);
+    // four heads a thread once that still leaves eight waves a CU
+    const long long all = (long long)rows * q->heads * a.shape.per_head;
+    n = !a.shape.wide ? 0 : q->heads >= ROPE_HEADS && all >= (long long)ROPE_HEADS * 256 * 8 * 64 ? ROPE_HEADS : 1;
+    const long long per_row = (long long)a.shape.per_head * (n > 1 ? (q->heads + n - 1) / n : q->heads);
+    if (per_row * batch->max_q > 0x7fffff00LL)
+      return set_err(BFP_EINVAL, "%s: max_q=%d rows of %d query heads are too many for one call", op, batch->max_q, q->heads);
+    a.q_row = FastDiv((uint32_t)per_row);
+    a.q_head = FastDiv((uint32_t)a.shape.per_head);
+    a.q_units = (uint32_t)(per_row * batch->max_q);
+    a.q_blocks = (int)((a.q_units + KV4_BS - 1) / KV4_BS);
+  }
+  hipLaunchKernelGGL(n == 0 ? k_kv4_append<0> : n == 1 ? k_kv4_append<1> : k_kv4_append<ROPE_HEADS>,
+                     dim3(a.q_blocks + (a.n_units + KV4_BS - 1) / KV4_BS, batch->n_seq), dim3(KV4_BS), 0,
                      (hipStream_t)stream, a);
   return launch_status(op);
 }

@@ -2,7 +2,30 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include "bfp_rows.h"
+
 namespace bfp {
+
+// How the heads of rows are cut into units of work, for 16-byte accesses
+// (`wide`: 8 pairs, that is two groups of 8 values, of the half layout, 4 of the
+// interleaved one, or 8 values to copy) or value by value (a pair, or a value
+// to copy): rows of any width, stride and alignment.
+struct RopeShape {
+  int half, interleaved, wide, turned, per_head;   // units that are turned, and all of them
+};
+inline RopeShape rope_shape(const bfp_rows &x, const bfp_rows &y, int hd, int rot, int interleaved) {
+  RopeShape s;
+  s.half = rot / 2;
+  s.interleaved = interleaved ? 1 : 0;
+  s.wide = rows_aligned(x, 8) && rows_aligned(y, 8) && hd % 8 == 0 && (interleaved ? rot % 8 == 0 : s.half % 8 == 0);
+  s.turned = s.wide ? (interleaved ? rot / 8 : s.half / 8) : s.half;
+  s.per_head = s.turned + (s.wide ? (hd - rot) / 8 : hd - rot);
+  return s;
+}
+// Heads a thread takes, one after the other, of wide units: their angles are
+// the same, and their loads are under way together.  A call of few units is
+// spread over more threads instead.
+constexpr int ROPE_HEADS = 4;
 
 __device__ __forceinline__ double2 rope_cs(float2 t) { return make_double2((double)t.x, (double)t.y); }
 
@@ -13,6 +36,71 @@ __device__ __forceinline__ double2 rope_cs(float2 t) { return make_double2((doub
 __device__ __forceinline__ void rope_pair(float a, float b, double2 cs, double &ya, double &yb) {
   ya = fma((double)a, cs.x, -((double)b * cs.y));
   yb = fma((double)b, cs.x, (double)a * cs.y);
+}
+
+// Unit j of head h of row t.  cs: the row's angles (null: it has none, NaN).
+__device__ __forceinline__ void rope_unit(const RopeShape &s, const bfp_rows &x, const bfp_rows &y, long long t, int h,
+                                          int j, const float2 *cs) {
+  const long long xo = t * x.row_stride + h * x.head_stride, yo = t * y.row_stride + h * y.head_stride;
+  if (j >= s.turned) {
+    const int d = j + s.half;
+    row_store(y, yo + d, row_load(x, xo + d));
+    return;
+  }
+  const int da = s.interleaved ? 2 * j : j, db = s.interleaved ? 2 * j + 1 : j + s.half;
+  double ya, yb;
+  rope_pair(row_load(x, xo + da), row_load(x, xo + db), cs ? rope_cs(cs[j]) : make_double2(NAN, NAN), ya, yb);
+  row_store(y, yo + da, ya);
+  row_store(y, yo + db, yb);
+}
+
+// Wide unit j of heads h0 .. h0 + N - 1 (those below `heads`) of row t.
+template <int N>
+__device__ __forceinline__ void rope_wide_unit(const RopeShape &s, const bfp_rows &x, const bfp_rows &y, long long t,
+                                               int h0, int heads, int j, const float2 *cs) {
+  const bool turn = j < s.turned;
+  const int da = turn ? 8 * j : 2 * s.half + (j - s.turned) * 8, db = da + s.half;
+  const bool two = turn && !s.interleaved;
+  float va[N][8], vb[N][8];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const int h = h0 + n < heads ? h0 + n : heads - 1;
+    row_load_n(x, t * x.row_stride + h * x.head_stride + da, va[n]);
+    if (two) row_load_n(x, t * x.row_stride + h * x.head_stride + db, vb[n]);
+  }
+  if (!turn) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (h0 + n < heads) row_store_n(y, t * y.row_stride + (h0 + n) * y.head_stride + da, va[n]);
+    return;
+  }
+  if (two) {
+    double2 c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = cs ? rope_cs(cs[8 * j + i]) : make_double2(NAN, NAN);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (h0 + n >= heads) break;
+      double ya[8], yb[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rope_pair(va[n][i], vb[n][i], c[i], ya[i], yb[i]);
+      const long long yo = t * y.row_stride + (h0 + n) * y.head_stride;
+      row_store_n(y, yo + da, ya);
+      row_store_n(y, yo + db, yb);
+    }
+  } else {
+    double2 c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = cs ? rope_cs(cs[4 * j + i]) : make_double2(NAN, NAN);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      if (h0 + n >= heads) break;
+      double ya[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rope_pair(va[n][2 * i], va[n][2 * i + 1], c[i], ya[2 * i], ya[2 * i + 1]);
+      row_store_n(y, t * y.row_stride + (h0 + n) * y.head_stride + da, ya);
+    }
+  }
 }
 
 }  // namespace bfp

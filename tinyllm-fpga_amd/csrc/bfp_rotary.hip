@@ -34,79 +34,28 @@ __global__ __launch_bounds__(ROPE_BS) void k_rope_table(RopeFreqs f, FastDiv n_f
 
 struct RopeArgs {
   bfp_rows x, y;
+  RopeShape shape;
   const int32_t *pos;
   const float2 *table;
-  int hd, n_pos, half, interleaved, row0;
-  FastDiv per_row, per_head;   // units of work of a row, of a head
+  int n_pos, row0;
+  FastDiv per_row, per_head;   // units of work of a row, of N heads
   uint32_t units;
 };
 
-// Every unit of a head is one pair, or one value past the rotated part:
-// rows of any width, stride and alignment.
-__global__ __launch_bounds__(ROPE_BS) void k_rope_pairs(RopeArgs a) {
+// N = 0: value by value.
+template <int N>
+__global__ __launch_bounds__(ROPE_BS) void k_rope(RopeArgs a) {
   const uint32_t u = blockIdx.x * ROPE_BS + threadIdx.x;
   if (u >= a.units) return;
   uint32_t rest, j;
-  const uint32_t t = a.row0 + a.per_row.div(u, rest);
-  const uint32_t h = a.per_head.div(rest, j);
-  const long long xo = t * a.x.row_stride + h * a.x.head_stride;
-  const long long yo = t * a.y.row_stride + h * a.y.head_stride;
-  if ((int)j >= a.half) {
-    const int d = (int)j + a.half;
-    row_store(a.y, yo + d, row_load(a.x, xo + d));
-    return;
-  }
+  const long long t = a.row0 + (long long)a.per_row.div(u, rest);
+  const int h = (int)a.per_head.div(rest, j);
   const int p = a.pos[t];
-  const int da = a.interleaved ? 2 * j : j, db = a.interleaved ? 2 * j + 1 : j + a.half;
-  const bool in = (unsigned)p < (unsigned)a.n_pos;
-  const double2 cs = in ? rope_cs(a.table[(long long)p * a.half + j]) : make_double2(NAN, NAN);
-  double ya, yb;
-  rope_pair(row_load(a.x, xo + da), row_load(a.x, xo + db), cs, ya, yb);
-  row_store(a.y, yo + da, ya);
-  row_store(a.y, yo + db, yb);
-}
-
-// Units of 8 values in 16-byte accesses: 8 pairs (two groups of 8 values) of
-// the half layout, 4 of the interleaved one, or 8 values to copy.
-__global__ __launch_bounds__(ROPE_BS) void k_rope_wide(RopeArgs a) {
-  const uint32_t u = blockIdx.x * ROPE_BS + threadIdx.x;
-  if (u >= a.units) return;
-  uint32_t rest, j;
-  const uint32_t t = a.row0 + a.per_row.div(u, rest);
-  const uint32_t h = a.per_head.div(rest, j);
-  const long long xo = t * a.x.row_stride + h * a.x.head_stride;
-  const long long yo = t * a.y.row_stride + h * a.y.head_stride;
-  const int turned = a.interleaved ? a.half / 4 : a.half / 8;
-  if ((int)j >= turned) {
-    const int d = 2 * a.half + ((int)j - turned) * 8;
-    float v[8];
-    row_load_n(a.x, xo + d, v);
-    row_store_n(a.y, yo + d, v);
-    return;
-  }
-  const int p = a.pos[t];
-  const bool in = (unsigned)p < (unsigned)a.n_pos;
-  const float2 *cs = a.table + (in ? (long long)p * a.half : 0);
-  if (a.interleaved) {
-    float v[8];
-    row_load_n(a.x, xo + 8 * j, v);
-    double y[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      rope_pair(v[2 * i], v[2 * i + 1], in ? rope_cs(cs[4 * j + i]) : make_double2(NAN, NAN), y[2 * i],
-                y[2 * i + 1]);
-    row_store_n(a.y, yo + 8 * j, y);
-  } else {
-    float va[8], vb[8];
-    row_load_n(a.x, xo + 8 * j, va);
-    row_load_n(a.x, xo + a.half + 8 * j, vb);
-    double ya[8], yb[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      rope_pair(va[i], vb[i], in ? rope_cs(cs[8 * j + i]) : make_double2(NAN, NAN), ya[i], yb[i]);
-    row_store_n(a.y, yo + 8 * j, ya);
-    row_store_n(a.y, yo + a.half + 8 * j, yb);
-  }
+  const float2 *cs = (unsigned)p < (unsigned)a.n_pos ? a.table + (long long)p * a.shape.half : nullptr;
+  if constexpr (N == 0)
+    rope_unit(a.shape, a.x, a.y, t, h, (int)j, cs);
+  else
+    rope_wide_unit<N>(a.shape, a.x, a.y, t, h * N, a.x.heads, (int)j, cs);
 }
 
 }  // namespace bfp
@@ -190,22 +139,20 @@ int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const 
   if (!pos || !table || n_pos < 1) return set_err(BFP_EINVAL, "rope: no positions or no table");
   if ((uintptr_t)table % 8) return set_err(BFP_EINVAL, "rope: table is not 8-byte aligned");
   if (n_rows == 0) return BFP_OK;
-  const int half = rot / 2;
-  // 16-byte accesses where the groups of 8 fall on them; else value by value
-  const bool wide = rows_aligned(*x, 8) && rows_aligned(*y, 8) && hd % 8 == 0 &&
-                    (interleaved ? rot % 8 == 0 : half % 8 == 0);
-  const int per_head = wide ? (interleaved ? rot / 8 : half / 8) + (hd - rot) / 8 : half + hd - rot;
-  const long long per_row = (long long)per_head * x->heads;
+  const RopeShape shape = rope_shape(*x, *y, hd, rot, interleaved);
+  // four heads a thread once that still leaves eight waves a CU
+  const long long all = (long long)n_rows * x->heads * shape.per_head;
+  const int n = shape.wide && x->heads >= ROPE_HEADS && all >= (long long)ROPE_HEADS * 256 * 8 * 64 ? ROPE_HEADS : 1;
+  const long long per_row = (long long)shape.per_head * ((x->heads + n - 1) / n);
   if (per_row > 0x3fffffffLL) return set_err(BFP_EINVAL, "rope: rows of %lld units", per_row);
-  RopeArgs a{*x, *y, pos, (const float2 *)table, hd, n_pos, half, interleaved ? 1 : 0, 0,
-             FastDiv((uint32_t)per_row), FastDiv((uint32_t)per_head), 0};
+  RopeArgs a{*x, *y, shape, pos, (const float2 *)table, n_pos, 0, FastDiv((uint32_t)per_row), FastDiv((uint32_t)shape.per_head), 0};
+  auto *fn = !shape.wide ? k_rope<0> : n == 1 ? k_rope<1> : k_rope<ROPE_HEADS>;
   const int step = (int)(0x7fffff00LL / per_row);
   for (int r = 0; r < n_rows;) {
     const int rows = n_rows - r < step ? n_rows - r : step;
     a.row0 = r;
     a.units = (uint32_t)((long long)rows * per_row);
-    hipLaunchKernelGGL(wide ? k_rope_wide : k_rope_pairs, dim3((a.units + ROPE_BS - 1) / ROPE_BS),
-                       dim3(ROPE_BS), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(fn, dim3((a.units + ROPE_BS - 1) / ROPE_BS), dim3(ROPE_BS), 0, (hipStream_t)stream, a);
     BFP_TRY(launch_status("rope"));
     r += rows;
   }
