@@ -296,7 +296,7 @@ int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp
   if (q) {
     a.q = *q, a.q_out = *q_out;
     a.shape = rope_shape(*q, *q_out, hd, 2 * a.half, interleaved);
-    // four heads a thread once that still leaves eight waves a CU
+    // two heads a thread once that still leaves eight waves a CU
     const long long all = (long long)rows * q->heads * a.shape.per_head;
     n = !a.shape.wide ? 0 : q->heads >= ROPE_HEADS && all >= (long long)ROPE_HEADS * 256 * 8 * 64 ? ROPE_HEADS : 1;
     const long long per_row = (long long)a.shape.per_head * (n > 1 ? (q->heads + n - 1) / n : q->heads);
