@@ -31,7 +31,8 @@ struct Kv4AttnArgs {
   int tiles, group, page_shift, window, row_tiles;
   int splits, chunk;   // k_kv4_prompt: pieces of the keys, and their length in tiles
   int stream;          // k_kv4_rows: workgroups that share all tiles (0: one takes all keys of its rows)
-  FastDiv by_seq, by_head, by_split;
+  int out_wide;        // out takes 16-byte stores
+  FastDiv by_seq, by_head, by_split, by_group;
   // A workgroup's piece: one sequence after the other, its last rows, which
   // see the most keys, first.  Neighbouring workgroups take different KV heads
   // of the same rows and keys: workgroups go to the XCDs and their shader
@@ -180,6 +181,26 @@ __device__ __forceinline__ void out_store(const bfp_rows &r, long long o, float 
   const int m = quantize16_lanes((double)v, e);
   ((int16_t *)r.p)[o] = (int16_t)m;
   if ((threadIdx.x & 15) == 0) r.e[o >> 4] = (int8_t)e;
+}
+
+// Eight values from o on; of a tile, the other eight are lane ^ 1's.
+__device__ __forceinline__ void out_store8(const bfp_rows &r, long long o, const float (&v)[8], bool wide) {
+  if (r.type != BFP_TILES) {
+    if (wide) {
+      row_store_n(r, o, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) row_store(r, o + i, v[i]);
+    }
+    return;
+  }
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+  const int e = tile_exp_of((double)fmaxf(top, __shfl_xor(top, 1, 64)));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ((int16_t *)r.p)[o + i] = (int16_t)tile_mant_of((double)v[i], e);
+  if (!(threadIdx.x & 1)) r.e[o >> 4] = (int8_t)e;
 }
 
 // What a row tile of k_kv4_rows costs beside its tiles (the queries, the first

@@ -152,6 +152,8 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   a.row_tiles = p.row_tiles;
   a.by_head = FastDiv(cache->heads);
   a.by_split = FastDiv(p.splits);
+  a.by_group = FastDiv((uint32_t)a.group);
+  a.out_wide = rows_aligned(*out, 8);
   const long long each = (long long)p.row_tiles * p.splits * cache->heads, blocks = p.stream ? p.stream : each * batch->n_seq;
   if (each > 0x7fffffLL || blocks > 0x7fffffLL)
     return set_err(BFP_EINVAL, "%s: max_q=%d is too large for one call", op, batch->max_q);

@@ -47,7 +47,8 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   const int tiles = a.tiles;
   const int wg0 = rt * ROWS, rr0 = wg0 + 32 * w, rr = rr0 + n;
   const bool mine = rr < rows;
-  const int i = mine ? rr / G : 0, qh = head * G + (mine ? rr % G : 0);
+  uint32_t qg;
+  const int i = (int)a.by_group.div((uint32_t)(mine ? rr : 0), qg), qh = head * G + (int)qg;
   const int hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
   // what this wave's rows all see, and any of the workgroup's
   const int wfirst = rr0 < rows ? rr0 : rows - 1, wlast = (rr0 + 32 < rows ? rr0 + 32 : rows) - 1;
@@ -276,39 +277,63 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   }
   __syncthreads();
 
-  // results: 32 values of the wave's rows at a time through LDS, 16 lanes to a tile
+  // results: 32 values of the wave's rows at a time through LDS, 4 lanes to a
+  // row with 8 values each
   sum += fpeer<32>(sum);
   float *ow = (float *)lds + w * 32 * OUT_PITCH, *ml = (float *)lds + W * 32 * OUT_PITCH + w * 64;
   if (h == 0) {
     ml[n] = m * a.scale2;
     ml[32 + n] = sum;
   }
-  const int hd = 16 * tiles;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  const int hd = 16 * tiles, piece = 8 * (lane & 3);
+  bool live[2];
+  long long to[2];   // of the row's first value, in out or in the unfinished sums
+  float over[2];     // 1 / sum (0: nothing seen), or 1
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int row = (lane >> 2) + 16 * k;
+    live[k] = rr0 + row < rows;
+    uint32_t rg;
+    const int ri = (int)a.by_group.div((uint32_t)(live[k] ? rr0 + row : 0), rg), rh = head * G + (int)rg;
+    const long long tok = sp.row0 + ri;
+    const float L = ml[32 + row];
+    if (a.splits > 1) {
+      const long long at = (tok * a.q.heads + rh) * a.splits + split;
+      if (live[k] && piece == 0) a.part_ml[at] = make_float2(ml[row], L);
+      to[k] = at * hd;
+      over[k] = 1.0f;
+    } else {
+      to[k] = tok * a.out.row_stride + rh * a.out.head_stride;
+      over[k] = L == 0.0f ? 0.0f : 1.0f / L;
+    }
+  }
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
-    if (2 * d >= tiles) continue;
-    const f32x16 v = o[d];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
+    if (2 * d < tiles) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-      *(f32x4 *)(ow + n * OUT_PITCH + 8 * b + 4 * h) = f32x4{v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]};
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int k = lane >> 4; k < 64; k += 4) {
-      const int row = k >> 1, dim = 32 * d + 16 * (k & 1) + (lane & 15);
-      if (rr0 + row >= rows) break;
-      if (dim >= hd) continue;   // all 16 lanes
-      const int ri = (rr0 + row) / G, rh = head * G + (rr0 + row) % G;
-      const long long tok = sp.row0 + ri;
-      const float L = ml[32 + row], acc = ow[row * OUT_PITCH + dim - 32 * d];
-      if (a.splits > 1) {
-        const long long at = (tok * a.q.heads + rh) * a.splits + split;
-        if (dim == 0) a.part_ml[at] = make_float2(ml[row], L);
-        a.part_o[at * hd + dim] = acc;
-      } else {
-        out_store(a.out, tok * a.out.row_stride + rh * a.out.head_stride + dim, L == 0.0f ? 0.0f : acc / L);
+      for (int b = 0; b < 4; ++b)
+        *(f32x4 *)(ow + n * OUT_PITCH + 8 * b + 4 * h) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (!live[k] || 32 * d + piece >= hd) continue;   // all of a tile's lanes
+        const float *from = ow + ((lane >> 2) + 16 * k) * OUT_PITCH + piece;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = from[e] * over[k];
+        const long long at = to[k] + 32 * d + piece;
+        if (a.splits > 1) {
+          float4 *p = (float4 *)(a.part_o + at);
+          p[0] = make_float4(v[0], v[1], v[2], v[3]);
+          p[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          out_store8(a.out, at, v, a.out_wide);
+        }
       }
     }
   }
