@@ -21,6 +21,7 @@ struct Kv4Plan {
   int terms, waves, row_tiles, splits, chunk, stream;
   size_t cells;      // of the workspace: rows of unfinished sums
   size_t work;       // its bytes
+  double us;
 };
 
 // The terms a row is carried in: one where queries, probabilities and results
@@ -40,11 +41,52 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   long long keys = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
   if (window > 0 && keys > (long long)window + b.max_q) keys = (long long)window + b.max_q;
   const long long key_tiles = (keys + KEYS - 1) / KEYS;
-  p.prompt = rows > 64;
-  p.splits = 1;
   p.chunk = (int)key_tiles;
-  if (p.prompt) {
-    const bool wide = q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES;
+  p.splits = 1;
+  // Both kernels' times in microseconds, from what a workgroup of each takes
+  // for itself (the first loads, the results) and for a round of 64-key tiles,
+  // one workgroup a CU at a time:
+  //                     few rows: itself, 16 / 8 / 4 tiles    prompts: itself, a tile
+  //   heads up to 64          7.0 (float32 8.9), 2.7                 8.8 (10.6), 1.4
+  //   up to 128               7.5 (9.5), 2.6                         12, 1.8
+  //   up to 192, 256          11, 13; 2.6                            16, 20; 2.1
+  // Measured, with both forced: 22 rows of 9 heads 7.4 against 8.8, 100 rows
+  // over 2000 keys 12.8 / 16.0 + 5.2, 5 x 300 rows in float32 74 / 18.9, 64 rows
+  // of 32 heads of 128 over 4000 keys 46 / 26 + 13.
+  const bool wide = q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES;
+  const int size = tiles <= 4 ? 0 : tiles <= 8 ? 1 : tiles <= 12 ? 2 : 3;
+  const long long all_rows = (b.n_rows < (long long)b.n_seq * b.max_q ? b.n_rows : (long long)b.n_seq * b.max_q) * group * c.heads;
+  const double seen = key_tiles - 0.5 * ((b.max_q < keys ? b.max_q : keys) / KEYS);   // on average
+  const double cus = 256.0;
+  Kv4Plan few = p;
+  {
+    static const double itself[4] = {7.0, 7.5, 11.0, 13.0};
+    few.prompt = false;
+    few.terms = terms_of(q, out, (int)(rows < 64 ? rows : 64));
+    const int R = 16 / few.terms;
+    few.row_tiles = (int)((rows + R - 1) / R);
+    few.waves = rows_waves(tiles);
+    const double each = itself[size] + (few.terms == 4 ? 2.0 : 0.0), per_tile = 2.65 / few.waves;
+    const double groups = (double)((all_rows + R - 1) / R);
+    const double rounds = groups < cus ? 1.0 : groups / cus;
+    // Short contexts: one workgroup takes a row tile's keys, four tiles a wave
+    // at most, and there is nothing to join.  Otherwise as many workgroups as
+    // run at once share all keys equally.
+    const long long most_groups = (long long)few.row_tiles * c.heads * b.n_seq, cap_tiles = (cap + KEYS - 1) / KEYS;
+    few.us = rounds * (each + per_tile * few.waves * ceil(seen / few.waves));
+    if (key_tiles > 4 * few.waves) {
+      few.waves = 4;
+      if (b.n_seq <= 256 && most_groups * (cap_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
+        const long long most = most_groups * (key_tiles + ROWS_EXTRA) / 4 + 1, slots = tiles <= 4 ? 768 : tiles <= 8 ? 512 : 256;
+        few.stream = (int)(most < slots ? most : slots);
+        few.cells = 2 * (size_t)few.stream * R;
+        few.us = each + R * c.hd / 128.0 + per_tile * groups * (seen + ROWS_EXTRA) / cus;   // joined by one workgroup
+      }
+    }
+  }
+  {
+    static const double itself[4] = {8.8, 12.0, 16.0, 20.0}, tile[4] = {1.4, 1.8, 2.1, 2.1};
+    p.prompt = true;
     p.terms = wide ? 3 : (q.type == BFP_BF16 && out.type == BFP_BF16 ? 1 : 2);
     p.waves = prompt_waves(tiles, p.terms);
     p.row_tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
@@ -57,25 +99,10 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
       p.chunk = (int)((key_tiles + s - 1) / s);
       p.cells = (size_t)b.n_rows * q.heads * p.splits;
     }
-  } else {
-    p.terms = terms_of(q, out, (int)rows);
-    const int R = 16 / p.terms;
-    p.row_tiles = (int)((rows + R - 1) / R);
-    p.waves = rows_waves(tiles);
-    const long long groups = (long long)p.row_tiles * c.heads * b.n_seq, cap_tiles = (cap + KEYS - 1) / KEYS;
-    // Short contexts: one workgroup takes a row tile's keys, four tiles a wave
-    // at most, and there is nothing to join.  Otherwise as many workgroups as
-    // run at once share all keys equally.
-    if (key_tiles > 4 * p.waves) {
-      p.waves = 4;
-      if (b.n_seq <= 256 && groups * (cap_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
-        const long long most = groups * (key_tiles + ROWS_EXTRA) / 4 + 1, slots = tiles <= 4 ? 768 : tiles <= 8 ? 512 : 256;
-        p.stream = (int)(most < slots ? most : slots);
-        if (p.stream < 1) p.stream = 1;
-        p.cells = 2 * (size_t)p.stream * R;
-      }
-    }
+    const double work = (double)all_rows / (32 * p.waves) * p.splits, rounds = work < cus ? 1.0 : work / cus;
+    p.us = rounds * (itself[size] + (p.terms == 3 ? 1.8 : 0.0) + tile[size] * (p.splits > 1 ? p.chunk : seen)) + (p.splits > 1 ? 5.0 : 0.0);
   }
+  if (few.us <= p.us) p = few;
   p.work = p.cells * (16 * tiles * sizeof(float) + sizeof(float2)) + 2 * p.stream * sizeof(unsigned long long);
   return p;
 }

@@ -354,13 +354,19 @@ __global__ __launch_bounds__(256) void k_kv4_join_prompt(Kv4AttnArgs a) {
   // a split that saw nothing (or NaN scores alone, whose sum is NaN): factor 0
   const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
   const float L = wave_sum(f * ml.y);
+  // four splits' loads under way together; past the last one: it again, with
+  // the factor 0 (its NaN, if it has one, is the row's anyway)
   float acc[4] = {0, 0, 0, 0};
-#pragma unroll 8
-  for (int k = 0; k < a.splits; ++k) {
-    const float fk = __shfl(f, k, 64);
+  for (int k0 = 0; k0 < a.splits; k0 += 4) {
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
-      if (64 * d + lane < hd) acc[d] += fk * a.part_o[(at + k) * hd + 64 * d + lane];
+    for (int e = 0; e < 4; ++e) {
+      const int k = k0 + e < a.splits ? k0 + e : a.splits - 1;
+      const float fk = k0 + e < a.splits ? __shfl(f, k, 64) : 0.0f;
+      const float *o = a.part_o + (at + k) * hd;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (64 * d < hd) acc[d] += fk * o[64 * d + lane < hd ? 64 * d + lane : hd - 1];
+    }
   }
 #pragma unroll
   for (int d = 0; d < 4; ++d)

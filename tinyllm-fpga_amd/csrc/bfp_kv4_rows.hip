@@ -528,6 +528,43 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
   }
 }
 
+// 64 E values of a part at a time, row after row; a lane has E of them under
+// way for each of its wave's parts.
+template <int E>
+__device__ __forceinline__ void join_values(const Kv4AttnArgs &a, const RowsSeq &sp, int head, int rr0, uint32_t p0, int parts,
+                                            int R, int values, const float *factor, const float *total, float *sums) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, G = a.group, hd = 16 * a.tiles;
+  for (int v0 = 0; v0 < values; v0 += 64 * E) {
+    float acc[E];
+    int at[E], row[E];   // past the last value: the last one, not taken
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      acc[e] = 0.0f;
+      at[e] = v0 + 64 * e + lane < values ? v0 + 64 * e + lane : values - 1;
+      row[e] = at[e] / hd;
+    }
+#pragma unroll 2
+    for (int k = w; k < parts; k += 4) {
+      const float *o = a.part_o + (long long)part_slot(p0, (uint32_t)k) * R * hd;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = get(o + at[e]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += factor[k * R + row[e]] * x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[w * 64 * E + 64 * e + lane] = acc[e];
+    __syncthreads();
+    for (int u = threadIdx.x; u < 64 * E && v0 + u < values; u += 256) {   // whole groups of 16 lanes
+      const int r = (v0 + u) / hd, rr = rr0 + r;
+      const float L = total[r], sum = (sums[u] + sums[64 * E + u]) + (sums[128 * E + u] + sums[192 * E + u]);
+      out_store(a.out, (long long)(sp.row0 + rr / G) * a.out.row_stride + (head * G + rr % G) * a.out.head_stride + (v0 + u) % hd,
+                L == 0.0f ? 0.0f : sum / L);
+    }
+    __syncthreads();
+  }
+}
+
 // A row tile's rows from the parts of their keys.  All of a workgroup of four
 // waves: the parts' factors first, then every wave takes each fourth part, a
 // lane the same values of all of them.
@@ -535,7 +572,7 @@ template <int C, int R>
 __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, int head, int rr0, uint32_t p0, int parts) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, G = a.group, hd = 16 * a.tiles;
   const int left = sp.n * G - rr0, rows = left < R ? left : R;
-  float *factor = (float *)lds, *total = factor + MAX_PARTS * R, *sums = total + R;   // [part][R], [R], [4][256]
+  float *factor = (float *)lds, *total = factor + MAX_PARTS * R, *sums = total + R;   // [part][R], [R], [4][1024]
   auto slot = [&](int k) { return (long long)part_slot(p0, (uint32_t)k) * R; };
   for (int row = w; row < rows; row += 4) {
     float2 ml[MAX_PARTS / 64];
@@ -557,40 +594,18 @@ __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, i
     if (lane == 0) total[row] = L;
   }
   __syncthreads();
-  const int values = rows * hd;   // of a part, row after row: multiples of 16
-  for (int v0 = 0; v0 < values; v0 += 256) {
-    float acc[4] = {0, 0, 0, 0};
-    int at[4], row[4];   // past the last value: the last one, not taken
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      at[e] = v0 + 64 * e + lane < values ? v0 + 64 * e + lane : values - 1;
-      row[e] = at[e] / hd;
-    }
-#pragma unroll 4
-    for (int k = w; k < parts; k += 4) {
-      const float *o = a.part_o + slot(k) * hd;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += factor[k * R + row[e]] * get(o + at[e]);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sums[w * 256 + 64 * e + lane] = acc[e];
-    __syncthreads();
-    const int v = v0 + threadIdx.x;
-    if (v < values) {   // whole groups of 16 lanes
-      const int r = v / hd, rr = rr0 + r;
-      const float L = total[r], acc4 = (sums[threadIdx.x] + sums[256 + threadIdx.x]) + (sums[512 + threadIdx.x] + sums[768 + threadIdx.x]);
-      out_store(a.out, (long long)(sp.row0 + rr / G) * a.out.row_stride + (head * G + rr % G) * a.out.head_stride + v % hd,
-                L == 0.0f ? 0.0f : acc4 / L);
-    }
-    __syncthreads();
-  }
+  const int values = rows * hd;
+  if (C == 1 || values <= 512)   // 16 need more registers than the narrow heads' kernels have
+    join_values<8>(a, sp, head, rr0, p0, parts, R, values, factor, total, sums);
+  else
+    join_values<16>(a, sp, head, rr0, p0, parts, R, values, factor, total, sums);
 }
 
 template <int C, int W>
 static AttnKernel pick(int tiles, int terms) {
   const int R = 16 / terms;
   int lds = W * V_ROWS * v_pitch(C);
-  for (int n : {W * join_floats(R, tiles) * 4, (MAX_PARTS * R + R + 1024) * 4}) lds = n > lds ? n : lds;
+  for (int n : {W * join_floats(R, tiles) * 4, (MAX_PARTS * R + R + 4096) * 4}) lds = n > lds ? n : lds;
   return {terms == 1 ? k_kv4_rows<C, 1, W> : terms == 2 ? k_kv4_rows<C, 2, W> : k_kv4_rows<C, 4, W>, lds};
 }
 
