@@ -35,7 +35,7 @@ def value(codes, exps):
     c = np.asarray(codes)
     v = GRID[c & 7] * np.where(c & 8, -1.0, 1.0)
     s = np.where(exps == E_NAN, np.nan, 2.0 ** (exps.astype(float) - 127))
-    return (v.reshape(*c.shape[:-1], -1, 16) * s[..., None]).reshape(c.shape)
+    return (v.reshape(*c.shape[:-1], c.shape[-1] // 16, 16) * s[..., None]).reshape(c.shape)
 
 
 def quant4(v):
@@ -118,3 +118,25 @@ def attend_bound(out, weight, big, n_keys, hd, out_half, p_half):
     result's out_half of its value."""
     d = big[..., None] * (3 * hd + 4) * 2.0 ** -23 + 2.0 ** -21
     return (2 * d + (2 * n_keys + 16) * 2.0 ** -23 + p_half) * weight + out_half * np.abs(out) + 1e-38
+
+
+def attend_all(q, keys, values, start, lens, group, scale, window=0, there=None):
+    """attend() a head at a time, for many rows or long contexts."""
+    out, weight, big = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:2])
+    for b in range(len(lens)):
+        rows = slice(start[b], start[b + 1])
+        n, m = start[b + 1] - start[b], len(keys[b])
+        p = (max(lens[b], 0) - n + np.arange(n))[:, None]
+        at = np.arange(m)[None]
+        see = (at <= p) & ((at > p - window) if window else True) & (True if there is None else there[b][None, :m])
+        some = see.any(-1)
+        if not some.any():
+            continue
+        for h in range(q.shape[1]):
+            k, v, x = keys[b][:, h // group], values[b][:, h // group], q[rows, h]
+            s = np.where(see, x @ k.T * scale, -np.inf)
+            w = np.exp(s - np.where(some, s.max(-1, initial=-np.inf), 0)[:, None])
+            w /= np.where(some, w.sum(-1), 1)[:, None]
+            out[rows, h], weight[rows, h] = w @ v, w @ np.abs(v)
+            big[rows, h] = np.where(see, np.abs(x) @ np.abs(k).T * abs(scale), 0).max(-1, initial=0)
+    return out, weight, big

@@ -257,3 +257,18 @@ def test_plain_format_is_nearest():
     assert (np.abs(got - v) == best).all()
     top = np.abs(v).max(-1)
     assert (top < 7 * scale[:, 0]).all() and (top >= 3.5 * scale[:, 0]).all()
+
+
+@pytest.mark.parametrize("window", [0, 1, 5])
+def test_plain_attention_both_ways(window):
+    """The tests' two plain implementations agree."""
+    rng = np.random.default_rng(5)
+    lens, news = [9, 0, 3, 20], [4, 0, 5, 20]
+    start = np.concatenate([[0], np.cumsum(news)])
+    keys, vals = ([rng.standard_normal((n, 2, 16)) for n in lens] for _ in range(2))
+    there = [rng.random(n) < 0.7 for n in lens]
+    q = rng.standard_normal((start[-1], 6, 16))
+    for t in (None, there):
+        one, two = (f(q, keys, vals, start, lens, 3, 0.4, window, t) for f in (ref.attend, ref.attend_all))
+        for x, y in zip(one, two):
+            assert np.abs(x - y).max() < 1e-12

@@ -82,11 +82,14 @@ __device__ __forceinline__ float cut_bf16(float x) {
   return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
 }
 
-// Term t of x's split by cuts (three hold any float32).  An infinity or a
-// NaN is its own first term.
-__device__ __forceinline__ float cut_term(float x, int t) {
-  const bool good = fabsf(x) < INFINITY;
-  if (!good) return t == 0 ? (x != x ? NAN : x) : 0.0f;
+// Term t of T of a query's value x: split by cuts (three hold any float32).
+// An infinite query has no score but infinities and NaN, so its row is NaN
+// whatever it sees: as a NaN it says so itself, where infinities of one sign
+// would leave probabilities of nothing but zeros.
+template <int T>
+__device__ __forceinline__ float query_term(float x, int t) {
+  if (!(fabsf(x) < INFINITY)) return t == 0 ? NAN : 0.0f;
+  if (T == 1) return x;
   for (int i = 0; i < t; ++i) x -= cut_bf16(x);
   return cut_bf16(x);
 }

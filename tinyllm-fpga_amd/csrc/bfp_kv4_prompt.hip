@@ -77,7 +77,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
     for (int t = 0; t < T; ++t) {
       float y[8];
 #pragma unroll
-      for (int d = 0; d < 8; ++d) y[d] = (T == 1 ? x[d] : cut_term(x[d], t)) * a.q_sign;
+      for (int d = 0; d < 8; ++d) y[d] = query_term<T>(x[d], t) * a.q_sign;
       qf[t][c] = pack8(y);
     }
   }

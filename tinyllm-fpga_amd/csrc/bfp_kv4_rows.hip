@@ -275,7 +275,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
       if (mine && g * C + c < tiles) {
         row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * (g * C + c), x);
 #pragma unroll
-        for (int d = 0; d < 16; ++d) x[d] = (T == 1 ? x[d] : cut_term(x[d], t)) * a.q_sign;
+        for (int d = 0; d < 16; ++d) x[d] = query_term<T>(x[d], t) * a.q_sign;
       } else {
 #pragma unroll
         for (int d = 0; d < 16; ++d) x[d] = 0.0f;
