@@ -84,6 +84,7 @@ LONG = [  # lens, news, page, heads, hd, group, type, out type, window
     ([2113, 4000], [1, 2], 128, 1, 112, 4, "f32", "f32", 0),
     ([2600, 2600, 2600], [1, 5, 1], 16, 2, 80, 3, "tile", "f16", 2200),
     ([1100, 3000], [1, 1], 16, 1, 192, 12, "bf16", "bf16", 0),
+    ([300, 100], [1, 1], 16, 2, 192, 9, "bf16", "bf16", 0),
     ([1100, 3000], [1, 1], 16, 1, 144, 3, "f16", "f32", 0),
     ([1100, 2000], [1, 1], 16, 3, 160, 2, "bf16", "bf16", 0),
     ([1900, 64], [1, 1], 64, 2, 256, 9, "bf16", "bf16", 0),
@@ -104,6 +105,7 @@ def test_long_contexts(gpu, case):
 PROMPTS = [  # lens, news, page, heads, hd, group, type, out type, window
     ([2000], [1500], 16, 2, 32, 4, "bf16", "bf16", 0),
     ([700, 41], [700, 41], 16, 2, 32, 3, "f16", "f16", 0),
+    ([1500], [1200], 16, 2, 32, 4, "f16", "f16", 0),
     ([600, 0, 333], [600, 0, 200], 32, 2, 16, 4, "f32", "f32", 0),
     ([2000, 900], [1500, 900], 64, 2, 64, 4, "bf16", "bf16", 0),
     ([1000, 3], [700, 3], 16, 3, 48, 2, "tile", "bf16", 0),
@@ -111,6 +113,7 @@ PROMPTS = [  # lens, news, page, heads, hd, group, type, out type, window
     ([900, 901], [900, 600], 16, 2, 64, 3, "f32", "f32", 100),
     ([1500, 800], [1500, 800], 256, 3, 96, 4, "bf16", "bf16", 0),
     ([700], [700], 16, 2, 96, 4, "f16", "f16", 0),
+    ([1500, 40], [1200, 40], 16, 2, 96, 4, "tile", "f16", 0),
     ([700, 64], [500, 64], 128, 2, 80, 3, "f32", "bf16", 0),
     ([2000, 1200], [1500, 1200], 64, 3, 128, 4, "bf16", "bf16", 0),
     ([1000, 1200], [1000, 1000], 64, 1, 128, 8, "f16", "f16", 333),
