@@ -564,7 +564,8 @@ int bfp_rope_table_d(const double *inv_freq, int n_freq, double mscale, long lon
                      float *table, void *stream);
 /* Rotates the first rot values of every head (rot even, 2 <= rot <= hd) and
  * copies the rest: with (c, s) = table[pos[t]][j], y_a = a c - b s, y_b = b c +
- * a s, in float64, where (a, b) are values (j, j + rot/2) of the head
+ * a s, rounded once for a BFP_F32 y (to within 2 float32 steps, then to 16 bits,
+ * for the others), where (a, b) are values (j, j + rot/2) of the head
  * (interleaved 0, as rope_fp pairs them) or (2j, 2j + 1) (interleaved 1).
  * x and y: n_rows rows, the same number of heads; y BFP_F32, BFP_BF16 or
  * BFP_F16; y may be x.  pos: n_rows positions; a row whose position is
@@ -606,9 +607,9 @@ typedef struct bfp_kv4_batch {
 /* Writes the new tokens' k and v (n_rows x heads x hd) into their slots, k
  * rotated as bfp_rope_d does at its position first (table NULL: not
  * rotated).  q and q_out (both or neither): queries rotated by the same
- * table in the same launch, q_out as bfp_rope_d's y.  pos: positions to
- * rotate at, per row (NULL: the position in the cache).  A row without a
- * slot writes nothing, and its q_out is zero; a position outside
+ * table in the same launch, q_out as bfp_rope_d's y, and not k or v.  pos:
+ * positions to rotate at, per row (NULL: the position in the cache).  A row
+ * without a slot writes nothing, and its q_out is zero; a position outside
  * [0, n_pos) gives NaN in the rotated part (whole tiles of k).  No two rows
  * of a call may have the same slot. */
 int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *k,
@@ -625,10 +626,12 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
  * Positions whose page is outside [0, n_pages) are not seen; a row that sees
  * nothing gives zeros.  What a row does not see does not reach it, whatever
  * its bytes.  Products are exact, sums and softmax in float32, probabilities
- * carried to at least the output's precision.  out: any type (BFP_TILES:
- * tile_quantize of the float32 result).  work: bfp_kv4_attn_work() bytes of
- * device scratch, 16-byte aligned (NULL if that is 0); calls that may run at
- * the same time need their own. */
+ * carried to at least the output's precision; scale q.k has to fit float32, and
+ * a query with a NaN or an infinity in it makes its row NaN.  out: any type
+ * (BFP_TILES: tile_quantize of the float32 result); it may be q.  work:
+ * bfp_kv4_attn_work() bytes of device scratch, 16-byte aligned (NULL if that
+ * is 0), whatever they hold; calls that may run at the same time need their
+ * own. */
 int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                    const bfp_rows *out, double scale, int window, void *work, size_t work_bytes,
                    void *stream);

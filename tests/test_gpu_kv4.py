@@ -199,6 +199,21 @@ def test_append_rotated_borders(gpu):
     assert (rk.double().cpu().numpy() == want).all()
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("hq,hd,rot,n", [(3, 64, 64, 5), (4, 96, 34, 40), (32, 128, 64, 1500), (5, 80, 40, 33)])
+def test_append_turns_queries_in_place(gpu, inter, hq, hd, rot, n):
+    import torch
+    s = Setup(4, [n, 3], [n, 5], 16, 1, hd)       # two rows without a slot: zeros
+    table = torch.from_numpy(ref.angles(n, rot).astype(np.float32)).cuda()
+    for kind in ("f32", "bf16"):
+        k = torch.randn(s.rows, 1, hd, device="cuda", dtype=_dt(kind))
+        q = torch.randn(s.rows, hq, hd, device="cuda", dtype=_dt(kind))
+        want = s.cache.append(s.batch, k, k, table, interleaved=inter, q=q)
+        same = q.clone()
+        assert s.cache.append(s.batch, k, k, table, interleaved=inter, q=same, q_out=same) is same
+        assert torch.equal(same, want) and (same[n:n + 2] == 0).all()
+
+
 def test_append_leaves_the_rest(gpu):
     """Rows past the last sequence, pages that do not exist, positions
     outside the table, own positions."""
@@ -629,7 +644,6 @@ def test_refusals(gpu):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: s.cache.attend(s.batch, q, window=-1), lambda: s.cache.attend(s.batch, q, scale=float("inf")),
-                lambda: s.cache.append(s.batch, k, k, q=q, q_out=q),
                 lambda: s.cache.attend(s.batch, torch.zeros(2 * 4 * 64 + 1, device="cuda")[1:].view(2, 4, 64))):
         with pytest.raises(BfpError):
             bad()

@@ -260,6 +260,33 @@ def test_where_results_go(gpu, lens, news, hd, kind):
     assert torch.equal(out[2:n + 2], want) and (out[:2] == 9).all() and (out[n + 2:] == 9).all()
 
 
+def test_as_many_sequences_as_a_batch_has(gpu):
+    """65535 sequences of one token, more heads than workgroups of many waves
+    could take in one launch: each gets its own value back."""
+    import torch
+    from bfp.kv4 import Batch, Fp4Cache
+    n, heads = 65535, 65
+    cache = Fp4Cache(n, 16, heads, 16)
+    v = torch.randn(n, heads, 16, device="cuda", dtype=torch.bfloat16)
+    one = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    batch = Batch(one[:n].view(n, 1).flip(0).contiguous(), one, torch.ones(n, dtype=torch.int32, device="cuda"), max_q=1, max_len=1)
+    cache.append(batch, v, v)
+    _, want = cache.read(batch, n, dtype=torch.bfloat16)
+    assert torch.equal(cache.attend(batch, v), want)
+
+
+def test_rows_cut_off_keep_their_positions(gpu):
+    """Row arrays that end inside a sequence, whatever kernel takes them."""
+    for lens, news in (([700, 500], [3, 4]), ([900, 800], [300, 700]), ([9000, 6000], [1, 3])):
+        s = Long(113, lens, news, 64, 1, 64)
+        q, _ = s.query(4, "f32")
+        want = s.cache.attend(s.batch, q)
+        n = s.rows - 2
+        got = s.cache.attend(s.batch, q[:n].contiguous())
+        # perhaps summed in another order; a position off by one changes a row by some 1e-3
+        assert (got - want[:n]).abs().max() < 2e-5
+
+
 def test_sequences_that_share_pages(gpu):
     """A common beginning cached once."""
     import torch

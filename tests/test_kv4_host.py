@@ -83,6 +83,16 @@ def test_page_zero_of_an_ordinary_span(tmp_path):
     assert out == "5 3 17 / 3 -2 / 2 17"
 
 
+def test_rows_that_are_cut_off_still_count(tmp_path):
+    """Row arrays that end inside a sequence: its rows keep their positions."""
+    out = run_host(tmp_path, """
+  Kv4Span s = kv4_span(5, 8, 20, 7, 4);
+  Kv4Span e = kv4_span(5, 8, 20, 5, 4);
+  Kv4Span n = kv4_span(-2, 3, 20, 9, 4);
+  printf("%d %d %d / %d / %d %d %d", s.row0, s.n, s.at, e.n, n.row0, n.n, n.at);""")
+    assert out == "5 2 17 / 0 / 0 3 17"
+
+
 # ------------------------------------------------------------------ refusals
 def _lib():
     from bfp import _lib
@@ -155,7 +165,7 @@ def test_refuses_bad_calls():
     app = lambda q, o, t, n, rot: _refused(L, "bfp_kv4_append_d", C.byref(c), C.byref(b), R, R, q, o, None, t, n, rot, 0, None)  # noqa: E731
     app(R, None, None, 0, 0)                    # q without q_out
     app(None, R, None, 0, 0)
-    app(R, R, None, 0, 0)                       # in place
+    app(R, R, None, 0, 0)                       # over k
     app(None, None, 4096, 16, 3)                # odd rot
     app(None, None, 4096, 16, 66)               # wider than the head
     app(None, None, 4096, 16, 0)
@@ -272,3 +282,25 @@ def test_plain_attention_both_ways(window):
         one, two = (f(q, keys, vals, start, lens, 3, 0.4, window, t) for f in (ref.attend, ref.attend_all))
         for x, y in zip(one, two):
             assert np.abs(x - y).max() < 1e-12
+
+
+def test_what_a_struct_points_to_cannot_be_replaced():
+    from bfp._rows import Fixed
+
+    class Thing(Fixed):
+        def __init__(self):
+            self.k, self._n = 1, 2
+    t = Thing()
+    t._n = 3
+    with pytest.raises(AttributeError):
+        t.k = 2
+    assert (t.k, t._n) == (1, 3)
+
+
+def test_more_threads_than_a_launch_has_are_refused():
+    """65535 prompts of a million rows each."""
+    L = _lib()
+    c = C.byref(_cache(L, heads=64))
+    b = C.byref(_batch(L, n_seq=65535, n_rows=2 ** 31 - 1, width=70000, max_q=1 << 20))
+    r = C.byref(_rows(L, heads=64, rs=4096))
+    assert "too many" in _refused(L, "bfp_kv4_attn_d", c, b, r, r, 1.0, 0, 4096, 1 << 62, None)

@@ -103,6 +103,19 @@ def gpu_of(t, what):
     return t.device
 
 
+MAX_ROWS = 0x7fffffff   # the entry points count rows in int
+
+
+class Fixed:
+    """An object whose C struct is made once: its tensors are written into,
+    never replaced."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__ and name[0] != "_":
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: write into it, or make a new object")
+        object.__setattr__(self, name, value)
+
+
 class Entry:
     """A stream-ordered entry point: called with the device its tensors are
     on, and its arguments without the stream.  The C entry points launch on

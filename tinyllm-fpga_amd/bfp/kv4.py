@@ -26,13 +26,13 @@ TILE = 16
 _append, _read, _attend = (_rows.Entry(f"bfp_kv4_{name}_d") for name in ("append", "read", "attn"))
 
 
-class Batch:
+class Batch(_rows.Fixed):
     """Which rows belong to which sequence, and where they are cached: row
     start[b] + i of the row arrays is a new token of sequence b, the last of
     them at position lens[b] - 1; position p lies in page pages[b, p // page].
     pages (sequences, width), start (sequences + 1) and lens are int32 tensors
     on the device; they are read when a call runs, so a program may write new
-    values into them.  max_q: the most new rows a sequence has; max_len: the
+    values into them (but not put other tensors in their place).  max_q: the most new rows a sequence has; max_len: the
     longest sequence (0: the table's width), which only chooses how the work
     is split."""
 
@@ -56,13 +56,15 @@ class Batch:
         it points to)."""
         n, c = self._made
         if n != n_rows:
+            if not 0 <= n_rows <= _rows.MAX_ROWS:
+                raise ValueError(f"{n_rows} rows")
             c = Kv4BatchC(self.pages.data_ptr(), self.start.data_ptr(), self.lens.data_ptr(), self.pages.shape[0],
                           n_rows, self.pages.shape[1], self.max_q, self.max_len)
             self._made = (n_rows, c)
         return C.byref(c)
 
 
-class Fp4Cache:
+class Fp4Cache(_rows.Fixed):
     """n_pages pages of `page` tokens of `heads` KV heads, hd wide, at 4.5
     bits a value.  Which sequence has which page is the program's to say
     (Batch.pages)."""
@@ -118,7 +120,7 @@ class Fp4Cache:
         or a new tensor of q's type (float32 for tiles) whose rows outside
         every sequence are undefined.  A row whose position is negative, or
         whose page is not one of the cache's, writes nothing, and its
-        rotated query is zero."""
+        rotated query is zero.  q_out may be q."""
         dev = self.device
         kt, vt = self._values(batch, k, "k"), self._values(batch, v, "v")
         n = kt.shape[0]

@@ -90,6 +90,8 @@ def rope(x, pos, table, interleaved=False, out=None, dtype=None):
         raise ValueError(f"out must be a tensor {tuple(t.shape)}" + (f" of {dtype}" if dtype else ""))
     else:
         yr = _rows.rows(out, "out", device)
+    if n > _rows.MAX_ROWS:
+        raise ValueError(f"{n} rows")
     n_pos, rot = check_table(table, device)
     p = _rows.ints(pos, "pos", device, n)
     if n:

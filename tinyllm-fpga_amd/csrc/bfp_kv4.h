@@ -33,10 +33,10 @@ struct Kv4Span {
 __host__ __device__ inline Kv4Span kv4_span(int start, int stop, int len, int n_rows, int max_q) {
   Kv4Span s;
   const int r0 = start < 0 ? 0 : (start > n_rows ? n_rows : start);
-  const int r1 = stop < r0 ? r0 : (stop > n_rows ? n_rows : stop);
+  const int all = stop < r0 ? 0 : stop - r0, n = all < n_rows - r0 ? all : n_rows - r0;
   s.row0 = r0;
-  s.n = r1 - r0 < max_q ? r1 - r0 : max_q;
-  s.at = (len < 0 ? 0 : len) - (r1 - r0);
+  s.n = n < max_q ? n : max_q;
+  s.at = (len < 0 ? 0 : len) - all;   // also of rows that are not there
   return s;
 }
 

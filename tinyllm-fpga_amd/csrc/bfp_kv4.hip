@@ -271,8 +271,8 @@ int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp
     BFP_TRY(check_out(op, "q_out", q_out, q->heads, hd, false, rows));
     if (!rows_aligned(*q, 8) || !rows_aligned(*q_out, 8))
       return set_err(BFP_EINVAL, "%s: q and q_out need 16-byte alignment and strides in multiples of 8", op);
-    // a lane turns one tile and reads its partner, which another lane may have written
-    if (q_out->p == q->p) return set_err(BFP_EINVAL, "%s: q_out cannot be q", op);
+    // q_out may be q: who writes a value has read its pair (rope_wide_unit)
+    if (q_out->p == k->p || q_out->p == v->p) return set_err(BFP_EINVAL, "%s: q_out cannot be k or v", op);
   }
   if (table) {
     if (rot < 2 || rot % 2 || rot > hd) return set_err(BFP_EINVAL, "%s: rot=%d, hd=%d", op, rot, hd);

@@ -74,7 +74,8 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
     // run at once share all keys equally.
     const long long most_groups = (long long)few.row_tiles * c.heads * b.n_seq, cap_tiles = (cap + KEYS - 1) / KEYS;
     few.us = rounds * (each + per_tile * few.waves * ceil(seen / few.waves));
-    if (key_tiles > 4 * few.waves) {
+    // (Four waves also where wider workgroups would be more than 2^32 threads.)
+    if (key_tiles > 4 * few.waves || most_groups * few.waves > 0x3ffffff) {
       few.waves = 4;
       if (b.n_seq <= 256 && most_groups * (cap_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
         const long long most = most_groups * (key_tiles + ROWS_EXTRA) / 4 + 1, slots = tiles <= 4 ? 768 : tiles <= 8 ? 512 : 256;
@@ -182,8 +183,8 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   a.by_group = FastDiv((uint32_t)a.group);
   a.out_wide = rows_aligned(*out, 8);
   const long long each = (long long)p.row_tiles * p.splits * cache->heads, blocks = p.stream ? p.stream : each * batch->n_seq;
-  if (each > 0x7fffffLL || blocks > 0x7fffffLL)
-    return set_err(BFP_EINVAL, "%s: max_q=%d is too large for one call", op, batch->max_q);
+  if (blocks > 0x3ffffff / p.waves || each > 0x7fffffff)   // 2^32 threads
+    return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, batch->n_seq, batch->max_q);
   a.by_seq = FastDiv((uint32_t)each);
   const AttnKernel k = p.prompt ? prompt_kernel(a.tiles, p.terms) : rows_kernel(a.tiles, p.terms, p.waves);
   if (k.lds > 65536)   // one limit for a kernel, whatever the call

@@ -134,7 +134,8 @@ __device__ __forceinline__ uint32_t stream_plan(const Kv4AttnArgs &a, int R, Str
 // store and load by load (device-scope accesses): a store is done when the
 // wait for it is over, so a workgroup's arrival after that wait and a barrier
 // says that its sums are there.  A device-scope fence instead would write back
-// and drop all of an L2 each time: 55 us for a call that takes 13 this way.
+// and drop all of an L2 each time: one sequence of 8192 tokens took 55 us with
+// fences, 16 this way.
 __device__ __forceinline__ void put(float *p, float v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
