@@ -94,22 +94,31 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   uint2 rk[UNITS], rv[UNITS];
   uint32_t rke[UNITS], rve[UNITS];
   bool there = false;
+  // The page number of this lane's key, where some row sees the key; looked at
+  // only when the page is fetched, a tile later: a use here would wait for it
+  // and for the bytes asked for before it (two prompts of 8192 tokens, 32 heads
+  // of 128: 870 us that way, 807 this way).
   auto page_of = [&](int tile) {
+    if (tile >= stop) return -1;
     const int key = tile * KEYS + lane;
-    return tile < stop && key >= begin && key < end ? kv4_page(pages, a.b.width, a.c.n_pages, key >> a.page_shift) : -1;
+    int id = -1;
+    if ((tile * KEYS >= begin && tile * KEYS <= end - KEYS) || (key >= begin && key < end)) id = pages[key >> a.page_shift];
+    return id;
   };
   // a key without a page reads the first one's bytes; they are not used
+  const uint32_t page_tiles = (uint32_t)a.c.heads * tiles * a.c.page;   // at most 2^24
   auto fetch = [&](int tile, int id) {
-    there = id >= 0;
-    const long long at = kv4_tile(there ? id : 0, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + lane) & (a.c.page - 1));
+    there = (unsigned)id < (unsigned)a.c.n_pages;
+    const uint32_t slot = (uint32_t)(tile * KEYS + lane) & (a.c.page - 1);
+    const unsigned long long at = (unsigned long long)(there ? (uint32_t)id : 0u) * page_tiles + slot;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int t = w + u * W;
-      const long long o8 = at + (long long)(t < tiles ? t : tiles - 1) * a.c.page;
-      rk[u] = *(const uint2 *)(a.c.k + o8 * KV4_TILE_BYTES);
-      rv[u] = *(const uint2 *)(a.c.v + o8 * KV4_TILE_BYTES);
-      rke[u] = a.c.k_e[o8];
-      rve[u] = a.c.v_e[o8];
+      const long long from = kv4_tile(0, a.c.heads, head, tiles, t < tiles ? t : tiles - 1, a.c.page, 0);   // the same in every lane
+      rk[u] = ((const uint2 *)(a.c.k + from * KV4_TILE_BYTES))[at];
+      rv[u] = ((const uint2 *)(a.c.v + from * KV4_TILE_BYTES))[at];
+      rke[u] = (a.c.k_e + from)[at];
+      rve[u] = (a.c.v_e + from)[at];
     }
   };
   char *const k_lds = lds, *const v_lds = lds + 2 * k_bytes(TB);
