@@ -7,7 +7,8 @@ Import the package with ``tinyllm-fpga_amd`` on ``sys.path``::
     m, e = bfp.tile_quantize(v)
 
 Modules: ``api`` (the reference simulator's functions on the GPU),
-``model`` (HBM-resident model, layer step and decode driver), ``synth``
+``model`` (HBM-resident model, layer step and decode driver), ``rotary`` and ``kv4``
+(rotary positions, the paged 4-bit key/value cache and its attention), ``synth``
 (seeded synthetic inputs), ``dims`` (model dimensions), ``_lib`` (ctypes
 binding of libbfp.so).
 """
