@@ -50,7 +50,8 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   //   heads up to 64          7.0 (float32 8.9), 2.7                 8.8 (10.6), 1.4
   //   up to 128               7.5 (9.5), 2.6                         12, 1.8
   //   up to 192, 256          11, 13; 2.6                            16, 20; 2.1
-  // Measured, with both forced: 22 rows of 9 heads 7.4 against 8.8, 100 rows
+  // Measured when the rule was made (prompts have become 2 to 7% faster since),
+  // with both forced: 22 rows of 9 heads 7.4 against 8.8, 100 rows
   // over 2000 keys 12.8 / 16.0 + 5.2, 5 x 300 rows in float32 74 / 18.9, 64 rows
   // of 32 heads of 128 over 4000 keys 46 / 26 + 13.
   const bool wide = q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES;
