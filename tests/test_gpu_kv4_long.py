@@ -377,3 +377,33 @@ def test_captured_and_replayed(gpu, news, kind):
             torch.cuda.synchronize()
             rows = sum(news)
             assert torch.equal(out[:rows], w[:rows]) and torch.equal(again[:rows], w[:rows])
+
+
+def test_rows_far_apart(gpu):
+    """Row strides whose offsets pass 2^31 values and 2^32 bytes: queries,
+    new keys and values, and results."""
+    import torch
+    from bfp import rotary
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of GPU memory")
+    n, far = 40, 1 << 26
+    s = Long(127, [700], [n], 64, 2, 64)
+    q, _ = s.query(6, "bf16")
+    wide_q = torch.empty(n * far, dtype=torch.bfloat16, device="cuda").as_strided((n, 6, 64), (far, 64, 1))
+    wide_o = torch.empty(n * far, dtype=torch.bfloat16, device="cuda").as_strided((n, 6, 64), (far, 64, 1))
+    wide_q.copy_(q)
+    s.cache.attend(s.batch, wide_q, out=wide_o)
+    assert torch.equal(wide_o, s.cache.attend(s.batch, q))
+    table = rotary.rope_table(rotary.rope_freqs(64)[0], 700)
+    pos = torch.arange(660, 700, dtype=torch.int32, device="cuda")
+    rotary.rope(wide_q, pos, table, out=wide_o)
+    assert torch.equal(wide_o, rotary.rope(q, pos, table))
+    k = wide_q[:, :2]
+    turned = s.cache.append(s.batch, k, wide_q[:, 2:4], table, q=wide_q, q_out=wide_o)
+    far_k, far_v = s.cache.read(s.batch, n)
+    assert turned is wide_o and torch.equal(turned, rotary.rope(q, pos, table))
+    s.cache.append(s.batch, q[:, :2], q[:, 2:4], table)
+    near_k, near_v = s.cache.read(s.batch, n)
+    assert torch.equal(far_k, near_k) and torch.equal(far_v, near_v)
+    s.cache.read(s.batch, k=wide_o[:, :2], v=wide_o[:, 2:4])
+    assert torch.equal(wide_o[:, :2].float(), near_k) and torch.equal(wide_o[:, 2:4].float(), near_v)
