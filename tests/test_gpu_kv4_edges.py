@@ -1,0 +1,69 @@
+"""The ends of what the rotary and 4-bit-cache operators allow: scales,
+magnitudes and exponents at the limits, results that cannot be held, strides
+that nothing uses, and the kernels that only large calls reach, against
+plain 64-bit numpy."""
+import numpy as np
+import pytest
+
+import kv4_ref as ref
+from test_gpu_kv4 import HALF, _dt, _int, _say
+from test_gpu_kv4_long import Long
+
+pytestmark = pytest.mark.gpu
+
+
+class Few:
+    """One sequence whose keys differ in value 0 of the head only and whose
+    values are alike in every place: k0 and v (tokens) are elements of the
+    format times 2^(exponent byte - 127)."""
+
+    def __init__(self, k0, v, k_exp=127, v_exp=127, news=1, page=16, hd=16):
+        import torch
+        from bfp.kv4 import Batch, Fp4Cache
+        self.heads, self.hd, self.n, self.rows = 1, hd, len(k0), news
+        code = {x * s: i + (8 if s < 0 else 0) for i, x in enumerate(ref.GRID.tolist()) for s in (1, -1) if x or s > 0}
+        n_pages = -(-self.n // page)
+        raw = {name: np.zeros((n_pages, 1, hd // 16, page, 8), np.uint8) for name in "kv"}
+        for t in range(self.n):
+            raw["k"][t // page, 0, 0, t % page, 0] = code[float(k0[t])]
+            raw["v"][t // page, 0, :, t % page] = code[float(v[t])] * 17
+        exps = {name: np.full((n_pages, 1, hd // 16, page), e, np.uint8) for name, e in (("k", k_exp), ("v", v_exp))}
+        self.cache = Fp4Cache.from_buffers(*(torch.from_numpy(x).cuda() for x in (raw["k"], exps["k"], raw["v"], exps["v"])))
+        self.batch = Batch(_int(np.arange(n_pages)[None]), _int([0, news]), _int([self.n]), max_q=news, max_len=self.n)
+        self.k0 = np.asarray(k0, float) * 2.0 ** (k_exp - 127)
+        self.v = np.asarray(v, float) * 2.0 ** (v_exp - 127)
+
+    def query(self, q0, kind):
+        """Queries (rows, query heads) of value 0, zeros elsewhere."""
+        import torch
+        q = torch.zeros(self.rows, q0.shape[1], self.hd, dtype=_dt(kind))
+        q[:, :, 0] = torch.from_numpy(q0).to(_dt(kind))
+        return q.cuda(), q[:, :, 0].double().numpy()
+
+    def want(self, q0, scale):
+        """(result, weighted magnitudes, largest score) of each row and query head."""
+        out = np.zeros(q0.shape + (3,))
+        for i in range(self.rows):
+            seen = self.n - self.rows + i + 1
+            s = q0[i][:, None] * self.k0[:seen] * scale
+            w = np.exp(s - s.max(-1, keepdims=True))
+            out[i, :, 0], out[i, :, 1] = (w @ self.v[:seen] / w.sum(-1), w @ np.abs(self.v[:seen]) / w.sum(-1))
+            out[i, :, 2] = np.abs(s).max(-1)
+        return out[..., 0], out[..., 1], out[..., 2]
+
+
+def test_lengths_counted_in_place(gpu):
+    """batch.lens += 1, as a decode loop has it."""
+    import torch
+    from bfp.kv4 import Batch
+    s = Long(157, [60, 9], [1, 1], 16, 1, 64)
+    lens = torch.tensor([40, 8], dtype=torch.int32, device="cuda")
+    b = Batch(s.batch.pages, s.batch.start, lens, max_q=1, max_len=60)
+    q = torch.randn(2, 3, 64, device="cuda")
+    for n in range(4):
+        b.lens += 1
+        assert b.lens is lens and lens.tolist() == [41 + n, 9 + n]
+    want = Batch(s.batch.pages, s.batch.start, _int([44, 12]), max_q=1, max_len=60)
+    got, want = s.cache.attend(b, q), s.cache.attend(want, q)
+    # the second sequence now counts slots that no token has written: noise, which may be NaN
+    assert torch.equal(got[0], want[0]) and torch.allclose(got, want, rtol=0, atol=0, equal_nan=True)

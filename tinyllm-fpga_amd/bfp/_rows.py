@@ -108,10 +108,11 @@ MAX_ROWS = 0x7fffffff   # the entry points count rows in int
 
 class Fixed:
     """An object whose C struct is made once: its tensors are written into,
-    never replaced."""
+    never replaced (an in-place form, x.lens += 1, assigns the tensor it has
+    written into: no other object)."""
 
     def __setattr__(self, name, value):
-        if name in self.__dict__ and name[0] != "_":
+        if name in self.__dict__ and name[0] != "_" and self.__dict__[name] is not value:
             raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: write into it, or make a new object")
         object.__setattr__(self, name, value)
 
