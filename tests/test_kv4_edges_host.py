@@ -25,3 +25,34 @@ def test_in_place_forms_put_back_the_same_object():
     with pytest.raises(AttributeError):
         t.lens = t.lens + 1
     assert t.lens is lens and lens.tolist() == [8, 10]
+
+
+OVERLAP = [  # heads, hd, rows, row stride, head stride, whether two rows share a value
+    (2, 64, 4, 128, 64, False), (2, 64, 4, 64, 64, True), (2, 64, 4, 127, 64, True), (2, 64, 4, 64, 256, False),   # heads before rows
+    (2, 64, 4, 64, 255, True), (3, 64, 2, 320, 128, False), (3, 64, 2, 192, 128, False), (3, 64, 2, 128, 192, False),
+    (3, 64, 3, 128, 192, False), (3, 64, 3, 127, 192, True), (2, 64, 1, 0, 64, False), (1, 64, 5, 64, 0, False), (1, 64, 5, 63, 0, True), (1, 64, 1, 0, 0, False),
+    (9, 16, 1000, 144, 16, False), (9, 16, 1000, 143, 16, True), (9, 16, 1000, 16, 16000, False), (9, 16, 1000, 16, 15999, True)]
+
+
+@pytest.mark.parametrize("case", OVERLAP, ids=str)
+def test_results_that_lie_on_each_other(case):
+    """Against a set of all values' places.  What passes this check is
+    refused by a later one: nothing is launched."""
+    heads, hd, n, rs, hs, shared = case
+    seen = (np.arange(n)[:, None, None] * rs + np.arange(heads)[:, None] * hs + np.arange(hd)).reshape(-1)
+    assert (len(np.unique(seen)) < len(seen)) == shared
+    L = _lib()
+    y = L.RowsC(1 << 30, None, 0, heads, rs, hs)
+    x = L.RowsC(1 << 20, None, 0, heads, heads * hd, hd)
+    msg = _refused(L, "bfp_rope_d", C.byref(x), n, hd, 4096, 4096, 16, hd + 2, 0, C.byref(y), None)
+    assert ("overlap" in msg) == shared and ("rot" in msg) != shared, msg
+    c, b = _cache(L, heads=heads, hd=hd), _batch(L, n_rows=n)
+    msg = _refused(L, "bfp_kv4_attn_d", C.byref(c), C.byref(b), C.byref(x), C.byref(y), 1.0, -1, None, 0, None)
+    assert ("overlap" in msg) == shared and ("window" in msg) != shared, msg
+
+
+def test_strides_whose_product_leaves_64_bits():
+    L = _lib()
+    for rs, hs in ((1 << 62, 64), (64, 1 << 62), (1 << 60, 1 << 60)):
+        x = L.RowsC(1 << 20, None, 0, 9, rs, hs)
+        assert "too large" in _refused(L, "bfp_rope_d", C.byref(x), 4, 64, 4096, 4096, 16, 66, 0, C.byref(x), None)

@@ -52,17 +52,39 @@ inline int check_rows(const char *op, const char *what, const bfp_rows *r, int h
   if ((uintptr_t)r->p % size) return set_err(BFP_EINVAL, "%s: %s is not aligned to its type", op, what);
   // offsets are 64-bit; the last one still has to fit
   const long long last = n_rows > 0 ? n_rows - 1 : 0;
-  if (r->row_stride > 0 && last > (1LL << 60) / r->row_stride)
+  if ((r->row_stride > 0 && last > (1LL << 60) / r->row_stride) ||
+      (r->head_stride > 0 && heads - 1 > (1LL << 60) / r->head_stride))
     return set_err(BFP_EINVAL, "%s: %s is too large", op, what);
   return BFP_OK;
+}
+
+// Whether two of n_rows x heads groups of hd values share a value: groups
+// (t, h) and (t', h') do where |(t - t') row_stride + (h - h') head_stride| < hd.
+// One dimension inside the other never does; strides between are looked at
+// difference by difference, of the dimension that has fewer.
+inline bool rows_share(long long row_stride, long long head_stride, long long n_rows, long long heads, long long hd) {
+  long long s = row_stride, n = n_rows, t = head_stride, m = heads;
+  if (n <= 1 || m <= 1) return n > 1 ? s < hd : m > 1 && t < hd;
+  if (s < hd || t < hd) return true;
+  if (s >= (m - 1) * t + hd || t >= (n - 1) * s + hd) return false;
+  if (m > n) {
+    const long long a = s, b = n;
+    s = t, n = m, t = a, m = b;
+  }
+  for (long long j = 1; j < m; ++j) {   // j steps of t against the two nearest numbers of steps of s
+    const long long i = j * t / s, rest = j * t - i * s;
+    if ((i < n && rest < hd) || (i + 1 < n && s - rest < hd)) return true;
+  }
+  return false;
 }
 
 // The same for rows that are written: no two of them may share a value.
 inline int check_out(const char *op, const char *what, const bfp_rows *r, int heads, int hd,
                      bool tiles, long long n_rows) {
   BFP_TRY(check_rows(op, what, r, heads, hd, tiles, n_rows));
-  if (r->row_stride < hd && n_rows > 1)
-    return set_err(BFP_EINVAL, "%s: rows of %s overlap (stride %lld, hd %d)", op, what, r->row_stride, hd);
+  if (rows_share(r->row_stride, r->head_stride, n_rows, heads, hd))
+    return set_err(BFP_EINVAL, "%s: rows of %s overlap (strides %lld and %lld, %d heads of %d)", op, what, r->row_stride,
+                   r->head_stride, heads, hd);
   return BFP_OK;
 }
 
