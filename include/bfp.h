@@ -534,7 +534,8 @@ enum bfp_type {
 /* rows x heads x hd values on the device, the hd values of a head side by
  * side: value (t, h, d) is p[t*row_stride + h*head_stride + d] (strides in
  * values).  BFP_TILES: p holds mantissas and e one exponent for 16 of them,
- * that of value offset o at e[o/16]; strides are then multiples of 16.  Rows
+ * that of value offset o at e[o/16]; strides are then multiples of 16.  What
+ * the stride of a single row or head is does not matter.  Rows
  * that are written may lie in any order (heads before rows, too) but share no
  * value. */
 typedef struct bfp_rows {

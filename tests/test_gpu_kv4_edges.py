@@ -67,3 +67,27 @@ def test_lengths_counted_in_place(gpu):
     got, want = s.cache.attend(b, q), s.cache.attend(want, q)
     # the second sequence now counts slots that no token has written: noise, which may be NaN
     assert torch.equal(got[0], want[0]) and torch.allclose(got, want, rtol=0, atol=0, equal_nan=True)
+
+
+def test_one_row_of_any_stride(gpu):
+    """The stride between rows where there is one, and between heads where
+    there is one, is nobody's."""
+    import torch
+    from bfp.kv4 import Batch
+    s = Long(139, [60], [1], 16, 1, 64)
+    b = Batch(s.batch.pages, s.batch.start, s.batch.lens, max_q=1, max_len=60)
+    for kind in (torch.float32, torch.bfloat16):
+        k = torch.randn(1, 1, 64, device="cuda", dtype=kind)
+        q = torch.randn(1, 3, 64, device="cuda", dtype=kind)
+        odd_k, odd_q = (torch.zeros(4096, device="cuda", dtype=kind).as_strided(x.shape, st) for x, st in ((k, (67, 3, 1)), (q, (193, 64, 1))))
+        odd_k.copy_(k)
+        odd_q.copy_(q)
+        s.cache.append(b, k, k)
+        want, wk = s.cache.attend(b, q), s.cache.read(b, 1)[0]
+        out = torch.zeros(4096, device="cuda", dtype=kind).as_strided((1, 3, 64), (193, 64, 1))
+        turned = torch.zeros_like(out)
+        assert s.cache.append(b, odd_k, odd_k, q=odd_q, q_out=turned) is turned and torch.equal(turned, q)
+        back = torch.zeros(4096, device="cuda").as_strided((1, 1, 64), (5, 7, 1))
+        s.cache.read(b, k=back)
+        assert torch.equal(back, wk)
+        assert torch.equal(s.cache.attend(b, odd_q, out=out), want) and torch.equal(out, want)

@@ -56,3 +56,19 @@ def test_strides_whose_product_leaves_64_bits():
     for rs, hs in ((1 << 62, 64), (64, 1 << 62), (1 << 60, 1 << 60)):
         x = L.RowsC(1 << 20, None, 0, 9, rs, hs)
         assert "too large" in _refused(L, "bfp_rope_d", C.byref(x), 4, 64, 4096, 4096, 16, 66, 0, C.byref(x), None)
+
+
+def test_strides_that_nothing_uses():
+    """One row, or one head: what its stride is does not matter.  The calls
+    are refused for what follows."""
+    L = _lib()
+    c, b = C.byref(_cache(L, heads=1)), C.byref(_batch(L, n_rows=1))
+    for kind, e in ((0, None), (1, None), (3, 4096)):
+        r = L.RowsC(4096, e, kind, 1, 131, 3)
+        free = L.RowsC(1 << 30, None, 1, 1, 131, 3)
+        assert "window" in _refused(L, "bfp_kv4_attn_d", c, b, C.byref(r), C.byref(free), 1.0, -1, None, 0, None)
+        assert "rot" in _refused(L, "bfp_kv4_append_d", c, b, C.byref(r), C.byref(r), None, None, None, 4096, 16, 66, 0, None)
+        assert "rot" in _refused(L, "bfp_rope_d", C.byref(r), 1, 64, 4096, 4096, 16, 66, 0, C.byref(free), None)
+    two = C.byref(_batch(L, n_rows=2))
+    r = L.RowsC(4096, None, 1, 1, 131, 3)
+    assert "strides" in _refused(L, "bfp_kv4_attn_d", c, two, C.byref(r), C.byref(L.RowsC(1 << 30, None, 1, 1, 64, 64)), 1.0, 0, None, 0, None)

@@ -262,14 +262,14 @@ int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp
   const int hd = cache->hd, rows = batch->n_rows;
   BFP_TRY(check_rows(op, "k", k, cache->heads, hd, true, rows));
   BFP_TRY(check_rows(op, "v", v, cache->heads, hd, true, rows));
-  if (!rows_aligned(*k, 8) || !rows_aligned(*v, 8))
+  if (!rows_aligned(*k, 8, rows) || !rows_aligned(*v, 8, rows))
     return set_err(BFP_EINVAL, "%s: k and v need 16-byte alignment and strides in multiples of 8", op);
   if (!q != !q_out) return set_err(BFP_EINVAL, "%s: q and q_out go together", op);
   if (q) {
     if (q->heads < 1 || q->heads > 65536) return set_err(BFP_EINVAL, "%s: q has %d heads", op, q->heads);
     BFP_TRY(check_rows(op, "q", q, q->heads, hd, true, rows));
     BFP_TRY(check_out(op, "q_out", q_out, q->heads, hd, false, rows));
-    if (!rows_aligned(*q, 8) || !rows_aligned(*q_out, 8))
+    if (!rows_aligned(*q, 8, rows) || !rows_aligned(*q_out, 8, rows))
       return set_err(BFP_EINVAL, "%s: q and q_out need 16-byte alignment and strides in multiples of 8", op);
     // q_out may be q: who writes a value has read its pair (rope_wide_unit)
     if (q_out->p == k->p || q_out->p == v->p) return set_err(BFP_EINVAL, "%s: q_out cannot be k or v", op);
@@ -295,7 +295,7 @@ int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp
   int n = 1;
   if (q) {
     a.q = *q, a.q_out = *q_out;
-    a.shape = rope_shape(*q, *q_out, hd, 2 * a.half, interleaved);
+    a.shape = rope_shape(*q, *q_out, rows, hd, 2 * a.half, interleaved);
     // two heads a thread once that still leaves eight waves a CU
     const long long all = (long long)rows * q->heads * a.shape.per_head;
     n = !a.shape.wide ? 0 : q->heads >= ROPE_HEADS && all >= (long long)ROPE_HEADS * 256 * 8 * 64 ? ROPE_HEADS : 1;
@@ -321,7 +321,7 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   for (const bfp_rows *r : {k, v}) {
     if (!r) continue;
     BFP_TRY(check_out(op, r == k ? "k" : "v", r, cache->heads, cache->hd, false, batch->n_rows));
-    if (!rows_aligned(*r, 8))
+    if (!rows_aligned(*r, 8, batch->n_rows))
       return set_err(BFP_EINVAL, "%s: k and v need 16-byte alignment and strides in multiples of 8", op);
   }
   if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;

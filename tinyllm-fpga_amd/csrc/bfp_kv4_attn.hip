@@ -127,7 +127,7 @@ static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch 
     return set_err(BFP_EINVAL, "%s: q has %d heads, the cache %d", op, q ? q->heads : 0, cache->heads);
   BFP_TRY(check_rows(op, "q", q, q->heads, cache->hd, true, batch->n_rows));
   BFP_TRY(check_out(op, "out", out, q->heads, cache->hd, true, batch->n_rows));
-  if (!rows_aligned(*q, 8)) return set_err(BFP_EINVAL, "%s: q needs 16-byte alignment and strides in multiples of 8", op);
+  if (!rows_aligned(*q, 8, batch->n_rows)) return set_err(BFP_EINVAL, "%s: q needs 16-byte alignment and strides in multiples of 8", op);
   if (window < 0) return set_err(BFP_EINVAL, "%s: window=%d", op, window);
   if ((long long)batch->max_q * (q->heads / cache->heads) > 0x3fffffffLL)
     return set_err(BFP_EINVAL, "%s: max_q=%d rows of %d heads are too many", op, batch->max_q, q->heads);
@@ -182,7 +182,7 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   a.by_head = FastDiv(cache->heads);
   a.by_split = FastDiv(p.splits);
   a.by_group = FastDiv((uint32_t)a.group);
-  a.out_wide = rows_aligned(*out, 8);
+  a.out_wide = rows_aligned(*out, 8, batch->n_rows);
   const long long each = (long long)p.row_tiles * p.splits * cache->heads, blocks = p.stream ? p.stream : each * batch->n_seq;
   if (blocks > 0x3ffffff / p.waves || each > 0x7fffffff)   // 2^32 threads
     return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, batch->n_seq, batch->max_q);

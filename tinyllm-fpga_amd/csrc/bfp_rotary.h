@@ -13,11 +13,11 @@ namespace bfp {
 struct RopeShape {
   int half, interleaved, wide, turned, per_head;   // units that are turned, and all of them
 };
-inline RopeShape rope_shape(const bfp_rows &x, const bfp_rows &y, int hd, int rot, int interleaved) {
+inline RopeShape rope_shape(const bfp_rows &x, const bfp_rows &y, long long n_rows, int hd, int rot, int interleaved) {
   RopeShape s;
   s.half = rot / 2;
   s.interleaved = interleaved ? 1 : 0;
-  s.wide = rows_aligned(x, 8) && rows_aligned(y, 8) && hd % 8 == 0 && (interleaved ? rot % 8 == 0 : s.half % 8 == 0);
+  s.wide = rows_aligned(x, 8, n_rows) && rows_aligned(y, 8, n_rows) && hd % 8 == 0 && (interleaved ? rot % 8 == 0 : s.half % 8 == 0);
   s.turned = s.wide ? (interleaved ? rot / 8 : s.half / 8) : s.half;
   s.per_head = s.turned + (s.wide ? (hd - rot) / 8 : hd - rot);
   return s;

@@ -166,7 +166,7 @@ int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const 
   if (!pos || !table || n_pos < 1) return set_err(BFP_EINVAL, "rope: no positions or no table");
   if ((uintptr_t)table % 8) return set_err(BFP_EINVAL, "rope: table is not 8-byte aligned");
   if (n_rows == 0) return BFP_OK;
-  const RopeShape shape = rope_shape(*x, *y, hd, rot, interleaved);
+  const RopeShape shape = rope_shape(*x, *y, n_rows, hd, rot, interleaved);
   // two heads a thread once that still leaves eight waves a CU
   const long long all = (long long)n_rows * x->heads * shape.per_head;
   const int n = shape.wide && x->heads >= ROPE_HEADS && all >= (long long)ROPE_HEADS * 256 * 8 * 64 ? ROPE_HEADS : 1;

@@ -46,7 +46,7 @@ inline int check_rows(const char *op, const char *what, const bfp_rows *r, int h
     return set_err(BFP_EINVAL, "%s: %s has a negative stride", op, what);
   if (r->head_stride < hd && heads > 1)
     return set_err(BFP_EINVAL, "%s: heads of %s overlap (stride %lld, hd %d)", op, what, r->head_stride, hd);
-  if (r->type == BFP_TILES && (hd % 16 || r->row_stride % 16 || r->head_stride % 16))
+  if (r->type == BFP_TILES && (hd % 16 || (n_rows > 1 && r->row_stride % 16) || (heads > 1 && r->head_stride % 16)))
     return set_err(BFP_EINVAL, "%s: tiles of %s need hd and strides in multiples of 16", op, what);
   const int size = r->type == BFP_F32 ? 4 : 2;
   if ((uintptr_t)r->p % size) return set_err(BFP_EINVAL, "%s: %s is not aligned to its type", op, what);
@@ -89,9 +89,10 @@ inline int check_out(const char *op, const char *what, const bfp_rows *r, int he
 }
 
 // Whether groups of n values (n values a multiple of 16 bytes) that start at
-// multiples of n in a head can be moved with 16-byte accesses.
-inline bool rows_aligned(const bfp_rows &r, int n) {
-  return (uintptr_t)r.p % 16 == 0 && r.row_stride % n == 0 && r.head_stride % n == 0;
+// multiples of n in a head can be moved with 16-byte accesses.  The stride of
+// a single row or head is not used, and may be anything.
+inline bool rows_aligned(const bfp_rows &r, int n, long long n_rows) {
+  return (uintptr_t)r.p % 16 == 0 && (n_rows <= 1 || r.row_stride % n == 0) && (r.heads <= 1 || r.head_stride % n == 0);
 }
 
 __device__ __forceinline__ float bf16_to_f32(uint32_t b) { return __uint_as_float(b << 16); }
