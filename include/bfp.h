@@ -571,7 +571,8 @@ int bfp_rope_table_d(const double *inv_freq, int n_freq, double mscale, long lon
  * for the others), where (a, b) are values (j, j + rot/2) of the head
  * (interleaved 0, as rope_fp pairs them) or (2j, 2j + 1) (interleaved 1).
  * x and y: n_rows rows, the same number of heads; y BFP_F32, BFP_BF16 or
- * BFP_F16; y may be x.  pos: n_rows positions; a row whose position is
+ * BFP_F16; y may be x (the same place and strides, values of the same size),
+ * and shares no memory with it otherwise.  pos: n_rows positions; a row whose position is
  * outside [0, n_pos) gets NaN in its rotated part. */
 int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const float *table,
                int n_pos, int rot, int interleaved, const bfp_rows *y, void *stream);
@@ -610,7 +611,8 @@ typedef struct bfp_kv4_batch {
 /* Writes the new tokens' k and v (n_rows x heads x hd) into their slots, k
  * rotated as bfp_rope_d does at its position first (table NULL: not
  * rotated).  q and q_out (both or neither): queries rotated by the same
- * table in the same launch, q_out as bfp_rope_d's y, and not k or v.  pos:
+ * table in the same launch, q_out as bfp_rope_d's y, and no value of it on k
+ * or v (joined rows are fine).  pos:
  * positions to rotate at, per row (NULL: the position in the cache).  A row
  * without a slot writes nothing, and its q_out is zero; a position outside
  * [0, n_pos) gives NaN in the rotated part (whole tiles of k).  No two rows
@@ -619,8 +621,8 @@ int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp
                      const bfp_rows *v, const bfp_rows *q, const bfp_rows *q_out, const int32_t *pos,
                      const float *table, int n_pos, int rot, int interleaved, void *stream);
 /* Reads the batch's rows back: k and v (either may be NULL; BFP_F32, BFP_BF16
- * or BFP_F16) hold the cached values, exact but for float16's range; a row
- * without a slot gives zeros. */
+ * or BFP_F16, apart from each other) hold the cached values, exact but for
+ * float16's range; a row without a slot gives zeros. */
 int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *k,
                    const bfp_rows *v, void *stream);
 /* out = softmax(scale q k^T) v per row and query head over the cache: the
@@ -631,7 +633,8 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
  * its bytes.  Products are exact, sums and softmax in float32, probabilities
  * carried to at least the output's precision; scale q.k has to fit float32, and
  * a query with a NaN or an infinity in it makes its row NaN.  out: any type
- * (BFP_TILES: tile_quantize of the float32 result); it may be q.  work:
+ * (BFP_TILES: tile_quantize of the float32 result); it may be q, as y may be
+ * x in bfp_rope_d.  work:
  * bfp_kv4_attn_work() bytes of device scratch, 16-byte aligned (NULL if that
  * is 0), whatever they hold; calls that may run at the same time need their
  * own. */

@@ -72,3 +72,82 @@ def test_strides_that_nothing_uses():
     two = C.byref(_batch(L, n_rows=2))
     r = L.RowsC(4096, None, 1, 1, 131, 3)
     assert "strides" in _refused(L, "bfp_kv4_attn_d", c, two, C.byref(r), C.byref(L.RowsC(1 << 30, None, 1, 1, 64, 64)), 1.0, 0, None, 0, None)
+
+
+def _places(p, size, n, heads, hd, rs, hs):
+    at = p + size * (np.arange(n)[:, None, None] * rs + np.arange(heads)[:, None] * hs + np.arange(hd))
+    return set((at.reshape(-1, 1) + np.arange(size)).reshape(-1).tolist())
+
+
+#  q_out's and k's first byte past 2^20, type (0: 4 bytes, 1: 2), heads, row stride, head stride; rows
+BETWEEN = [
+    ((0, 1, 4, 384, 64), (512, 1, 1, 384, 64), 5),              # joined rows q | k
+    ((512, 1, 4, 384, 64), (0, 1, 4, 384, 64), 5),              # q runs into the next row's k
+    ((0, 1, 4, 384, 64), (384, 1, 1, 384, 64), 5),              # k is one of q's heads
+    ((0, 1, 4, 384, 64), (384, 1, 1, 320, 64), 5),              # other rows
+    ((0, 1, 2, 768, 384), (128, 1, 2, 768, 384), 5),            # q, k and v side by side within a group
+    ((0, 1, 2, 768, 384), (64, 1, 2, 768, 384), 5),
+    ((0, 1, 2, 768, 384), (896, 1, 1, 768, 64), 5),             # between two groups' q
+    ((0, 1, 2, 768, 384), (704, 1, 1, 768, 64), 5),
+    ((0, 1, 4, 384, 64), (5 * 768, 1, 1, 384, 64), 5),          # behind the last row
+    ((0, 1, 4, 384, 64), (4 * 768 + 256, 1, 1, 384, 64), 5),
+    ((0, 0, 4, 384, 64), (1024, 0, 1, 384, 64), 5),
+    ((0, 0, 4, 384, 64), (0, 1, 1, 384, 64), 5),                # another type's rows in the same place
+    ((0, 1, 4, 384, 64), (512, 1, 1, 9999, 7), 1),              # one row, one head: strides that nothing uses
+    ((0, 1, 4, 384, 64), (496, 1, 1, 9999, 7), 1),
+    ((0, 1, 4, 64, 320), (4 * 640, 1, 1, 64, 64), 5),           # heads before rows
+    ((0, 1, 4, 64, 320), (2 * 640, 1, 1, 64, 64), 5)]
+
+
+@pytest.mark.parametrize("a,b,n", BETWEEN)
+def test_results_that_lie_on_operands(a, b, n):
+    """Against sets of bytes; the calls stop there or at a later check."""
+    shared = bool(_places(a[0], 2 if a[1] else 4, n, a[2], 64, *a[3:]) & _places(b[0], 2 if b[1] else 4, n, b[2], 64, *b[3:]))
+    L = _lib()
+    make = lambda x: L.RowsC((1 << 20) + x[0], None, x[1], x[2], x[3], x[4])  # noqa: E731
+    free = L.RowsC(1 << 30, None, 1, b[2], 1 << 12, 64)
+    cache = C.byref(_cache(L, heads=b[2]))
+    batch = C.byref(_batch(L, n_rows=n))
+    for k, v in ((make(b), free), (free, make(b))):
+        q = make(a)
+        msg = _refused(L, "bfp_kv4_append_d", cache, batch, C.byref(k), C.byref(v), C.byref(q), C.byref(q), None, 4096, 16, 66, 0, None)
+        assert ("q_out" in msg) == shared and ("rot" in msg) != shared, msg
+
+
+def test_results_over_their_own_rows():
+    """In place means the same place: not shifted, not in another stride or
+    size of value."""
+    L = _lib()
+    x = L.RowsC(1 << 20, None, 1, 3, 192, 64)
+    other = [L.RowsC((1 << 20) + 16, None, 1, 3, 192, 64), L.RowsC(1 << 20, None, 1, 3, 256, 64), L.RowsC(1 << 20, None, 0, 3, 192, 64),
+             L.RowsC((1 << 20) + 384, None, 1, 3, 192, 64)]
+    apart = [x, L.RowsC(1 << 20, None, 2, 3, 192, 64), L.RowsC((1 << 20) + 4 * 384, None, 1, 3, 192, 64), L.RowsC(1 << 24, None, 0, 3, 192, 64)]
+    c, b = C.byref(_cache(L, heads=1)), C.byref(_batch(L, n_rows=4))
+    kv = C.byref(L.RowsC(1 << 30, None, 1, 1, 64, 64))
+    for y in other + apart:
+        shared = any(y is o for o in other)
+        msg = _refused(L, "bfp_rope_d", C.byref(x), 4, 64, 4096, 4096, 16, 66, 0, C.byref(y), None)
+        assert ("y lies" in msg) == shared and ("rot" in msg) != shared, msg
+        msg = _refused(L, "bfp_kv4_attn_d", c, b, C.byref(x), C.byref(y), 1.0, -1, None, 0, None)
+        assert ("out lies" in msg) == shared and ("window" in msg) != shared, msg
+        msg = _refused(L, "bfp_kv4_append_d", c, b, kv, kv, C.byref(x), C.byref(y), None, 4096, 16, 66, 0, None)
+        assert ("q_out lies" in msg) == shared and ("rot" in msg) != shared, msg
+
+
+def test_tiles_over_their_own_rows():
+    L = _lib()
+    q = L.RowsC(1 << 20, 1 << 21, 3, 3, 192, 64)
+    c, b = C.byref(_cache(L, heads=1)), C.byref(_batch(L, n_rows=4))
+    for out, shared in ((q, False), (L.RowsC(1 << 22, 1 << 23, 3, 3, 192, 64), False), (L.RowsC(1 << 20, 1 << 23, 3, 3, 192, 64), False),
+                        (L.RowsC(1 << 22, 1 << 21, 3, 3, 192, 64), False), (L.RowsC(1 << 22, (1 << 21) + 4, 3, 3, 192, 64), True),
+                        (L.RowsC(1 << 22, 1 << 20, 3, 3, 192, 64), True), (L.RowsC(1 << 22, (1 << 21) + 48, 3, 3, 192, 64), False)):
+        msg = _refused(L, "bfp_kv4_attn_d", c, b, C.byref(q), C.byref(out), 1.0, -1, None, 0, None)
+        assert ("out lies" in msg) == shared and ("window" in msg) != shared, msg
+
+
+def test_keys_and_values_read_into_the_same_place():
+    L = _lib()
+    c, b = C.byref(_cache(L)), C.byref(_batch(L))
+    k = L.RowsC(1 << 20, None, 1, 2, 128, 64)
+    for v in (k, L.RowsC((1 << 20) + 128, None, 1, 2, 128, 64)):
+        assert "v lies" in _refused(L, "bfp_kv4_read_d", c, b, C.byref(k), C.byref(v), None)

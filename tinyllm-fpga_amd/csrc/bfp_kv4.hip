@@ -272,7 +272,9 @@ int bfp_kv4_append_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp
     if (!rows_aligned(*q, 8, rows) || !rows_aligned(*q_out, 8, rows))
       return set_err(BFP_EINVAL, "%s: q and q_out need 16-byte alignment and strides in multiples of 8", op);
     // q_out may be q: who writes a value has read its pair (rope_wide_unit)
-    if (q_out->p == k->p || q_out->p == v->p) return set_err(BFP_EINVAL, "%s: q_out cannot be k or v", op);
+    BFP_TRY(check_apart(op, "q_out", *q_out, "q", *q, rows, hd, true));
+    BFP_TRY(check_apart(op, "q_out", *q_out, "k", *k, rows, hd, false));
+    BFP_TRY(check_apart(op, "q_out", *q_out, "v", *v, rows, hd, false));
   }
   if (table) {
     if (rot < 2 || rot % 2 || rot > hd) return set_err(BFP_EINVAL, "%s: rot=%d, hd=%d", op, rot, hd);
@@ -325,6 +327,7 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
       return set_err(BFP_EINVAL, "%s: k and v need 16-byte alignment and strides in multiples of 8", op);
   }
   if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
+  if (k && v) BFP_TRY(check_apart(op, "v", *v, "k", *k, batch->n_rows, cache->hd, false));
   Kv4ReadArgs a{};
   a.c = *cache;
   a.b = *batch;

@@ -128,6 +128,8 @@ static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch 
   BFP_TRY(check_rows(op, "q", q, q->heads, cache->hd, true, batch->n_rows));
   BFP_TRY(check_out(op, "out", out, q->heads, cache->hd, true, batch->n_rows));
   if (!rows_aligned(*q, 8, batch->n_rows)) return set_err(BFP_EINVAL, "%s: q needs 16-byte alignment and strides in multiples of 8", op);
+  // out may be q: a workgroup has read its rows' queries before anyone writes their results
+  BFP_TRY(check_apart(op, "out", *out, "q", *q, batch->n_rows, cache->hd, true));
   if (window < 0) return set_err(BFP_EINVAL, "%s: window=%d", op, window);
   if ((long long)batch->max_q * (q->heads / cache->heads) > 0x3fffffffLL)
     return set_err(BFP_EINVAL, "%s: max_q=%d rows of %d heads are too many", op, batch->max_q, q->heads);

@@ -162,6 +162,7 @@ int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const 
     return set_err(BFP_EINVAL, "rope: x %s", x ? "has no heads, or too many" : "is null");
   BFP_TRY(check_rows("rope", "x", x, x->heads, hd, true, n_rows));
   BFP_TRY(check_out("rope", "y", y, x->heads, hd, false, n_rows));
+  BFP_TRY(check_apart("rope", "y", *y, "x", *x, n_rows, hd, true));   // who writes a value has read its pair
   if (rot < 2 || rot % 2 || rot > hd) return set_err(BFP_EINVAL, "rope: rot=%d, hd=%d", rot, hd);
   if (!pos || !table || n_pos < 1) return set_err(BFP_EINVAL, "rope: no positions or no table");
   if ((uintptr_t)table % 8) return set_err(BFP_EINVAL, "rope: table is not 8-byte aligned");

@@ -88,6 +88,71 @@ inline int check_out(const char *op, const char *what, const bfp_rows *r, int he
   return BFP_OK;
 }
 
+// Rows in bytes: n rows s apart of m heads t apart, each w bytes from p on.
+struct RowPlaces {
+  long long p, s, t, n, m, w;
+};
+inline RowPlaces row_places(const bfp_rows &r, long long n_rows, int hd, bool exponents) {
+  const long long size = r.type == BFP_F32 ? 4 : 2;
+  if (exponents) return {(long long)(uintptr_t)r.e, r.row_stride / 16, r.head_stride / 16, n_rows, r.heads, hd / 16};
+  return {(long long)(uintptr_t)r.p, r.row_stride * size, r.head_stride * size, n_rows, r.heads, hd * size};
+}
+inline bool same_places(const RowPlaces &a, const RowPlaces &b) {
+  return a.p == b.p && a.m == b.m && a.w == b.w && (a.n <= 1 || a.s == b.s) && (a.m <= 1 || a.t == b.t);
+}
+
+// Whether a byte lies in both.  Exact where the rows are equally far apart,
+// as in joined rows (and the heads, or there are few): a head of one against
+// a head of the other is then a question of their distance modulo the rows'.
+// Rows of another stride in the same memory count as sharing some.
+inline bool places_share(const RowPlaces &a, const RowPlaces &b) {
+  typedef __int128 wide;
+  const auto row = [](const RowPlaces &r) { return (wide)(r.m - 1) * r.t + r.w; };
+  const auto end = [&](const RowPlaces &r) { return (wide)r.p + (wide)(r.n - 1) * r.s + row(r); };
+  if (end(a) <= b.p || end(b) <= a.p) return false;
+  if (a.n > 1 && a.s != b.s) return true;
+  const long long s = a.s, most = a.n - 1;
+  if (s > 0) {   // b's rows in the gaps between a's: joined rows, without the search
+    const long long gap = (b.p - a.p) % s, at = gap < 0 ? gap + s : gap;
+    if (at >= row(a) && at + row(b) <= s) return false;
+  }
+  const auto meet = [&](wide d) {   // b's bytes d behind a's, in any two rows: -b.w < d + k s < a.w, |k| <= most
+    if (most == 0 || s == 0) return -b.w < d && d < a.w;
+    const wide x = -b.w - d;
+    wide k = x / s - (x % s < 0 ? 1 : 0) + 1;   // the least with k s > x
+    k = k < -most ? -most : k;
+    return k <= most && k * s + d < a.w;
+  };
+  const wide d = (wide)b.p - a.p;
+  if (a.m == 1 || b.m == 1 || a.t == b.t) {
+    const long long t = a.m == 1 ? b.t : a.t;
+    for (long long j = 1 - a.m; j < b.m; ++j)
+      if (meet(d + (wide)j * t)) return true;
+    return false;
+  }
+  if (a.m * b.m > 65536) return true;
+  for (long long i = 0; i < a.m; ++i)
+    for (long long j = 0; j < b.m; ++j)
+      if (meet(d + (wide)j * b.t - (wide)i * a.t)) return true;
+  return false;
+}
+
+// Results may lie on operands where each value takes its own operand's place
+// (in_place), or nowhere near them.
+inline int check_apart(const char *op, const char *what, const bfp_rows &y, const char *other, const bfp_rows &x,
+                       long long n_rows, int hd, bool in_place) {
+  if (n_rows <= 0) return BFP_OK;
+  for (int i = 0; i < 4; ++i) {
+    const bool ye = i & 1, xe = i & 2;
+    if ((ye && y.type != BFP_TILES) || (xe && x.type != BFP_TILES)) continue;
+    const RowPlaces a = row_places(y, n_rows, hd, ye), b = row_places(x, n_rows, hd, xe);
+    if (in_place && ye == xe && same_places(a, b)) continue;
+    if (places_share(a, b))
+      return set_err(BFP_EINVAL, "%s: %s lies on %s%s", op, what, other, in_place ? ", but not in its place" : "");
+  }
+  return BFP_OK;
+}
+
 // Whether groups of n values (n values a multiple of 16 bytes) that start at
 // multiples of n in a head can be moved with 16-byte accesses.  The stride of
 // a single row or head is not used, and may be anything.
