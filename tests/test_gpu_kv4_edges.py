@@ -91,3 +91,18 @@ def test_one_row_of_any_stride(gpu):
         s.cache.read(b, k=back)
         assert torch.equal(back, wk)
         assert torch.equal(s.cache.attend(b, odd_q, out=out), want) and torch.equal(out, want)
+
+
+def test_a_type_that_the_result_does_not_have(gpu):
+    import torch
+    s = Long(149, [60], [2], 16, 1, 64)
+    q = torch.randn(2, 3, 64, device="cuda")
+    pair = (torch.empty(2, 3, 64, dtype=torch.int16, device="cuda"), torch.empty(2, 3, 4, dtype=torch.int8, device="cuda"))
+    out, kv = torch.empty_like(q), torch.empty(2, 1, 64, device="cuda")
+    for bad in (lambda: s.cache.attend(s.batch, q, out=out, dtype=torch.bfloat16), lambda: s.cache.attend(s.batch, q, out=pair, dtype=torch.float32),
+                lambda: s.cache.attend_work(s.batch, q, out=out, dtype=torch.float16), lambda: s.cache.read(s.batch, k=kv, dtype=torch.bfloat16),
+                lambda: s.cache.read(s.batch, n_rows=3, v=kv)):
+        with pytest.raises(ValueError):
+            bad()
+    assert s.cache.attend(s.batch, q, out=out, dtype=torch.float32) is out
+    assert s.cache.read(s.batch, n_rows=2, k=kv, dtype=torch.float32)[0] is kv

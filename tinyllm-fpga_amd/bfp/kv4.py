@@ -168,7 +168,7 @@ class Fp4Cache(_rows.Fixed):
             if n_rows:
                 _read(self.device, self._c, batch._c(int(n_rows)), C.byref(kr), C.byref(vr))
             return k, v
-        n, rs = None, []
+        n, rs = None if n_rows is None else int(n_rows), []
         for x, what in ((k, "k"), (v, "v")):
             if x is None:
                 rs.append(None)
@@ -176,6 +176,8 @@ class Fp4Cache(_rows.Fixed):
             t = self._values(batch, x, what)
             if t.shape[1] != self.heads or n not in (None, t.shape[0]):
                 raise ValueError(f"{what} has shape {tuple(t.shape)}, not ({'rows' if n is None else n}, {self.heads}, {self.hd})")
+            if dtype is not None and t.dtype != dtype:
+                raise ValueError(f"{what} is not of {dtype}")
             n = t.shape[0]
             rs.append(C.byref(_rows.rows(x, what, self.device)))
         if n:
@@ -220,6 +222,8 @@ class Fp4Cache(_rows.Fixed):
         else:
             if self._values(batch, out, "out").shape != t.shape:
                 raise ValueError(f"out must be {tuple(t.shape)}")
+            if dtype is not None and (type(out) is tuple or out.dtype != dtype):
+                raise ValueError(f"out is not of {dtype}")
             orow = _rows.rows(out, "out", self.device)
         return t, qr, out, orow
 
