@@ -106,3 +106,18 @@ def test_a_type_that_the_result_does_not_have(gpu):
             bad()
     assert s.cache.attend(s.batch, q, out=out, dtype=torch.float32) is out
     assert s.cache.read(s.batch, n_rows=2, k=kv, dtype=torch.float32)[0] is kv
+
+
+def test_numbers_that_an_int_does_not_hold(gpu):
+    """They do not come back from the other end."""
+    import torch
+    from bfp.kv4 import Batch
+    s = Long(151, [60], [2], 16, 1, 64)
+    q = torch.randn(2, 3, 64, device="cuda")
+    for bad in (2 ** 32 + 16, 2 ** 31, 2 ** 64 + 1):
+        for call in (lambda: s.cache.attend(s.batch, q, window=bad), lambda: s.cache.attend_work(s.batch, q, window=bad),
+                     lambda: Batch(s.batch.pages, s.batch.start, s.batch.lens, max_q=bad),
+                     lambda: Batch(s.batch.pages, s.batch.start, s.batch.lens, max_q=1, max_len=bad)):
+            with pytest.raises(ValueError):
+                call()
+    assert torch.equal(s.cache.attend(s.batch, q, window=2 ** 31 - 1), s.cache.attend(s.batch, q))

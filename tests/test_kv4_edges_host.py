@@ -151,3 +151,18 @@ def test_keys_and_values_read_into_the_same_place():
     k = L.RowsC(1 << 20, None, 1, 2, 128, 64)
     for v in (k, L.RowsC((1 << 20) + 128, None, 1, 2, 128, 64)):
         assert "v lies" in _refused(L, "bfp_kv4_read_d", c, b, C.byref(k), C.byref(v), None)
+
+
+def test_numbers_that_an_int_does_not_hold():
+    """They do not come back from the other end."""
+    import torch
+    from bfp import rotary
+    inv, _ = rotary.rope_freqs(4)
+    for bad in (2 ** 31, 2 ** 32 + 4, 2 ** 64 + 4, -2 ** 32 + 4):
+        for call in (lambda: rotary.rope_freqs(bad), lambda: rotary.rope_freqs(64, 1e4, "parts", 4.0, bad),
+                     lambda: rotary.rope_table(inv, bad, out=torch.zeros(4, 2, 2))):
+            with pytest.raises(ValueError):
+                call()
+    for first in (2 ** 64, -2 ** 64 + 1, 2 ** 63):
+        with pytest.raises(ValueError):
+            rotary.rope_table(inv, 4, first=first, out=torch.zeros(4, 2, 2))

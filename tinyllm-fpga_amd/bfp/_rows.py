@@ -103,7 +103,16 @@ def gpu_of(t, what):
     return t.device
 
 
-MAX_ROWS = 0x7fffffff   # the entry points count rows in int
+MAX_INT = MAX_ROWS = 0x7fffffff   # the entry points count rows in int
+
+
+def c_int(n, what: str, least=0, most=MAX_INT):
+    """n as an int of the entry points: ctypes would take the lowest bits of
+    a larger one."""
+    n = int(n)
+    if not least <= n <= most:
+        raise ValueError(f"{what}={n}")
+    return n
 
 
 class Fixed:

@@ -26,6 +26,10 @@ TILE = 16
 _append, _read, _attend = (_rows.Entry(f"bfp_kv4_{name}_d") for name in ("append", "read", "attn"))
 
 
+def _window(n):
+    return _rows.c_int(n, "window", -1 - _rows.MAX_INT)   # negative ones are the entry point's to refuse
+
+
 class Batch(_rows.Fixed):
     """Which rows belong to which sequence, and where they are cached: row
     start[b] + i of the row arrays is a new token of sequence b, the last of
@@ -44,10 +48,8 @@ class Batch(_rows.Fixed):
             if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != pages.device \
                     or not t.is_cuda:
                 raise ValueError(f"{what} must be a contiguous int32 tensor {shape} on one GPU")
-        if max_q < 0 or max_len < 0:
-            raise ValueError(f"max_q={max_q}, max_len={max_len}")
         self.pages, self.start, self.lens = pages, start, lens
-        self.max_q, self.max_len = int(max_q), int(max_len)
+        self.max_q, self.max_len = _rows.c_int(max_q, "max_q"), _rows.c_int(max_len, "max_len")
         self.device = pages.device
         self._made = (-1, None)
 
@@ -198,7 +200,7 @@ class Fp4Cache(_rows.Fixed):
         n = t.shape[0]
         if n == 0:
             return out
-        b, qb, ob, window = batch._c(n), C.byref(qr), C.byref(orow), int(window)
+        b, qb, ob, window = batch._c(n), C.byref(qr), C.byref(orow), _window(window)
         if work is None:
             size = lib().bfp_kv4_attn_work(self._c, b, qb, ob, window)
             if size:
@@ -230,4 +232,4 @@ class Fp4Cache(_rows.Fixed):
     def attend_work(self, batch, q, out=None, dtype=None, window=0):
         """Scratch bytes attend() needs for such a call."""
         t, qr, out, orow = self._attend_rows(batch, q, out, dtype)
-        return lib().bfp_kv4_attn_work(self._c, batch._c(t.shape[0]), C.byref(qr), C.byref(orow), int(window))
+        return lib().bfp_kv4_attn_work(self._c, batch._c(t.shape[0]), C.byref(qr), C.byref(orow), _window(window))

@@ -32,10 +32,9 @@ def rope_freqs(rot, base=10000.0, scaling="none", factor=1.0, orig_ctx=0):
       "bands"   above 4 turns stay, below 1 divided, linear in the turns"""
     if scaling not in SCALINGS:
         raise ValueError(f"scaling {scaling!r}: one of {', '.join(SCALINGS)}")
-    n = max(int(rot) // 2, 1)
-    inv, mscale = (C.c_double * n)(), C.c_double()
-    call("bfp_rope_freqs", int(rot), float(base), SCALINGS[scaling], float(factor), int(orig_ctx), inv,
-         C.byref(mscale))
+    rot, orig_ctx = (_rows.c_int(x, what, -1 - _rows.MAX_INT) for x, what in ((rot, "rot"), (orig_ctx, "orig_ctx")))
+    inv, mscale = (C.c_double * max(rot // 2, 1))(), C.c_double()
+    call("bfp_rope_freqs", rot, float(base), SCALINGS[scaling], float(factor), orig_ctx, inv, C.byref(mscale))
     return np.frombuffer(inv, np.float64), mscale.value
 
 
@@ -52,15 +51,14 @@ def rope_table(inv_freq, n_pos, mscale=1.0, first=0, out=None):
     inv = inv_freq
     if type(inv) is not np.ndarray or inv.dtype != np.float64 or inv.ndim != 1 or not inv.flags.c_contiguous:
         inv = np.ascontiguousarray(np.asarray(inv_freq, np.float64).reshape(-1))
-    shape = (int(n_pos), inv.size, 2)
+    shape = (_rows.c_int(n_pos, "n_pos"), inv.size, 2)
+    first = _rows.c_int(first, "first", -1 << 63, (1 << 63) - 1)
     if out is None:
-        if shape[0] < 0:
-            raise ValueError(f"n_pos={n_pos}")
         out = torch.empty(shape, dtype=torch.float32, device="cuda")
     elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or not out.is_cuda:
         raise ValueError(f"out must be a contiguous float32 tensor {shape} on a GPU")
     if shape[0]:
-        _table(out.device, _address(inv), inv.size, float(mscale), int(first), shape[0], out.data_ptr())
+        _table(out.device, _address(inv), inv.size, float(mscale), first, shape[0], out.data_ptr())
     return out
 
 
