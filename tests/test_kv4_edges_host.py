@@ -166,3 +166,10 @@ def test_numbers_that_an_int_does_not_hold():
     for first in (2 ** 64, -2 ** 64 + 1, 2 ** 63):
         with pytest.raises(ValueError):
             rotary.rope_table(inv, 4, first=first, out=torch.zeros(4, 2, 2))
+
+
+def test_positions_past_64_bits():
+    L = _lib()
+    inv = np.zeros(4)
+    for first, n in ((2 ** 63 - 1, 1), (2 ** 63 - 5, 100), (2 ** 31, 1), (2 ** 31 - 1, 2)):
+        assert "first" in _refused(L, "bfp_rope_table_d", inv.ctypes.data, 4, 1.0, first, n, 4096, None)

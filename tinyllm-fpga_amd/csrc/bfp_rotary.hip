@@ -135,7 +135,7 @@ int bfp_rope_table_d(const double *inv_freq, int n_freq, double mscale, long lon
   if (!inv_freq || !table) return set_err(BFP_EINVAL, "rope_table: null pointer");
   if (n_freq < 1 || n_freq > ROPE_MAX_FREQ)
     return set_err(BFP_EINVAL, "rope_table: n_freq=%d must be in [1, %d]", n_freq, ROPE_MAX_FREQ);
-  if (n_pos < 0 || first < 0 || first + n_pos > (1LL << 31))
+  if (n_pos < 0 || first < 0 || first > (1LL << 31) - n_pos)
     return set_err(BFP_EINVAL, "rope_table: first=%lld, n_pos=%d", first, n_pos);
   if ((uintptr_t)table % 8) return set_err(BFP_EINVAL, "rope_table: table is not 8-byte aligned");
   RopeFreqs f;
