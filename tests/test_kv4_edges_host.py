@@ -173,3 +173,9 @@ def test_positions_past_64_bits():
     inv = np.zeros(4)
     for first, n in ((2 ** 63 - 1, 1), (2 ** 63 - 5, 100), (2 ** 31, 1), (2 ** 31 - 1, 2)):
         assert "first" in _refused(L, "bfp_rope_table_d", inv.ctypes.data, 4, 1.0, first, n, 4096, None)
+
+
+def test_positions_that_are_not_aligned():
+    L = _lib()
+    x = L.RowsC(1 << 20, None, 0, 1, 64, 64)
+    assert "pos" in _refused(L, "bfp_rope_d", C.byref(x), 4, 64, 4098, 4096, 16, 64, 0, C.byref(x), None)

@@ -166,6 +166,7 @@ int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const 
   if (rot < 2 || rot % 2 || rot > hd) return set_err(BFP_EINVAL, "rope: rot=%d, hd=%d", rot, hd);
   if (!pos || !table || n_pos < 1) return set_err(BFP_EINVAL, "rope: no positions or no table");
   if ((uintptr_t)table % 8) return set_err(BFP_EINVAL, "rope: table is not 8-byte aligned");
+  if ((uintptr_t)pos % 4) return set_err(BFP_EINVAL, "rope: pos is not aligned");
   if (n_rows == 0) return BFP_OK;
   const RopeShape shape = rope_shape(*x, *y, n_rows, hd, rot, interleaved);
   // two heads a thread once that still leaves eight waves a CU
