@@ -121,3 +121,29 @@ def test_numbers_that_an_int_does_not_hold(gpu):
             with pytest.raises(ValueError):
                 call()
     assert torch.equal(s.cache.attend(s.batch, q, window=2 ** 31 - 1), s.cache.attend(s.batch, q))
+
+
+SCALES = [  # scale, exponent byte of the keys, size of the queries
+    (2.0 ** -110, 227, 2.0 ** 8), (2.0 ** -120, 227, 2.0 ** 18), (2.0 ** -125, 227, 2.0 ** 22),
+    (0.0, 227, 2.0 ** 20), (-0.0, 227, 2.0 ** 20), (1e-40, 227, 2.0 ** 20), (-1e-46, 227, 2.0 ** 20), (1e-320, 227, 1.0),
+    (2.0 ** -20, 127, 2.0 ** 20), (2.0 ** 110, 27, 2.0 ** -10), (-2.0 ** 100, 27, 1.0), (2.0 ** 100, 67, 2.0 ** -40)]
+
+
+@pytest.mark.parametrize("news", [1, 6, 700])
+@pytest.mark.parametrize("scale,k_exp,size", SCALES)
+def test_scales_at_the_ends(gpu, scale, k_exp, size, news):
+    """Any scale that float32 holds, whatever the products' size, and those
+    too small for it, which leave all scores alike."""
+    rng = np.random.default_rng(3)
+    n = 700
+    s = Few(rng.choice(np.concatenate([ref.GRID, -ref.GRID[1:]]), n), rng.choice(ref.GRID, n), k_exp, news=news)
+    for kind in ("f32", "bf16"):
+        q, q0 = s.query(rng.uniform(-1, 1, (news, 4)) * size, kind)
+        want, weight, big = s.want(q0, scale)
+        got = s.cache.attend(s.batch, q, scale=scale).double().cpu().numpy()
+        # a scale below float32's normal numbers is off by half of 2^-149, its score by that times q.k < 2^126
+        lost = 2.0 ** -23 if abs(scale) < 2.0 ** -126 else 0.0
+        bound = ref.attend_bound(want[..., None], weight[..., None], big, n, s.hd, HALF[kind],
+                                 (2.0 ** -24 if kind == "f32" else 2.0 ** -8) + 2 * lost)
+        assert np.isfinite(got).all()
+        assert (np.abs(got - want[..., None]) <= bound).all(), (kind, np.abs(got - want[..., None]).max())

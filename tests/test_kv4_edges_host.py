@@ -179,3 +179,11 @@ def test_positions_that_are_not_aligned():
     L = _lib()
     x = L.RowsC(1 << 20, None, 0, 1, 64, 64)
     assert "pos" in _refused(L, "bfp_rope_d", C.byref(x), 4, 64, 4098, 4096, 16, 64, 0, C.byref(x), None)
+
+
+def test_scales_past_float32():
+    L = _lib()
+    c, b = C.byref(_cache(L)), C.byref(_batch(L))
+    r = C.byref(_rows(L))
+    for scale in (1e300, -1e300, 3e38, float("inf"), float("nan")):
+        assert "scale" in _refused(L, "bfp_kv4_attn_d", c, b, r, r, scale, 0, None, 0, None)

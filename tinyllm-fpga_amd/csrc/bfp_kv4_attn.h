@@ -47,9 +47,9 @@ struct Kv4AttnArgs {
     head = (int)h + split % c.heads;
     head = head < c.heads ? head : head - c.heads;
   }
-  float scale2;        // |scale| * log2(e), kept above 0; the queries take the sign
+  float scale2;        // |scale| * log2(e), kept above 0
   float slack;         // M_SLACK in scores: M_SLACK / scale2
-  float q_sign;
+  float q_sign;        // the scale's sign, or 0, which the queries take
   // unfinished rows: the sums, and (maximum, sum of probabilities)
   float *part_o;       // k_kv4_prompt [row][query head][split][hd]; k_kv4_rows [slot][R][hd]
   float2 *part_ml;     // without [hd]

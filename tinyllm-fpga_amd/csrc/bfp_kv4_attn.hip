@@ -153,7 +153,8 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
                    void *stream) {
   const char *op = "kv4_attn";
   BFP_TRY(check_attn(op, cache, batch, q, out, window));
-  if (!isfinite(scale)) return set_err(BFP_EINVAL, "%s: scale=%g", op, scale);
+  const float scale2 = (float)(fabs(scale) * 1.44269504088896340736);
+  if (!isfinite(scale2)) return set_err(BFP_EINVAL, "%s: scale=%g is not float32's", op, scale);
   if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
   const Kv4Plan p = plan_attn(*cache, *batch, *q, *out, window);
   if (p.work && (!work || (uintptr_t)work % 16 || work_bytes < p.work))
@@ -169,10 +170,11 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
   a.window = window;
   a.splits = p.splits;
   a.chunk = p.chunk;
-  // a scale of zero (all scores alike) is taken as one that leaves nothing of them
-  a.scale2 = fmaxf((float)(fabs(scale) * 1.44269504088896340736), 0x1p-100f);
-  a.slack = M_SLACK / a.scale2;
-  a.q_sign = scale < 0 ? -1.0f : 1.0f;
+  // a scale of zero, or too small for float32: all scores alike, from queries of zeros
+  a.scale2 = scale2 == 0.0f ? 1.0f : scale2;
+  a.q_sign = scale2 == 0.0f ? 0.0f : scale < 0 ? -1.0f : 1.0f;
+  // (kept finite, and so that no score below 2^126 passes float32 with it)
+  a.slack = fminf(M_SLACK / a.scale2, 0x1p125f);
   a.stream = p.stream;
   if (p.work) {
     a.part_o = (float *)work;
