@@ -632,8 +632,10 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
  * nothing gives zeros.  What a row does not see does not reach it, whatever
  * its bytes.  Products are exact, sums and softmax in float32, probabilities
  * carried to at least the output's precision.  q.k and scale q.k have to stay
- * below 2^126; products q_d k_d below 2^-126 may count as zero.  A scale that
- * is not finite in float32 is refused, one below 2^-150 leaves all scores alike.
+ * below 2^126, and the sum of the |v| that a row sees has to fit float32;
+ * products below 2^-126, of q_d k_d or of v and a probability (which the kernels
+ * carry at 2^-8 to 1 for the largest), may count as zero.  A scale that is not
+ * finite in float32 is refused, one below 2^-150 leaves all scores alike.
  * A query with a NaN or an infinity in it makes its row NaN.  out: any type
  * (BFP_TILES: tile_quantize of the float32 result); it may be q, as y may be
  * x in bfp_rope_d.  work:

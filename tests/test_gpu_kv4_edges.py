@@ -147,3 +147,21 @@ def test_scales_at_the_ends(gpu, scale, k_exp, size, news):
                                  (2.0 ** -24 if kind == "f32" else 2.0 ** -8) + 2 * lost)
         assert np.isfinite(got).all()
         assert (np.abs(got - want[..., None]) <= bound).all(), (kind, np.abs(got - want[..., None]).max())
+
+
+def test_sums_of_the_largest_values(gpu):
+    """The largest value the cache holds in 200192 tokens whose scores all
+    lie just under the point where the running maximum would follow: the
+    result is that value."""
+    import torch
+    from bfp.kv4 import Batch
+    n, news, page = 200192, 33024, 256
+    s = Few(np.concatenate([np.full(page, -6.0), np.zeros(page)]), np.full(2 * page, 6.0), v_exp=227, page=page)
+    batch = Batch(_int([[0] + [1] * (n // page - 1)]), _int([0, news]), _int([n]), max_q=news, max_len=n)
+    q = torch.zeros(news, 1, 16, dtype=torch.bfloat16, device="cuda")
+    q[:, :, 0] = 1
+    out = s.cache.attend(batch, q, scale=7.9 / 6 * np.log(2)).double()
+    top = 6 * 2.0 ** 100
+    assert torch.isfinite(out).all()
+    # two sums of n terms, 2^-23 each at most, and the result's own rounding
+    assert float((out / top - 1).abs().max()) <= (2 * n + 16) * 2.0 ** -23 + 2.0 ** -8

@@ -14,10 +14,12 @@
 namespace bfp {
 
 constexpr int KEYS = 64;             // keys a wave takes at a time
-// The running maximum is raised only when a score passes it by this many
-// powers of two: probabilities up to 2^8 are as exact as those up to 1, and
-// the sums are rescaled a few times in a whole context instead of whenever a
-// new maximum turns up.
+// The running maximum is raised only when a score passes it, and then to this
+// many powers of two above the score: the sums are rescaled a few times in a
+// whole context instead of whenever a new maximum turns up.  No probability
+// passes 1, so a sum of n values stays below n of the largest; the largest is
+// at least 2^-8 where it was set, and none is worse off for that (a float has
+// no fewer bits there, and those below 2^-126 are lost to the sum anyway).
 constexpr float M_SLACK = 8.0f;
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
@@ -48,7 +50,7 @@ struct Kv4AttnArgs {
     head = head < c.heads ? head : head - c.heads;
   }
   float scale2;        // |scale| * log2(e), kept above 0
-  float slack;         // M_SLACK in scores: M_SLACK / scale2
+  float slack;         // M_SLACK in scores: M_SLACK / scale2, above the score that raises the maximum
   float q_sign;        // the scale's sign, or 0, which the queries take
   // unfinished rows: the sums, and (maximum, sum of probabilities)
   float *part_o;       // k_kv4_prompt [row][query head][split][hd]; k_kv4_rows [slot][R][hd]

@@ -207,9 +207,9 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (u == 1) __syncthreads();
-      const bool raise = top > m + a.slack;
+      const bool raise = top > m;
       if (__any(raise)) {
-        const float mn = raise ? top : m;
+        const float mn = raise ? top + a.slack : m;
         const float f = raise ? exp2f((m - mn) * a.scale2) : 1.0f;
         m = mn;
         sum *= f;

@@ -384,9 +384,9 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
         for (int e = 0; e < 4; ++e) top = fmaxf(top, s[j][e]);
       top = fmaxf(top, fpeer<16>(top));
       top = fmaxf(top, fpeer<32>(top));
-      const bool raise = top > m + a.slack;
+      const bool raise = top > m;
       if (__any(raise)) {
-        const float mn = raise ? top : m;
+        const float mn = raise ? top + a.slack : m;
         const float f = raise ? exp2f((m - mn) * a.scale2) : 1.0f;   // from -infinity: 0
         m = mn;
         sum *= f;
