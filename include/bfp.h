@@ -630,7 +630,8 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
  * its own sequence; query head h reads KV head h / (q->heads / heads).
  * Positions whose page is outside [0, n_pages) are not seen; a row that sees
  * nothing gives zeros.  What a row does not see does not reach it, whatever
- * its bytes.  Products are exact, sums and softmax in float32, probabilities
+ * its bytes; a row that sees a tile of v whose exponent byte is 253 or more gets
+ * NaN there (bytes that append does not write: 0..26 and 228..254).  Products are exact, sums and softmax in float32, probabilities
  * carried to at least the output's precision.  q.k and scale q.k have to stay
  * below 2^126, and the sum of the |v| that a row sees has to fit float32;
  * products below 2^-126, of q_d k_d or of v and a probability (which the kernels

@@ -165,3 +165,30 @@ def test_sums_of_the_largest_values(gpu):
     assert torch.isfinite(out).all()
     # two sums of n terms, 2^-23 each at most, and the result's own rounding
     assert float((out / top - 1).abs().max()) <= (2 * n + 16) * 2.0 ** -23 + 2.0 ** -8
+
+
+@pytest.mark.parametrize("lens,news,window,hd,group", [(130, 100, 0, 64, 3), (130, 3, 0, 64, 3), (5001, 3, 0, 64, 3), (5001, 2, 4500, 128, 2),
+                                                       (1200, 1000, 0, 128, 4), (900, 600, 300, 64, 4), (700, 400, 0, 256, 2)])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_any_byte_stays_with_those_who_see_it(gpu, lens, news, window, hd, group, kind):
+    """Exponent bytes that no append writes, the largest elements beside
+    them: rows that do not see the token are as they were."""
+    s = Long(131, [lens], [news], 16, 1, hd)
+    q, _ = s.query(group, kind)
+    clean = s.cache.attend(s.batch, q, window=window).double().cpu().numpy()
+    pos = np.arange(lens - news, lens)
+    for p, tile in ((lens - 1, 1), (lens - news // 2 - 1, 0), (lens - news, 3), (2, 2)):
+        page, slot = int(s.table[0, p // 16]), p % 16
+        sees = (pos >= p) & ((pos - window < p) if window else True)
+        for exps, data, dims in ((s.cache.v_exp, s.cache.v, slice(16 * tile, 16 * tile + 16)), (s.cache.k_exp, s.cache.k, slice(0, hd))):
+            old = int(exps[page, 0, tile, slot]), data[page, 0, tile, slot].clone()
+            data[page, 0, tile, slot] = 0x7f
+            for byte in (252, 253, 254, 255, 0):
+                exps[page, 0, tile, slot] = byte
+                got = s.cache.attend(s.batch, q, window=window).double().cpu().numpy()
+                apart = np.ones(got.shape, bool)
+                apart[sees, :, dims] = False
+                assert (got[apart] == clean[apart]).all(), (p, tile, byte)
+                if byte >= 253 and exps is s.cache.v_exp:
+                    assert np.isnan(got[~apart]).all(), (p, tile, byte)
+            exps[page, 0, tile, slot], data[page, 0, tile, slot] = old[0], old[1]

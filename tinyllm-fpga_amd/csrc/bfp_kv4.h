@@ -22,6 +22,11 @@ namespace bfp {
 
 constexpr int KV4_E_MIN = -100, KV4_E_MAX = 100;   // exponents of a tile
 constexpr int KV4_BIAS = 127, KV4_NAN = 255;
+// Exponent bytes from here on can pass bfloat16's range (6 x 2^126).  Only
+// KV4_NAN is ever written; the attention takes values with the others as NaN,
+// too, since an infinity times a probability of zero would reach rows that do
+// not see it.
+constexpr int KV4_PAST = 253;
 constexpr int KV4_TILE_BYTES = 8;
 
 // The rows of a sequence in a batch, clamped to what the row arrays hold:

@@ -168,8 +168,10 @@ __device__ __forceinline__ float wave_sum(float v) {
   return sum16(v + fpeer<16>(v));
 }
 
-__device__ __forceinline__ bool has_byte_255(uint32_t w) {
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u;
+// Whether a byte of w is at least KV4_PAST: its lower seven bits carry into the
+// eighth, which is set.
+__device__ __forceinline__ bool has_byte_past(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u * (256 - KV4_PAST)) & w & 0x80808080u;
 }
 // w with its bytes kept where keep has a bit (byte i: bit i).
 __device__ __forceinline__ uint32_t byte_mask(uint32_t keep) {

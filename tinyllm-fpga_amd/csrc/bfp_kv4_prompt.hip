@@ -136,9 +136,9 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       kd[1] = kv4_decode8(t < tiles ? rk[u].y : 0u, ks);
       // NaN tiles of V count as zeros in the product; the rows that see them are set after
       const uint32_t E = ok ? rve[u] : 0u;
-      const bool take = ok && E != KV4_NAN;
+      const bool take = ok && E < KV4_PAST;
       vt[KEYS * VP + lane * 16 + t] = (char)E;
-      if (E == KV4_NAN) nan_tiles[t1 & 3] = 1;
+      if (E >= KV4_PAST) nan_tiles[t1 & 3] = 1;
       const float vs = kv4_scale(take ? E : 0u);
       *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1)) ^ sw)) = kv4_decode8(take ? rv[u].x : 0u, vs);
       *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1) + 1) ^ sw)) = kv4_decode8(take ? rv[u].y : 0u, vs);
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       for (int c = 0; c < TB; ++c) {
         bool hit = false;
 #pragma unroll 1
-        for (int k = 0; k < KEYS; ++k) hit |= (ve[16 * k + c] == KV4_NAN) & (t0 + k >= lo) & (t0 + k < hi);
+        for (int k = 0; k < KEYS; ++k) hit |= (ve[16 * k + c] >= KV4_PAST) & (t0 + k >= lo) & (t0 + k < hi);
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[c >> 1][8 * (c & 1) + e] = hit ? NAN : o[c >> 1][8 * (c & 1) + e];
       }

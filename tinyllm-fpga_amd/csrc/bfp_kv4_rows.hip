@@ -413,7 +413,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
       // cannot reach a row that does not see it; the rows that do are set below.
       uint32_t bad = 0;
 #pragma unroll
-      for (int c = 0; c < C; ++c) bad |= has_byte_255(v.e[c]) && g * C + c < tiles ? 1u << c : 0u;
+      for (int c = 0; c < C; ++c) bad |= has_byte_past(v.e[c]) && g * C + c < tiles ? 1u << c : 0u;
       const bool any_nan = __any(bad);
       uint32_t ve[C];
       if (any_nan) {
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
           ve[c] = v.e[c];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if (((ve[c] >> (8 * j)) & 255u) != KV4_NAN) continue;
+            if (((ve[c] >> (8 * j)) & 255u) < KV4_PAST) continue;
             v.e[c] &= ~(255u << (8 * j));
             (j & 1 ? v.w[c][j >> 1].z : v.w[c][j >> 1].x) = 0;
             (j & 1 ? v.w[c][j >> 1].w : v.w[c][j >> 1].y) = 0;
@@ -468,7 +468,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
         for (int d = 0; d < 4 * C; ++d) {
           bool hit = false;
 #pragma unroll 1
-          for (int key = 0; key < KEYS; ++key) hit |= (le[16 * key + d] == KV4_NAN) & (t0 + key >= lo) & (t0 + key < hi);
+          for (int key = 0; key < KEYS; ++key) hit |= (le[16 * key + d] >= KV4_PAST) & (t0 + key >= lo) & (t0 + key < hi);
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[d][e] = hit ? NAN : o[d][e];
         }
