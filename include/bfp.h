@@ -638,11 +638,11 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
  * carry at 2^-8 to 1 for the largest), may count as zero.  A scale that is not
  * finite in float32 is refused, one below 2^-150 leaves all scores alike.
  * A query with a NaN or an infinity in it makes its row NaN.  out: any type
- * (BFP_TILES: tile_quantize of the float32 result); it may be q, as y may be
- * x in bfp_rope_d.  work:
- * bfp_kv4_attn_work() bytes of device scratch, 16-byte aligned (NULL if that
- * is 0), whatever they hold; calls that may run at the same time need their
- * own. */
+ * (BFP_TILES: tile_quantize of the float32 result; tiles cannot hold a NaN, which
+ * is written as -2^127, mantissa -32768 and exponent 127); it may be q, as y may
+ * be x in bfp_rope_d.  work: bfp_kv4_attn_work() bytes of device scratch, 16-byte
+ * aligned (NULL if that is 0), whatever they hold; calls that may run at the
+ * same time need their own. */
 int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                    const bfp_rows *out, double scale, int window, void *work, size_t work_bytes,
                    void *stream);

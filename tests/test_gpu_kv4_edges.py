@@ -192,3 +192,37 @@ def test_any_byte_stays_with_those_who_see_it(gpu, lens, news, window, hd, group
                 if byte >= 253 and exps is s.cache.v_exp:
                     assert np.isnan(got[~apart]).all(), (p, tile, byte)
             exps[page, 0, tile, slot], data[page, 0, tile, slot] = old[0], old[1]
+
+
+@pytest.mark.parametrize("lens,news,hd,group", [([40, 7], [1, 1], 64, 2), ([5000, 7], [2, 1], 64, 2), ([300, 7], [1, 1], 256, 2),
+                                                ([900, 7], [600, 7], 64, 2), ([6000], [64], 64, 4), ([900], [800], 112, 3)])
+def test_what_tiles_cannot_hold(gpu, lens, news, hd, group):
+    """16-bit tiles have no NaN: such values are the most negative number
+    that they have, whoever joins the rows."""
+    import torch
+    s = Long(137, lens, news, 16, 1, hd)
+    n = s.rows
+
+    def tiles(q):
+        m = torch.empty(n, group, hd, dtype=torch.int16, device="cuda")
+        e = torch.empty(n, group, hd // 16, dtype=torch.int8, device="cuda")
+        s.cache.attend(s.batch, q, out=(m, e))
+        return m, e
+    for kind in ("f32", "bf16"):
+        q, _ = s.query(group, kind)
+        m, e = tiles(q)
+        for value, row in ((float("nan"), 0), (float("inf"), n - 1), (float("-inf"), n // 2)):
+            q2 = q.clone()
+            q2[row, 1, 3] = value
+            m2, e2 = tiles(q2)
+            wm, we = m.clone(), e.clone()
+            wm[row, 1], we[row, 1] = -32768, 127
+            assert torch.equal(m2, wm) and torch.equal(e2, we), (kind, value, row)
+    # a tile of a value that all rows of the last sequence see
+    b, tile = len(lens) - 1, hd // 16 - 1
+    s.cache.v_exp[int(s.table[b, 0]), 0, tile, 0] = 255
+    m2, e2 = tiles(q)
+    first = int(s.start[b])
+    wm, we = m.clone(), e.clone()
+    wm[first:, :, 16 * tile:], we[first:, :, tile] = -32768, 127
+    assert torch.equal(m2, wm) and torch.equal(e2, we)

@@ -193,7 +193,7 @@ class Fp4Cache(_rows.Fixed):
         heads in groups of neighbours.  Returns out -- a tensor, or a pair
         (m, e) of 16-bit tiles -- or a new tensor of dtype (q's; float32 for
         tiles) whose rows outside every sequence are undefined.  A row that
-        sees nothing is zero.  work: uint8 scratch of attend_work() bytes
+        sees nothing is zero; tiles hold a NaN as -2^127.  work: uint8 scratch of attend_work() bytes
         (allocated per call otherwise)."""
         dev = self.device
         t, qr, out, orow = self._attend_rows(batch, q, out, dtype)

@@ -178,6 +178,13 @@ __device__ __forceinline__ uint32_t byte_mask(uint32_t keep) {
   return (((keep & 1) | ((keep & 2) << 7) | ((keep & 4) << 14) | ((keep & 8) << 21)) * 255u);
 }
 
+// Tiles have no NaN and no infinity: -2^127 (mantissa -32768, exponent 127),
+// the largest magnitude they hold, stands for a NaN, so that whatever reads the
+// row sees that it is no result; infinities stand as far out as tiles go.
+__device__ __forceinline__ float tile_holds(float v) {
+  return fabsf(v) <= 0x1.fffffep127f ? v : v > 0.0f ? 0x1.fffffep127f : -0x1.fffffep127f;
+}
+
 // Value o of a finished row: one of 16 neighbouring lanes with neighbouring o.
 __device__ __forceinline__ void out_store(const bfp_rows &r, long long o, float v) {
   if (r.type != BFP_TILES) {
@@ -185,7 +192,7 @@ __device__ __forceinline__ void out_store(const bfp_rows &r, long long o, float 
     return;
   }
   int e;
-  const int m = quantize16_lanes((double)v, e);
+  const int m = quantize16_lanes((double)tile_holds(v), e);
   ((int16_t *)r.p)[o] = (int16_t)m;
   if ((threadIdx.x & 15) == 0) r.e[o >> 4] = (int8_t)e;
 }
@@ -201,12 +208,15 @@ __device__ __forceinline__ void out_store8(const bfp_rows &r, long long o, const
     }
     return;
   }
-  float top = 0.0f;
+  float x[8], top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+  for (int i = 0; i < 8; ++i) {
+    x[i] = tile_holds(v[i]);
+    top = fmaxf(top, fabsf(x[i]));
+  }
   const int e = tile_exp_of((double)fmaxf(top, __shfl_xor(top, 1, 64)));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ((int16_t *)r.p)[o + i] = (int16_t)tile_mant_of((double)v[i], e);
+  for (int i = 0; i < 8; ++i) ((int16_t *)r.p)[o + i] = (int16_t)tile_mant_of((double)x[i], e);
   if (!(threadIdx.x & 1)) r.e[o >> 4] = (int8_t)e;
 }
 
