@@ -226,3 +226,22 @@ def test_what_tiles_cannot_hold(gpu, lens, news, hd, group):
     wm, we = m.clone(), e.clone()
     wm[first:, :, 16 * tile:], we[first:, :, tile] = -32768, 127
     assert torch.equal(m2, wm) and torch.equal(e2, we)
+
+
+def test_one_term_probabilities_and_their_sum(gpu):
+    """Where probabilities go into the product rounded to bfloat16, their
+    sum takes them rounded too.  In every 64 keys one has the largest score,
+    the others a probability that rounds up by nearly half a step: a sum of
+    unrounded ones would leave the results 2^-8 too large."""
+    k0 = np.where(np.arange(512) % 64 == 5, 0.0, -1.0)
+    v = np.full(512, 2.0)
+    v[[1, 90, 200, 300, 400, 511]] = 1.5
+    s = Few(k0, v)
+    scale = -np.log(0.5 + 2.0 ** -9 + 2.0 ** -13)
+    q, q0 = s.query(np.ones((1, 16)), "bf16")
+    want, _, _ = s.want(q0, scale)
+    got = s.cache.attend(s.batch, q, scale=scale).double().cpu().numpy()
+    assert 1.993 < want.min() and want.max() < 1.996
+    # half a bfloat16 step of a result in [1, 2); one key in 64 (3% of the weight) is not rounded up as the
+    # others are, by 2^-8, which moves the mean by 0.03 * 2^-8 of the values' spread of 0.5 at most
+    assert (np.abs(got - want[..., None]) <= 2.0 ** -8 + 2.0 ** -14).all(), np.abs(got - want[..., None]).max()

@@ -403,10 +403,16 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float p = __builtin_amdgcn_exp2f(fmaf(s[2 * jp + jj][e], a.scale2, m0));
-            sum += p;
+            if (T > 1) sum += p;
             pv[4 * jj + e] = p;
           }
         pb[jp] = pack_terms<T>(pv, t);
+        if constexpr (T == 1) {   // the sum takes the probabilities as the product takes them
+#pragma unroll
+          for (int e = 0; e < 8; e += 2)
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, bf16x2{pb[jp][e], pb[jp][e + 1]}), s16x2{0x3f80, 0x3f80},
+                                                  sum, false);
+        }
       }
 
       // A tile of V that holds a NaN counts as zeros in the product, so that it
