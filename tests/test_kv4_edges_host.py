@@ -187,3 +187,13 @@ def test_scales_past_float32():
     r = C.byref(_rows(L))
     for scale in (1e300, -1e300, 3e38, float("inf"), float("nan")):
         assert "scale" in _refused(L, "bfp_kv4_attn_d", c, b, r, r, scale, 0, None, 0, None)
+
+
+def test_scratch_does_not_grow_with_rows_that_no_sequence_has():
+    """Row arrays that hold room for more: the scratch is the sequences'."""
+    L = _lib()
+    for news, heads, width in ((64, 4, 4000), (1, 3, 4000), (300, 4, 1000), (500, 1, 4000)):
+        c, r = C.byref(_cache(L, heads=1)), _rows(L, heads=heads)
+        sizes = [L.lib().bfp_kv4_attn_work(c, C.byref(_batch(L, n_seq=1, n_rows=n, width=width, max_q=news)), C.byref(r), C.byref(r), 0)
+                 for n in (news, 4 * news, 1 << 20)]
+        assert sizes[0] > 0 and len(set(sizes)) == 1, sizes

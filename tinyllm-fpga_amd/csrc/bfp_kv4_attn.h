@@ -53,7 +53,7 @@ struct Kv4AttnArgs {
   float slack;         // M_SLACK in scores: M_SLACK / scale2, above the score that raises the maximum
   float q_sign;        // the scale's sign, or 0, which the queries take
   // unfinished rows: the sums, and (maximum, sum of probabilities)
-  float *part_o;       // k_kv4_prompt [row][query head][split][hd]; k_kv4_rows [slot][R][hd]
+  float *part_o;       // k_kv4_prompt [sequence][row of max_q][query head][split][hd]; k_kv4_rows [slot][R][hd]
   float2 *part_ml;     // without [hd]
   unsigned long long *there, number;   // k_kv4_rows: which slots are filled, and this call's number
 };

@@ -99,7 +99,7 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
     if (s > 1) {
       p.splits = (int)s;
       p.chunk = (int)((key_tiles + s - 1) / s);
-      p.cells = (size_t)b.n_rows * q.heads * p.splits;
+      p.cells = (size_t)b.n_seq * b.max_q * q.heads * p.splits;   // at most 256 row tiles
     }
     const double work = (double)all_rows / (32 * p.waves) * p.splits, rounds = work < cus ? 1.0 : work / cus;
     p.us = rounds * (itself[size] + (p.terms == 3 ? 1.8 : 0.0) + tile[size] * (p.splits > 1 ? p.chunk : seen)) + (p.splits > 1 ? 5.0 : 0.0);

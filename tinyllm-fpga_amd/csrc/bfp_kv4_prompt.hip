@@ -308,8 +308,8 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
     const int ri = (int)a.by_group.div((uint32_t)(live[k] ? rr0 + row : 0), rg), rh = head * G + (int)rg;
     const long long tok = sp.row0 + ri;
     const float L = ml[32 + row];
-    if (a.splits > 1) {
-      const long long at = (tok * a.q.heads + rh) * a.splits + split;
+    if (a.splits > 1) {   // by the row's place in its sequence: the scratch holds no more than they have
+      const long long at = (((long long)seq * a.b.max_q + ri) * a.q.heads + rh) * a.splits + split;
       if (live[k] && piece == 0) a.part_ml[at] = make_float2(ml[row], L);
       to[k] = at * hd;
       over[k] = 1.0f;
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(256) void k_kv4_join_prompt(Kv4AttnArgs a) {
   const int u = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int i = u / a.q.heads, qh = u % a.q.heads;
   if (i >= sp.n) return;
-  const long long tok = sp.row0 + i, at = (tok * a.q.heads + qh) * a.splits;
+  const long long tok = sp.row0 + i, at = (((long long)seq * a.b.max_q + i) * a.q.heads + qh) * a.splits;
   const int hd = 16 * a.tiles;
   // lane k holds split k's maximum and sum (at most 64 splits)
   const float2 ml = lane < a.splits ? a.part_ml[at + lane] : make_float2(-INFINITY, 0.0f);
