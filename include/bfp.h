@@ -646,8 +646,8 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
 int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                    const bfp_rows *out, double scale, int window, void *work, size_t work_bytes,
                    void *stream);
-/* Scratch bytes bfp_kv4_attn_d needs for these arguments (0: none, or
- * arguments that it refuses). */
+/* Scratch bytes bfp_kv4_attn_d needs for these arguments, wherever q and out
+ * lie (0: none, or arguments that it refuses). */
 size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                          const bfp_rows *out, int window);
 

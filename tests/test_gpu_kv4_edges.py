@@ -245,3 +245,14 @@ def test_one_term_probabilities_and_their_sum(gpu):
     # half a bfloat16 step of a result in [1, 2); one key in 64 (3% of the weight) is not rounded up as the
     # others are, by 2^-8, which moves the mean by 0.03 * 2^-8 of the values' spread of 0.5 at most
     assert (np.abs(got - want[..., None]) <= 2.0 ** -8 + 2.0 ** -14).all(), np.abs(got - want[..., None]).max()
+
+
+def test_scratch_size_allocates_nothing(gpu):
+    import torch
+    s = Long(163, [9000], [1], 64, 2, 64)
+    q = torch.zeros(1, 6, 64, device="cuda").expand(1 << 15, 6, 64)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    assert s.cache.attend_work(s.batch, q) > 0
+    assert torch.cuda.max_memory_allocated() == before

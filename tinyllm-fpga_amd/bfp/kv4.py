@@ -213,14 +213,14 @@ class Fp4Cache(_rows.Fixed):
                 work.data_ptr() if work is not None else None, size)
         return out
 
-    def _attend_rows(self, batch, q, out, dtype):
+    def _attend_rows(self, batch, q, out, dtype, make=True):
         t = self._values(batch, q, "q")
         heads = t.shape[1]
         if heads % self.heads or not heads:
             raise ValueError(f"{heads} query heads for {self.heads} KV heads")
         qr = _rows.rows(q, "q", self.device)
         if out is None:
-            out, orow = _rows.new(q, t, dtype)
+            out, orow = _rows.new(q, t, dtype) if make else _rows.like(q, t, dtype)
         else:
             if self._values(batch, out, "out").shape != t.shape:
                 raise ValueError(f"out must be {tuple(t.shape)}")
@@ -231,5 +231,6 @@ class Fp4Cache(_rows.Fixed):
 
     def attend_work(self, batch, q, out=None, dtype=None, window=0):
         """Scratch bytes attend() needs for such a call."""
-        t, qr, out, orow = self._attend_rows(batch, q, out, dtype)
+        t, qr, _, orow = self._attend_rows(batch, q, out, dtype, make=False)
+        orow.p = orow.p or 16   # the size depends on no address
         return lib().bfp_kv4_attn_work(self._c, batch._c(t.shape[0]), C.byref(qr), C.byref(orow), _window(window))

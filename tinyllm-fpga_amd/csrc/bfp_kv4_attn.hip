@@ -121,7 +121,7 @@ static unsigned long long call_number() {
 }
 
 static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
-                      const bfp_rows *out, int window) {
+                      const bfp_rows *out, int window, bool placed) {
   BFP_TRY(check_kv4(op, cache, batch));
   if (!q || q->heads < cache->heads || q->heads % cache->heads || q->heads > 65536)
     return set_err(BFP_EINVAL, "%s: q has %d heads, the cache %d", op, q ? q->heads : 0, cache->heads);
@@ -129,7 +129,7 @@ static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch 
   BFP_TRY(check_out(op, "out", out, q->heads, cache->hd, true, batch->n_rows));
   if (!rows_aligned(*q, 8, batch->n_rows)) return set_err(BFP_EINVAL, "%s: q needs 16-byte alignment and strides in multiples of 8", op);
   // out may be q: a workgroup has read its rows' queries before anyone writes their results
-  BFP_TRY(check_apart(op, "out", *out, "q", *q, batch->n_rows, cache->hd, true));
+  if (placed) BFP_TRY(check_apart(op, "out", *out, "q", *q, batch->n_rows, cache->hd, true));
   if (window < 0) return set_err(BFP_EINVAL, "%s: window=%d", op, window);
   if ((long long)batch->max_q * (q->heads / cache->heads) > 0x3fffffffLL)
     return set_err(BFP_EINVAL, "%s: max_q=%d rows of %d heads are too many", op, batch->max_q, q->heads);
@@ -144,7 +144,7 @@ extern "C" {
 
 size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                          const bfp_rows *out, int window) {
-  if (check_attn("kv4_attn_work", cache, batch, q, out, window)) return 0;
+  if (check_attn("kv4_attn_work", cache, batch, q, out, window, false)) return 0;
   return plan_attn(*cache, *batch, *q, *out, window).work;
 }
 
@@ -152,7 +152,7 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
                    const bfp_rows *out, double scale, int window, void *work, size_t work_bytes,
                    void *stream) {
   const char *op = "kv4_attn";
-  BFP_TRY(check_attn(op, cache, batch, q, out, window));
+  BFP_TRY(check_attn(op, cache, batch, q, out, window, true));
   const float scale2 = (float)(fabs(scale) * 1.44269504088896340736);
   if (!isfinite(scale2)) return set_err(BFP_EINVAL, "%s: scale=%g is not float32's", op, scale);
   if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
