@@ -599,10 +599,10 @@ typedef struct bfp_kv4 {
  * pages[b*width + p/page] at slot p % page.  start (n_seq + 1, ascending), len
  * (n_seq) and pages are device arrays of int32.  max_q: no sequence has more
  * new rows; max_len: no sequence is longer (0: width * page) -- it only
- * chooses how the work is split.  n_rows bounds the row arrays.  A row whose
- * position is negative (more rows than len) or whose page is outside
- * [0, n_pages) has no slot.  Rows outside every sequence are left as they
- * were. */
+ * chooses how the work is split.  width * page is at most 2^31 - 2^16.  n_rows
+ * bounds the row arrays.  A row whose position is negative (more rows than
+ * len) or whose page is outside [0, n_pages) has no slot.  Rows outside every
+ * sequence are left as they were. */
 typedef struct bfp_kv4_batch {
   const int32_t *pages, *start, *len;
   int n_seq, n_rows, width, max_q, max_len;

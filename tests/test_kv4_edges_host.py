@@ -197,3 +197,17 @@ def test_scratch_does_not_grow_with_rows_that_no_sequence_has():
         sizes = [L.lib().bfp_kv4_attn_work(c, C.byref(_batch(L, n_seq=1, n_rows=n, width=width, max_q=news)), C.byref(r), C.byref(r), 0)
                  for n in (news, 4 * news, 1 << 20)]
         assert sizes[0] > 0 and len(set(sizes)) == 1, sizes
+
+
+def test_positions_past_31_bits():
+    """A table of pages for more positions than an int counts."""
+    L = _lib()
+    r = _rows(L)
+    for width, page in ((1 << 23, 256), ((1 << 27) - 1, 16), ((1 << 31) - 1, 16)):
+        c, b = C.byref(_cache(L, page=page)), C.byref(_batch(L, width=width))
+        k = C.byref(r)
+        assert "positions" in _refused(L, "bfp_kv4_append_d", c, b, k, k, None, None, None, None, 0, 0, 0, None)
+        assert "positions" in _refused(L, "bfp_kv4_read_d", c, b, k, None, None)
+        assert "positions" in _refused(L, "bfp_kv4_attn_d", c, b, k, k, 1.0, 0, None, 0, None)
+    c, b = C.byref(_cache(L, page=256)), C.byref(_batch(L, width=(1 << 23) - 256, max_q=0))
+    assert L.lib().bfp_kv4_attn_d(c, b, C.byref(r), C.byref(r), 1.0, 0, None, 0, None) == 0

@@ -28,6 +28,7 @@ constexpr int KV4_BIAS = 127, KV4_NAN = 255;
 // not see it.
 constexpr int KV4_PAST = 253;
 constexpr int KV4_TILE_BYTES = 8;
+constexpr int KV4_MAX_POS = 0x7fff0000;   // that a table of pages has room for
 
 // The rows of a sequence in a batch, clamped to what the row arrays hold:
 // rows row0 .. row0 + n - 1, row i at position at + i (which may be negative, or

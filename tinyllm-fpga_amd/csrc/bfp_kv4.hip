@@ -26,6 +26,9 @@ int check_kv4(const char *op, const bfp_kv4 *c, const bfp_kv4_batch *b) {
   if (b->n_seq < 0 || b->n_seq > 65535 || b->n_rows < 0 || b->width < 1 || b->max_q < 0 || b->max_len < 0)
     return set_err(BFP_EINVAL, "%s: n_seq=%d (at most 65535), n_rows=%d, width=%d, max_q=%d, max_len=%d",
                    op, b->n_seq, b->n_rows, b->width, b->max_q, b->max_len);
+  // positions, and the keys of the tiles that begin before the last one, are ints
+  if ((long long)b->width * c->page > KV4_MAX_POS)
+    return set_err(BFP_EINVAL, "%s: width=%d pages of %d are more than %d positions", op, b->width, c->page, KV4_MAX_POS);
   if (b->n_seq > 0 && (!b->pages || !b->start || !b->len))
     return set_err(BFP_EINVAL, "%s: the batch's arrays are null", op);
   if (((uintptr_t)b->pages | (uintptr_t)b->start | (uintptr_t)b->len) % 4)
