@@ -256,3 +256,64 @@ def test_scratch_size_allocates_nothing(gpu):
     before = torch.cuda.memory_allocated()
     assert s.cache.attend_work(s.batch, q) > 0
     assert torch.cuda.max_memory_allocated() == before
+
+
+LARGE = [  # rows, heads, hd, rot, type in, type out, heads beside them
+    (2000, 33, 64, 64, "bf16", "bf16", 0), (2000, 33, 64, 64, "f32", "f32", 3), (1500, 33, 128, 64, "f16", "f16", 2),
+    (1500, 33, 128, 64, "f32", "bf16", 1), (2100, 33, 64, 32, "bf16", "f32", 5), (4200, 17, 64, 64, "tile", "f32", 0),
+    (4200, 17, 64, 32, "tile", "f16", 2), (8200, 8, 64, 64, "f16", "bf16", 0)]
+
+
+def _large(seed, rows, heads, hd, kind, extra):
+    """Rows inside wider ones and the values they hold."""
+    import torch
+    from bfp import api
+    v = np.random.default_rng(seed).standard_normal((rows, heads + extra, hd)).astype(np.float32)
+    if kind == "tile":
+        m, e = api.tile_quantize(v.astype(np.float64).reshape(-1))
+        m, e = np.asarray(m, np.int16).reshape(v.shape), np.asarray(e, np.int8).reshape(*v.shape[:2], hd // 16)
+        held = m * np.repeat(2.0 ** (e.astype(float) - 15), 16, -1)
+        return tuple(torch.from_numpy(np.ascontiguousarray(x)).cuda()[:, :heads] for x in (m, e)), held[:, :heads]
+    t = torch.from_numpy(v).to(_dt(kind))
+    return t.cuda()[:, :heads], t.double().numpy()[:, :heads]
+
+
+def _rotated(got, want, name):
+    # a float32 result is rounded once; a 16-bit one comes from a float32 value at most two steps off
+    tiny = {"f32": 2.0 ** -149, "bf16": 2.0 ** -133, "f16": 2.0 ** -24}[name] / 2
+    slack = 0 if name == "f32" else 2.0 ** -22
+    return (np.abs(got.double().cpu().numpy() - want) <= (HALF[name] + slack) * np.abs(want) + 2.0 ** -49 + tiny).all()
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("case", LARGE, ids=str)
+def test_rotations_of_many_rows(gpu, case, inter):
+    """Calls of 262144 units and more, where a thread turns two heads: odd
+    head counts leave the last one alone; into new rows, into joined ones
+    and, with the new keys' append, beside the cache."""
+    import torch
+    from bfp import rotary
+    rows, heads, hd, rot, kind, out_kind, extra = case
+    x, val = _large(rows + rot, rows, heads, hd, kind, extra)
+    n_pos = 3000
+    table = ref.angles(n_pos, rot).astype(np.float32)
+    dev = torch.from_numpy(table).cuda()
+    pos = np.random.default_rng(9).integers(0, n_pos, rows)
+    want = ref.rotate(val, pos, table, inter)
+    per_head = rot // (8 if inter else 16) + (hd - rot) // 8
+    assert rows * heads * per_head >= 2 * 256 * 8 * 64      # the line above which two heads go together
+    _say(case, inter)
+    assert _rotated(rotary.rope(x, _int(pos), dev, interleaved=inter, dtype=_dt(out_kind)), want, out_kind)
+    joined = torch.full((rows, heads + 3, hd), 7.0, device="cuda", dtype=_dt(out_kind))
+    rotary.rope(x, _int(pos), dev, interleaved=inter, out=joined[:, 1:1 + heads])
+    assert _rotated(joined[:, 1:1 + heads], want, out_kind)
+    assert (joined[:, 0] == 7).all() and (joined[:, 1 + heads:] == 7).all()
+    # queries with the append: sequences of ragged lengths, at the given positions
+    cut = rows // 3
+    s = Long(167, [cut, rows - cut - 2], [cut, rows - cut], 64, 1, hd)      # two rows without a slot: zeros
+    k = torch.randn(rows, 1, hd, device="cuda")
+    joined.fill_(7.0)
+    s.cache.append(s.batch, k, k, dev, interleaved=inter, pos=_int(pos), q=x, q_out=joined[:, 2:2 + heads])
+    want[cut:cut + 2] = 0
+    assert _rotated(joined[:, 2:2 + heads], want, out_kind)
+    assert (joined[:, :2] == 7).all() and (joined[:, 2 + heads:] == 7).all()
