@@ -317,3 +317,29 @@ def test_rotations_of_many_rows(gpu, case, inter):
     want[cut:cut + 2] = 0
     assert _rotated(joined[:, 2:2 + heads], want, out_kind)
     assert (joined[:, :2] == 7).all() and (joined[:, 2 + heads:] == 7).all()
+
+
+def test_few_rows_carry_probabilities_in_two_terms(gpu):
+    """bfloat16 calls of up to 8 rows a KV head: two kinds of keys whose
+    probabilities differ by 2^-10, which one bfloat16 does not hold, and
+    whose values cancel."""
+    n = 128
+    s = Few(np.where(np.arange(n) % 2, -1.0, 0.0), np.where(np.arange(n) % 2, -1.0, 1.0))
+    for group in (1, 3, 8):
+        q, q0 = s.query(np.ones((1, group)), "bf16")
+        want, weight, big = s.want(q0, 2.0 ** -10)
+        got = s.cache.attend(s.batch, q, scale=2.0 ** -10).double().cpu().numpy()
+        bound = ref.attend_bound(want[..., None], weight[..., None], big, n, 1, HALF["bf16"], 2.0 ** -16)
+        assert (bound < np.abs(want[..., None]) / 2).all()
+        assert (np.abs(got - want[..., None]) <= bound).all(), (group, np.abs(got - want[..., None]).max())
+
+
+@pytest.mark.parametrize("lens,news,page,heads,hd,group", [([1, 0, 2, 15, 16, 17], [1, 0, 1, 1, 1, 1], 16, 3, 64, 3), ([300, 555], [1, 1], 64, 2, 128, 8),
+                                                           ([2000], [1], 16, 3, 64, 3), ([40, 7, 130], [4, 2, 3], 16, 2, 64, 2)])
+def test_few_rows_within_two_terms(gpu, lens, news, page, heads, hd, group):
+    """The bound of two terms on ordinary calls of few rows."""
+    from test_gpu_kv4 import Setup, _typed, check
+    s = Setup(59, lens, news, page, heads, hd)
+    q, qv = _typed(s.rng.standard_normal((s.rows, heads * group, hd)) * 2, "bf16")
+    assert max(news) * group <= 8
+    check(s, q, qv, "bf16", "bf16", got=s.cache.attend(s.batch, q), max_p=2.0 ** -16)
