@@ -36,9 +36,10 @@ class Batch(_rows.Fixed):
     them at position lens[b] - 1; position p lies in page pages[b, p // page].
     pages (sequences, width), start (sequences + 1) and lens are int32 tensors
     on the device; they are read when a call runs, so a program may write new
-    values into them (but not put other tensors in their place).  max_q: the most new rows a sequence has; max_len: the
-    longest sequence (0: the table's width), which only chooses how the work
-    is split."""
+    values into them (batch.lens += 1, but not put other tensors in their
+    place).  max_q: the most new rows a sequence has; max_len: the longest
+    sequence (0: the table's width), which only chooses how the work is
+    split."""
 
     def __init__(self, pages, start, lens, max_q, max_len=0):
         if pages.dim() != 2 or pages.shape[1] < 1:
@@ -193,7 +194,9 @@ class Fp4Cache(_rows.Fixed):
         heads in groups of neighbours.  Returns out -- a tensor, or a pair
         (m, e) of 16-bit tiles -- or a new tensor of dtype (q's; float32 for
         tiles) whose rows outside every sequence are undefined.  A row that
-        sees nothing is zero; tiles hold a NaN as -2^127.  work: uint8 scratch of attend_work() bytes
+        sees nothing is zero; tiles hold a NaN as -2^127.  Probabilities are
+        carried to at least the result's precision: bfloat16 calls of many
+        rows round them to bfloat16, dtype=torch.float32 keeps them whole.  work: uint8 scratch of attend_work() bytes
         (allocated per call otherwise)."""
         dev = self.device
         t, qr, out, orow = self._attend_rows(batch, q, out, dtype)

@@ -24,10 +24,17 @@ struct Kv4Plan {
   double us;
 };
 
-// The terms a row is carried in: one where queries, probabilities and results
-// are bfloat16 and the rows fill the tile's 16 columns anyway; two hold a
-// float16 or 16-bit-tile query and leave probabilities 2^-18 off; three
-// (of four places) hold float32 queries and results.
+// The terms a row is carried in: three (of four places) hold float32 queries
+// and results; two hold a float16 or 16-bit-tile query and leave probabilities
+// 2^-16 off (cut, then rounded; k_kv4_prompt rounds both, 2^-17).  One, for
+// bfloat16 queries and results of more than 8 rows, rounds probabilities to
+// bfloat16 as the result is: a second term would need a second row tile (8
+// documents of 131072 tokens with 4 new ones, 16 rows a KV head: 158 us; 32
+// rows, two tiles: 250).  Prompts
+// the same: two prompts of 8192 with 32 heads of 128 take 811 us in one term and
+// 1250 in two (float16), with a relative error against 64 bits of 0.0021 where
+// float32 probabilities leave 0.0016, the result's own rounding.  float32
+// results carry all of them.
 static int terms_of(const bfp_rows &q, const bfp_rows &out, int rows) {
   if (q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES) return 4;
   return q.type == BFP_BF16 && out.type == BFP_BF16 && rows > 8 ? 1 : 2;
