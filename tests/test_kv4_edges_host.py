@@ -27,6 +27,21 @@ def test_in_place_forms_put_back_the_same_object():
     assert t.lens is lens and lens.tolist() == [8, 10]
 
 
+def test_what_a_struct_points_to_cannot_be_taken_away():
+    """Else another object could take its name, while the struct points to
+    the first one's memory."""
+    from bfp._rows import Fixed
+
+    class Thing(Fixed):
+        def __init__(self):
+            self.lens, self._n = [1], 2
+    t = Thing()
+    with pytest.raises(AttributeError):
+        del t.lens
+    del t._n
+    assert t.lens == [1]
+
+
 OVERLAP = [  # heads, hd, rows, row stride, head stride, whether two rows share a value
     (2, 64, 4, 128, 64, False), (2, 64, 4, 64, 64, True), (2, 64, 4, 127, 64, True), (2, 64, 4, 64, 256, False),   # heads before rows
     (2, 64, 4, 64, 255, True), (3, 64, 2, 320, 128, False), (3, 64, 2, 192, 128, False), (3, 64, 2, 128, 192, False),

@@ -145,6 +145,11 @@ class Fixed:
             raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: write into it, or make a new object")
         object.__setattr__(self, name, value)
 
+    def __delattr__(self, name):
+        if name[0] != "_":
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be taken away")
+        object.__delattr__(self, name)
+
 
 class Entry:
     """A stream-ordered entry point: called with the device its tensors are
