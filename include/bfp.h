@@ -572,8 +572,8 @@ int bfp_rope_table_d(const double *inv_freq, int n_freq, double mscale, long lon
  * (interleaved 0, as rope_fp pairs them) or (2j, 2j + 1) (interleaved 1).
  * x and y: n_rows rows, the same number of heads; y BFP_F32, BFP_BF16 or
  * BFP_F16; y may be x (the same place and strides, values of the same size),
- * and shares no memory with it otherwise.  pos: n_rows positions; a row whose position is
- * outside [0, n_pos) gets NaN in its rotated part. */
+ * and shares no memory with it otherwise.  pos: n_rows positions; a row whose
+ * position is outside [0, n_pos) gets NaN in its rotated part. */
 int bfp_rope_d(const bfp_rows *x, int n_rows, int hd, const int32_t *pos, const float *table,
                int n_pos, int rot, int interleaved, const bfp_rows *y, void *stream);
 
@@ -630,19 +630,20 @@ int bfp_kv4_read_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
  * its own sequence; query head h reads KV head h / (q->heads / heads).
  * Positions whose page is outside [0, n_pages) are not seen; a row that sees
  * nothing gives zeros.  What a row does not see does not reach it, whatever
- * its bytes; a row that sees a tile of v whose exponent byte is 253 or more gets
- * NaN there (bytes that append does not write: 0..26 and 228..254).  Products are exact, sums and softmax in float32, probabilities
- * carried to at least the output's precision.  q.k and scale q.k have to stay
- * below 2^126, and the sum of the |v| that a row sees has to fit float32;
- * products below 2^-126, of q_d k_d or of v and a probability (which the kernels
- * carry at 2^-8 to 1 for the largest), may count as zero.  A scale that is not
- * finite in float32 is refused, one below 2^-150 leaves all scores alike.
- * A query with a NaN or an infinity in it makes its row NaN.  out: any type
- * (BFP_TILES: tile_quantize of the float32 result; tiles cannot hold a NaN, which
- * is written as -2^127, mantissa -32768 and exponent 127); it may be q, as y may
- * be x in bfp_rope_d.  work: bfp_kv4_attn_work() bytes of device scratch, 16-byte
- * aligned (NULL if that is 0), whatever they hold; calls that may run at the
- * same time need their own. */
+ * its bytes; a row that sees a tile of v whose exponent byte is 253 or more
+ * gets NaN there (append writes 27..227 and 255).  Products are exact, sums
+ * and softmax in float32, probabilities carried to at least the output's
+ * precision.  q.k and scale q.k have to stay below 2^126, and the sum of the
+ * |v| that a row sees has to fit float32; products below 2^-126, of q_d k_d or
+ * of v and a probability (which the kernels carry at 2^-8 to 1 for the
+ * largest), may count as zero.  A scale that is not finite in float32 is
+ * refused, one below 2^-150 leaves all scores alike.  A query with a NaN or an
+ * infinity in it makes its row NaN.  out: any type (BFP_TILES: tile_quantize
+ * of the float32 result; tiles cannot hold a NaN, which is written as -2^127,
+ * mantissa -32768 and exponent 127); it may be q, as y may be x in bfp_rope_d.
+ * work: bfp_kv4_attn_work() bytes of device scratch, 16-byte aligned (NULL if
+ * that is 0), whatever they hold; calls that may run at the same time need
+ * their own. */
 int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                    const bfp_rows *out, double scale, int window, void *work, size_t work_bytes,
                    void *stream);

@@ -68,17 +68,6 @@ def _tiles(x, what, device):
 
 
 def like(x, t, dtype):
-    """The type of results of dtype for x, whose values are t (None: x's;
-    float32 for tiles), and the RowsC of contiguous ones where t lies."""
-    if dtype is None:
-        dtype = t.dtype if t is x else torch.float32
-    elif dtype not in TYPES:
-        raise ValueError(f"results are float32, bfloat16 or float16, not {dtype}")
-    _, heads, hd = t.shape
-    return dtype, RowsC(t.data_ptr(), None, TYPES[dtype], heads, heads * hd, hd)
-
-
-def like(x, t, dtype):
     """Results of dtype for x, whose values are t (None: x's type; float32
     for tiles), that lie nowhere yet: the type, and the RowsC of contiguous
     ones without their address."""

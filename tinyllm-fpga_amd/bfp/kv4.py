@@ -196,8 +196,9 @@ class Fp4Cache(_rows.Fixed):
         tiles) whose rows outside every sequence are undefined.  A row that
         sees nothing is zero; tiles hold a NaN as -2^127.  Probabilities are
         carried to at least the result's precision: bfloat16 calls of many
-        rows round them to bfloat16, dtype=torch.float32 keeps them whole.  work: uint8 scratch of attend_work() bytes
-        (allocated per call otherwise)."""
+        rows round them to bfloat16, dtype=torch.float32 keeps them whole.
+        work: uint8 scratch of attend_work() bytes (allocated per call
+        otherwise)."""
         dev = self.device
         t, qr, out, orow = self._attend_rows(batch, q, out, dtype)
         n = t.shape[0]

@@ -17,9 +17,8 @@ constexpr int KEYS = 64;             // keys a wave takes at a time
 // The running maximum is raised only when a score passes it, and then to this
 // many powers of two above the score: the sums are rescaled a few times in a
 // whole context instead of whenever a new maximum turns up.  No probability
-// passes 1, so a sum of n values stays below n of the largest; the largest is
-// at least 2^-8 where it was set, and none is worse off for that (a float has
-// no fewer bits there, and those below 2^-126 are lost to the sum anyway).
+// passes 1, so a sum of n values stays below n times the largest; the largest
+// probability is 2^-8 where the maximum was set, which a float holds as well.
 constexpr float M_SLACK = 8.0f;
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));

@@ -30,11 +30,10 @@ struct Kv4Plan {
 // bfloat16 queries and results of more than 8 rows, rounds probabilities to
 // bfloat16 as the result is: a second term would need a second row tile (8
 // documents of 131072 tokens with 4 new ones, 16 rows a KV head: 158 us; 32
-// rows, two tiles: 250).  Prompts
-// the same: two prompts of 8192 with 32 heads of 128 take 811 us in one term and
-// 1250 in two (float16), with a relative error against 64 bits of 0.0021 where
-// float32 probabilities leave 0.0016, the result's own rounding.  float32
-// results carry all of them.
+// rows, two tiles: 250).  Prompts the same: two of 8192 tokens with 32 heads of
+// 128 take 811 us in one term and 1250 in two (float16), with a relative error
+// against 64 bits of 0.0021 where float32 probabilities leave 0.0016, the
+// result's own rounding.  float32 results carry all of them.
 static int terms_of(const bfp_rows &q, const bfp_rows &out, int rows) {
   if (q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES) return 4;
   return q.type == BFP_BF16 && out.type == BFP_BF16 && rows > 8 ? 1 : 2;

@@ -22,7 +22,8 @@ struct RopeFreqs {
 // sin and cos in float64 for results that are rounded to float32: x less k
 // quarter turns (pi/2 in two parts: off by 2^-53 for k up to 2^31), then the
 // power series at |r| <= pi/4, cut where its next term is below 2^-63 (sine)
-// and 2^-58 (cosine), far below half a step of the float32 they become.  A third of the library's work, which also serves larger arguments: 131072
+// and 2^-58 (cosine), far below half a step of the float32 they become.  A
+// third of the library's work, which also serves larger arguments: 131072
 // positions of 64 frequencies 22.4 -> 18.6 us.
 __device__ __forceinline__ void sin_cos(double x, double &s, double &c) {
   if (!(fabs(x) <= 0x1p31)) {   // frequencies above one

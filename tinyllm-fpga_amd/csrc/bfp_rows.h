@@ -88,17 +88,18 @@ inline int check_out(const char *op, const char *what, const bfp_rows *r, int he
   return BFP_OK;
 }
 
-// Rows in bytes: n rows s apart of m heads t apart, each w bytes from p on.
+// Rows in bytes: n rows s apart of m heads t apart, each w bytes from p on
+// (0 apart where there is one).
 struct RowPlaces {
   long long p, s, t, n, m, w;
 };
 inline RowPlaces row_places(const bfp_rows &r, long long n_rows, int hd, bool exponents) {
-  const long long size = r.type == BFP_F32 ? 4 : 2;
-  if (exponents) return {(long long)(uintptr_t)r.e, r.row_stride / 16, r.head_stride / 16, n_rows, r.heads, hd / 16};
-  return {(long long)(uintptr_t)r.p, r.row_stride * size, r.head_stride * size, n_rows, r.heads, hd * size};
+  const long long size = r.type == BFP_F32 ? 4 : 2, s = n_rows > 1 ? r.row_stride : 0, t = r.heads > 1 ? r.head_stride : 0;
+  if (exponents) return {(long long)(uintptr_t)r.e, s / 16, t / 16, n_rows, r.heads, hd / 16};
+  return {(long long)(uintptr_t)r.p, s * size, t * size, n_rows, r.heads, hd * size};
 }
 inline bool same_places(const RowPlaces &a, const RowPlaces &b) {
-  return a.p == b.p && a.m == b.m && a.w == b.w && (a.n <= 1 || a.s == b.s) && (a.m <= 1 || a.t == b.t);
+  return a.p == b.p && a.m == b.m && a.w == b.w && a.s == b.s && a.t == b.t;
 }
 
 // Whether a byte lies in both.  Exact where the rows are equally far apart,
