@@ -652,6 +652,63 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
 size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                          const bfp_rows *out, int window);
 
+/* The pages of one or several caches that share their tables (a model's
+ * layers): refs[p] says how many entries of the tables hold page p, and a page
+ * is free where that is 0.  Free pages are given lowest number first, in the
+ * order of the tables' entries.
+ *   refs      n_pages int32 on the device, 16-byte aligned; the calls change it
+ *   n_short   one int32 on the device (or NULL), raised by the number of pages
+ *             that were asked for and not there
+ *   arrays    n_arrays arrays on the device whose pages go together: page p is
+ *             the `bytes` bytes from p + p * bytes on (16-byte aligned,
+ *             multiples of 16 bytes).  The list itself is the host's, read
+ *             during the call.
+ * Tables are device arrays of int32; an entry outside [0, n_pages) holds no
+ * page.  work: bfp_pages_work() bytes of device scratch, 16-byte aligned,
+ * whatever they hold.  No two of a call's arrays may share memory. */
+typedef struct bfp_page_array {
+  uint8_t *p;
+  long long bytes;
+} bfp_page_array;
+typedef struct bfp_pages {
+  int32_t *refs, *n_short;
+  const bfp_page_array *arrays;
+  int n_pages, page, n_arrays;
+} bfp_pages;
+typedef struct bfp_page_table {
+  int32_t *pages;
+  long long n;
+} bfp_page_table;
+/* Scratch bytes of bfp_pages_fork_d for n children; the other calls need those
+ * for none (0: a pool that they refuse). */
+size_t bfp_pages_work(const bfp_pages *pool, int n);
+/* Page src[i] of every array to page dst[i], for i < n.  No page may be in dst
+ * twice, or in both; a pair with a page outside the pool copies nothing. */
+int bfp_pages_copy_d(const bfp_pages *pool, const int32_t *src, const int32_t *dst, int n, void *stream);
+/* A page for every entry of the batch's table that its new rows lie in (as
+ * bfp_kv4_append_d writes them) and that holds none; the entry becomes -1
+ * where there is none left.  Writes batch->pages. */
+int bfp_pages_reserve_d(const bfp_pages *pool, const bfp_kv4_batch *batch, void *work, size_t work_bytes, void *stream);
+/* Branches: row i of out_pages (n x out_width) and out_len[i] go on from
+ * sequence parents[i] of pages (n_seq x width) and len, which counts the
+ * tokens that its pages hold.  Whole pages are shared (their refs rise); the
+ * page in which the tokens end is copied to a page of its own.  Entries past
+ * those are -1, also where no page was left for the copy, and what lies past
+ * out_width is left out.  A parent outside [0, n_seq) gives an empty row.  What
+ * out_pages held before is not looked at. */
+int bfp_pages_fork_d(const bfp_pages *pool, const int32_t *pages, const int32_t *len, int n_seq, int width,
+                     const int32_t *parents, int n, int32_t *out_pages, int32_t *out_len, int out_width, void *work,
+                     size_t work_bytes, void *stream);
+/* Gives up what the n entries of a table hold: their pages' refs fall by one
+ * each (never below 0), the entries become -1. */
+int bfp_pages_free_d(const bfp_pages *pool, int32_t *pages, long long n, void *stream);
+/* Moves the L pages that are held into pages 0 .. L-1: the k-th of those from
+ * L on to the k-th free one below L, in every array, in refs and in the tables
+ * (at most 16, all that hold any of the pool's).  An entry with a free page
+ * from L on becomes -1.  *live = L (on the device). */
+int bfp_pages_compact_d(const bfp_pages *pool, const bfp_page_table *tables, int n_tables, int32_t *live, void *work,
+                        size_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

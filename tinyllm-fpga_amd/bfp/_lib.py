@@ -56,7 +56,24 @@ class Kv4BatchC(C.Structure):
                 ("n_rows", C.c_int), ("width", C.c_int), ("max_q", C.c_int), ("max_len", C.c_int)]
 
 
+class PageArrayC(C.Structure):
+    """struct bfp_page_array."""
+    _fields_ = [("p", C.c_void_p), ("bytes", C.c_longlong)]
+
+
+class PagesC(C.Structure):
+    """struct bfp_pages."""
+    _fields_ = [("refs", C.c_void_p), ("n_short", C.c_void_p), ("arrays", C.POINTER(PageArrayC)),
+                ("n_pages", C.c_int), ("page", C.c_int), ("n_arrays", C.c_int)]
+
+
+class PageTableC(C.Structure):
+    """struct bfp_page_table."""
+    _fields_ = [("pages", C.c_void_p), ("n", C.c_longlong)]
+
+
 _rows, _kv4, _kvb = C.POINTER(RowsC), C.POINTER(Kv4C), C.POINTER(Kv4BatchC)
+_pool, _tables = C.POINTER(PagesC), C.POINTER(PageTableC)
 
 # name -> (restype, argtypes); the list of exported symbols is checked by the
 # CPU test suite against include/bfp.h.
@@ -129,6 +146,12 @@ SIGNATURES = {
     "bfp_kv4_read_d": (i32, [_kv4, _kvb, _rows, _rows, vp]),
     "bfp_kv4_attn_d": (i32, [_kv4, _kvb, _rows, _rows, C.c_double, i32, vp, sz, vp]),
     "bfp_kv4_attn_work": (sz, [_kv4, _kvb, _rows, _rows, i32]),
+    "bfp_pages_work": (sz, [_pool, i32]),
+    "bfp_pages_copy_d": (i32, [_pool, vp, vp, i32, vp]),
+    "bfp_pages_reserve_d": (i32, [_pool, _kvb, vp, sz, vp]),
+    "bfp_pages_fork_d": (i32, [_pool, vp, vp, i32, i32, vp, i32, vp, vp, i32, vp, sz, vp]),
+    "bfp_pages_free_d": (i32, [_pool, vp, i64, vp]),
+    "bfp_pages_compact_d": (i32, [_pool, _tables, i32, vp, vp, sz, vp]),
     "bfp_embed_gather_d": (i32, [vp, vp, i32, i32, i32, vp, i32, vp, vp, vp]),
 }
 

@@ -52,11 +52,16 @@ class Batch(_rows.Fixed):
         self.pages, self.start, self.lens = pages, start, lens
         self.max_q, self.max_len = _rows.c_int(max_q, "max_q"), _rows.c_int(max_len, "max_len")
         self.device = pages.device
-        self._made = (-1, None)
+        self._made, self._all = (-1, None), None
 
     def _c(self, n_rows):
-        """The struct for row arrays of n_rows (this object keeps the tensors
-        it points to)."""
+        """The struct for row arrays of n_rows, or for calls that have none
+        (this object keeps the tensors it points to)."""
+        if n_rows is None:
+            if self._all is None:
+                self._all = Kv4BatchC(self.pages.data_ptr(), self.start.data_ptr(), self.lens.data_ptr(), self.pages.shape[0],
+                                      _rows.MAX_ROWS, self.pages.shape[1], self.max_q, self.max_len)
+            return C.byref(self._all)
         n, c = self._made
         if n != n_rows:
             if not 0 <= n_rows <= _rows.MAX_ROWS:
@@ -105,6 +110,10 @@ class Fp4Cache(_rows.Fixed):
         self._scale = 1.0 / math.sqrt(self.hd)
         self._made = Kv4C(k.data_ptr(), k_exp.data_ptr(), v.data_ptr(), v_exp.data_ptr(), n_pages, page, heads, self.hd)
         self._c = C.byref(self._made)
+
+    def _page_arrays(self):
+        """(address, bytes of a page) of what a page's copy has to copy."""
+        return [(t.data_ptr(), t.stride(0)) for t in (self.k, self.k_exp, self.v, self.v_exp)]
 
     def _values(self, batch, x, what):
         """x's values, checked against the batch and the head width."""

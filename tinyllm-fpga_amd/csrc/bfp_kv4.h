@@ -129,5 +129,7 @@ __device__ __forceinline__ void kv4_decode(uint2 w, uint32_t E, float (&v)[16]) 
 
 // The checks every entry point of the cache makes (bfp_kv4.hip).
 int check_kv4(const char *op, const bfp_kv4 *c, const bfp_kv4_batch *b);
+// Of those, the batch's, for pages of `page` tokens.
+int check_batch(const char *op, const bfp_kv4_batch *b, int page);
 
 }  // namespace bfp
