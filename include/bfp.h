@@ -652,6 +652,39 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
 size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                          const bfp_rows *out, int window);
 
+/* Bounds of each page's keys: bounds (n_pages, heads, 2, hd) bfloat16, 16-byte
+ * aligned, hold the least key of every channel and then the largest, over the
+ * tokens of the page; exact, but NaN for a tile that has a NaN in any token
+ * (an exponent byte of 253 or more).  This call makes those of the pages that
+ * the batch's new rows lie in anew, from all tokens up to the sequence's last:
+ * after bfp_kv4_append_d. */
+int bfp_kv4_bounds_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, uint16_t *bounds, void *stream);
+/* picks (n_rows, heads, n) int32: for every row of q and KV head the page
+ * numbers in its sequence's table (0: the first page) that it is to see, in
+ * ascending order, -1 behind the last.  Of the pages up to the row's own that
+ * the cache has: the first `first` ones, the last `last` (at least 1: the
+ * row's own), and those with the best scores, n in all.  The score is
+ *   sum over the KV head's query heads and d of max(q_d lo_d, q_d hi_d),
+ * the largest sum of products that a key within the page's bounds can have.
+ * The choice is by the scores in 64 bits (products below 2^-126 may count as
+ * zero); of equal ones the lower pages; a NaN counts as the largest.  A
+ * row that sees nothing gets -1 alone; rows outside every sequence are left as
+ * they were.  n * page at most 2^31 - 2^16, first + last at most n, width at
+ * most 16384.
+ * work: bfp_kv4_select_work() bytes of device scratch, 16-byte aligned,
+ * whatever they hold. */
+int bfp_kv4_select_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const uint16_t *bounds, const bfp_rows *q, int n, int first,
+                     int last, int32_t *picks, void *work, size_t work_bytes, void *stream);
+size_t bfp_kv4_select_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q);
+/* bfp_kv4_attn_d over listed pages: a row sees, of the positions up to its
+ * own, those in the pages of picks (n_rows, heads, n_picks), a list for every
+ * row and KV head, in any order; a page that is listed twice counts twice, and
+ * numbers outside [0, width) list nothing.  n_picks * page is at most
+ * 2^31 - 2^16. */
+int bfp_kv4_attn_picks_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const int32_t *picks, int n_picks, const bfp_rows *q,
+                         const bfp_rows *out, double scale, void *work, size_t work_bytes, void *stream);
+size_t bfp_kv4_attn_picks_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, int n_picks, const bfp_rows *q, const bfp_rows *out);
+
 /* The pages of one or several caches that share their tables (a model's
  * layers): refs[p] says how many entries of the tables hold page p, and a page
  * is free where that is 0.  Free pages are given lowest number first, in the

@@ -146,6 +146,11 @@ SIGNATURES = {
     "bfp_kv4_read_d": (i32, [_kv4, _kvb, _rows, _rows, vp]),
     "bfp_kv4_attn_d": (i32, [_kv4, _kvb, _rows, _rows, C.c_double, i32, vp, sz, vp]),
     "bfp_kv4_attn_work": (sz, [_kv4, _kvb, _rows, _rows, i32]),
+    "bfp_kv4_bounds_d": (i32, [_kv4, _kvb, vp, vp]),
+    "bfp_kv4_select_d": (i32, [_kv4, _kvb, vp, _rows, i32, i32, i32, vp, vp, sz, vp]),
+    "bfp_kv4_select_work": (sz, [_kv4, _kvb, _rows]),
+    "bfp_kv4_attn_picks_d": (i32, [_kv4, _kvb, vp, i32, _rows, _rows, C.c_double, vp, sz, vp]),
+    "bfp_kv4_attn_picks_work": (sz, [_kv4, _kvb, i32, _rows, _rows]),
     "bfp_pages_work": (sz, [_pool, i32]),
     "bfp_pages_copy_d": (i32, [_pool, vp, vp, i32, vp]),
     "bfp_pages_reserve_d": (i32, [_pool, _kvb, vp, sz, vp]),

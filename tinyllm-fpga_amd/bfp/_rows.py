@@ -104,6 +104,13 @@ def ints(t, what: str, device, n):
     return t.data_ptr()
 
 
+def scratch(work, device):
+    """The bytes of a scratch tensor that a caller gives."""
+    if work.device != device or not work.is_contiguous():
+        raise ValueError(f"work must be a contiguous tensor on {device}")
+    return work.numel() * work.element_size()
+
+
 def gpu_of(t, what):
     """The device of a tensor that has to be on a GPU."""
     if not t.is_cuda:

@@ -23,7 +23,8 @@ from ._lib import Kv4BatchC, Kv4C, lib
 from .rotary import check_table
 
 TILE = 16
-_append, _read, _attend = (_rows.Entry(f"bfp_kv4_{name}_d") for name in ("append", "read", "attn"))
+_append, _read, _attend, _attend_picks, _bounds, _select = (
+    _rows.Entry(f"bfp_kv4_{name}_d") for name in ("append", "read", "attn", "attn_picks", "bounds", "select"))
 
 
 def _window(n):
@@ -196,7 +197,7 @@ class Fp4Cache(_rows.Fixed):
             _read(self.device, self._c, batch._c(n), *rs)
         return k, v
 
-    def attend(self, batch, q, scale=None, window=0, out=None, dtype=None, work=None):
+    def attend(self, batch, q, scale=None, window=0, out=None, dtype=None, work=None, picks=None):
         """softmax(scale q k^T) v of every row of q (rows, query heads, hd)
         over its sequence's cached tokens up to its own, the last `window` of
         them (0: all).  scale: 1/sqrt(hd) by default.  Query heads share KV
@@ -207,24 +208,44 @@ class Fp4Cache(_rows.Fixed):
         carried to at least the result's precision: bfloat16 calls of many
         rows round them to bfloat16, dtype=torch.float32 keeps them whole.
         work: uint8 scratch of attend_work() bytes (allocated per call
-        otherwise)."""
+        otherwise).
+
+        picks: int32 (rows, KV heads, n), as PageBounds.select gives them: a
+        row sees, of those tokens, the ones in the listed pages of its
+        sequence's table (any order, each once; -1 for none).  No window
+        then."""
         dev = self.device
         t, qr, out, orow = self._attend_rows(batch, q, out, dtype)
         n = t.shape[0]
+        if picks is not None:
+            n_picks = self._picks(picks, n, window)
         if n == 0:
             return out
         b, qb, ob, window = batch._c(n), C.byref(qr), C.byref(orow), _window(window)
+        scale = self._scale if scale is None else float(scale)
         if work is None:
-            size = lib().bfp_kv4_attn_work(self._c, b, qb, ob, window)
+            if picks is not None:
+                size = lib().bfp_kv4_attn_picks_work(self._c, b, n_picks, qb, ob)
+            else:
+                size = lib().bfp_kv4_attn_work(self._c, b, qb, ob, window)
             if size:
                 work = torch.empty(size, dtype=torch.uint8, device=dev)
-        elif work.device != dev or not work.is_contiguous():
-            raise ValueError(f"work must be a contiguous tensor on {dev}")
         else:
-            size = work.numel() * work.element_size()
-        _attend(dev, self._c, b, qb, ob, self._scale if scale is None else float(scale), window,
-                work.data_ptr() if work is not None else None, size)
+            size = _rows.scratch(work, dev)
+        p = work.data_ptr() if work is not None else None
+        if picks is not None:
+            _attend_picks(dev, self._c, b, picks.data_ptr(), n_picks, qb, ob, scale, p, size)
+        else:
+            _attend(dev, self._c, b, qb, ob, scale, window, p, size)
         return out
+
+    def _picks(self, picks, n, window):
+        if picks.dim() != 3 or tuple(picks.shape[:2]) != (n, self.heads) or picks.dtype != torch.int32 \
+                or not picks.is_contiguous() or picks.device != self.device:
+            raise ValueError(f"picks must be a contiguous int32 tensor ({n}, {self.heads}, pages) on {self.device}")
+        if window:
+            raise ValueError("picks and a window")
+        return picks.shape[2]
 
     def _attend_rows(self, batch, q, out, dtype, make=True):
         t = self._values(batch, q, "q")
@@ -242,8 +263,93 @@ class Fp4Cache(_rows.Fixed):
             orow = _rows.rows(out, "out", self.device)
         return t, qr, out, orow
 
-    def attend_work(self, batch, q, out=None, dtype=None, window=0):
+    def attend_work(self, batch, q, out=None, dtype=None, window=0, picks=None):
         """Scratch bytes attend() needs for such a call."""
         t, qr, _, orow = self._attend_rows(batch, q, out, dtype, make=False)
         orow.p = orow.p or 16   # the size depends on no address
+        if picks is not None:
+            n_picks = self._picks(picks, t.shape[0], window)
+            return lib().bfp_kv4_attn_picks_work(self._c, batch._c(t.shape[0]), n_picks, C.byref(qr), C.byref(orow))
         return lib().bfp_kv4_attn_work(self._c, batch._c(t.shape[0]), C.byref(qr), C.byref(orow), _window(window))
+
+
+class PageBounds(_rows.Fixed):
+    """The least and the largest key of each page's channels, and the pages
+    that they let a row pick: buf (n_pages, heads, 2, hd) bfloat16, for one
+    cache.
+
+        bounds = PageBounds(cache)
+        bounds.update(batch)                               # after every append
+        picks = bounds.select(batch, q, 32)                # rows x KV heads x 32
+        out = cache.attend(batch, q, picks=picks)
+
+    Bounds belong to pages: a PagePool that has this object among its caches
+    copies and moves them with the keys."""
+
+    def __init__(self, cache):
+        self._set(cache, torch.zeros((cache.n_pages, cache.heads, 2, cache.hd), dtype=torch.bfloat16, device=cache.device))
+
+    @classmethod
+    def from_buffer(cls, cache, buf):
+        """Bounds in existing memory."""
+        self = cls.__new__(cls)
+        self._set(cache, buf)
+        return self
+
+    def _set(self, cache, buf):
+        shape = (cache.n_pages, cache.heads, 2, cache.hd)
+        if tuple(buf.shape) != shape or buf.dtype != torch.bfloat16 or not buf.is_contiguous() or buf.device != cache.device:
+            raise ValueError(f"bounds must be a contiguous bfloat16 tensor {shape} on {cache.device}")
+        self.cache, self.buf = cache, buf
+        self.n_pages, self.page, self.device = cache.n_pages, cache.page, cache.device
+
+    def _page_arrays(self):
+        return [(self.buf.data_ptr(), 2 * self.buf.stride(0))]
+
+    def update(self, batch):
+        """Make the bounds of the pages that the batch's new rows lie in anew,
+        from all of their tokens: after append, before select."""
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on {batch.device}, the cache on {self.device}")
+        _bounds(self.device, self.cache._c, batch._c(None), self.buf.data_ptr())
+
+    def select(self, batch, q, n, first=1, last=2, out=None, work=None):
+        """For every row of q (rows, query heads, hd) and KV head the n pages
+        of its sequence to look at, numbers in the batch's table, ascending,
+        -1 behind the last: the first `first` and the last `last` (at least 1)
+        of those up to the row's own, and of the others the ones with the best
+        scores, the sum over the KV head's query heads and d of max(q_d lo_d,
+        q_d hi_d).  Equal scores: the lower page.  Returns out, or a new int32
+        tensor (rows, heads, n), whose rows outside every sequence are
+        undefined.  work: uint8 scratch of select_work() bytes (allocated
+        per call otherwise)."""
+        c = self.cache
+        t, qr, n, first, last = self._select(batch, q, n, first, last)
+        rows, shape = t.shape[0], (t.shape[0], c.heads, n)
+        if out is None:
+            out = torch.empty(shape, dtype=torch.int32, device=self.device)
+        elif tuple(out.shape) != shape or out.dtype != torch.int32 or not out.is_contiguous() or out.device != self.device:
+            raise ValueError(f"out must be a contiguous int32 tensor {shape} on {self.device}")
+        if rows == 0:
+            return out
+        b, qb = batch._c(rows), C.byref(qr)
+        if work is None:
+            size = lib().bfp_kv4_select_work(c._c, b, qb)
+            work = torch.empty(size, dtype=torch.uint8, device=self.device)
+        else:
+            size = _rows.scratch(work, self.device)
+        _select(self.device, c._c, b, self.buf.data_ptr(), qb, n, first, last, out.data_ptr(), work.data_ptr(), size)
+        return out
+
+    def _select(self, batch, q, n, first, last):
+        c = self.cache
+        t = c._values(batch, q, "q")
+        if t.shape[1] % c.heads or not t.shape[1]:
+            raise ValueError(f"{t.shape[1]} query heads for {c.heads} KV heads")
+        return (t, _rows.rows(q, "q", self.device), _rows.c_int(n, "n", 1), _rows.c_int(first, "first"),
+                _rows.c_int(last, "last", 1))
+
+    def select_work(self, batch, q):
+        """Scratch bytes select() needs for such a call."""
+        t, qr, *_ = self._select(batch, q, 1, 0, 1)
+        return lib().bfp_kv4_select_work(self.cache._c, batch._c(t.shape[0]), C.byref(qr))

@@ -62,10 +62,8 @@ class PagePool(_rows.Fixed):
         size = self._size + 8 * n
         if work is None:
             work = torch.empty(size, dtype=torch.uint8, device=self.device)
-        elif work.device != self.device or not work.is_contiguous():
-            raise ValueError(f"work must be a contiguous tensor on {self.device}")
         else:
-            size = work.numel() * work.element_size()
+            size = _rows.scratch(work, self.device)
         return work, work.data_ptr(), size
 
     def work(self, n=0):

@@ -55,6 +55,9 @@ struct Kv4AttnArgs {
   float *part_o;       // k_kv4_prompt [sequence][row of max_q][query head][split][hd]; k_kv4_rows [slot][R][hd]
   float2 *part_ml;     // without [hd]
   unsigned long long *there, number;   // k_kv4_rows: which slots are filled, and this call's number
+  // listed pages: n_picks a row and KV head, and the row tiles of a token's query heads
+  const int32_t *picks;
+  int n_picks, token_tiles;
 };
 
 // Position p's visible keys are [lo, hi).
@@ -232,6 +235,7 @@ struct AttnKernel {
   int lds;
 };
 AttnKernel rows_kernel(int tiles, int terms, int waves);
+AttnKernel picks_kernel(int tiles, int terms, int waves);
 AttnKernel prompt_kernel(int tiles, int terms);
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }

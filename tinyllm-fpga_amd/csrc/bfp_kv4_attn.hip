@@ -115,6 +115,35 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   return p;
 }
 
+static bool picks_fit(const bfp_kv4 &c, int n) { return n >= 1 && (long long)n * c.page <= KV4_MAX_POS; }
+
+// Rows that see the pages a list names: few rows to a list, one token's query
+// heads, so always k_kv4_rows, its keys those of the list.
+static Kv4Plan plan_picks(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_rows &q, const bfp_rows &out, int n, int &token_tiles) {
+  Kv4Plan p{};
+  const int group = q.heads / c.heads, tiles = c.hd / 16;
+  p.terms = terms_of(q, out, group);
+  const int R = 16 / p.terms;
+  token_tiles = (group + R - 1) / R;
+  p.row_tiles = b.max_q * token_tiles;
+  p.splits = 1;
+  const long long key_tiles = ((long long)n * c.page + KEYS - 1) / KEYS;
+  p.chunk = (int)key_tiles;
+  const long long rows = b.n_rows < (long long)b.n_seq * b.max_q ? b.n_rows : (long long)b.n_seq * b.max_q;
+  const long long groups = rows * token_tiles * c.heads, most_groups = (long long)p.row_tiles * c.heads * b.n_seq;
+  p.waves = rows_waves(tiles);
+  if (key_tiles > 4 * p.waves || most_groups * p.waves > 0x3ffffff || groups >= 1024) {
+    p.waves = 4;
+    if (groups < 1024 && key_tiles > 16 && b.n_seq <= 256 && most_groups * (key_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
+      const long long most = groups * (key_tiles + ROWS_EXTRA) / 4 + 1, slots = tiles <= 4 ? 768 : tiles <= 8 ? 512 : 256;
+      p.stream = (int)(most < slots ? most : slots);
+      p.cells = 2 * (size_t)p.stream * R;
+    }
+  }
+  p.work = p.cells * (16 * tiles * sizeof(float) + sizeof(float2)) + 2 * p.stream * sizeof(unsigned long long);
+  return p;
+}
+
 // A number no other call has: what k_kv4_rows knows its flags in the
 // workspace by, whatever the workspace held before.
 static unsigned long long call_number() {
@@ -142,6 +171,55 @@ static int check_attn(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch 
   return BFP_OK;
 }
 
+// The arguments that follow from a call's; the scale's checks.
+static int attn_args(const char *op, Kv4AttnArgs &a, const bfp_kv4 &cache, const bfp_kv4_batch &batch, const bfp_rows &q,
+                     const bfp_rows &out, double scale, int window) {
+  const float scale2 = (float)(fabs(scale) * 1.44269504088896340736);
+  if (!isfinite(scale2)) return set_err(BFP_EINVAL, "%s: scale=%g is not float32's", op, scale);
+  a = Kv4AttnArgs{};
+  a.c = cache;
+  a.b = batch;
+  a.q = q;
+  a.out = out;
+  a.tiles = cache.hd / 16;
+  a.group = q.heads / cache.heads;
+  a.page_shift = __builtin_ctz((unsigned)cache.page);
+  a.window = window;
+  // a scale of zero, or too small for float32: all scores alike, from queries of zeros
+  a.scale2 = scale2 == 0.0f ? 1.0f : scale2;
+  a.q_sign = scale2 == 0.0f ? 0.0f : scale < 0 ? -1.0f : 1.0f;
+  // (kept finite, and so that no score below 2^126 passes float32 with it)
+  a.slack = fminf(M_SLACK / a.scale2, 0x1p125f);
+  a.by_head = FastDiv(cache.heads);
+  a.by_group = FastDiv((uint32_t)a.group);
+  a.out_wide = rows_aligned(out, 8, batch.n_rows);
+  return BFP_OK;
+}
+
+static int launch_attn(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, void *work, size_t work_bytes, hipStream_t s) {
+  if (p.work && (!work || (uintptr_t)work % 16 || work_bytes < p.work))
+    return set_err(BFP_EINVAL, "%s: needs %zu bytes of 16-byte-aligned scratch, got %zu", op, p.work, work ? work_bytes : (size_t)0);
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  a.stream = p.stream;
+  if (p.work) {
+    a.part_o = (float *)work;
+    a.part_ml = (float2 *)((float *)work + p.cells * 16 * a.tiles);
+    a.there = (unsigned long long *)(a.part_ml + p.cells);
+    a.number = call_number();
+  }
+  a.row_tiles = p.row_tiles;
+  a.by_split = FastDiv(p.splits);
+  const long long each = (long long)p.row_tiles * p.splits * a.c.heads, blocks = p.stream ? p.stream : each * a.b.n_seq;
+  if (blocks > 0x3ffffff / p.waves || each > 0x7fffffff)   // 2^32 threads
+    return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, a.b.n_seq, a.b.max_q);
+  a.by_seq = FastDiv((uint32_t)each);
+  if (k.lds > 65536)   // one limit for a kernel, whatever the call
+    HIP_TRY(hipFuncSetAttribute((const void *)k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024));
+  hipLaunchKernelGGL(k.fn, dim3((unsigned)blocks), dim3(64 * p.waves), k.lds, s, a);
+  return launch_status(op);
+}
+
 }  // namespace bfp
 
 using namespace bfp;
@@ -159,52 +237,36 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
                    void *stream) {
   const char *op = "kv4_attn";
   BFP_TRY(check_attn(op, cache, batch, q, out, window, true));
-  const float scale2 = (float)(fabs(scale) * 1.44269504088896340736);
-  if (!isfinite(scale2)) return set_err(BFP_EINVAL, "%s: scale=%g is not float32's", op, scale);
+  Kv4AttnArgs a;
+  BFP_TRY(attn_args(op, a, *cache, *batch, *q, *out, scale, window));
   if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
   const Kv4Plan p = plan_attn(*cache, *batch, *q, *out, window);
-  if (p.work && (!work || (uintptr_t)work % 16 || work_bytes < p.work))
-    return set_err(BFP_EINVAL, "%s: needs %zu bytes of 16-byte-aligned scratch, got %zu", op, p.work, work ? work_bytes : (size_t)0);
-  Kv4AttnArgs a{};
-  a.c = *cache;
-  a.b = *batch;
-  a.q = *q;
-  a.out = *out;
-  a.tiles = cache->hd / 16;
-  a.group = q->heads / cache->heads;
-  a.page_shift = __builtin_ctz((unsigned)cache->page);
-  a.window = window;
-  a.splits = p.splits;
-  a.chunk = p.chunk;
-  // a scale of zero, or too small for float32: all scores alike, from queries of zeros
-  a.scale2 = scale2 == 0.0f ? 1.0f : scale2;
-  a.q_sign = scale2 == 0.0f ? 0.0f : scale < 0 ? -1.0f : 1.0f;
-  // (kept finite, and so that no score below 2^126 passes float32 with it)
-  a.slack = fminf(M_SLACK / a.scale2, 0x1p125f);
-  a.stream = p.stream;
-  if (p.work) {
-    a.part_o = (float *)work;
-    a.part_ml = (float2 *)((float *)work + p.cells * 16 * a.tiles);
-    a.there = (unsigned long long *)(a.part_ml + p.cells);
-    a.number = call_number();
-  }
-  a.row_tiles = p.row_tiles;
-  a.by_head = FastDiv(cache->heads);
-  a.by_split = FastDiv(p.splits);
-  a.by_group = FastDiv((uint32_t)a.group);
-  a.out_wide = rows_aligned(*out, 8, batch->n_rows);
-  const long long each = (long long)p.row_tiles * p.splits * cache->heads, blocks = p.stream ? p.stream : each * batch->n_seq;
-  if (blocks > 0x3ffffff / p.waves || each > 0x7fffffff)   // 2^32 threads
-    return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, batch->n_seq, batch->max_q);
-  a.by_seq = FastDiv((uint32_t)each);
-  const AttnKernel k = p.prompt ? prompt_kernel(a.tiles, p.terms) : rows_kernel(a.tiles, p.terms, p.waves);
-  if (k.lds > 65536)   // one limit for a kernel, whatever the call
-    HIP_TRY(hipFuncSetAttribute((const void *)k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024));
-  hipLaunchKernelGGL(k.fn, dim3((unsigned)blocks), dim3(64 * p.waves), k.lds, (hipStream_t)stream, a);
-  BFP_TRY(launch_status(op));
+  BFP_TRY(launch_attn(op, a, p, p.prompt ? prompt_kernel(a.tiles, p.terms) : rows_kernel(a.tiles, p.terms, p.waves), work, work_bytes,
+                      (hipStream_t)stream));
   if (p.splits == 1) return BFP_OK;
   launch_join_prompt(a, (hipStream_t)stream);
   return launch_status(op);
+}
+
+size_t bfp_kv4_attn_picks_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, int n_picks, const bfp_rows *q, const bfp_rows *out) {
+  int token_tiles;
+  if (check_attn("kv4_attn_picks_work", cache, batch, q, out, 0, false) || !picks_fit(*cache, n_picks)) return 0;
+  return plan_picks(*cache, *batch, *q, *out, n_picks, token_tiles).work;
+}
+
+int bfp_kv4_attn_picks_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const int32_t *picks, int n_picks, const bfp_rows *q,
+                         const bfp_rows *out, double scale, void *work, size_t work_bytes, void *stream) {
+  const char *op = "kv4_attn_picks";
+  BFP_TRY(check_attn(op, cache, batch, q, out, 0, true));
+  if (!picks_fit(*cache, n_picks)) return set_err(BFP_EINVAL, "%s: n_picks=%d", op, n_picks);
+  Kv4AttnArgs a;
+  BFP_TRY(attn_args(op, a, *cache, *batch, *q, *out, scale, 0));
+  if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
+  if (!picks || (uintptr_t)picks % 4) return set_err(BFP_EINVAL, "%s: picks are null or not aligned", op);
+  const Kv4Plan p = plan_picks(*cache, *batch, *q, *out, n_picks, a.token_tiles);
+  a.picks = picks;
+  a.n_picks = n_picks;
+  return launch_attn(op, a, p, picks_kernel(a.tiles, p.terms, p.waves), work, work_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,593 @@
+// Bounds of each page's keys, and the pages that a score picks for each row.
+//
+// lo_d and hi_d are the least and the largest key of channel d in a page.  No
+// key of the page has a product with q above sum_d max(q_d lo_d, q_d hi_d), and
+// summed over the heads that share the keys that is
+//   score = sum_d hi_d P_d + lo_d N_d,  P_d = sum max(q_d, 0),  N_d = sum min(q_d, 0):
+// one product of length 2 hd a page, whatever the heads.  Cached keys have two
+// significant bits, so bounds are exact in bfloat16 and lie in memory as the
+// matrix cores take them.
+#include <math.h>
+
+#include "bfp_kv4_attn.h"
+
+namespace bfp {
+
+constexpr int BOUND_T = 256;
+constexpr uint32_t BOUND_NAN = 0x7fc07fc0u;
+
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+
+struct Kv4BoundArgs {
+  bfp_kv4 c;
+  bfp_kv4_batch b;
+  uint16_t *bounds;
+  int touched, lanes_shift;   // pages that a sequence's new rows can lie in; log2 of page / 4
+  FastDiv by_group, by_head, by_touched;   // groups of tiles, one a wave; heads; pages of a sequence
+  long long n_units;
+};
+
+// bfloat16 as numbers that compare as whole ones do (and back).
+__device__ __forceinline__ i16x2 sortable(i16x2 v) { return v ^ ((v >> 15) & (short)0x7fff); }
+__device__ __forceinline__ i16x2 lane_xor(i16x2 v, int m) {
+  return __builtin_bit_cast(i16x2, __shfl_xor(__builtin_bit_cast(int, v), m, 64));
+}
+
+// A lane takes four tokens of one tile, as they lie side by side; the lanes
+// of a tile join.  Bound by the bytes of k.
+__global__ __launch_bounds__(BOUND_T) void k_kv4_bounds(Kv4BoundArgs a) {
+  const long long u64 = (long long)blockIdx.x * (BOUND_T / 64) + (threadIdx.x >> 6);
+  if (u64 >= a.n_units) return;
+  uint32_t group, head, j;
+  const uint32_t seq = a.by_touched.div(a.by_head.div(a.by_group.div((uint32_t)u64, group), head), j);
+  const Kv4Span s = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
+  const int stop = s.at + s.n, first = s.at > 0 ? s.at : 0;
+  if (s.n == 0 || stop <= first) return;
+  const int page = a.c.page, p = first / page + (int)j;
+  if (p > (stop - 1) / page) return;
+  const int id = kv4_page(a.b.pages + (long long)seq * a.b.width, a.b.width, a.c.n_pages, p);
+  if (id < 0) return;
+  const int lane = threadIdx.x & 63, tiles = a.c.hd / 16, lanes = 1 << a.lanes_shift;
+  const int tile = (int)group * (64 >> a.lanes_shift) + (lane >> a.lanes_shift), slot = 4 * (lane & (lanes - 1));
+  const bool mine = tile < tiles;
+  const long long o = kv4_tile(id, a.c.heads, (int)head, tiles, mine ? tile : tiles - 1, page, slot);
+  const uint4 *d = (const uint4 *)(a.c.k + o * KV4_TILE_BYTES);
+  const uint4 w[2] = {d[0], d[1]};
+  const uint32_t e = *(const uint32_t *)(a.c.k_e + o);
+  const int held = stop - p * page;   // slots of this page that hold a token
+
+  i16x2 lo[8], hi[8];
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lo[i] = i16x2{0x7fff, 0x7fff}, hi[i] = i16x2{-0x8000, -0x8000};
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const bool have = slot + t < held;
+    const uint32_t E = (e >> (8 * t)) & 255u;
+    bad |= have && E >= KV4_PAST ? 1u : 0u;
+    const float sc = kv4_scale(E);
+    const uint32_t words[2] = {t & 1 ? w[t >> 1].z : w[t >> 1].x, t & 1 ? w[t >> 1].w : w[t >> 1].y};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 v = __builtin_bit_cast(uint4, kv4_decode8(words[h], sc));
+      const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const i16x2 y = sortable(__builtin_bit_cast(i16x2, x[i]));
+        if (have) {
+          lo[4 * h + i] = __builtin_elementwise_min(lo[4 * h + i], y);
+          hi[4 * h + i] = __builtin_elementwise_max(hi[4 * h + i], y);
+        }
+      }
+    }
+  }
+  for (int m = 1; m < lanes; m *= 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo[i] = __builtin_elementwise_min(lo[i], lane_xor(lo[i], m));
+      hi[i] = __builtin_elementwise_max(hi[i], lane_xor(hi[i], m));
+    }
+    bad |= __shfl_xor(bad, m, 64);
+  }
+  if (!mine || (lane & (lanes - 1)) > 1) return;
+  // the tile's first lane writes the least ones, its second the largest
+  const bool upper = lane & 1;
+  uint32_t y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const i16x2 x = sortable(upper ? hi[i] : lo[i]);
+    y[i] = bad ? BOUND_NAN : __builtin_bit_cast(uint32_t, x);
+  }
+  uint4 *to = (uint4 *)(a.bounds + (((long long)id * a.c.heads + head) * 2 + (upper ? 1 : 0)) * a.c.hd + 16 * tile);
+  to[0] = make_uint4(y[0], y[1], y[2], y[3]);
+  to[1] = make_uint4(y[4], y[5], y[6], y[7]);
+}
+
+// ------------------------------------------------------------------- scores
+// Scores in float32 on the bfloat16 matrix cores, P and N in three terms of
+// eight bits, and how far they may be from the exact ones.  The choice is
+// exact all the same: with every score within e of its value, pages more than
+// 2 e above the n-th largest are surely picked and those more than 2 e below it
+// surely not; what lies between is scored again in float64 (k_kv4_pick).
+struct Kv4PickArgs {
+  bfp_kv4 c;
+  bfp_kv4_batch b;
+  bfp_rows q;
+  const uint16_t *bounds;
+  int group, i0, rows;        // rows i0 .. i0 + rows - 1 of every sequence
+  int n, first, last;         // pages to pick; of these the first and the last ones, whatever their scores
+  int chunks;                 // pieces of the pages, SCORE_CHUNK each
+  FastDiv by_chunk, by_tile;
+  float *score;               // [sequence][row][head][width]
+  float *off;                 // [sequence][row][head][chunk]: sums of the products' magnitudes, at most
+  int32_t *picks;
+};
+
+constexpr int SCORE_W = 4;                // waves
+constexpr int SCORE_PAGES = 64;           // of a wave
+constexpr int SCORE_CHUNK = SCORE_W * SCORE_PAGES;
+
+// The last page that row i of a span sees, -1: none.
+__device__ __forceinline__ int own_page(const Kv4PickArgs &a, const Kv4Span &s, int i) {
+  const int p = s.at + i;
+  if (p < 0) return -1;
+  const int q = p / a.c.page;
+  return q < a.b.width ? q : a.b.width - 1;
+}
+
+// R: rows of a wave's matrix tile.  16: their terms multiply one after the
+// other; 4: the terms are columns of the tile.  K: steps of 32 values (hd / 16).
+// Bound by the bytes of the bounds: 16 pages' operands are loaded as they lie.
+template <int R, int K>
+__global__ __launch_bounds__(64 * SCORE_W) void k_kv4_score(Kv4PickArgs a) {
+  constexpr int T = R == 16 ? 3 : 1;
+  const int head = blockIdx.y;
+  uint32_t chunk, rt;
+  const int seq = (int)a.by_tile.div(a.by_chunk.div(blockIdx.x, chunk), rt);
+  const Kv4Span s = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
+  const int i0 = a.i0 + (int)rt * R, stop = a.i0 + a.rows < s.n ? a.i0 + a.rows : s.n;
+  if (i0 >= stop) return;
+  const int ilast = i0 + R < stop ? i0 + R - 1 : stop - 1;
+  const int pages = own_page(a, s, ilast) + 1;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int base = (int)chunk * SCORE_CHUNK;
+  // all of them are taken, or there are none here
+  if (pages <= a.n || base >= pages) return;
+  const int hd = a.c.hd, i = i0 + col % R;
+  const bool mine = i < stop;
+  // this lane's column: dims 32 k + 8 g .. + 7 of [N | P]
+  bf16x8 coef[T][K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int at = 32 * k + 8 * g;
+    const bool upper = at >= hd;
+    const int d = upper ? at - hd : at;
+    float sum[8], x[8], rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] = rest[e] = 0.0f;
+    if (mine)
+      for (int h = 0; h < a.group; ++h) {
+        row_load_n(a.q, (long long)(s.row0 + i) * a.q.row_stride + (head * a.group + h) * a.q.head_stride + d, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = upper ? fmaxf(x[e], 0.0f) : fminf(x[e], 0.0f);
+          sum[e] += x[e] == x[e] ? v : NAN;
+        }
+      }
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      const int term = R == 16 ? t : col / R;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = term < 3 ? query_term<3>(sum[e], term) : 0.0f;
+      coef[t][k] = pack8(y);
+    }
+  }
+  const int32_t *table = a.b.pages + (long long)seq * a.b.width;
+  const long long out = ((long long)seq * a.rows + (i - a.i0)) * a.c.heads + head;
+  float most = 0.0f;
+#pragma unroll 1
+  for (int t = 0; t < SCORE_PAGES / 16; ++t) {
+    const int p0 = base + w * SCORE_PAGES + 16 * t;
+    if (p0 >= pages) break;
+    const int p = p0 + col;
+    const int id = p < pages ? kv4_page(table, a.b.width, a.c.n_pages, p) : -1;
+    const bf16x8 *from = (const bf16x8 *)(a.bounds + ((long long)(id < 0 ? 0 : id) * a.c.heads + head) * 2 * hd + 8 * g);
+    bf16x8 v[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = from[4 * k];
+    f32x4 sc = {0, 0, 0, 0}, mag = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int u = 0; u < T; ++u) sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[k], coef[u][k], sc, 0, 0, 0);
+      typedef unsigned u4 __attribute__((ext_vector_type(4)));
+      const u4 va = __builtin_bit_cast(u4, v[k]) & 0x7fff7fffu, ca = __builtin_bit_cast(u4, coef[0][k]) & 0x7fff7fffu;
+      mag = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, ca), mag, 0, 0, 0);
+    }
+    const unsigned long long there = __ballot(id >= 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = sc[e], m = mag[e];
+      if (R == 4) {
+        x = term_sum<4>(x);
+        m = term_sum<4>(m);
+      }
+      const int page = p0 + 4 * g + e;
+      if (!mine || page >= pages || (R == 4 && col >= R)) continue;
+      const bool ok = (there >> (4 * g + e)) & 1;
+      if (ok) most = fabsf(x) < INFINITY ? fmaxf(most, m) : INFINITY;
+      a.score[out * a.b.width + page] = ok ? x : -INFINITY;
+    }
+  }
+  // over the column's four lanes, then the waves
+  most = fmaxf(most, fpeer<16>(most));
+  most = fmaxf(most, fpeer<32>(most));
+  __shared__ float waves[SCORE_W][16];
+  if (g == 0) waves[w][col] = most;
+  __syncthreads();
+  if (threadIdx.x < R && mine)
+    a.off[out * a.chunks + chunk] = fmaxf(fmaxf(waves[0][col], waves[1][col]), fmaxf(waves[2][col], waves[3][col]));
+}
+
+// -------------------------------------------------------------------- picks
+__device__ __forceinline__ uint32_t key_of(float f) {
+  const uint32_t b = __float_as_uint(f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+__device__ __forceinline__ unsigned long long key_of(double f) {
+  if (f != f) return ~0ull;   // a NaN counts as the largest
+  const unsigned long long b = (unsigned long long)__double_as_longlong(f + 0.0);   // -0 is 0
+  return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+// Sums over a workgroup of W waves of what each wave counted; two sets of
+// places in turn, one barrier a call.
+template <int W>
+struct Counter {
+  int (*place)[W][3];
+  int turn;
+  __device__ void add(int (&n)[3]) {
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+      place[turn][w][0] = n[0];
+      place[turn][w][1] = n[1];
+      place[turn][w][2] = n[2];
+    }
+    __syncthreads();
+    n[0] = n[1] = n[2] = 0;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      n[0] += place[turn][k][0];
+      n[1] += place[turn][k][1];
+      n[2] += place[turn][k][2];
+    }
+    turn ^= 1;
+  }
+};
+
+// The largest key that at least `want` of the n keys reach.  Two bits a round.
+template <int W, typename Key>
+__device__ __forceinline__ Key nth_key(int n, int want, const Key *key, Counter<W> &count) {
+  Key at = 0;
+#pragma unroll 1
+  for (int bit = 8 * (int)sizeof(Key) - 2; bit >= 0; bit -= 2) {
+    const Key q[3] = {at | (Key)1 << bit, at | (Key)2 << bit, at | (Key)3 << bit};
+    int c[3] = {0, 0, 0};
+    for (int p0 = 0; p0 < n; p0 += 64 * W) {
+      const int p = p0 + threadIdx.x;
+      const Key k = p < n ? key[p] : 0;
+#pragma unroll
+      for (int u = 0; u < 3; ++u) c[u] += __popcll(__ballot(k >= q[u]));
+    }
+    count.add(c);
+    at = c[2] >= want ? q[2] : c[1] >= want ? q[1] : c[0] >= want ? q[0] : at;
+  }
+  return at;
+}
+
+// The exact score of a page, by eight neighbouring lanes; coef: N and P in
+// float64.
+__device__ __forceinline__ double exact_score(const Kv4PickArgs &a, int id, int head, const double *coef) {
+  const int hd = a.c.hd, l = threadIdx.x & 7;
+  const uint16_t *v = a.bounds + ((long long)id * a.c.heads + head) * 2 * hd;
+  double sum = 0.0;
+  for (int d = 8 * l; d < 2 * hd; d += 64) {
+    const uint4 x = *(const uint4 *)(v + d);
+    const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum = __builtin_fma((double)__uint_as_float(y[i] << 16), coef[d + 2 * i], sum);
+      sum = __builtin_fma((double)__uint_as_float(y[i] & 0xffff0000u), coef[d + 2 * i + 1], sum);
+    }
+  }
+  sum += __shfl_xor(sum, 1, 64);
+  sum += __shfl_xor(sum, 2, 64);
+  return sum + __shfl_xor(sum, 4, 64);
+}
+
+// One row and KV head a workgroup of W waves.  words: a bit for every page
+// that is taken, and for every one that may be; then the scores as keys, in
+// float32 and, of those at the border, in float64.
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_kv4_pick(Kv4PickArgs a) {
+  extern __shared__ __align__(16) unsigned long long words[];
+  __shared__ int places[2][W][3];
+  __shared__ float tops[W];
+  __shared__ double coef[512];
+  const int head = blockIdx.y, seq = (int)(blockIdx.x / (unsigned)a.rows), i = a.i0 + (int)(blockIdx.x % (unsigned)a.rows);
+  const Kv4Span s = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
+  if (i >= s.n) return;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int n = own_page(a, s, i) + 1;   // pages that it sees
+  const int32_t *table = a.b.pages + (long long)seq * a.b.width;
+  int32_t *to = a.picks + ((long long)(s.row0 + i) * a.c.heads + head) * a.n;
+  const long long in = ((long long)seq * a.rows + (i - a.i0)) * a.c.heads + head;
+  const float *score = a.score + in * a.b.width;
+  const int n_words = (n + 63) / 64;
+  unsigned long long *take = words, *border = words + n_words, *keys = border + n_words;
+  uint32_t *key32 = (uint32_t *)keys;   // 0: not to be picked
+  Counter<W> count{places, 0};
+  auto forced = [&](int p) { return p < a.first || p >= n - a.last; };
+
+  // The forced pages that exist, the others that do, and how far scores may be off.
+  int c[3] = {0, 0, 0};
+  const bool all = n <= a.n;
+  for (int p0 = 0; p0 < n; p0 += 64 * W) {
+    const int p = p0 + threadIdx.x;
+    const float x = p < n && !all && !forced(p) ? score[p] : -INFINITY;
+    const bool there = p < n && (all || forced(p) ? kv4_page(table, a.b.width, a.c.n_pages, p) >= 0 : x != -INFINITY);
+    if (p < n) key32[p] = x == -INFINITY ? 0u : key_of(x);
+    const unsigned long long f = __ballot(there && (all || forced(p)));
+    c[0] += __popcll(f);
+    c[1] += __popcll(__ballot(there && !all && !forced(p)));
+    if (lane == 0 && p0 + 64 * w < n) take[p0 / 64 + w] = f;
+  }
+  count.add(c);
+  int want = a.n - c[0];
+  want = want < c[1] ? want : c[1];
+  if (want > 0 && want == c[1]) {
+    for (int p0 = 0; p0 < n; p0 += 64 * W) {
+      const int p = p0 + threadIdx.x;
+      const unsigned long long f = __ballot(p < n && key32[p] != 0);
+      if (lane == 0 && p0 + 64 * w < n) take[p0 / 64 + w] |= f;
+    }
+  } else if (want > 0) {
+    float most = 0.0f;
+    for (int k = threadIdx.x; k * SCORE_CHUNK < n; k += 64 * W) most = fmaxf(most, a.off[in * a.chunks + k]);
+    most = wave_max(most);
+    if (lane == 0) tops[w] = most;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < W; ++k) most = fmaxf(most, tops[k]);
+    // A product of 2 hd terms, 2^-23 of the sum of their magnitudes each (the
+    // matrix cores may cut); the second and third terms' sums, which are 2^-7
+    // and 2^-14 of the first's, P and N themselves (sums of the group's
+    // queries in float32, 2^-24 each) and the joining of the terms in what is
+    // added; magnitudes are of the first terms, at least 1 - 2^-7 of the whole.
+    const float e2 = 2.0f * (2 * a.c.hd + a.group + 16) * 0x1.06p-23f * most + 0x1p-120f;
+    const bool exact_all = !(e2 < 0x1p120f);
+    float A = 0.0f;
+    if (!exact_all) A = of_key(nth_key<W, uint32_t>(n, want, key32, count));
+    c[0] = c[1] = c[2] = 0;
+    for (int p0 = 0; p0 < n; p0 += 64 * W) {
+      const int p = p0 + threadIdx.x;
+      const uint32_t k = p < n ? key32[p] : 0u;
+      const bool free = exact_all ? p < n && !forced(p) && kv4_page(table, a.b.width, a.c.n_pages, p) >= 0 : k != 0;
+      const float x = free && !exact_all ? of_key(k) - A : 0.0f;
+      const unsigned long long in_set = __ballot(free && x > e2), between = __ballot(free && !(x > e2) && !(x < -e2));
+      c[0] += __popcll(in_set);
+      c[1] += __popcll(between);
+      if (lane == 0 && p0 + 64 * w < n) {
+        take[p0 / 64 + w] |= in_set;
+        border[p0 / 64 + w] = between;
+      }
+    }
+    count.add(c);
+    want -= c[0];
+    if (want >= c[1]) {   // all of them
+      for (int k = threadIdx.x; k < n_words; k += 64 * W) take[k] |= border[k];
+    } else {
+      // P and N, then the border's scores in float64 over the approximate ones' keys
+      for (int d = threadIdx.x; d < 2 * a.c.hd; d += 64 * W) {
+        double sum = 0.0;
+        const bool upper = d >= a.c.hd;
+        for (int h = 0; h < a.group; ++h) {
+          const double x = row_load(a.q, (long long)(s.row0 + i) * a.q.row_stride + (head * a.group + h) * a.q.head_stride + (upper ? d - a.c.hd : d));
+          sum += x != x ? x : upper ? fmax(x, 0.0) : fmin(x, 0.0);
+        }
+        coef[d] = sum;
+      }
+      __syncthreads();
+      int before = 0;   // keys: of the border's pages, in their order
+      for (int k = 0; k < n_words; ++k) {
+        const unsigned long long m = border[k];
+        const int mine = __popcll(m);
+        for (int u = threadIdx.x >> 3; u < mine; u += 8 * W) {   // eight lanes a page
+          unsigned long long rest = m;
+          for (int x = 0; x < u; ++x) rest &= rest - 1;
+          const int p = 64 * k + __ffsll((long long)rest) - 1;
+          const int id = kv4_page(table, a.b.width, a.c.n_pages, p);
+          const double sc = exact_score(a, id < 0 ? 0 : id, head, coef);
+          if ((threadIdx.x & 7) == 0) keys[before + u] = key_of(sc);
+        }
+        before += mine;
+      }
+      __syncthreads();
+      const unsigned long long T = nth_key<W, unsigned long long>(before, want, keys, count);
+      c[0] = c[1] = c[2] = 0;
+      for (int u0 = 0; u0 < before; u0 += 64 * W) {
+        const int u = u0 + threadIdx.x;
+        c[0] += __popcll(__ballot(u < before && keys[u] > T));
+      }
+      count.add(c);
+      int ties = want - c[0];   // of those at T the first
+      // page by page, in order: one wave
+      if (w == 0) {
+        int at = 0;
+        for (int k = 0; k < n_words; ++k) {
+          const unsigned long long m = border[k], below = m & ((1ull << lane) - 1);
+          const bool is = (m >> lane) & 1;
+          const unsigned long long x = is ? keys[at + __popcll(below)] : 0;
+          const unsigned long long equal = __ballot(is && x == T), above = __ballot(is && x > T);
+          const bool tie = is && x == T && __popcll(equal & ((1ull << lane) - 1)) < ties;
+          const unsigned long long got = above | __ballot(tie);
+          const int used = __popcll(equal);
+          ties = ties > used ? ties - used : 0;
+          if (lane == 0) take[k] |= got;
+          at += __popcll(m);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // in the pages' order: a wave takes 64 words at a time
+  int before = 0;
+  for (int k0 = 0; k0 < n_words; k0 += 64) {
+    const unsigned long long m = k0 + lane < n_words ? take[k0 + lane] : 0;
+    int up = __popcll(m);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int x = __shfl_up(up, d, 64);
+      up += lane >= d ? x : 0;
+    }
+    const int mine = before + up - __popcll(m);
+    for (int k = k0 + w; k < k0 + 64 && k < n_words; k += W) {
+      const unsigned long long word = take[k];
+      const int at = __shfl(mine, k - k0, 64) + __popcll(word & ((1ull << lane) - 1));
+      if ((word >> lane) & 1) to[at] = 64 * k + lane;
+    }
+    before += __shfl(up, 63, 64);
+  }
+  for (int k = before + threadIdx.x; k < a.n; k += 64 * W) to[k] = -1;
+}
+
+// ---------------------------------------------------------------------- host
+static int check_bounds(const char *op, const void *bounds) {
+  if (!bounds || (uintptr_t)bounds % 16) return set_err(BFP_EINVAL, "%s: bounds are null or not 16-byte aligned", op);
+  return BFP_OK;
+}
+
+constexpr size_t PICK_SCRATCH = (size_t)256 << 20;   // at most, unless one row of each sequence needs more
+struct PickPlan {
+  int rows, chunks;   // rows of a sequence in a piece
+  size_t scores, work;
+};
+static PickPlan plan_pick(const bfp_kv4 &c, const bfp_kv4_batch &b) {
+  PickPlan p;
+  p.chunks = (b.width + SCORE_CHUNK - 1) / SCORE_CHUNK;
+  const int rows = b.max_q < b.n_rows ? b.max_q : b.n_rows;
+  const size_t row = (size_t)b.n_seq * c.heads * ((size_t)b.width + p.chunks) * sizeof(float);
+  size_t most = PICK_SCRATCH / row;
+  if (most >= 16) most = most / 16 * 16;
+  p.rows = most < 1 ? 1 : most < (size_t)rows ? (int)most : rows;
+  p.scores = (size_t)b.n_seq * p.rows * c.heads * b.width;
+  p.work = (p.scores + (size_t)b.n_seq * p.rows * c.heads * p.chunks) * sizeof(float);
+  return p;
+}
+
+static int check_pick(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q) {
+  BFP_TRY(check_kv4(op, cache, batch));
+  if (!q || q->heads < cache->heads || q->heads % cache->heads || q->heads > 65536)
+    return set_err(BFP_EINVAL, "%s: q has %d heads, the cache %d", op, q ? q->heads : 0, cache->heads);
+  BFP_TRY(check_rows(op, "q", q, q->heads, cache->hd, true, batch->n_rows));
+  if (!rows_aligned(*q, 8, batch->n_rows)) return set_err(BFP_EINVAL, "%s: q needs 16-byte alignment and strides in multiples of 8", op);
+  // a bit a page, twice, and the border's scores have to fit the LDS
+  if (batch->width > 16384) return set_err(BFP_EINVAL, "%s: width=%d pages, at most 16384", op, batch->width);
+  return BFP_OK;
+}
+
+typedef void (*score_fn)(Kv4PickArgs);
+template <int R>
+static score_fn score_kernel(int k) {
+  static const score_fn fn[16] = {k_kv4_score<R, 1>,  k_kv4_score<R, 2>,  k_kv4_score<R, 3>,  k_kv4_score<R, 4>,
+                                  k_kv4_score<R, 5>,  k_kv4_score<R, 6>,  k_kv4_score<R, 7>,  k_kv4_score<R, 8>,
+                                  k_kv4_score<R, 9>,  k_kv4_score<R, 10>, k_kv4_score<R, 11>, k_kv4_score<R, 12>,
+                                  k_kv4_score<R, 13>, k_kv4_score<R, 14>, k_kv4_score<R, 15>, k_kv4_score<R, 16>};
+  return fn[k - 1];
+}
+
+}  // namespace bfp
+
+using namespace bfp;
+
+extern "C" {
+
+int bfp_kv4_bounds_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, uint16_t *bounds, void *stream) {
+  const char *op = "kv4_bounds";
+  BFP_TRY(check_kv4(op, cache, batch));
+  BFP_TRY(check_bounds(op, bounds));
+  if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
+  Kv4BoundArgs a{};
+  a.c = *cache;
+  a.b = *batch;
+  a.bounds = bounds;
+  const int rows = batch->max_q < batch->n_rows ? batch->max_q : batch->n_rows;
+  a.touched = (int)(((long long)rows + cache->page - 2) / cache->page + 1);
+  a.touched = a.touched < batch->width ? a.touched : batch->width;
+  a.lanes_shift = __builtin_ctz((unsigned)cache->page) - 2;
+  const int each = 64 >> a.lanes_shift, groups = (cache->hd / 16 + each - 1) / each;
+  a.by_group = FastDiv(groups);
+  a.by_head = FastDiv(cache->heads);
+  a.by_touched = FastDiv(a.touched);
+  a.n_units = (long long)batch->n_seq * a.touched * cache->heads * groups;
+  if (a.n_units > 0x3ffffff) return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, batch->n_seq, batch->max_q);
+  hipLaunchKernelGGL(k_kv4_bounds, dim3((unsigned)((a.n_units + BOUND_T / 64 - 1) / (BOUND_T / 64))), dim3(BOUND_T), 0,
+                     (hipStream_t)stream, a);
+  return launch_status(op);
+}
+
+size_t bfp_kv4_select_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q) {
+  if (check_pick("kv4_select_work", cache, batch, q) || batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return 0;
+  return plan_pick(*cache, *batch).work;
+}
+
+int bfp_kv4_select_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const uint16_t *bounds, const bfp_rows *q, int n, int first,
+                     int last, int32_t *picks, void *work, size_t work_bytes, void *stream) {
+  const char *op = "kv4_select";
+  BFP_TRY(check_pick(op, cache, batch, q));
+  BFP_TRY(check_bounds(op, bounds));
+  if (n < 1 || (long long)n * cache->page > KV4_MAX_POS || first < 0 || last < 1 || first > n - last)
+    return set_err(BFP_EINVAL, "%s: n=%d pages, first=%d and last=%d of them", op, n, first, last);
+  if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
+  if (!picks || (uintptr_t)picks % 4) return set_err(BFP_EINVAL, "%s: picks are null or not aligned", op);
+  const PickPlan p = plan_pick(*cache, *batch);
+  if (!work || (uintptr_t)work % 16 || work_bytes < p.work)
+    return set_err(BFP_EINVAL, "%s: needs %zu bytes of 16-byte-aligned scratch, got %zu", op, p.work, work ? work_bytes : (size_t)0);
+  const int rows = batch->max_q < batch->n_rows ? batch->max_q : batch->n_rows;
+  const int R = p.rows > 4 ? 16 : 4;
+  const long long tiles = (p.rows + R - 1) / R, blocks = tiles * p.chunks * batch->n_seq, pick_blocks = (long long)p.rows * batch->n_seq;
+  // 2^32 threads a launch
+  if (blocks * cache->heads > 0xffffff || pick_blocks * cache->heads > 0x3fffff)
+    return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, batch->n_seq, batch->max_q);
+  Kv4PickArgs a{};
+  a.c = *cache;
+  a.b = *batch;
+  a.q = *q;
+  a.bounds = bounds;
+  a.group = q->heads / cache->heads;
+  a.rows = p.rows;
+  a.n = n, a.first = first, a.last = last;
+  a.chunks = p.chunks;
+  a.by_chunk = FastDiv(p.chunks);
+  a.by_tile = FastDiv((uint32_t)tiles);
+  a.score = (float *)work;
+  a.off = a.score + p.scores;
+  a.picks = picks;
+  const score_fn score = R == 4 ? score_kernel<4>(cache->hd / 16) : score_kernel<16>(cache->hd / 16);
+  const size_t lds = (size_t)(batch->width + 63) / 64 * 16 + (size_t)batch->width * 8;
+  // few workgroups: more waves each
+  const bool wide = pick_blocks * cache->heads <= 512;
+  const score_fn pick = wide ? k_kv4_pick<16> : k_kv4_pick<4>;
+  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void *)pick, hipFuncAttributeMaxDynamicSharedMemorySize, 140 * 1024));
+  for (a.i0 = 0; a.i0 < rows; a.i0 += p.rows) {
+    hipLaunchKernelGGL(score, dim3((unsigned)blocks, cache->heads), dim3(64 * SCORE_W), 0, (hipStream_t)stream, a);
+    BFP_TRY(launch_status(op));
+    hipLaunchKernelGGL(pick, dim3((unsigned)pick_blocks, cache->heads), dim3(wide ? 1024 : 256), lds, (hipStream_t)stream, a);
+    BFP_TRY(launch_status(op));
+  }
+  return BFP_OK;
+}
+
+}  // extern "C"
