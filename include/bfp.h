@@ -652,6 +652,27 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
 size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_rows *q,
                          const bfp_rows *out, int window);
 
+/* Sequences that share their first tokens, in groups of neighbours: sequences
+ * start[g] .. start[g+1]-1 of a batch have their first len[g] tokens in common,
+ * position p of them in page pages[g*width + p/page].  start (n_groups + 1,
+ * ascending), len (n_groups) and pages are device arrays of int32.  max_rows:
+ * no group has more new rows (0: n_rows); max_len: none shares more (0: width
+ * * page) -- it only chooses how the work is split.  Sequences outside every
+ * group share nothing. */
+typedef struct bfp_kv4_shared {
+  const int32_t *pages, *start, *len;
+  int n_groups, width, max_rows, max_len;
+} bfp_kv4_shared;
+/* bfp_kv4_attn_d where positions 0 .. len[g]-1 of a group's sequences are read
+ * from the group's pages, once for all of the group's rows, and only the later
+ * ones from each sequence's own: the entries of a sequence's table before
+ * position len[g] are not looked at.  A row sees of the shared tokens those up
+ * to its own position and within its window, as of any. */
+int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,
+                          const bfp_rows *out, double scale, int window, void *work, size_t work_bytes, void *stream);
+size_t bfp_kv4_attn_shared_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,
+                                const bfp_rows *out, int window);
+
 /* Bounds of each page's keys: bounds (n_pages, heads, 2, hd) bfloat16, 16-byte
  * aligned, hold the least key of every channel and then the largest, over the
  * tokens of the page; exact, but NaN for a tile that has a NaN in any token

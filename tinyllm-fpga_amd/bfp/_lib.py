@@ -56,6 +56,12 @@ class Kv4BatchC(C.Structure):
                 ("n_rows", C.c_int), ("width", C.c_int), ("max_q", C.c_int), ("max_len", C.c_int)]
 
 
+class Kv4SharedC(C.Structure):
+    """struct bfp_kv4_shared."""
+    _fields_ = [("pages", C.c_void_p), ("start", C.c_void_p), ("len", C.c_void_p), ("n_groups", C.c_int),
+                ("width", C.c_int), ("max_rows", C.c_int), ("max_len", C.c_int)]
+
+
 class PageArrayC(C.Structure):
     """struct bfp_page_array."""
     _fields_ = [("p", C.c_void_p), ("bytes", C.c_longlong)]
@@ -73,6 +79,7 @@ class PageTableC(C.Structure):
 
 
 _rows, _kv4, _kvb = C.POINTER(RowsC), C.POINTER(Kv4C), C.POINTER(Kv4BatchC)
+_shared = C.POINTER(Kv4SharedC)
 _pool, _tables = C.POINTER(PagesC), C.POINTER(PageTableC)
 
 # name -> (restype, argtypes); the list of exported symbols is checked by the
@@ -146,6 +153,8 @@ SIGNATURES = {
     "bfp_kv4_read_d": (i32, [_kv4, _kvb, _rows, _rows, vp]),
     "bfp_kv4_attn_d": (i32, [_kv4, _kvb, _rows, _rows, C.c_double, i32, vp, sz, vp]),
     "bfp_kv4_attn_work": (sz, [_kv4, _kvb, _rows, _rows, i32]),
+    "bfp_kv4_attn_shared_d": (i32, [_kv4, _kvb, _shared, _rows, _rows, C.c_double, i32, vp, sz, vp]),
+    "bfp_kv4_attn_shared_work": (sz, [_kv4, _kvb, _shared, _rows, _rows, i32]),
     "bfp_kv4_bounds_d": (i32, [_kv4, _kvb, vp, vp]),
     "bfp_kv4_select_d": (i32, [_kv4, _kvb, vp, _rows, i32, i32, i32, vp, vp, sz, vp]),
     "bfp_kv4_select_work": (sz, [_kv4, _kvb, _rows]),

@@ -19,12 +19,12 @@ import math
 import torch
 
 from . import _rows
-from ._lib import Kv4BatchC, Kv4C, lib
+from ._lib import Kv4BatchC, Kv4C, Kv4SharedC, lib
 from .rotary import check_table
 
 TILE = 16
-_append, _read, _attend, _attend_picks, _bounds, _select = (
-    _rows.Entry(f"bfp_kv4_{name}_d") for name in ("append", "read", "attn", "attn_picks", "bounds", "select"))
+_append, _read, _attend, _attend_shared, _attend_picks, _bounds, _select = (
+    _rows.Entry(f"bfp_kv4_{name}_d") for name in ("append", "read", "attn", "attn_shared", "attn_picks", "bounds", "select"))
 
 
 def _window(n):
@@ -71,6 +71,30 @@ class Batch(_rows.Fixed):
                           n_rows, self.pages.shape[1], self.max_q, self.max_len)
             self._made = (n_rows, c)
         return C.byref(c)
+
+
+class Shared(_rows.Fixed):
+    """Groups of a batch's sequences that share their first tokens: sequences
+    start[g] .. start[g + 1] - 1 have lens[g] tokens in common, position p of
+    them in page pages[g, p // page].  pages (groups, width), start (groups +
+    1, ascending) and lens are int32 tensors on the device, read when a call
+    runs, as a Batch's.  max_rows: the most new rows a group has (0: all);
+    max_len: the most tokens one shares (0: the table's width), which only
+    chooses how the work is split.  Sequences outside every group share
+    nothing."""
+
+    def __init__(self, pages, start, lens, max_rows=0, max_len=0):
+        if pages.dim() != 2 or pages.shape[1] < 1 or pages.shape[0] < 1:
+            raise ValueError(f"pages has shape {tuple(pages.shape)}, not (groups, width)")
+        n = pages.shape[0]
+        for t, what, shape in ((pages, "pages", tuple(pages.shape)), (start, "start", (n + 1,)), (lens, "lens", (n,))):
+            if tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous() or t.device != pages.device \
+                    or not t.is_cuda:
+                raise ValueError(f"{what} must be a contiguous int32 tensor {shape} on one GPU")
+        self.pages, self.start, self.lens, self.device = pages, start, lens, pages.device
+        self.max_rows, self.max_len = _rows.c_int(max_rows, "max_rows"), _rows.c_int(max_len, "max_len")
+        self._made = Kv4SharedC(pages.data_ptr(), start.data_ptr(), lens.data_ptr(), n, pages.shape[1], self.max_rows, self.max_len)
+        self._c = C.byref(self._made)
 
 
 class Fp4Cache(_rows.Fixed):
@@ -197,7 +221,7 @@ class Fp4Cache(_rows.Fixed):
             _read(self.device, self._c, batch._c(n), *rs)
         return k, v
 
-    def attend(self, batch, q, scale=None, window=0, out=None, dtype=None, work=None, picks=None):
+    def attend(self, batch, q, scale=None, window=0, out=None, dtype=None, work=None, shared=None, picks=None):
         """softmax(scale q k^T) v of every row of q (rows, query heads, hd)
         over its sequence's cached tokens up to its own, the last `window` of
         them (0: all).  scale: 1/sqrt(hd) by default.  Query heads share KV
@@ -210,15 +234,21 @@ class Fp4Cache(_rows.Fixed):
         work: uint8 scratch of attend_work() bytes (allocated per call
         otherwise).
 
+        shared: a Shared that says which sequences have their first tokens in
+        common; those are read from its pages, once for a group's rows, and
+        the sequences' own tables are looked at behind them alone.
+
         picks: int32 (rows, KV heads, n), as PageBounds.select gives them: a
         row sees, of those tokens, the ones in the listed pages of its
         sequence's table (any order, each once; -1 for none).  No window
-        then."""
+        and no shared then."""
         dev = self.device
         t, qr, out, orow = self._attend_rows(batch, q, out, dtype)
         n = t.shape[0]
         if picks is not None:
-            n_picks = self._picks(picks, n, window)
+            n_picks = self._picks(picks, n, window, shared)
+        elif shared is not None and shared.device != dev:
+            raise ValueError(f"the groups are on {shared.device}, the cache on {dev}")
         if n == 0:
             return out
         b, qb, ob, window = batch._c(n), C.byref(qr), C.byref(orow), _window(window)
@@ -226,6 +256,8 @@ class Fp4Cache(_rows.Fixed):
         if work is None:
             if picks is not None:
                 size = lib().bfp_kv4_attn_picks_work(self._c, b, n_picks, qb, ob)
+            elif shared is not None:
+                size = lib().bfp_kv4_attn_shared_work(self._c, b, shared._c, qb, ob, window)
             else:
                 size = lib().bfp_kv4_attn_work(self._c, b, qb, ob, window)
             if size:
@@ -235,16 +267,18 @@ class Fp4Cache(_rows.Fixed):
         p = work.data_ptr() if work is not None else None
         if picks is not None:
             _attend_picks(dev, self._c, b, picks.data_ptr(), n_picks, qb, ob, scale, p, size)
+        elif shared is not None:
+            _attend_shared(dev, self._c, b, shared._c, qb, ob, scale, window, p, size)
         else:
             _attend(dev, self._c, b, qb, ob, scale, window, p, size)
         return out
 
-    def _picks(self, picks, n, window):
+    def _picks(self, picks, n, window, shared):
         if picks.dim() != 3 or tuple(picks.shape[:2]) != (n, self.heads) or picks.dtype != torch.int32 \
                 or not picks.is_contiguous() or picks.device != self.device:
             raise ValueError(f"picks must be a contiguous int32 tensor ({n}, {self.heads}, pages) on {self.device}")
-        if window:
-            raise ValueError("picks and a window")
+        if window or shared is not None:
+            raise ValueError("picks go with no window and no shared prefix")
         return picks.shape[2]
 
     def _attend_rows(self, batch, q, out, dtype, make=True):
@@ -263,13 +297,15 @@ class Fp4Cache(_rows.Fixed):
             orow = _rows.rows(out, "out", self.device)
         return t, qr, out, orow
 
-    def attend_work(self, batch, q, out=None, dtype=None, window=0, picks=None):
+    def attend_work(self, batch, q, out=None, dtype=None, window=0, shared=None, picks=None):
         """Scratch bytes attend() needs for such a call."""
         t, qr, _, orow = self._attend_rows(batch, q, out, dtype, make=False)
         orow.p = orow.p or 16   # the size depends on no address
         if picks is not None:
-            n_picks = self._picks(picks, t.shape[0], window)
+            n_picks = self._picks(picks, t.shape[0], window, shared)
             return lib().bfp_kv4_attn_picks_work(self._c, batch._c(t.shape[0]), n_picks, C.byref(qr), C.byref(orow))
+        if shared is not None:
+            return lib().bfp_kv4_attn_shared_work(self._c, batch._c(t.shape[0]), shared._c, C.byref(qr), C.byref(orow), _window(window))
         return lib().bfp_kv4_attn_work(self._c, batch._c(t.shape[0]), C.byref(qr), C.byref(orow), _window(window))
 
 

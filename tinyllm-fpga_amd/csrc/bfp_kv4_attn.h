@@ -25,6 +25,14 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
+// What a launch's rows see.
+enum Kv4Sees {
+  SEES_ALL,      // their sequence up to their position
+  SEES_PICKS,    // of that the pages that a list of each row and KV head names
+  SEES_PREFIX,   // of that what their sequence's group shares: one "sequence" is a group's rows
+  SEES_REST      // of that what lies behind the shared tokens
+};
+
 struct Kv4AttnArgs {
   bfp_kv4 c;
   bfp_kv4_batch b;
@@ -58,6 +66,15 @@ struct Kv4AttnArgs {
   // listed pages: n_picks a row and KV head, and the row tiles of a token's query heads
   const int32_t *picks;
   int n_picks, token_tiles;
+  // Shared prefixes.  SEES_PREFIX: b's sequences are the groups (pages, width,
+  // n_seq, max_q), its start and len still the batch's.  Both launches leave
+  // unfinished rows in part_o [row][query head][slot][hd], sum_slots of them a
+  // row, from sum_slot on, and part_ml; k_kv4_rows its own parts in slot_o, slot_ml.
+  bfp_kv4_shared sh;
+  int sh_seqs;   // sequences of the batch
+  int sum_slots, sum_slot;
+  float *slot_o;
+  float2 *slot_ml;
 };
 
 // Position p's visible keys are [lo, hi).
@@ -65,6 +82,82 @@ __device__ __forceinline__ int key_hi(int p) { return p < 0 ? 0 : p + 1; }
 __device__ __forceinline__ int key_lo(int hi, int window) {
   return window > 0 && hi > window ? hi - window : 0;
 }
+
+// Group g's sequences, within the batch.
+struct Kv4Group {
+  int first, stop;
+};
+__device__ __forceinline__ Kv4Group kv4_group(const Kv4AttnArgs &a, int g) {
+  const int f = a.sh.start[g], t = a.sh.start[g + 1];
+  Kv4Group x;
+  x.first = f < 0 ? 0 : f < a.sh_seqs ? f : a.sh_seqs;
+  x.stop = t < x.first ? x.first : t < a.sh_seqs ? t : a.sh_seqs;
+  return x;
+}
+// The rows of a group, as one sequence's, and the tokens that they share and
+// the pages have room for (at).
+__device__ __forceinline__ Kv4Span kv4_group_span(const Kv4AttnArgs &a, int g, Kv4Group &x) {
+  x = kv4_group(a, g);
+  Kv4Span s = kv4_span(a.b.start[x.first], a.b.start[x.stop], 0, a.b.n_rows, a.b.max_q);
+  const long long cap = (long long)a.b.width << a.page_shift;
+  const int len = a.sh.len[g];
+  s.at = len < 0 ? 0 : len < cap ? len : (int)cap;
+  return s;
+}
+// The least position that any row of a group sees.
+__device__ __forceinline__ int kv4_group_low(const Kv4AttnArgs &a, const Kv4Group &x) {
+  if (a.window == 0) return 0;
+  int low = 0x7fffffff;
+#pragma unroll 4
+  for (int b = x.first; b < x.stop; ++b) {
+    const int len = a.b.len[b], n = a.b.start[b + 1] - a.b.start[b];
+    const int at = len > n ? len - n : 0;
+    if (len > 0 && n > 0) low = key_lo(key_hi(at), a.window) < low ? key_lo(key_hi(at), a.window) : low;
+  }
+  return low == 0x7fffffff ? 0 : low;
+}
+// The tokens that sequence b's group shares, 0 outside every group.
+__device__ __forceinline__ int kv4_shared_len(const Kv4AttnArgs &a, int b) {
+  int g = 0, past = a.sh.n_groups;   // the last group that begins at b or before
+  while (past - g > 1) {
+    const int mid = g + (past - g) / 2;
+    (a.sh.start[mid] <= b ? g : past) = mid;
+  }
+  const int n = a.sh.len[g];
+  return a.sh.start[g] <= b && b < a.sh.start[g + 1] && n > 0 ? n : 0;
+}
+// The position of row t of a group: of the sequence in which it lies.  Lane x
+// < N of every N neighbouring ones has the wave's x-th row; each gets its own's.
+template <int N>
+__device__ __forceinline__ int kv4_row_position(const Kv4AttnArgs &a, const Kv4Group &x, int t) {
+  const int lane = threadIdx.x & 63;
+  int n = 0;
+  for (int b0 = x.first; b0 < x.stop; b0 += 64) {
+    const int past = b0 + lane < x.stop ? a.b.start[b0 + lane + 1] : 0x7fffffff;   // the first row behind sequence b0 + lane
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int c = __popcll(__ballot(past <= __builtin_amdgcn_readlane(t, k)));
+      n += lane % N == k ? c : 0;
+    }
+  }
+  const int b = x.first + n < x.stop ? x.first + n : x.stop - 1;
+  if (b < x.first) return -1;
+  const int len = a.b.len[b];
+  const long long p = (long long)(len < 0 ? 0 : len) - a.b.start[b + 1] + t;
+  return p < 0 ? -1 : (int)(p < KV4_MAX_POS ? p : KV4_MAX_POS);
+}
+
+// Over N neighbouring lanes (16 or 32).
+template <int N>
+__device__ __forceinline__ int min_lanes(int v) {
+  if (N == 32) v = min(v, peer<16>(v));
+  v = min(v, peer<8>(v));
+  v = min(v, peer<4>(v));
+  v = min(v, peer<2>(v));
+  return min(v, peer<1>(v));
+}
+template <int N>
+__device__ __forceinline__ int max_lanes(int v) { return -min_lanes<N>(-v); }
 
 // The tiles of split `split` out of a row tile's n: chunks as long as the
 // longest sequence's splits are, so that workgroups take equally long
@@ -237,9 +330,16 @@ struct AttnKernel {
 AttnKernel rows_kernel(int tiles, int terms, int waves);
 AttnKernel picks_kernel(int tiles, int terms, int waves);
 AttnKernel prompt_kernel(int tiles, int terms);
+// Of a shared prefix, and of what lies behind it.
+AttnKernel prefix_rows_kernel(int tiles, int terms, int waves);
+AttnKernel prefix_prompt_kernel(int tiles, int terms);
+AttnKernel rest_rows_kernel(int tiles, int terms, int waves);
+AttnKernel rest_prompt_kernel(int tiles, int terms);
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }
 // Queues the kernel that joins what k_kv4_prompt left in pieces.
 void launch_join_prompt(const Kv4AttnArgs &a, hipStream_t s);
+// The same of a row's two parts.
+void launch_join_shared(const Kv4AttnArgs &a, hipStream_t s);
 
 }  // namespace bfp

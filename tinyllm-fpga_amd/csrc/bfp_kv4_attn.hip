@@ -39,13 +39,22 @@ static int terms_of(const bfp_rows &q, const bfp_rows &out, int rows) {
   return q.type == BFP_BF16 && out.type == BFP_BF16 && rows > 8 ? 1 : 2;
 }
 
-static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_rows &q, const bfp_rows &out, int window) {
+// The longest sequence's keys that any of its rows sees, from position `from` on.
+static long long keys_of(const bfp_kv4 &c, const bfp_kv4_batch &b, int window, long long from) {
+  const long long cap = (long long)b.width * c.page;
+  long long keys = (b.max_len > 0 && b.max_len < cap ? b.max_len : cap) - from;
+  keys = keys < 1 ? 1 : keys;
+  return window > 0 && keys > (long long)window + b.max_q ? (long long)window + b.max_q : keys;
+}
+
+// keys: of the longest sequence; whole: all rows see all of them, else up to
+// their own; most: splits.
+static Kv4Plan plan_keys(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_rows &q, const bfp_rows &out, long long keys, bool whole,
+                         int most) {
   Kv4Plan p{};
   const int group = q.heads / c.heads, tiles = c.hd / 16;
   const long long rows = (long long)b.max_q * group;
   const long long cap = (long long)b.width * c.page;
-  long long keys = b.max_len > 0 && b.max_len < cap ? b.max_len : cap;
-  if (window > 0 && keys > (long long)window + b.max_q) keys = (long long)window + b.max_q;
   const long long key_tiles = (keys + KEYS - 1) / KEYS;
   p.chunk = (int)key_tiles;
   p.splits = 1;
@@ -63,7 +72,7 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   const bool wide = q.type == BFP_F32 || out.type == BFP_F32 || out.type == BFP_TILES;
   const int size = tiles <= 4 ? 0 : tiles <= 8 ? 1 : tiles <= 12 ? 2 : 3;
   const long long all_rows = (b.n_rows < (long long)b.n_seq * b.max_q ? b.n_rows : (long long)b.n_seq * b.max_q) * group * c.heads;
-  const double seen = key_tiles - 0.5 * ((b.max_q < keys ? b.max_q : keys) / KEYS);   // on average
+  const double seen = whole ? key_tiles : key_tiles - 0.5 * ((b.max_q < keys ? b.max_q : keys) / KEYS);   // on average
   const double cus = 256.0;
   Kv4Plan few = p;
   {
@@ -101,7 +110,7 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
     const long long groups = (long long)p.row_tiles * c.heads * b.n_seq;
     long long s = groups > 0 ? 256 / groups : 1;
     if (s > key_tiles / 4) s = key_tiles / 4;
-    if (s > 64) s = 64;   // a lane of k_kv4_join_prompt each
+    if (s > most) s = most;   // a lane of the joining wave each
     if (s > 1) {
       p.splits = (int)s;
       p.chunk = (int)((key_tiles + s - 1) / s);
@@ -112,6 +121,40 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   }
   if (few.us <= p.us) p = few;
   p.work = p.cells * (16 * tiles * sizeof(float) + sizeof(float2)) + 2 * p.stream * sizeof(unsigned long long);
+  return p;
+}
+
+static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_rows &q, const bfp_rows &out, int window) {
+  return plan_keys(c, b, q, out, keys_of(c, b, window, 0), false, 64);
+}
+
+// Shared prefixes: the groups' rows as sequences against the groups' tokens,
+// then every sequence's tokens behind them; the parts of a row side by side.
+struct SharedPlan {
+  Kv4Plan prefix, rest;
+  bfp_kv4_batch groups;
+  int slots;
+  size_t sums, own, work;   // parts of rows; bytes of the launches' own parts
+};
+static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_kv4_shared &sh, const bfp_rows &q, const bfp_rows &out,
+                              int window) {
+  SharedPlan p;
+  p.groups = b;
+  p.groups.pages = sh.pages;
+  p.groups.n_seq = sh.n_groups;
+  p.groups.width = sh.width;
+  p.groups.max_len = sh.max_len;
+  p.groups.max_q = sh.max_rows > 0 && sh.max_rows < b.n_rows ? sh.max_rows : b.n_rows;
+  const long long prefix = keys_of(c, p.groups, window, 0);
+  p.prefix = plan_keys(c, p.groups, q, out, prefix, true, 48);
+  const long long cap = (long long)sh.width * c.page;
+  p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len > 0 && sh.max_len < cap ? sh.max_len : cap), false, 16);
+  p.slots = p.prefix.splits + p.rest.splits;
+  p.sums = (size_t)b.n_rows * q.heads * p.slots;
+  // (a split launch's parts are the rows', not its own)
+  const size_t one = p.prefix.splits > 1 ? 0 : p.prefix.work, two = p.rest.splits > 1 ? 0 : p.rest.work;
+  p.own = one > two ? one : two;
+  p.work = p.sums * (c.hd * sizeof(float) + sizeof(float2)) + p.own;
   return p;
 }
 
@@ -196,18 +239,16 @@ static int attn_args(const char *op, Kv4AttnArgs &a, const bfp_kv4 &cache, const
   return BFP_OK;
 }
 
-static int launch_attn(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, void *work, size_t work_bytes, hipStream_t s) {
-  if (p.work && (!work || (uintptr_t)work % 16 || work_bytes < p.work))
-    return set_err(BFP_EINVAL, "%s: needs %zu bytes of 16-byte-aligned scratch, got %zu", op, p.work, work ? work_bytes : (size_t)0);
+static int check_work(const char *op, size_t need, const void *work, size_t work_bytes) {
+  if (need && (!work || (uintptr_t)work % 16 || work_bytes < need))
+    return set_err(BFP_EINVAL, "%s: needs %zu bytes of 16-byte-aligned scratch, got %zu", op, need, work ? work_bytes : (size_t)0);
+  return BFP_OK;
+}
+
+static int launch_plan(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, hipStream_t s) {
   a.splits = p.splits;
   a.chunk = p.chunk;
   a.stream = p.stream;
-  if (p.work) {
-    a.part_o = (float *)work;
-    a.part_ml = (float2 *)((float *)work + p.cells * 16 * a.tiles);
-    a.there = (unsigned long long *)(a.part_ml + p.cells);
-    a.number = call_number();
-  }
   a.row_tiles = p.row_tiles;
   a.by_split = FastDiv(p.splits);
   const long long each = (long long)p.row_tiles * p.splits * a.c.heads, blocks = p.stream ? p.stream : each * a.b.n_seq;
@@ -218,6 +259,43 @@ static int launch_attn(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const A
     HIP_TRY(hipFuncSetAttribute((const void *)k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024));
   hipLaunchKernelGGL(k.fn, dim3((unsigned)blocks), dim3(64 * p.waves), k.lds, s, a);
   return launch_status(op);
+}
+
+static int launch_attn(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, void *work, size_t work_bytes, hipStream_t s) {
+  BFP_TRY(check_work(op, p.work, work, work_bytes));
+  if (p.work) {
+    a.part_o = (float *)work;
+    a.part_ml = (float2 *)((float *)work + p.cells * 16 * a.tiles);
+    a.there = (unsigned long long *)(a.part_ml + p.cells);
+    a.number = call_number();
+  }
+  return launch_plan(op, a, p, k, s);
+}
+
+// One of the two parts: its slots of the rows' parts, and its own workspace.
+static int launch_part(const char *op, Kv4AttnArgs a, const Kv4Plan &p, const AttnKernel &k, int slot, void *own, hipStream_t s) {
+  a.sum_slot = slot;
+  if (p.stream) {
+    a.slot_o = (float *)own;
+    a.slot_ml = (float2 *)((float *)own + p.cells * 16 * a.tiles);
+    a.there = (unsigned long long *)(a.slot_ml + p.cells);
+    a.number = call_number();
+  }
+  return launch_plan(op, a, p, k, s);
+}
+
+static int check_shared(const char *op, const bfp_kv4_batch *b, const bfp_kv4_shared *sh, const bfp_kv4 *c, const bfp_rows *q) {
+  if (!sh || !sh->pages || !sh->start || !sh->len) return set_err(BFP_EINVAL, "%s: no groups", op);
+  if (((uintptr_t)sh->pages | (uintptr_t)sh->start | (uintptr_t)sh->len) % 4)
+    return set_err(BFP_EINVAL, "%s: the groups' arrays are not aligned", op);
+  if (sh->n_groups < 1 || sh->n_groups > 65535 || sh->width < 1 || sh->max_rows < 0 || sh->max_len < 0)
+    return set_err(BFP_EINVAL, "%s: n_groups=%d (1 to 65535), width=%d, max_rows=%d, max_len=%d", op, sh->n_groups, sh->width,
+                   sh->max_rows, sh->max_len);
+  if ((long long)sh->width * c->page > KV4_MAX_POS)
+    return set_err(BFP_EINVAL, "%s: width=%d pages of %d are more than %d positions", op, sh->width, c->page, KV4_MAX_POS);
+  if ((long long)b->n_rows * (q->heads / c->heads) > 0x3fffffffLL && (sh->max_rows == 0 || (long long)sh->max_rows * (q->heads / c->heads) > 0x3fffffffLL))
+    return set_err(BFP_EINVAL, "%s: groups of max_rows=%d rows of %d heads are too many", op, sh->max_rows, q->heads);
+  return BFP_OK;
 }
 
 }  // namespace bfp
@@ -245,6 +323,43 @@ int bfp_kv4_attn_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_r
                       (hipStream_t)stream));
   if (p.splits == 1) return BFP_OK;
   launch_join_prompt(a, (hipStream_t)stream);
+  return launch_status(op);
+}
+
+size_t bfp_kv4_attn_shared_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,
+                                const bfp_rows *out, int window) {
+  const char *op = "kv4_attn_shared_work";
+  if (check_attn(op, cache, batch, q, out, window, false) || check_shared(op, batch, shared, cache, q)) return 0;
+  if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return 0;
+  return plan_shared(*cache, *batch, *shared, *q, *out, window).work;
+}
+
+int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,
+                          const bfp_rows *out, double scale, int window, void *work, size_t work_bytes, void *stream) {
+  const char *op = "kv4_attn_shared";
+  BFP_TRY(check_attn(op, cache, batch, q, out, window, true));
+  BFP_TRY(check_shared(op, batch, shared, cache, q));
+  Kv4AttnArgs a;
+  BFP_TRY(attn_args(op, a, *cache, *batch, *q, *out, scale, window));
+  if (batch->n_seq == 0 || batch->max_q == 0 || batch->n_rows == 0) return BFP_OK;
+  const SharedPlan p = plan_shared(*cache, *batch, *shared, *q, *out, window);
+  BFP_TRY(check_work(op, p.work, work, work_bytes));
+  hipStream_t s = (hipStream_t)stream;
+  a.sh = *shared;
+  a.sh_seqs = batch->n_seq;
+  a.sum_slots = p.slots;
+  a.part_o = (float *)work;
+  a.part_ml = (float2 *)(a.part_o + p.sums * cache->hd);
+  void *own = a.part_ml + p.sums;
+  Kv4AttnArgs g = a;
+  g.b = p.groups;
+  const Kv4Plan &one = p.prefix, &two = p.rest;
+  BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms) : prefix_rows_kernel(a.tiles, one.terms, one.waves),
+                      0, own, s));
+  BFP_TRY(launch_part(op, a, two, two.prompt ? rest_prompt_kernel(a.tiles, two.terms) : rest_rows_kernel(a.tiles, two.terms, two.waves),
+                      one.splits, own, s));
+  a.sum_slot = one.splits;
+  launch_join_shared(a, s);
   return launch_status(op);
 }
 

@@ -4,6 +4,6 @@
 
 namespace bfp {
 
-AttnKernel picks_kernel(int tiles, int terms, int waves) { return rows_kernel_for<true>(tiles, terms, waves); }
+AttnKernel picks_kernel(int tiles, int terms, int waves) { return rows_kernel_for<SEES_PICKS>(tiles, terms, waves); }
 
 }  // namespace bfp

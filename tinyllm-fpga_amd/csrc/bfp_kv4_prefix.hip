@@ -1,0 +1,11 @@
+// Attention over a prefix that a group of sequences shares: the kernels of the
+// first part, all rows of a group against the group's pages.
+#include "bfp_kv4_prompt.h"
+#include "bfp_kv4_rows.h"
+
+namespace bfp {
+
+AttnKernel prefix_rows_kernel(int tiles, int terms, int waves) { return rows_kernel_for<SEES_PREFIX>(tiles, terms, waves); }
+AttnKernel prefix_prompt_kernel(int tiles, int terms) { return prompt_kernel_for<SEES_PREFIX>(tiles, terms); }
+
+}  // namespace bfp

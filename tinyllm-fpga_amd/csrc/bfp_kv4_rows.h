@@ -10,10 +10,12 @@
 // has to be turned over: its decoded tiles go through the wave's own piece of
 // LDS and come back with the transposing reads.
 //
-// PICK: every row and KV head sees the pages that a list of its own names (in
-// any order; each once) instead of all up to its position.  The keys of the
-// listed pages, one after the other, are the key tiles then, and a row tile
-// is one token's query heads.
+// SEES_PICKS: every row and KV head sees the pages that a list of its own names
+// (in any order; each once) instead of all up to its position.  The keys of
+// the listed pages, one after the other, are the key tiles then, and a row
+// tile is one token's query heads.
+// SEES_PREFIX, SEES_REST: the two parts of rows that share a prefix, left
+// unfinished.  All rows of a group are one sequence in the first.
 #pragma once
 #include "bfp_kv4_attn.h"
 
@@ -78,20 +80,27 @@ struct RowsSeq {
   int row0, n, at;     // Kv4Span
   int tile0, tiles;    // the keys that any of its rows sees, in tiles (at least one: somebody writes the zeros)
   int groups;          // row tiles x KV heads
+  int low;             // SEES_REST: the first position
+  Kv4Group of;         // SEES_PREFIX: the group
   __device__ uint32_t span() const { return (uint32_t)tiles + ROWS_EXTRA; }
 };
-template <bool PICK>
+template <Kv4Sees SEES>
 __device__ __forceinline__ RowsSeq rows_seq(const Kv4AttnArgs &a, int R, int b) {
-  const Kv4Span sp = kv4_span(a.b.start[b], a.b.start[b + 1], a.b.len[b], a.b.n_rows, a.b.max_q);
-  RowsSeq s{sp.row0, sp.n, sp.at, 0, 1, 0};
+  RowsSeq s;
+  const Kv4Span sp = SEES == SEES_PREFIX ? kv4_group_span(a, b, s.of)
+                                         : kv4_span(a.b.start[b], a.b.start[b + 1], a.b.len[b], a.b.n_rows, a.b.max_q);
+  s.row0 = sp.row0, s.n = sp.n, s.at = sp.at, s.tile0 = 0, s.tiles = 1, s.groups = 0;
+  if (SEES == SEES_REST) s.low = kv4_shared_len(a, b);
   if (sp.n == 0) return s;
-  if (PICK) {
+  if (SEES == SEES_PICKS) {
     s.tiles = (int)((((long long)a.n_picks << a.page_shift) + KEYS - 1) / KEYS);
     s.groups = sp.n * a.token_tiles * a.c.heads;
     return s;
   }
   const long long cap = (long long)a.b.width << a.page_shift;
-  const int hi = key_hi(sp.at + sp.n - 1), end = hi < cap ? hi : (int)cap, lo = key_lo(key_hi(sp.at), a.window);
+  const int hi = SEES == SEES_PREFIX ? sp.at : key_hi(sp.at + sp.n - 1), end = hi < cap ? hi : (int)cap;
+  int lo = SEES == SEES_PREFIX ? kv4_group_low(a, s.of) : key_lo(key_hi(sp.at), a.window);
+  if (SEES == SEES_REST) lo = lo > s.low ? lo : s.low;
   s.tile0 = lo / KEYS;
   s.tiles = end > lo ? (end + KEYS - 1) / KEYS - s.tile0 : 1;
   s.groups = (sp.n * a.group + R - 1) / R * a.c.heads;
@@ -105,12 +114,12 @@ struct Stream {
   uint32_t wave[4], longest[4];
   int last;
 };
-template <bool PICK>
+template <Kv4Sees SEES>
 __device__ __forceinline__ uint32_t stream_plan(const Kv4AttnArgs &a, int R, Stream &st) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   uint32_t n = 0, most = 0;
   if (t < a.b.n_seq) {
-    const RowsSeq s = rows_seq<PICK>(a, R, t);
+    const RowsSeq s = rows_seq<SEES>(a, R, t);
     n = (uint32_t)s.groups * s.span();
     most = (uint32_t)s.tiles;
   }
@@ -193,34 +202,46 @@ __device__ __forceinline__ bool arrive(unsigned long long *there, unsigned long 
 
 // C: head tiles a lane group holds (hd <= 64 C); T: terms of a row (columns
 // R = 16 / T rows share); W: waves.
-template <int C, int R, bool PICK>
+template <int C, int R, Kv4Sees SEES>
 __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, int head, int rt, uint32_t p0, int parts);
 
 // Where row tile rt's rows lie: rows rr0 .. rows - 1 of the KV head's, row rr
-// being query head rr % G of token rr / G (PICK: head rr of token i).
+// being query head rr % G of token rr / G (SEES_PICKS: head rr of token i).
 struct RowTile {
   int rr0, rows, i;
 };
-template <int R, bool PICK>
+template <int R, Kv4Sees SEES>
 __device__ __forceinline__ RowTile row_tile(const Kv4AttnArgs &a, const RowsSeq &sp, int rt) {
-  if (!PICK) return {rt * R, sp.n * a.group, 0};
+  if (SEES != SEES_PICKS) return {rt * R, sp.n * a.group, 0};
   const int i = rt / a.token_tiles, rr0 = (rt - i * a.token_tiles) * R;
   return {rr0, i < sp.n ? a.group : 0, i};
 }
-template <bool PICK>
-__device__ __forceinline__ int token_of(const Kv4AttnArgs &a, const RowTile &t, int rr) { return PICK ? t.i : rr / a.group; }
-template <bool PICK>
-__device__ __forceinline__ int head_of(const Kv4AttnArgs &a, int rr) { return PICK ? rr : rr % a.group; }
+template <Kv4Sees SEES>
+__device__ __forceinline__ int token_of(const Kv4AttnArgs &a, const RowTile &t, int rr) { return SEES == SEES_PICKS ? t.i : rr / a.group; }
+template <Kv4Sees SEES>
+__device__ __forceinline__ int head_of(const Kv4AttnArgs &a, int rr) { return SEES == SEES_PICKS ? rr : rr % a.group; }
 
-template <int C, int T, int W, bool PICK>
+// The workspace of a launch's own parts, and where unfinished rows go.
+template <Kv4Sees SEES>
+__device__ __forceinline__ float *slot_o(const Kv4AttnArgs &a) { return SEES >= SEES_PREFIX ? a.slot_o : a.part_o; }
+template <Kv4Sees SEES>
+__device__ __forceinline__ float2 *slot_ml(const Kv4AttnArgs &a) { return SEES >= SEES_PREFIX ? a.slot_ml : a.part_ml; }
+__device__ __forceinline__ void leave_sum(const Kv4AttnArgs &a, long long tok, int qh, int d, float2 ml, float v) {
+  const long long at = (tok * a.q.heads + qh) * a.sum_slots + a.sum_slot;
+  if (d == 0) a.part_ml[at] = ml;
+  a.part_o[at * (16 * a.tiles) + d] = v;
+}
+
+template <int C, int T, int W, Kv4Sees SEES>
 __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 2 : 1) void k_kv4_rows(Kv4AttnArgs a) {
   constexpr int R = 16 / T;
+  constexpr bool PICK = SEES == SEES_PICKS;
   extern __shared__ __align__(16) char lds[];
   __shared__ Stream st;
   int seq, head, rt, split;
   uint32_t x = 0, x_stop = 1, piece = 0;
   if (W == 4 && a.stream) {
-    piece = stream_plan<PICK>(a, R, st);
+    piece = stream_plan<SEES>(a, R, st);
     x = blockIdx.x * piece;
     const uint32_t all = st.before[a.b.n_seq];
     if (x >= all) return;
@@ -248,14 +269,14 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
     KvSide<C> k, v;
     int id = -1;
     long long at = 0;
-    const bool early = !PICK && !(W == 4 && a.stream) && a.window == 0;
+    const bool early = SEES == SEES_ALL && !(W == 4 && a.stream) && a.window == 0;
     if (early) {
       id = kv4_page(pages, a.b.width, a.c.n_pages, (w * KEYS + 4 * r) >> a.page_shift);
       at = offset_of(w, id);
       load_side(k, a.c.k, a.c.k_e, at, a.c.page, g * C, tiles);
       load_side(v, a.c.v, a.c.v_e, at, a.c.page, g * C, tiles);
     }
-    const RowsSeq sp = rows_seq<PICK>(a, R, seq);
+    const RowsSeq sp = rows_seq<SEES>(a, R, seq);
     int from = 0, upto = sp.tiles, slot = -1;
     uint32_t begin = 0;
     if (W == 4 && a.stream) {
@@ -278,19 +299,33 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
     } else {
       x = x_stop;
     }
-    const RowTile row_t = row_tile<R, PICK>(a, sp, rt);
+    const RowTile row_t = row_tile<R, SEES>(a, sp, rt);
     const int rows = row_t.rows, rr0 = row_t.rr0;   // rows of this KV head: (token, query head)
     if (rr0 >= rows) return;     // never with shared work
 
     // this lane's column
     const int rr = rr0 + r % R;
     const bool mine = rr < rows;
-    const int i = mine ? token_of<PICK>(a, row_t, rr) : 0, qh = head * G + (mine ? head_of<PICK>(a, rr) : 0);
-    const int hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
+    const int i = mine ? token_of<SEES>(a, row_t, rr) : 0, qh = head * G + (mine ? head_of<SEES>(a, rr) : 0);
+    int hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
     // what all of them see, and any of them
     const int last = (rr0 + R < rows ? rr0 + R : rows) - 1;
-    const int hi_min = key_hi(sp.at + rr0 / G), hi_max = key_hi(sp.at + last / G);
-    const int lo_min = key_lo(hi_min, a.window), lo_max = key_lo(hi_max, a.window);
+    int hi_min = key_hi(sp.at + rr0 / G), hi_max = key_hi(sp.at + last / G);
+    int lo_min = key_lo(hi_min, a.window), lo_max = key_lo(hi_max, a.window);
+    if constexpr (SEES == SEES_REST) {
+      lo = lo > sp.low ? lo : sp.low;
+      lo_min = lo_min > sp.low ? lo_min : sp.low;
+      lo_max = lo_max > sp.low ? lo_max : sp.low;
+    }
+    if constexpr (SEES == SEES_PREFIX) {   // rows of several sequences: by each one's position
+      const int ends = key_hi(kv4_row_position<R>(a, sp.of, sp.row0 + (rr < rows ? rr : rows - 1) / G));
+      lo = mine ? key_lo(ends, a.window) : 0;
+      hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
+      hi_min = min_lanes<16>(mine ? hi : 0x7fffffff);
+      hi_max = max_lanes<16>(hi);
+      lo_min = min_lanes<16>(mine ? lo : 0x7fffffff);
+      lo_max = max_lanes<16>(lo);
+    }
     const long long cap = (long long)a.b.width << a.page_shift;
     const int end = hi_max < cap ? hi_max : (int)cap;
     const int first = PICK ? from : sp.tile0 + from > lo_min / KEYS ? sp.tile0 + from : lo_min / KEYS;
@@ -586,11 +621,13 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
 #pragma unroll
       for (int k = 0; k < W; ++k)
         acc += __shfl(f, (lane & 48) + k, 64) * jf[k * stride + 32 + row * (hd + 4) + d];
-      const int ri = token_of<PICK>(a, row_t, rr0 + row), rh = head * G + head_of<PICK>(a, rr0 + row);
+      const int ri = token_of<SEES>(a, row_t, rr0 + row), rh = head * G + head_of<SEES>(a, rr0 + row);
       const long long tok = sp.row0 + ri;
       if (slot >= 0) {
-        if (d == 0) put(a.part_ml + slot * R + row, make_float2(M, L));
-        put(a.part_o + ((long long)slot * R + row) * hd + d, acc);
+        if (d == 0) put(slot_ml<SEES>(a) + slot * R + row, make_float2(M, L));
+        put(slot_o<SEES>(a) + ((long long)slot * R + row) * hd + d, acc);
+      } else if (SEES >= SEES_PREFIX) {
+        leave_sum(a, tok, rh, d, make_float2(M, L), acc);
       } else {
         out_store(a.out, tok * a.out.row_stride + rh * a.out.head_stride + d, L == 0.0f ? 0.0f : acc / L);
       }
@@ -606,7 +643,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
         if (lane == 0) st.last = all;
       }
       __syncthreads();
-      if (st.last) join_parts<C, R, PICK>(a, lds, sp, head, rt, p0, (int)parts);
+      if (st.last) join_parts<C, R, SEES>(a, lds, sp, head, rt, p0, (int)parts);
     }
     while (x < x_stop && x == st.before[seq + 1]) ++seq;   // and past sequences without rows
   }
@@ -614,9 +651,10 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
 
 // 64 E values of a part at a time, row after row; a lane has E of them under
 // way for each of its wave's parts.
-template <int E, bool PICK>
+template <int E, Kv4Sees SEES>
 __device__ __forceinline__ void join_values(const Kv4AttnArgs &a, const RowsSeq &sp, int head, const RowTile &row_t, uint32_t p0,
-                                            int parts, int R, int values, const float *factor, const float *total, float *sums) {
+                                            int parts, int R, int values, const float *factor, const float *total,
+                                            const float *top, float *sums) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, G = a.group, hd = 16 * a.tiles;
   for (int v0 = 0; v0 < values; v0 += 64 * E) {
     float acc[E];
@@ -629,7 +667,7 @@ __device__ __forceinline__ void join_values(const Kv4AttnArgs &a, const RowsSeq 
     }
 #pragma unroll 2
     for (int k = w; k < parts; k += 4) {
-      const float *o = a.part_o + (long long)part_slot(p0, (uint32_t)k) * R * hd;
+      const float *o = slot_o<SEES>(a) + (long long)part_slot(p0, (uint32_t)k) * R * hd;
       float x[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = get(o + at[e]);
@@ -642,9 +680,12 @@ __device__ __forceinline__ void join_values(const Kv4AttnArgs &a, const RowsSeq 
     for (int u = threadIdx.x; u < 64 * E && v0 + u < values; u += 256) {   // whole groups of 16 lanes
       const int r = (v0 + u) / hd, rr = row_t.rr0 + r;
       const float L = total[r], sum = (sums[u] + sums[64 * E + u]) + (sums[128 * E + u] + sums[192 * E + u]);
-      out_store(a.out, (long long)(sp.row0 + token_of<PICK>(a, row_t, rr)) * a.out.row_stride
-                           + (head * G + head_of<PICK>(a, rr)) * a.out.head_stride + (v0 + u) % hd,
-                L == 0.0f ? 0.0f : sum / L);
+      const long long tok = sp.row0 + token_of<SEES>(a, row_t, rr);
+      const int qh = head * G + head_of<SEES>(a, rr);
+      if (SEES >= SEES_PREFIX)
+        leave_sum(a, tok, qh, (v0 + u) % hd, make_float2(top[r], L), sum);
+      else
+        out_store(a.out, tok * a.out.row_stride + qh * a.out.head_stride + (v0 + u) % hd, L == 0.0f ? 0.0f : sum / L);
     }
     __syncthreads();
   }
@@ -653,19 +694,19 @@ __device__ __forceinline__ void join_values(const Kv4AttnArgs &a, const RowsSeq 
 // A row tile's rows from the parts of their keys.  All of a workgroup of four
 // waves: the parts' factors first, then every wave takes each fourth part, a
 // lane the same values of all of them.
-template <int C, int R, bool PICK>
+template <int C, int R, Kv4Sees SEES>
 __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, int head, int rt, uint32_t p0, int parts) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, hd = 16 * a.tiles;
-  const RowTile row_t = row_tile<R, PICK>(a, sp, rt);
+  const RowTile row_t = row_tile<R, SEES>(a, sp, rt);
   const int left = row_t.rows - row_t.rr0, rows = left < R ? left : R;
-  float *factor = (float *)lds, *total = factor + MAX_PARTS * R, *sums = total + R;   // [part][R], [R], [4][1024]
+  float *factor = (float *)lds, *total = factor + MAX_PARTS * R, *top = total + R, *sums = top + R;   // [part][R], [R] x 2, [4][1024]
   auto slot = [&](int k) { return (long long)part_slot(p0, (uint32_t)k) * R; };
   for (int row = w; row < rows; row += 4) {
     float2 ml[MAX_PARTS / 64];
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
     for (int k = 0; k < MAX_PARTS / 64; ++k) {
-      ml[k] = 64 * k + lane < parts ? get(a.part_ml + slot(64 * k + lane) + row) : make_float2(-INFINITY, 0.0f);
+      ml[k] = 64 * k + lane < parts ? get(slot_ml<SEES>(a) + slot(64 * k + lane) + row) : make_float2(-INFINITY, 0.0f);
       M = fmaxf(M, ml[k].x);
     }
     M = wave_max(M);
@@ -677,30 +718,30 @@ __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, i
       if (64 * k + lane < parts) factor[(64 * k + lane) * R + row] = f;
     }
     L = wave_sum(L);
-    if (lane == 0) total[row] = L;
+    if (lane == 0) total[row] = L, top[row] = M;
   }
   __syncthreads();
   const int values = rows * hd;
   if (C == 1 || values <= 512)   // 16 need more registers than the narrow heads' kernels have
-    join_values<8, PICK>(a, sp, head, row_t, p0, parts, R, values, factor, total, sums);
+    join_values<8, SEES>(a, sp, head, row_t, p0, parts, R, values, factor, total, top, sums);
   else
-    join_values<16, PICK>(a, sp, head, row_t, p0, parts, R, values, factor, total, sums);
+    join_values<16, SEES>(a, sp, head, row_t, p0, parts, R, values, factor, total, top, sums);
 }
 
-template <int C, int W, bool PICK>
+template <int C, int W, Kv4Sees SEES>
 static AttnKernel rows_kernel_of(int tiles, int terms) {
   const int R = 16 / terms;
   int lds = W * V_ROWS * v_pitch(C);
-  for (int n : {W * join_floats(R, tiles) * 4, (MAX_PARTS * R + R + 4096) * 4}) lds = n > lds ? n : lds;
-  return {terms == 1 ? k_kv4_rows<C, 1, W, PICK> : terms == 2 ? k_kv4_rows<C, 2, W, PICK> : k_kv4_rows<C, 4, W, PICK>, lds};
+  for (int n : {W * join_floats(R, tiles) * 4, (MAX_PARTS * R + 2 * R + 4096) * 4}) lds = n > lds ? n : lds;
+  return {terms == 1 ? k_kv4_rows<C, 1, W, SEES> : terms == 2 ? k_kv4_rows<C, 2, W, SEES> : k_kv4_rows<C, 4, W, SEES>, lds};
 }
 
-template <bool PICK>
+template <Kv4Sees SEES>
 static AttnKernel rows_kernel_for(int tiles, int terms, int waves) {
   const int C = (tiles + 3) / 4;
-  if (C == 1) return waves == 4 ? rows_kernel_of<1, 4, PICK>(tiles, terms) : rows_kernel_of<1, 16, PICK>(tiles, terms);
-  if (C == 2) return waves == 4 ? rows_kernel_of<2, 4, PICK>(tiles, terms) : rows_kernel_of<2, 8, PICK>(tiles, terms);
-  return C == 3 ? rows_kernel_of<3, 4, PICK>(tiles, terms) : rows_kernel_of<4, 4, PICK>(tiles, terms);
+  if (C == 1) return waves == 4 ? rows_kernel_of<1, 4, SEES>(tiles, terms) : rows_kernel_of<1, 16, SEES>(tiles, terms);
+  if (C == 2) return waves == 4 ? rows_kernel_of<2, 4, SEES>(tiles, terms) : rows_kernel_of<2, 8, SEES>(tiles, terms);
+  return C == 3 ? rows_kernel_of<3, 4, SEES>(tiles, terms) : rows_kernel_of<4, 4, SEES>(tiles, terms);
 }
 
 }  // namespace bfp
