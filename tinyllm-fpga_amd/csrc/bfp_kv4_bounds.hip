@@ -116,16 +116,15 @@ struct Kv4PickArgs {
   const uint16_t *bounds;
   int group, i0, rows;        // rows i0 .. i0 + rows - 1 of every sequence
   int n, first, last;         // pages to pick; of these the first and the last ones, whatever their scores
-  int chunks;                 // pieces of the pages, SCORE_CHUNK each
-  FastDiv by_chunk, by_tile;
+  int chunks, chunk;          // pieces of the pages, and how many pages each has
+  FastDiv by_head, by_chunk, by_tile;
   float *score;               // [sequence][row][head][width]
   float *off;                 // [sequence][row][head][chunk]: sums of the products' magnitudes, at most
   int32_t *picks;
 };
 
+constexpr int PICK_WIDTH = 16384;         // pages of a table: a bit each, twice, and scores have to fit the LDS
 constexpr int SCORE_W = 4;                // waves
-constexpr int SCORE_PAGES = 64;           // of a wave
-constexpr int SCORE_CHUNK = SCORE_W * SCORE_PAGES;
 
 // The last page that row i of a span sees, -1: none.
 __device__ __forceinline__ int own_page(const Kv4PickArgs &a, const Kv4Span &s, int i) {
@@ -135,95 +134,136 @@ __device__ __forceinline__ int own_page(const Kv4PickArgs &a, const Kv4Span &s, 
   return q < a.b.width ? q : a.b.width - 1;
 }
 
+// Eight values of P or N from offset o on, for query heads `stride` apart.
+// One branch on the type, so that the heads' loads are under way together
+// (behind a branch each they took a microsecond apiece).
+template <int TYPE>
+__device__ __forceinline__ void group_sum_of(bfp_rows q, long long o, long long stride, int group, bool upper, float (&sum)[8]) {
+  q.type = TYPE;
+#pragma unroll 4
+  for (int h = 0; h < group; ++h) {
+    float x[8];
+    row_load_n(q, o + h * stride, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float y = upper ? fmaxf(x[e], 0.0f) : fminf(x[e], 0.0f);
+      sum[e] += x[e] == x[e] ? y : NAN;
+    }
+  }
+}
+__device__ __forceinline__ void group_sum(const bfp_rows &q, long long o, int group, bool upper, float (&sum)[8]) {
+  switch (q.type) {
+    case BFP_F32: group_sum_of<BFP_F32>(q, o, q.head_stride, group, upper, sum); break;
+    case BFP_BF16: group_sum_of<BFP_BF16>(q, o, q.head_stride, group, upper, sum); break;
+    case BFP_F16: group_sum_of<BFP_F16>(q, o, q.head_stride, group, upper, sum); break;
+    default: group_sum_of<BFP_TILES>(q, o, q.head_stride, group, upper, sum); break;
+  }
+}
+
 // R: rows of a wave's matrix tile.  16: their terms multiply one after the
 // other; 4: the terms are columns of the tile.  K: steps of 32 values (hd / 16).
-// Bound by the bytes of the bounds: 16 pages' operands are loaded as they lie.
+// The waves share P and N, each works out some of the steps, and each takes
+// every fourth 16 pages, whose operands are loaded as they lie, the next ones
+// while these are multiplied.  Bound by the bytes of the bounds.
 template <int R, int K>
 __global__ __launch_bounds__(64 * SCORE_W) void k_kv4_score(Kv4PickArgs a) {
   constexpr int T = R == 16 ? 3 : 1;
-  const int head = blockIdx.y;
-  uint32_t chunk, rt;
-  const int seq = (int)a.by_tile.div(a.by_chunk.div(blockIdx.x, chunk), rt);
+  __shared__ bf16x8 coefs[T * K * 64];
+  __shared__ float waves[SCORE_W][16];
+  uint32_t chunk, rt, head;   // neighbours take the heads of the same pages
+  const int seq = (int)a.by_tile.div(a.by_chunk.div(a.by_head.div(blockIdx.x, head), chunk), rt);
   const Kv4Span s = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
   const int i0 = a.i0 + (int)rt * R, stop = a.i0 + a.rows < s.n ? a.i0 + a.rows : s.n;
   if (i0 >= stop) return;
   const int ilast = i0 + R < stop ? i0 + R - 1 : stop - 1;
-  const int pages = own_page(a, s, ilast) + 1;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int base = (int)chunk * SCORE_CHUNK;
+  const int base = (int)chunk * a.chunk, all = own_page(a, s, ilast) + 1, pages = base + a.chunk < all ? base + a.chunk : all;
   // all of them are taken, or there are none here
-  if (pages <= a.n || base >= pages) return;
+  if (all <= a.n || base >= pages) return;
   const int hd = a.c.hd, i = i0 + col % R;
   const bool mine = i < stop;
-  // this lane's column: dims 32 k + 8 g .. + 7 of [N | P]
-  bf16x8 coef[T][K];
+  const int32_t *table = a.b.pages + (long long)seq * a.b.width;
+  auto page_of = [&](int p0) { return p0 + col < pages ? kv4_page(table, a.b.width, a.c.n_pages, p0 + col) : -1; };
+  auto fetch = [&](int id, bf16x8 (&v)[K]) {   // a page that does not exist: the first one's, not used
+    const bf16x8 *from = (const bf16x8 *)(a.bounds + ((long long)(id < 0 ? 0 : id) * a.c.heads + head) * 2 * hd + 8 * g);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < K; ++k) v[k] = from[4 * k];
+  };
+  int p0 = base + 16 * w;
+  constexpr int STEP = 16 * SCORE_W;
+  int id = page_of(p0), next_id = page_of(p0 + STEP);
+  bf16x8 v[2][K];
+  fetch(id, v[0]);
+  fetch(next_id, v[1]);
+  // a column: dims 32 k + 8 g .. + 7 of [N | P]
+#pragma unroll
+  for (int k0 = 0; k0 < K; k0 += SCORE_W) {
+    const int k = k0 + w;
+    if (K % SCORE_W && k >= K) break;
     const int at = 32 * k + 8 * g;
     const bool upper = at >= hd;
     const int d = upper ? at - hd : at;
-    float sum[8], x[8], rest[8];
+    float sum[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = rest[e] = 0.0f;
+    for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
     if (mine)
-      for (int h = 0; h < a.group; ++h) {
-        row_load_n(a.q, (long long)(s.row0 + i) * a.q.row_stride + (head * a.group + h) * a.q.head_stride + d, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = upper ? fmaxf(x[e], 0.0f) : fminf(x[e], 0.0f);
-          sum[e] += x[e] == x[e] ? v : NAN;
-        }
-      }
+      group_sum(a.q, (long long)(s.row0 + i) * a.q.row_stride + (long long)head * a.group * a.q.head_stride + d, a.group, upper, sum);
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const int term = R == 16 ? t : col / R;
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = term < 3 ? query_term<3>(sum[e], term) : 0.0f;
-      coef[t][k] = pack8(y);
+      coefs[(t * K + k) * 64 + lane] = pack8(y);
     }
   }
-  const int32_t *table = a.b.pages + (long long)seq * a.b.width;
+  __syncthreads();
+  bf16x8 coef[T][K];
+#pragma unroll
+  for (int t = 0; t < T; ++t)
+#pragma unroll
+    for (int k = 0; k < K; ++k) coef[t][k] = coefs[(t * K + k) * 64 + lane];
   const long long out = ((long long)seq * a.rows + (i - a.i0)) * a.c.heads + head;
   float most = 0.0f;
 #pragma unroll 1
-  for (int t = 0; t < SCORE_PAGES / 16; ++t) {
-    const int p0 = base + w * SCORE_PAGES + 16 * t;
-    if (p0 >= pages) break;
-    const int p = p0 + col;
-    const int id = p < pages ? kv4_page(table, a.b.width, a.c.n_pages, p) : -1;
-    const bf16x8 *from = (const bf16x8 *)(a.bounds + ((long long)(id < 0 ? 0 : id) * a.c.heads + head) * 2 * hd + 8 * g);
-    bf16x8 v[K];
+  for (; p0 < pages; p0 += 2 * STEP) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) v[k] = from[4 * k];
-    f32x4 sc = {0, 0, 0, 0}, mag = {0, 0, 0, 0};
+    for (int u = 0; u < 2; ++u) {   // the bytes of the tile after the next are asked for when this one's have been used
+      const int first = p0 + u * STEP;
+      if (first >= pages) break;
+      f32x4 sc = {0, 0, 0, 0}, mag = {0, 0, 0, 0};
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+      for (int k = 0; k < K; ++k) {
 #pragma unroll
-      for (int u = 0; u < T; ++u) sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[k], coef[u][k], sc, 0, 0, 0);
-      typedef unsigned u4 __attribute__((ext_vector_type(4)));
-      const u4 va = __builtin_bit_cast(u4, v[k]) & 0x7fff7fffu, ca = __builtin_bit_cast(u4, coef[0][k]) & 0x7fff7fffu;
-      mag = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, ca), mag, 0, 0, 0);
-    }
-    const unsigned long long there = __ballot(id >= 0);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = sc[e], m = mag[e];
-      if (R == 4) {
-        x = term_sum<4>(x);
-        m = term_sum<4>(m);
+        for (int t = 0; t < T; ++t) sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][k], coef[t][k], sc, 0, 0, 0);
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        const u4 va = __builtin_bit_cast(u4, v[u][k]) & 0x7fff7fffu, ca = __builtin_bit_cast(u4, coef[0][k]) & 0x7fff7fffu;
+        mag = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, ca), mag, 0, 0, 0);
       }
-      const int page = p0 + 4 * g + e;
-      if (!mine || page >= pages || (R == 4 && col >= R)) continue;
-      const bool ok = (there >> (4 * g + e)) & 1;
-      if (ok) most = fabsf(x) < INFINITY ? fmaxf(most, m) : INFINITY;
-      a.score[out * a.b.width + page] = ok ? x : -INFINITY;
+      const unsigned long long there = __ballot(id >= 0);
+      id = next_id;
+      if (first + 2 * STEP < pages) {
+        next_id = page_of(first + 2 * STEP);
+        fetch(next_id, v[u]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = sc[e], m = mag[e];
+        if (R == 4) {
+          x = term_sum<4>(x);
+          m = term_sum<4>(m);
+        }
+        const int page = first + 4 * g + e;
+        if (!mine || page >= pages || (R == 4 && col >= R)) continue;
+        const bool ok = (there >> (4 * g + e)) & 1;
+        if (ok) most = fabsf(x) < INFINITY ? fmaxf(most, m) : INFINITY;
+        a.score[out * a.b.width + page] = ok ? x : -INFINITY;
+      }
     }
   }
   // over the column's four lanes, then the waves
   most = fmaxf(most, fpeer<16>(most));
   most = fmaxf(most, fpeer<32>(most));
-  __shared__ float waves[SCORE_W][16];
   if (g == 0) waves[w][col] = most;
   __syncthreads();
   if (threadIdx.x < R && mine)
@@ -242,32 +282,34 @@ __device__ __forceinline__ unsigned long long key_of(double f) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// Sums over a workgroup of W waves of what each wave counted; two sets of
-// places in turn, one barrier a call.
+// Sums over a workgroup of W waves of three numbers that each wave counted
+// (below 2^21 in all): one word a wave, which as many lanes read and add up.  Two
+// sets of places in turn, one barrier a call.  (Every thread reading all of the
+// waves' counts took 0.9 us a call with 16 waves.)
 template <int W>
 struct Counter {
-  int (*place)[W][3];
+  unsigned long long (*place)[W];
   int turn;
   __device__ void add(int (&n)[3]) {
-    const int w = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-      place[turn][w][0] = n[0];
-      place[turn][w][1] = n[1];
-      place[turn][w][2] = n[2];
-    }
+    if ((threadIdx.x & 63) == 0)
+      place[turn][threadIdx.x >> 6] = (unsigned long long)n[0] | (unsigned long long)n[1] << 21 | (unsigned long long)n[2] << 42;
     __syncthreads();
-    n[0] = n[1] = n[2] = 0;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      n[0] += place[turn][k][0];
-      n[1] += place[turn][k][1];
-      n[2] += place[turn][k][2];
-    }
+    long long v = (long long)place[turn][threadIdx.x & (W - 1)];
+    if (W > 8) v += peer<8>(v);
+    if (W > 4) v += peer<4>(v);
+    v += peer<2>(v);
+    v += peer<1>(v);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)((unsigned long long)v >> 32));
+    const unsigned long long u = (unsigned long long)hi << 32 | lo;
+    n[0] = (int)(u & 0x1fffff);
+    n[1] = (int)((u >> 21) & 0x1fffff);
+    n[2] = (int)(u >> 42);
     turn ^= 1;
   }
 };
 
-// The largest key that at least `want` of the n keys reach.  Two bits a round.
+// A key that exactly `want` of the n keys reach, or, where there is none, the
+// largest that more do.  Two bits a round.
 template <int W, typename Key>
 __device__ __forceinline__ Key nth_key(int n, int want, const Key *key, Counter<W> &count) {
   Key at = 0;
@@ -282,9 +324,92 @@ __device__ __forceinline__ Key nth_key(int n, int want, const Key *key, Counter<
       for (int u = 0; u < 3; ++u) c[u] += __popcll(__ballot(k >= q[u]));
     }
     count.add(c);
-    at = c[2] >= want ? q[2] : c[1] >= want ? q[1] : c[0] >= want ? q[0] : at;
+    int reach = 0;
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (c[u] >= want) at = q[u], reach = c[u];
+    if (reach == want) break;
   }
   return at;
+}
+
+// The least of the keys that reach `at` (there is one).
+template <int W>
+__device__ __forceinline__ uint32_t least_key(int n, uint32_t at, const uint32_t *key, uint32_t *waves) {
+  uint32_t v = 0xffffffffu;
+  for (int p = threadIdx.x; p < n; p += 64 * W) v = key[p] >= at && key[p] < v ? key[p] : v;
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) {
+    const uint32_t x = __shfl_xor(v, d, 64);
+    v = x < v ? x : v;
+  }
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < W; ++k) v = waves[k] < v ? waves[k] : v;
+  return v;
+}
+
+// The want-th largest of the n values whose keys are not 0, out of `count` of
+// them, between least and most.  Bins of equal width first, then, in one wave,
+// those of the bin in which it lies; by its bits where they are more than a
+// wave's lanes.  (By bits alone: 9 us of 14 for 2048 pages.)
+constexpr int BINS = 256;
+struct BinSpace {
+  int bins[BINS], n;
+  uint32_t list[64], found;
+};
+template <int W>
+__device__ __forceinline__ float nth_value(int n, int want, const uint32_t *key, float least, float most, BinSpace &b, uint32_t *waves,
+                                           Counter<W> &count) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const float scale = (BINS - 1) / (most - least);   // 0, infinite or NaN: all in one bin
+  auto bin_of = [&](uint32_t k) {
+    const float x = (of_key(k) - least) * scale;     // does not fall where the value rises
+    return x > 0.0f ? (int)fminf(x, (float)(BINS - 1)) : 0;
+  };
+  for (int i = threadIdx.x; i < BINS; i += 64 * W) b.bins[i] = 0;
+  if (threadIdx.x == 0) b.n = 0;
+  __syncthreads();
+  for (int p = threadIdx.x; p < n; p += 64 * W)
+    if (key[p]) atomicAdd(&b.bins[bin_of(key[p])], 1);
+  __syncthreads();
+  // every wave: the bin, from above, in which the count reaches `want`
+  int mine[BINS / 64], sum = 0;   // lane l: bins from BINS - 1 - 4 l down
+#pragma unroll
+  for (int i = 0; i < BINS / 64; ++i) sum += mine[i] = b.bins[BINS - 1 - (BINS / 64 * lane + i)];
+  int up = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int x = __shfl_up(up, d, 64);
+    up += lane >= d ? x : 0;
+  }
+  int above = up - sum, bin = -1, held = 0;
+#pragma unroll
+  for (int i = 0; i < BINS / 64; ++i) {
+    if (bin < 0 && above + mine[i] >= want) bin = BINS - 1 - (BINS / 64 * lane + i), held = mine[i];
+    if (bin < 0) above += mine[i];
+  }
+  const int from = __ffsll((unsigned long long)__ballot(bin >= 0)) - 1;   // the first lane that reaches it
+  bin = __shfl(bin, from, 64);
+  held = __shfl(held, from, 64);
+  const int rank = want - __shfl(above, from, 64);   // in the bin, from 1
+  if (held > 64) return of_key(least_key<W>(n, nth_key<W, uint32_t>(n, want, key, count), key, waves));
+  for (int p = threadIdx.x; p < n; p += 64 * W)
+    if (key[p] && bin_of(key[p]) == bin) b.list[atomicAdd(&b.n, 1)] = key[p];
+  __syncthreads();
+  if (w == 0) {
+    const uint32_t x = lane < held ? b.list[lane] : 0;
+    int r = 0, same = 0;   // how many are larger, and how many are alike
+    for (int u = 0; u < held; ++u) {
+      const uint32_t y = (uint32_t)__builtin_amdgcn_readlane((int)x, u);
+      r += y > x;
+      same += y == x;
+    }
+    if (lane < held && r < rank && rank <= r + same) b.found = x;   // all that write it write the same
+  }
+  __syncthreads();
+  return of_key(b.found);
 }
 
 // The exact score of a page, by eight neighbouring lanes; coef: N and P in
@@ -313,9 +438,12 @@ __device__ __forceinline__ double exact_score(const Kv4PickArgs &a, int id, int 
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_kv4_pick(Kv4PickArgs a) {
   extern __shared__ __align__(16) unsigned long long words[];
-  __shared__ int places[2][W][3];
-  __shared__ float tops[W];
+  __shared__ unsigned long long places[2][W];
+  __shared__ float tops[W], ends[W][2];
+  __shared__ uint32_t least[W];
+  __shared__ BinSpace bins;
   __shared__ double coef[512];
+  __shared__ int lie_before[PICK_WIDTH / 64];   // pages of the border before each word
   const int head = blockIdx.y, seq = (int)(blockIdx.x / (unsigned)a.rows), i = a.i0 + (int)(blockIdx.x % (unsigned)a.rows);
   const Kv4Span s = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
   if (i >= s.n) return;
@@ -334,15 +462,23 @@ __global__ __launch_bounds__(64 * W) void k_kv4_pick(Kv4PickArgs a) {
   // The forced pages that exist, the others that do, and how far scores may be off.
   int c[3] = {0, 0, 0};
   const bool all = n <= a.n;
+  float low = INFINITY, high = -INFINITY;
   for (int p0 = 0; p0 < n; p0 += 64 * W) {
     const int p = p0 + threadIdx.x;
     const float x = p < n && !all && !forced(p) ? score[p] : -INFINITY;
     const bool there = p < n && (all || forced(p) ? kv4_page(table, a.b.width, a.c.n_pages, p) >= 0 : x != -INFINITY);
     if (p < n) key32[p] = x == -INFINITY ? 0u : key_of(x);
+    low = x == -INFINITY ? low : fminf(low, x);
+    high = fmaxf(high, x);
     const unsigned long long f = __ballot(there && (all || forced(p)));
     c[0] += __popcll(f);
     c[1] += __popcll(__ballot(there && !all && !forced(p)));
     if (lane == 0 && p0 + 64 * w < n) take[p0 / 64 + w] = f;
+  }
+  if (!all) {
+    low = -wave_max(-low);
+    high = wave_max(high);
+    if (lane == 0) ends[w][0] = low, ends[w][1] = high;
   }
   count.add(c);
   int want = a.n - c[0];
@@ -355,7 +491,7 @@ __global__ __launch_bounds__(64 * W) void k_kv4_pick(Kv4PickArgs a) {
     }
   } else if (want > 0) {
     float most = 0.0f;
-    for (int k = threadIdx.x; k * SCORE_CHUNK < n; k += 64 * W) most = fmaxf(most, a.off[in * a.chunks + k]);
+    for (int k = threadIdx.x; k * a.chunk < n; k += 64 * W) most = fmaxf(most, a.off[in * a.chunks + k]);
     most = wave_max(most);
     if (lane == 0) tops[w] = most;
     __syncthreads();
@@ -369,7 +505,11 @@ __global__ __launch_bounds__(64 * W) void k_kv4_pick(Kv4PickArgs a) {
     const float e2 = 2.0f * (2 * a.c.hd + a.group + 16) * 0x1.06p-23f * most + 0x1p-120f;
     const bool exact_all = !(e2 < 0x1p120f);
     float A = 0.0f;
-    if (!exact_all) A = of_key(nth_key<W, uint32_t>(n, want, key32, count));
+    if (!exact_all) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) low = fminf(low, ends[k][0]), high = fmaxf(high, ends[k][1]);
+      A = nth_value<W>(n, want, key32, low, high, bins, least, count);
+    }
     c[0] = c[1] = c[2] = 0;
     for (int p0 = 0; p0 < n; p0 += 64 * W) {
       const int p = p0 + threadIdx.x;
@@ -399,44 +539,81 @@ __global__ __launch_bounds__(64 * W) void k_kv4_pick(Kv4PickArgs a) {
         }
         coef[d] = sum;
       }
-      __syncthreads();
-      int before = 0;   // keys: of the border's pages, in their order
-      for (int k = 0; k < n_words; ++k) {
-        const unsigned long long m = border[k];
-        const int mine = __popcll(m);
-        for (int u = threadIdx.x >> 3; u < mine; u += 8 * W) {   // eight lanes a page
-          unsigned long long rest = m;
-          for (int x = 0; x < u; ++x) rest &= rest - 1;
-          const int p = 64 * k + __ffsll((long long)rest) - 1;
-          const int id = kv4_page(table, a.b.width, a.c.n_pages, p);
-          const double sc = exact_score(a, id < 0 ? 0 : id, head, coef);
-          if ((threadIdx.x & 7) == 0) keys[before + u] = key_of(sc);
-        }
-        before += mine;
-      }
-      __syncthreads();
-      const unsigned long long T = nth_key<W, unsigned long long>(before, want, keys, count);
-      c[0] = c[1] = c[2] = 0;
-      for (int u0 = 0; u0 < before; u0 += 64 * W) {
-        const int u = u0 + threadIdx.x;
-        c[0] += __popcll(__ballot(u < before && keys[u] > T));
-      }
-      count.add(c);
-      int ties = want - c[0];   // of those at T the first
-      // page by page, in order: one wave
       if (w == 0) {
-        int at = 0;
-        for (int k = 0; k < n_words; ++k) {
-          const unsigned long long m = border[k], below = m & ((1ull << lane) - 1);
-          const bool is = (m >> lane) & 1;
-          const unsigned long long x = is ? keys[at + __popcll(below)] : 0;
-          const unsigned long long equal = __ballot(is && x == T), above = __ballot(is && x > T);
-          const bool tie = is && x == T && __popcll(equal & ((1ull << lane) - 1)) < ties;
-          const unsigned long long got = above | __ballot(tie);
-          const int used = __popcll(equal);
-          ties = ties > used ? ties - used : 0;
-          if (lane == 0) take[k] |= got;
-          at += __popcll(m);
+        int before = 0;
+        for (int k0 = 0; k0 < n_words; k0 += 64) {
+          const int mine = k0 + lane < n_words ? __popcll(border[k0 + lane]) : 0;
+          int up = mine;
+#pragma unroll
+          for (int d = 1; d < 64; d *= 2) {
+            const int x = __shfl_up(up, d, 64);
+            up += lane >= d ? x : 0;
+          }
+          if (k0 + lane < n_words) lie_before[k0 + lane] = before + up - mine;
+          before += __shfl(up, 63, 64);
+        }
+      }
+      __syncthreads();
+      // Page u of the border: the last word with no more than u before it, and its bit.
+      auto page_at = [&](int u) {
+        int k = 0, past = n_words;
+        while (past - k > 1) {
+          const int mid = k + (past - k) / 2;
+          (lie_before[mid] <= u ? k : past) = mid;
+        }
+        unsigned long long m = border[k];
+        int left = u - lie_before[k], at = 0;
+#pragma unroll
+        for (int half = 32; half > 0; half /= 2) {
+          const int low = __popcll(m & ((1ull << half) - 1));
+          if (left >= low) left -= low, m >>= half, at += half;
+        }
+        return 64 * k + at;
+      };
+      const int m = c[1];   // pages of the border; keys: their scores, in order
+      for (int u = threadIdx.x >> 3; u < m; u += 8 * W) {   // eight lanes a page
+        const int id = kv4_page(table, a.b.width, a.c.n_pages, page_at(u));
+        const double sc = exact_score(a, id < 0 ? 0 : id, head, coef);
+        if ((threadIdx.x & 7) == 0) keys[u] = key_of(sc);
+      }
+      __syncthreads();
+      if (m <= 64) {   // one wave: each page by how many come before it
+        if (w == 0) {
+          const unsigned long long mine = lane < m ? keys[lane] : 0;
+          int r = 0;
+          for (int u = 0; u < m; ++u) {
+            const unsigned long long x = keys[u];
+            r += x > mine || (x == mine && u < lane);
+          }
+          if (lane < m && r < want) {
+            const int p = page_at(lane);
+            atomicOr(take + p / 64, 1ull << (p & 63));
+          }
+        }
+      } else {
+        // T: what the last one taken has (or more reach: then the first of those at T)
+        const unsigned long long T = nth_key<W, unsigned long long>(m, want, keys, count);
+        c[0] = c[1] = c[2] = 0;
+        for (int u0 = 0; u0 < m; u0 += 64 * W) {
+          const int u = u0 + threadIdx.x;
+          c[0] += __popcll(__ballot(u < m && keys[u] >= T));
+          c[1] += __popcll(__ballot(u < m && keys[u] > T));
+        }
+        count.add(c);
+        int ties = c[0] == want ? m : want - c[1];   // of those at T the first
+        // page by page, in order: one wave
+        if (w == 0) {
+          for (int k = 0; k < n_words; ++k) {
+            const unsigned long long b = border[k], below = (1ull << lane) - 1;
+            const bool is = (b >> lane) & 1;
+            const unsigned long long x = is ? keys[lie_before[k] + __popcll(b & below)] : 0;
+            const unsigned long long equal = __ballot(is && x == T), above = __ballot(is && x > T);
+            const bool tie = is && x == T && __popcll(equal & below) < ties;
+            const unsigned long long got = above | __ballot(tie);
+            const int used = __popcll(equal);
+            ties = ties > used ? ties - used : 0;
+            if (lane == 0) take[k] |= got;
+          }
         }
       }
     }
@@ -470,18 +647,28 @@ static int check_bounds(const char *op, const void *bounds) {
 }
 
 constexpr size_t PICK_SCRATCH = (size_t)256 << 20;   // at most, unless one row of each sequence needs more
+constexpr int PICK_CHUNKS = 256;
+
 struct PickPlan {
-  int rows, chunks;   // rows of a sequence in a piece
+  int rows, R, chunks, chunk;   // rows of a sequence in a piece, and of a matrix tile
   size_t scores, work;
 };
 static PickPlan plan_pick(const bfp_kv4 &c, const bfp_kv4_batch &b) {
   PickPlan p;
-  p.chunks = (b.width + SCORE_CHUNK - 1) / SCORE_CHUNK;
   const int rows = b.max_q < b.n_rows ? b.max_q : b.n_rows;
-  const size_t row = (size_t)b.n_seq * c.heads * ((size_t)b.width + p.chunks) * sizeof(float);
+  const size_t row = (size_t)b.n_seq * c.heads * ((size_t)b.width + PICK_CHUNKS) * sizeof(float);
   size_t most = PICK_SCRATCH / row;
   if (most >= 16) most = most / 16 * 16;
   p.rows = most < 1 ? 1 : most < (size_t)rows ? (int)most : rows;
+  p.R = p.rows > 4 ? 16 : 4;
+  // a thousand workgroups, each with 64 pages or more
+  const long long tiles = (long long)((p.rows + p.R - 1) / p.R) * c.heads * b.n_seq;
+  long long chunks = 1024 / tiles;
+  if (chunks > (b.width + 63) / 64) chunks = (b.width + 63) / 64;
+  if (chunks > PICK_CHUNKS) chunks = PICK_CHUNKS;
+  if (chunks < 1) chunks = 1;
+  p.chunk = (int)((b.width + chunks - 1) / chunks + 63) / 64 * 64;
+  p.chunks = (b.width + p.chunk - 1) / p.chunk;
   p.scores = (size_t)b.n_seq * p.rows * c.heads * b.width;
   p.work = (p.scores + (size_t)b.n_seq * p.rows * c.heads * p.chunks) * sizeof(float);
   return p;
@@ -493,8 +680,7 @@ static int check_pick(const char *op, const bfp_kv4 *cache, const bfp_kv4_batch 
     return set_err(BFP_EINVAL, "%s: q has %d heads, the cache %d", op, q ? q->heads : 0, cache->heads);
   BFP_TRY(check_rows(op, "q", q, q->heads, cache->hd, true, batch->n_rows));
   if (!rows_aligned(*q, 8, batch->n_rows)) return set_err(BFP_EINVAL, "%s: q needs 16-byte alignment and strides in multiples of 8", op);
-  // a bit a page, twice, and the border's scores have to fit the LDS
-  if (batch->width > 16384) return set_err(BFP_EINVAL, "%s: width=%d pages, at most 16384", op, batch->width);
+  if (batch->width > PICK_WIDTH) return set_err(BFP_EINVAL, "%s: width=%d pages, at most %d", op, batch->width, PICK_WIDTH);
   return BFP_OK;
 }
 
@@ -556,8 +742,7 @@ int bfp_kv4_select_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const uin
   if (!work || (uintptr_t)work % 16 || work_bytes < p.work)
     return set_err(BFP_EINVAL, "%s: needs %zu bytes of 16-byte-aligned scratch, got %zu", op, p.work, work ? work_bytes : (size_t)0);
   const int rows = batch->max_q < batch->n_rows ? batch->max_q : batch->n_rows;
-  const int R = p.rows > 4 ? 16 : 4;
-  const long long tiles = (p.rows + R - 1) / R, blocks = tiles * p.chunks * batch->n_seq, pick_blocks = (long long)p.rows * batch->n_seq;
+  const long long tiles = (p.rows + p.R - 1) / p.R, blocks = tiles * p.chunks * batch->n_seq, pick_blocks = (long long)p.rows * batch->n_seq;
   // 2^32 threads a launch
   if (blocks * cache->heads > 0xffffff || pick_blocks * cache->heads > 0x3fffff)
     return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, batch->n_seq, batch->max_q);
@@ -570,19 +755,21 @@ int bfp_kv4_select_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const uin
   a.rows = p.rows;
   a.n = n, a.first = first, a.last = last;
   a.chunks = p.chunks;
+  a.chunk = p.chunk;
+  a.by_head = FastDiv(cache->heads);
   a.by_chunk = FastDiv(p.chunks);
   a.by_tile = FastDiv((uint32_t)tiles);
   a.score = (float *)work;
   a.off = a.score + p.scores;
   a.picks = picks;
-  const score_fn score = R == 4 ? score_kernel<4>(cache->hd / 16) : score_kernel<16>(cache->hd / 16);
+  const score_fn score = p.R == 4 ? score_kernel<4>(cache->hd / 16) : score_kernel<16>(cache->hd / 16);
   const size_t lds = (size_t)(batch->width + 63) / 64 * 16 + (size_t)batch->width * 8;
   // few workgroups: more waves each
   const bool wide = pick_blocks * cache->heads <= 512;
   const score_fn pick = wide ? k_kv4_pick<16> : k_kv4_pick<4>;
-  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void *)pick, hipFuncAttributeMaxDynamicSharedMemorySize, 140 * 1024));
+  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void *)pick, hipFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024));
   for (a.i0 = 0; a.i0 < rows; a.i0 += p.rows) {
-    hipLaunchKernelGGL(score, dim3((unsigned)blocks, cache->heads), dim3(64 * SCORE_W), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(score, dim3((unsigned)(blocks * cache->heads)), dim3(64 * SCORE_W), 0, (hipStream_t)stream, a);
     BFP_TRY(launch_status(op));
     hipLaunchKernelGGL(pick, dim3((unsigned)pick_blocks, cache->heads), dim3(wide ? 1024 : 256), lds, (hipStream_t)stream, a);
     BFP_TRY(launch_status(op));
