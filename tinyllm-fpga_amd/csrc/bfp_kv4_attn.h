@@ -56,6 +56,7 @@ struct Kv4AttnArgs {
     head = (int)h + split % c.heads;
     head = head < c.heads ? head : head - c.heads;
   }
+  __device__ bool piece(int rows, int &g, int &head, int &split, int &rt, int &splits, int &chunk) const;
   float scale2;        // |scale| * log2(e), kept above 0
   float slack;         // M_SLACK in scores: M_SLACK / scale2, above the score that raises the maximum
   float q_sign;        // the scale's sign, or 0, which the queries take
@@ -73,6 +74,8 @@ struct Kv4AttnArgs {
   bfp_kv4_shared sh;
   int sh_seqs;   // sequences of the batch
   int sum_slots, sum_slot;
+  int pieces, prefix_slots;   // k_kv4_prompt: workgroups that share the keys of up to 64 groups (0: splits of one length), and a row's slots
+  int32_t *split_of;   // with them: the splits of each group
   float *slot_o;
   float2 *slot_ml;
 };
@@ -116,15 +119,20 @@ __device__ __forceinline__ int kv4_group_low(const Kv4AttnArgs &a, const Kv4Grou
   }
   return low == 0x7fffffff ? 0 : low;
 }
-// The tokens that sequence b's group shares, 0 outside every group.
-__device__ __forceinline__ int kv4_shared_len(const Kv4AttnArgs &a, int b) {
-  int g = 0, past = a.sh.n_groups;   // the last group that begins at b or before
+// The tokens that sequence b's group (g) shares, 0 outside every group.
+__device__ __forceinline__ int kv4_shared_len(const Kv4AttnArgs &a, int b, int &g) {
+  int past = a.sh.n_groups;   // the last group that begins at b or before
+  g = 0;
   while (past - g > 1) {
     const int mid = g + (past - g) / 2;
     (a.sh.start[mid] <= b ? g : past) = mid;
   }
   const int n = a.sh.len[g];
   return a.sh.start[g] <= b && b < a.sh.start[g + 1] && n > 0 ? n : 0;
+}
+__device__ __forceinline__ int kv4_shared_len(const Kv4AttnArgs &a, int b) {
+  int g;
+  return kv4_shared_len(a, b, g);
 }
 // The position of row t of a group: of the sequence in which it lies.  Lane x
 // < N of every N neighbouring ones has the wave's x-th row; each gets its own's.
@@ -158,6 +166,61 @@ __device__ __forceinline__ int min_lanes(int v) {
 }
 template <int N>
 __device__ __forceinline__ int max_lanes(int v) { return -min_lanes<N>(-v); }
+
+// Workgroup blockIdx.x's part of the groups' prefixes, at most 64 of them,
+// where the longest takes its keys in prefix_slots splits at most: all workgroups
+// take equally many tiles, whatever the groups' lengths, as long as a round of
+// them (a.pieces) has room for every row tile.  False: there is nothing for it.
+__device__ __forceinline__ bool Kv4AttnArgs::piece(int rows, int &g, int &head, int &split, int &rt, int &splits, int &chunk) const {
+  const int lane = threadIdx.x & 63;
+  int units = 0, tiles = 0;   // row tiles x KV heads, and key tiles
+  if (lane < b.n_seq) {
+    Kv4Group x;
+    const Kv4Span s = kv4_group_span(*this, lane, x);
+    const int low = kv4_group_low(*this, x) / KEYS;
+    units = (int)(((long long)s.n * group + rows - 1) / rows) * c.heads;
+    tiles = s.at > low * KEYS ? (s.at + KEYS - 1) / KEYS - low : 1;
+  }
+  auto sum = [&](long long v) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
+    return v;
+  };
+  int most = units ? tiles : 0;
+#pragma unroll
+  for (int d = 32; d > 0; d /= 2) most = max(most, __shfl_xor(most, d, 64));
+  const long long all = sum((long long)units * tiles), places = sum(units);
+  int least = (int)((all + pieces - 1) / pieces);
+  least = max(max(least, (most + prefix_slots - 1) / prefix_slots), 4);
+  chunk = max(most, 1);
+  if (places <= pieces && least < chunk) {   // the shortest pieces of which there are no more than `pieces`
+    int too_short = least - 1;
+    while (chunk - too_short > 1) {
+      const int mid = too_short + (chunk - too_short) / 2;
+      (sum((long long)units * ((tiles + mid - 1) / mid)) <= pieces ? chunk : too_short) = mid;
+    }
+  }
+  const int mine = (tiles + chunk - 1) / chunk;
+  if (blockIdx.x == 0 && threadIdx.x < b.n_seq) split_of[lane] = mine;
+  int up = units * mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int x = __shfl_up(up, d, 64);
+    up += lane >= d ? x : 0;
+  }
+  const unsigned long long past = __ballot(up > (int)blockIdx.x);
+  if (!past) return false;
+  g = __ffsll((long long)past) - 1;
+  splits = __builtin_amdgcn_readlane(mine, g);
+  chunk = __builtin_amdgcn_readfirstlane(chunk);
+  const int before = __builtin_amdgcn_readlane(up - units * mine, g), its = __builtin_amdgcn_readlane(units, g) / c.heads;
+  uint32_t h;
+  const uint32_t u = by_head.div(blockIdx.x - (uint32_t)before, h);
+  head = (int)h;
+  split = (int)(u / (uint32_t)its);
+  rt = (int)(u - (uint32_t)split * its);
+  return true;
+}
 
 // The tiles of split `split` out of a row tile's n: chunks as long as the
 // longest sequence's splits are, so that workgroups take equally long

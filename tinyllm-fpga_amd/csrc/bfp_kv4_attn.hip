@@ -133,7 +133,8 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
 struct SharedPlan {
   Kv4Plan prefix, rest;
   bfp_kv4_batch groups;
-  int slots;
+  int slots, pieces;
+  long long blocks;         // of the first launch, where its pieces are shared out (0: its plan's)
   size_t sums, own, work;   // parts of rows; bytes of the launches' own parts
 };
 static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_kv4_shared &sh, const bfp_rows &q, const bfp_rows &out,
@@ -149,12 +150,25 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   p.prefix = plan_keys(c, p.groups, q, out, prefix, true, 48);
   const long long cap = (long long)sh.width * c.page;
   p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len > 0 && sh.max_len < cap ? sh.max_len : cap), false, 16);
+  // Prompts' kernel, up to 64 groups: the device shares the keys out, whatever
+  // the groups' lengths; no group has more splits than workgroups a KV head.
+  p.pieces = p.blocks = 0;
+  if (p.prefix.prompt && sh.n_groups <= 64) {
+    const int group = q.heads / c.heads, rows = 32 * p.prefix.waves;
+    const long long key_tiles = (prefix + KEYS - 1) / KEYS;
+    const long long most = ((long long)b.n_rows * group + rows - 1) / rows * c.heads + (long long)sh.n_groups * c.heads;
+    int s = 256 / c.heads;
+    if (s > key_tiles / 4) s = (int)(key_tiles / 4);
+    p.prefix.splits = s < 1 ? 1 : s < 48 ? s : 48;
+    p.pieces = 256;
+    p.blocks = most > 256 ? most : 256;
+  }
   p.slots = p.prefix.splits + p.rest.splits;
   p.sums = (size_t)b.n_rows * q.heads * p.slots;
   // (a split launch's parts are the rows', not its own)
   const size_t one = p.prefix.splits > 1 ? 0 : p.prefix.work, two = p.rest.splits > 1 ? 0 : p.rest.work;
   p.own = one > two ? one : two;
-  p.work = p.sums * (c.hd * sizeof(float) + sizeof(float2)) + p.own;
+  p.work = p.sums * (c.hd * sizeof(float) + sizeof(float2)) + p.own + 64 * sizeof(int32_t);
   return p;
 }
 
@@ -245,13 +259,14 @@ static int check_work(const char *op, size_t need, const void *work, size_t work
   return BFP_OK;
 }
 
-static int launch_plan(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, hipStream_t s) {
+static int launch_plan(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, hipStream_t s, long long blocks = 0) {
   a.splits = p.splits;
   a.chunk = p.chunk;
   a.stream = p.stream;
   a.row_tiles = p.row_tiles;
   a.by_split = FastDiv(p.splits);
-  const long long each = (long long)p.row_tiles * p.splits * a.c.heads, blocks = p.stream ? p.stream : each * a.b.n_seq;
+  const long long each = (long long)p.row_tiles * p.splits * a.c.heads;
+  if (!blocks) blocks = p.stream ? p.stream : each * a.b.n_seq;
   if (blocks > 0x3ffffff / p.waves || each > 0x7fffffff)   // 2^32 threads
     return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, a.b.n_seq, a.b.max_q);
   a.by_seq = FastDiv((uint32_t)each);
@@ -273,7 +288,8 @@ static int launch_attn(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const A
 }
 
 // One of the two parts: its slots of the rows' parts, and its own workspace.
-static int launch_part(const char *op, Kv4AttnArgs a, const Kv4Plan &p, const AttnKernel &k, int slot, void *own, hipStream_t s) {
+static int launch_part(const char *op, Kv4AttnArgs a, const Kv4Plan &p, const AttnKernel &k, int slot, void *own, hipStream_t s,
+                       long long blocks = 0) {
   a.sum_slot = slot;
   if (p.stream) {
     a.slot_o = (float *)own;
@@ -281,7 +297,7 @@ static int launch_part(const char *op, Kv4AttnArgs a, const Kv4Plan &p, const At
     a.there = (unsigned long long *)(a.slot_ml + p.cells);
     a.number = call_number();
   }
-  return launch_plan(op, a, p, k, s);
+  return launch_plan(op, a, p, k, s, blocks);
 }
 
 static int check_shared(const char *op, const bfp_kv4_batch *b, const bfp_kv4_shared *sh, const bfp_kv4 *c, const bfp_rows *q) {
@@ -351,11 +367,14 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
   a.part_o = (float *)work;
   a.part_ml = (float2 *)(a.part_o + p.sums * cache->hd);
   void *own = a.part_ml + p.sums;
+  a.split_of = p.pieces ? (int32_t *)((char *)own + p.own) : nullptr;
+  a.pieces = p.pieces;
+  a.prefix_slots = p.prefix.splits;
   Kv4AttnArgs g = a;
   g.b = p.groups;
   const Kv4Plan &one = p.prefix, &two = p.rest;
   BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms) : prefix_rows_kernel(a.tiles, one.terms, one.waves),
-                      0, own, s));
+                      0, own, s, p.blocks));
   BFP_TRY(launch_part(op, a, two, two.prompt ? rest_prompt_kernel(a.tiles, two.terms) : rest_rows_kernel(a.tiles, two.terms, two.waves),
                       one.splits, own, s));
   a.sum_slot = one.splits;

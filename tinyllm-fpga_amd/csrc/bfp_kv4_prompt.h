@@ -42,8 +42,12 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), NV = v_buffers(TB);
   extern __shared__ __align__(16) char lds[];
   __shared__ int nan_tiles[4];
-  int seq, head, rt, split;
-  a.place(seq, head, split, rt);
+  int seq, head, rt, split, splits = a.splits, chunk = a.chunk;
+  if (SEES == SEES_PREFIX && a.pieces) {
+    if (!a.piece(ROWS, seq, head, split, rt, splits, chunk)) return;
+  } else {
+    a.place(seq, head, split, rt);
+  }
   Kv4Group of{};
   const Kv4Span sp = SEES == SEES_PREFIX ? kv4_group_span(a, seq, of)
                                          : kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
@@ -56,54 +60,61 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   const bool mine = rr < rows;
   uint32_t qg;
   const int i = (int)a.by_group.div((uint32_t)(mine ? rr : 0), qg), qh = head * G + (int)qg;
-  int hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
-  // what this wave's rows all see, and any of the workgroup's
-  const int wfirst = rr0 < rows ? rr0 : rows - 1, wlast = (rr0 + 32 < rows ? rr0 + 32 : rows) - 1;
-  int hi_min = key_hi(sp.at + wfirst / G), hi_max = rr0 < rows ? key_hi(sp.at + wlast / G) : 0;
-  int lo_max = key_lo(hi_max, a.window);
+  // what any of the workgroup's rows sees
   const int glast = (wg0 + ROWS < rows ? wg0 + ROWS : rows) - 1;
   int begin = key_lo(key_hi(sp.at + wg0 / G), a.window);
   int top_hi = key_hi(sp.at + glast / G);
-  if constexpr (SEES == SEES_REST) {
-    lo = lo > low ? lo : low;
-    lo_max = lo_max > low ? lo_max : low;
-    begin = begin > low ? begin : low;
-  }
-  if constexpr (SEES == SEES_PREFIX) {   // rows of several sequences: by each one's position
-    uint32_t rest;
-    const int row = (int)a.by_group.div((uint32_t)(mine ? rr : rows - 1), rest);
-    const int ends = key_hi(kv4_row_position<32>(a, of, sp.row0 + row));
-    lo = mine ? key_lo(ends, a.window) : 0;
-    hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
-    hi_min = min_lanes<32>(mine ? hi : 0x7fffffff);
-    lo_max = max_lanes<32>(lo);
-    begin = kv4_group_low(a, of);
+  if (SEES == SEES_REST) begin = begin > low ? begin : low;
+  if (SEES == SEES_PREFIX) {
+    begin = __builtin_amdgcn_readfirstlane(kv4_group_low(a, of));
     top_hi = sp.at;
   }
   const long long cap = (long long)a.b.width << a.page_shift;
   const int end = top_hi < cap ? top_hi : (int)cap;
   const int tile0 = begin / KEYS, n_tiles = end > begin ? (end + KEYS - 1) / KEYS - tile0 : 0;
-  const KeyPart part = key_part(n_tiles, split, a.splits, a.chunk);
+  const KeyPart part = key_part(n_tiles, split, splits, chunk);
   const int first = tile0 + part.first, stop = tile0 + part.stop;
 
+  // this lane's row, and what the wave's rows all see
+  int hi, lo, hi_min, lo_max;
   bf16x8 qf[T][TB];
-#pragma unroll
-  for (int c = 0; c < TB; ++c) {
-    float x[8];
-    if (mine && c < tiles) {
-      row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * c + 8 * h, x);
-    } else {
-#pragma unroll
-      for (int d = 0; d < 8; ++d) x[d] = 0.0f;
+  auto take_rows = [&]() __attribute__((always_inline)) {
+    hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
+    const int wfirst = rr0 < rows ? rr0 : rows - 1, wlast = (rr0 + 32 < rows ? rr0 + 32 : rows) - 1;
+    hi_min = key_hi(sp.at + wfirst / G);
+    lo_max = key_lo(rr0 < rows ? key_hi(sp.at + wlast / G) : 0, a.window);
+    if constexpr (SEES == SEES_REST) {
+      lo = lo > low ? lo : low;
+      lo_max = lo_max > low ? lo_max : low;
+    }
+    if constexpr (SEES == SEES_PREFIX) {   // rows of several sequences: by each one's position
+      uint32_t rest;
+      const int row = (int)a.by_group.div((uint32_t)(mine ? rr : rows - 1), rest);
+      const int ends = key_hi(kv4_row_position<32>(a, of, sp.row0 + row));
+      lo = mine ? key_lo(ends, a.window) : 0;
+      hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
+      hi_min = __builtin_amdgcn_readfirstlane(min_lanes<32>(mine ? hi : 0x7fffffff));
+      lo_max = __builtin_amdgcn_readfirstlane(max_lanes<32>(lo));
     }
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      float y[8];
+    for (int c = 0; c < TB; ++c) {
+      float x[8];
+      if (mine && c < tiles) {
+        row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * c + 8 * h, x);
+      } else {
 #pragma unroll
-      for (int d = 0; d < 8; ++d) y[d] = query_term<T>(x[d], t) * a.q_sign;
-      qf[t][c] = pack8(y);
+        for (int d = 0; d < 8; ++d) x[d] = 0.0f;
+      }
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        float y[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) y[d] = query_term<T>(x[d], t) * a.q_sign;
+        qf[t][c] = pack8(y);
+      }
     }
-  }
+  };
+  if (SEES != SEES_PREFIX) take_rows();
 
   float m = -INFINITY, sum = 0.0f;
   f32x16 o[DT];
@@ -114,9 +125,12 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
 
   const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
   // wave w brings in head tiles w, w + W, ... of K and V, a key a lane
-  uint2 rk[UNITS], rv[UNITS];
-  uint32_t rke[UNITS], rve[UNITS];
-  bool there = false;
+  struct Bytes {
+    uint2 k[UNITS], v[UNITS];
+    uint32_t ke[UNITS], ve[UNITS];
+    bool there;
+    unsigned long long ok;   // whose keys are there
+  };
   // The page number of this lane's key, where some row sees the key; looked at
   // only when the page is fetched, a tile later: a use here would wait for it
   // and for the bytes asked for before it (two prompts of 8192 tokens, 32 heads
@@ -130,41 +144,42 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   };
   // a key without a page reads the first one's bytes; they are not used
   const uint32_t page_tiles = (uint32_t)a.c.heads * tiles * a.c.page;   // at most 2^24
-  auto fetch = [&](int tile, int id) {
-    there = (unsigned)id < (unsigned)a.c.n_pages;
+  auto fetch = [&](Bytes &x, int tile, int id) __attribute__((always_inline)) {
+    x.there = (unsigned)id < (unsigned)a.c.n_pages;
+    x.ok = __ballot(x.there);
     const uint32_t slot = (uint32_t)(tile * KEYS + lane) & (a.c.page - 1);
-    const unsigned long long at = (unsigned long long)(there ? (uint32_t)id : 0u) * page_tiles + slot;
+    const unsigned long long at = (unsigned long long)(x.there ? (uint32_t)id : 0u) * page_tiles + slot;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int t = w + u * W;
       const long long from = kv4_tile(0, a.c.heads, head, tiles, t < tiles ? t : tiles - 1, a.c.page, 0);   // the same in every lane
-      rk[u] = ((const uint2 *)(a.c.k + from * KV4_TILE_BYTES))[at];
-      rv[u] = ((const uint2 *)(a.c.v + from * KV4_TILE_BYTES))[at];
-      rke[u] = (a.c.k_e + from)[at];
-      rve[u] = (a.c.v_e + from)[at];
+      x.k[u] = ((const uint2 *)(a.c.k + from * KV4_TILE_BYTES))[at];
+      x.v[u] = ((const uint2 *)(a.c.v + from * KV4_TILE_BYTES))[at];
+      x.ke[u] = (a.c.k_e + from)[at];
+      x.ve[u] = (a.c.v_e + from)[at];
     }
   };
   char *const k_lds = lds, *const v_lds = lds + 2 * k_bytes(TB);
-  auto decode = [&](int t1) {   // tile first + t1
+  auto decode = [&](const Bytes &x, int t1) __attribute__((always_inline)) {   // tile first + t1
     char *kb = k_lds + (t1 & 1) * k_bytes(TB) + lane * KP, *vt = v_lds + t1 % NV * v_bytes(TB), *vb = vt + lane * VP;
     const int sw = (lane >> 1) & 3;   // 16-byte pieces of each 64 change places, for the writes' banks
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int t = w + u * W;
       if (UNITS * W > TB && t >= TB) break;
-      const bool ok = there && t < tiles;   // zeros for what the head or the cache does not have
-      const float ks = kv4_scale(rke[u]);
+      const bool ok = x.there && t < tiles;   // zeros for what the head or the cache does not have
+      const float ks = kv4_scale(x.ke[u]);
       bf16x8 *kd = (bf16x8 *)(kb + 32 * t);
-      kd[0] = kv4_decode8(t < tiles ? rk[u].x : 0u, ks);
-      kd[1] = kv4_decode8(t < tiles ? rk[u].y : 0u, ks);
+      kd[0] = kv4_decode8(t < tiles ? x.k[u].x : 0u, ks);
+      kd[1] = kv4_decode8(t < tiles ? x.k[u].y : 0u, ks);
       // NaN tiles of V count as zeros in the product; the rows that see them are set after
-      const uint32_t E = ok ? rve[u] : 0u;
+      const uint32_t E = ok ? x.ve[u] : 0u;
       const bool take = ok && E < KV4_PAST;
       vt[KEYS * VP + lane * 16 + t] = (char)E;
       if (E >= KV4_PAST) nan_tiles[t1 & 3] = 1;
       const float vs = kv4_scale(take ? E : 0u);
-      *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1)) ^ sw)) = kv4_decode8(take ? rv[u].x : 0u, vs);
-      *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1) + 1) ^ sw)) = kv4_decode8(take ? rv[u].y : 0u, vs);
+      *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1)) ^ sw)) = kv4_decode8(take ? x.v[u].x : 0u, vs);
+      *(bf16x8 *)(vb + 64 * (t >> 1) + 16 * ((2 * (t & 1) + 1) ^ sw)) = kv4_decode8(take ? x.v[u].y : 0u, vs);
     }
   };
   // scores of half a tile (32 keys), before any mask: s[e] is key 8 (e / 4) + 4 h + e % 4 of row n
@@ -210,22 +225,36 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   // tile t is read between barriers t - 1 and t and written between t - 2 and
   // t - 1, V is read between t - 1 and t + 1.  nan_tiles[t % 4] is cleared before
   // barrier t - 2, set between t - 2 and t - 1, read between t and t + 1.
+  //
+  // A prefix's keys are read by few workgroups, or one, so they come from
+  // memory, not from an L2 cache: they are asked for two tiles ahead, in two
+  // sets of registers, and before the rows' queries.
+  constexpr bool FAR = SEES == SEES_PREFIX;
   if (threadIdx.x < 4) nan_tiles[threadIdx.x] = 0;
   __syncthreads();
+  Bytes one, two;
   int id = page_of(first);
-  fetch(first, id);
-  unsigned long long ok = __ballot(there);
-  decode(0);
-  id = page_of(first + 1);
+  if (FAR) {
+    const int id1 = page_of(first + 1), id2 = page_of(first + 2);
+    fetch(one, first, id);
+    fetch(two, first + 1, id1);
+    id = id2;
+    take_rows();
+  } else {
+    fetch(one, first, id);
+  }
+  unsigned long long ok = one.ok;
+  decode(one, 0);
+  if (!FAR) id = page_of(first + 1);
   __syncthreads();
   f32x16 s = scores(0, 0);
   mask(s, first, 0, ok);
   float top = top_of(s);
-  for (int tile = first; tile < stop; ++tile) {
+  // One tile: next holds the following one's bytes, or gets them (far: the one's after it)
+  auto step = [&](int tile, Bytes &next, Bytes &far) __attribute__((always_inline)) {
     const int t1 = tile - first;
-    fetch(tile + 1, id);
-    const unsigned long long ok_next = __ballot(there);
-    id = page_of(tile + 2);
+    fetch(far, tile + (FAR ? 2 : 1), id);
+    id = page_of(tile + (FAR ? 3 : 2));
     if (threadIdx.x == 0) nan_tiles[(t1 + 2) & 3] = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -284,15 +313,15 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
         }
       }
       if (u == 0) {
-        decode(t1 + 1);
+        decode(next, t1 + 1);
         mask(sn, tile, 1, ok);
       } else {
-        mask(sn, tile + 1, 0, ok_next);
+        mask(sn, tile + 1, 0, next.ok);
       }
       s = sn;
       top = top_of(s);
     }
-    ok = ok_next;
+    ok = next.ok;
     if (nan_tiles[t1 & 3]) {
       const uint8_t *ve = (const uint8_t *)v_lds + t1 % NV * v_bytes(TB) + KEYS * VP;
       const int t0 = tile * KEYS;
@@ -306,6 +335,14 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       }
     }
     if constexpr (NV == 2) __syncthreads();   // before V of tile t - 1 gives way to t + 1
+  };
+  if constexpr (FAR) {
+    for (int tile = first; tile < stop; tile += 2) {
+      step(tile, two, one);
+      if (tile + 1 < stop) step(tile + 1, one, two);
+    }
+  } else {
+    for (int tile = first; tile < stop; ++tile) step(tile, one, one);
   }
   __syncthreads();
 

@@ -40,35 +40,57 @@ __global__ __launch_bounds__(256) void k_kv4_join_prompt(Kv4AttnArgs a) {
 }
 
 // Joins the two parts of rows that share a prefix: the prefix's slots, which
-// are not there outside every group, and those of the rest.
+// are not there outside every group, and those of the rest.  A wave takes one
+// row and query head, 16 bytes a lane, so that several slots' values are
+// loaded at once, and four such loads are under way.
 __global__ __launch_bounds__(256) void k_kv4_join_shared(Kv4AttnArgs a) {
+  __shared__ float rows[4][256];
   const int seq = blockIdx.y;
   const Kv4Span sp = kv4_span(a.b.start[seq], a.b.start[seq + 1], a.b.len[seq], a.b.n_rows, a.b.max_q);
-  const int u = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int w = threadIdx.x >> 6, u = blockIdx.x * 4 + w, lane = threadIdx.x & 63;
   const int i = u / a.q.heads, qh = u % a.q.heads;
-  if (i >= sp.n) return;
+  if (i >= sp.n) return;   // (no barrier below)
   const long long tok = sp.row0 + i, at = (tok * a.q.heads + qh) * a.sum_slots;
-  const int hd = 16 * a.tiles, first = kv4_shared_len(a, seq) > 0 ? 0 : a.sum_slot;
-  const float2 ml = lane >= first && lane < a.sum_slots ? a.part_ml[at + lane] : make_float2(-INFINITY, 0.0f);
-  const float M = wave_max(ml.x);
-  const float f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
-  const float L = wave_sum(f * ml.y);
-  float acc[4] = {0, 0, 0, 0};
-  for (int k0 = first; k0 < a.sum_slots; k0 += 4) {
+  const int hd = 16 * a.tiles;
+  int g, before = 0;
+  if (kv4_shared_len(a, seq, g) > 0) before = a.split_of ? a.split_of[g] : a.prefix_slots;
+  const int n = before + a.sum_slots - a.prefix_slots;   // slot k of them
+  auto slot = [&](int k) { return k < before ? k : k - before + a.prefix_slots; };
+  const float2 ml = lane < n ? a.part_ml[at + slot(lane)] : make_float2(-INFINITY, 0.0f);
+  // lanes of a slot, slots at a time; this lane's
+  const int lanes = hd / 4, each = 64 / lanes, mine = lane / lanes, d = 4 * (lane - mine * lanes);
+  f32x4 acc = {0, 0, 0, 0}, x[4];
+  float M, f, L;
+  for (int k0 = 0; k0 < n; k0 += 4 * each) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {   // past the last slot: it again, with the factor 0 (its NaN, if it has one, is the row's anyway)
+      const int k = k0 + e * each + mine;
+      x[e] = *(const f32x4 *)(a.part_o + (at + slot(k < n ? k : n - 1)) * hd + d);
+    }
+    if (k0 == 0) {   // while the first ones are under way
+      M = wave_max(ml.x);
+      f = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+      L = wave_sum(f * ml.y);
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int k = k0 + e < a.sum_slots ? k0 + e : a.sum_slots - 1;
-      const float fk = k0 + e < a.sum_slots ? __shfl(f, k, 64) : 0.0f;
-      const float *o = a.part_o + (at + k) * hd;
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-        if (64 * d < hd) acc[d] += fk * o[64 * d + lane < hd ? 64 * d + lane : hd - 1];
+      const int k = k0 + e * each + mine;
+      const float fk = __shfl(f, k < n ? k : n - 1, 64);
+      acc += (k < n && mine < each ? fk : 0.0f) * x[e];
     }
   }
+  // the slots' sums, always in the same order
+  float *row = rows[w];
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
-    if (64 * d + lane < hd)
-      out_store(a.out, tok * a.out.row_stride + qh * a.out.head_stride + 64 * d + lane, L == 0.0f ? 0.0f : acc[d] / L);
+  for (int e = 0; e < 4; ++e) {
+    float v = acc[e];
+    for (int k = 1; k < each; ++k) v += __shfl(acc[e], (lane + k * lanes) & 63, 64);
+    if (mine == 0) row[d + e] = v;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  for (int o = lane; o < hd; o += 64)   // whole groups of 16 lanes
+    out_store(a.out, tok * a.out.row_stride + qh * a.out.head_stride + o, L == 0.0f ? 0.0f : row[o] / L);
 }
 
 AttnKernel prompt_kernel(int tiles, int terms) { return prompt_kernel_for<SEES_ALL>(tiles, terms); }

@@ -321,10 +321,10 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
       const int ends = key_hi(kv4_row_position<R>(a, sp.of, sp.row0 + (rr < rows ? rr : rows - 1) / G));
       lo = mine ? key_lo(ends, a.window) : 0;
       hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
-      hi_min = min_lanes<16>(mine ? hi : 0x7fffffff);
-      hi_max = max_lanes<16>(hi);
-      lo_min = min_lanes<16>(mine ? lo : 0x7fffffff);
-      lo_max = max_lanes<16>(lo);
+      hi_min = __builtin_amdgcn_readfirstlane(min_lanes<16>(mine ? hi : 0x7fffffff));
+      hi_max = __builtin_amdgcn_readfirstlane(max_lanes<16>(hi));
+      lo_min = __builtin_amdgcn_readfirstlane(min_lanes<16>(mine ? lo : 0x7fffffff));
+      lo_max = __builtin_amdgcn_readfirstlane(max_lanes<16>(lo));
     }
     const long long cap = (long long)a.b.width << a.page_shift;
     const int end = hi_max < cap ? hi_max : (int)cap;
