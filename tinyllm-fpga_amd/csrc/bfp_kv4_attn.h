@@ -181,23 +181,18 @@ __device__ __forceinline__ bool Kv4AttnArgs::piece(int rows, int &g, int &head, 
     units = (int)(((long long)s.n * group + rows - 1) / rows) * c.heads;
     tiles = s.at > low * KEYS ? (s.at + KEYS - 1) / KEYS - low : 1;
   }
-  auto sum = [&](long long v) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d, 64);
-    return v;
-  };
+  const auto sum = [](int v) { return (int)psum<1>(psum<2>(psum<4>(psum<8>(psum<16>(psum<32>(v)))))); };
   int most = units ? tiles : 0;
 #pragma unroll
   for (int d = 32; d > 0; d /= 2) most = max(most, __shfl_xor(most, d, 64));
-  const long long all = sum((long long)units * tiles), places = sum(units);
-  int least = (int)((all + pieces - 1) / pieces);
-  least = max(max(least, (most + prefix_slots - 1) / prefix_slots), 4);
+  const int places = sum(min(units, 1 << 20));
+  int least = max((most + prefix_slots - 1) / prefix_slots, 4);
   chunk = max(most, 1);
   if (places <= pieces && least < chunk) {   // the shortest pieces of which there are no more than `pieces`
     int too_short = least - 1;
     while (chunk - too_short > 1) {
       const int mid = too_short + (chunk - too_short) / 2;
-      (sum((long long)units * ((tiles + mid - 1) / mid)) <= pieces ? chunk : too_short) = mid;
+      (sum(units * ((tiles + mid - 1) / mid)) <= pieces ? chunk : too_short) = mid;   // (units are 256 at most here, and tiles / mid 48)
     }
   }
   const int mine = (tiles + chunk - 1) / chunk;
@@ -391,12 +386,12 @@ struct AttnKernel {
   int lds;
 };
 AttnKernel rows_kernel(int tiles, int terms, int waves);
-AttnKernel picks_kernel(int tiles, int terms, int waves);
+AttnKernel picks_kernel(int tiles, int terms, int waves, bool share);
 AttnKernel prompt_kernel(int tiles, int terms);
 // Of a shared prefix, and of what lies behind it.
-AttnKernel prefix_rows_kernel(int tiles, int terms, int waves);
+AttnKernel prefix_rows_kernel(int tiles, int terms, int waves, bool share);
 AttnKernel prefix_prompt_kernel(int tiles, int terms);
-AttnKernel rest_rows_kernel(int tiles, int terms, int waves);
+AttnKernel rest_rows_kernel(int tiles, int terms, int waves, bool share);
 AttnKernel rest_prompt_kernel(int tiles, int terms);
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }

@@ -150,6 +150,10 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   p.prefix = plan_keys(c, p.groups, q, out, prefix, true, 48);
   const long long cap = (long long)sh.width * c.page;
   p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len > 0 && sh.max_len < cap ? sh.max_len : cap), false, 16);
+  for (Kv4Plan *k : {&p.prefix, &p.rest}) {
+    const long long n = (long long)k->row_tiles * c.heads * (k == &p.rest ? b.n_seq : sh.n_groups);
+    if (!k->prompt && !k->stream && n > 256) k->waves = 4;
+  }
   // Prompts' kernel, up to 64 groups: the device shares the keys out, whatever
   // the groups' lengths; no group has more splits than workgroups a KV head.
   p.pieces = p.blocks = 0;
@@ -189,7 +193,7 @@ static Kv4Plan plan_picks(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_ro
   const long long rows = b.n_rows < (long long)b.n_seq * b.max_q ? b.n_rows : (long long)b.n_seq * b.max_q;
   const long long groups = rows * token_tiles * c.heads, most_groups = (long long)p.row_tiles * c.heads * b.n_seq;
   p.waves = rows_waves(tiles);
-  if (key_tiles > 4 * p.waves || most_groups * p.waves > 0x3ffffff || groups >= 1024) {
+  if (key_tiles > 4 * p.waves || most_groups * p.waves > 0x3ffffff || groups > 256) {
     p.waves = 4;
     if (groups < 1024 && key_tiles > 16 && b.n_seq <= 256 && most_groups * (key_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
       const long long most = groups * (key_tiles + ROWS_EXTRA) / 4 + 1, slots = tiles <= 4 ? 768 : tiles <= 8 ? 512 : 256;
@@ -361,6 +365,7 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
   const SharedPlan p = plan_shared(*cache, *batch, *shared, *q, *out, window);
   BFP_TRY(check_work(op, p.work, work, work_bytes));
   hipStream_t s = (hipStream_t)stream;
+  a.slack = fminf(2 * M_SLACK / a.scale2, 0x1p125f);   // few tiles a workgroup, whose first one sets the maximum: it is raised less often
   a.sh = *shared;
   a.sh_seqs = batch->n_seq;
   a.sum_slots = p.slots;
@@ -373,9 +378,9 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
   Kv4AttnArgs g = a;
   g.b = p.groups;
   const Kv4Plan &one = p.prefix, &two = p.rest;
-  BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms) : prefix_rows_kernel(a.tiles, one.terms, one.waves),
+  BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms) : prefix_rows_kernel(a.tiles, one.terms, one.waves, one.stream > 0),
                       0, own, s, p.blocks));
-  BFP_TRY(launch_part(op, a, two, two.prompt ? rest_prompt_kernel(a.tiles, two.terms) : rest_rows_kernel(a.tiles, two.terms, two.waves),
+  BFP_TRY(launch_part(op, a, two, two.prompt ? rest_prompt_kernel(a.tiles, two.terms) : rest_rows_kernel(a.tiles, two.terms, two.waves, two.stream > 0),
                       one.splits, own, s));
   a.sum_slot = one.splits;
   launch_join_shared(a, s);
@@ -400,7 +405,7 @@ int bfp_kv4_attn_picks_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const
   const Kv4Plan p = plan_picks(*cache, *batch, *q, *out, n_picks, a.token_tiles);
   a.picks = picks;
   a.n_picks = n_picks;
-  return launch_attn(op, a, p, picks_kernel(a.tiles, p.terms, p.waves), work, work_bytes, (hipStream_t)stream);
+  return launch_attn(op, a, p, picks_kernel(a.tiles, p.terms, p.waves, p.stream > 0), work, work_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

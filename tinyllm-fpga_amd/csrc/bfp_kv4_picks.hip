@@ -4,6 +4,8 @@
 
 namespace bfp {
 
-AttnKernel picks_kernel(int tiles, int terms, int waves) { return rows_kernel_for<SEES_PICKS>(tiles, terms, waves); }
+AttnKernel picks_kernel(int tiles, int terms, int waves, bool share) {
+  return rows_kernel_for<SEES_PICKS>(tiles, terms, waves, share);
+}
 
 }  // namespace bfp

@@ -5,7 +5,9 @@
 
 namespace bfp {
 
-AttnKernel prefix_rows_kernel(int tiles, int terms, int waves) { return rows_kernel_for<SEES_PREFIX>(tiles, terms, waves); }
+AttnKernel prefix_rows_kernel(int tiles, int terms, int waves, bool share) {
+  return rows_kernel_for<SEES_PREFIX>(tiles, terms, waves, share);
+}
 AttnKernel prefix_prompt_kernel(int tiles, int terms) { return prompt_kernel_for<SEES_PREFIX>(tiles, terms); }
 
 }  // namespace bfp

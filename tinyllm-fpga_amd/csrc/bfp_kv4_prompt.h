@@ -33,6 +33,30 @@ constexpr int prompt_lds(int tb, int waves) {
   return in > out ? in : out;
 }
 
+// A lane's part of a row's query, all loads under way together: behind a branch
+// on the type each, as where one row tile follows another, they take 3 us.
+template <int TB, int T, int TYPE>
+__device__ __forceinline__ void prompt_query(const Kv4AttnArgs &a, long long at, bool mine, bf16x8 (&qf)[T][TB]) {
+  bfp_rows q = a.q;
+  q.type = TYPE;
+  float x[TB][8];
+#pragma unroll
+  for (int c = 0; c < TB; ++c) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) x[c][d] = 0.0f;
+    if (mine && c < a.tiles) row_load_n(q, at + 16 * c, x[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < TB; ++c)
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      float y[8];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) y[d] = query_term<T>(x[c][d], t) * a.q_sign;
+      qf[t][c] = pack8(y);
+    }
+}
+
 // TB: tiles of the head the loops are built for (even; a narrower head's
 // missing tiles are zeros in K, and columns of V whose results nobody
 // takes); T: terms; W: waves.
@@ -77,6 +101,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
 
   // this lane's row, and what the wave's rows all see
   int hi, lo, hi_min, lo_max;
+  bool blind = false;   // SEES_PREFIX: the row sees none of it; what is worked out for it is thrown away, not masked
   bf16x8 qf[T][TB];
   auto take_rows = [&]() __attribute__((always_inline)) {
     hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
@@ -93,8 +118,19 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       const int ends = key_hi(kv4_row_position<32>(a, of, sp.row0 + row));
       lo = mine ? key_lo(ends, a.window) : 0;
       hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
-      hi_min = __builtin_amdgcn_readfirstlane(min_lanes<32>(mine ? hi : 0x7fffffff));
-      lo_max = __builtin_amdgcn_readfirstlane(max_lanes<32>(lo));
+      blind = hi <= lo;
+      hi_min = __builtin_amdgcn_readfirstlane(min_lanes<32>(blind ? 0x7fffffff : hi));
+      lo_max = __builtin_amdgcn_readfirstlane(max_lanes<32>(blind ? 0 : lo));
+    }
+    const long long q_at = (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 8 * h;
+    if constexpr (SEES == SEES_PREFIX) {
+      switch (a.q.type) {
+        case BFP_F32: prompt_query<TB, T, BFP_F32>(a, q_at, mine, qf); break;
+        case BFP_BF16: prompt_query<TB, T, BFP_BF16>(a, q_at, mine, qf); break;
+        case BFP_F16: prompt_query<TB, T, BFP_F16>(a, q_at, mine, qf); break;
+        default: prompt_query<TB, T, BFP_TILES>(a, q_at, mine, qf); break;
+      }
+      return;
     }
 #pragma unroll
     for (int c = 0; c < TB; ++c) {
@@ -146,7 +182,6 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   const uint32_t page_tiles = (uint32_t)a.c.heads * tiles * a.c.page;   // at most 2^24
   auto fetch = [&](Bytes &x, int tile, int id) __attribute__((always_inline)) {
     x.there = (unsigned)id < (unsigned)a.c.n_pages;
-    x.ok = __ballot(x.there);
     const uint32_t slot = (uint32_t)(tile * KEYS + lane) & (a.c.page - 1);
     const unsigned long long at = (unsigned long long)(x.there ? (uint32_t)id : 0u) * page_tiles + slot;
 #pragma unroll
@@ -158,6 +193,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       x.ke[u] = (a.c.k_e + from)[at];
       x.ve[u] = (a.c.v_e + from)[at];
     }
+    x.ok = __ballot(x.there);
   };
   char *const k_lds = lds, *const v_lds = lds + 2 * k_bytes(TB);
   auto decode = [&](const Bytes &x, int t1) __attribute__((always_inline)) {   // tile first + t1
@@ -225,36 +261,23 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   // tile t is read between barriers t - 1 and t and written between t - 2 and
   // t - 1, V is read between t - 1 and t + 1.  nan_tiles[t % 4] is cleared before
   // barrier t - 2, set between t - 2 and t - 1, read between t and t + 1.
-  //
-  // A prefix's keys are read by few workgroups, or one, so they come from
-  // memory, not from an L2 cache: they are asked for two tiles ahead, in two
-  // sets of registers, and before the rows' queries.
-  constexpr bool FAR = SEES == SEES_PREFIX;
   if (threadIdx.x < 4) nan_tiles[threadIdx.x] = 0;
   __syncthreads();
-  Bytes one, two;
+  Bytes next;
   int id = page_of(first);
-  if (FAR) {
-    const int id1 = page_of(first + 1), id2 = page_of(first + 2);
-    fetch(one, first, id);
-    fetch(two, first + 1, id1);
-    id = id2;
-    take_rows();
-  } else {
-    fetch(one, first, id);
-  }
-  unsigned long long ok = one.ok;
-  decode(one, 0);
-  if (!FAR) id = page_of(first + 1);
+  fetch(next, first, id);
+  unsigned long long ok = next.ok;
+  if (SEES == SEES_PREFIX) take_rows();   // while the first tile is under way
+  decode(next, 0);
+  id = page_of(first + 1);
   __syncthreads();
   f32x16 s = scores(0, 0);
   mask(s, first, 0, ok);
   float top = top_of(s);
-  // One tile: next holds the following one's bytes, or gets them (far: the one's after it)
-  auto step = [&](int tile, Bytes &next, Bytes &far) __attribute__((always_inline)) {
+  for (int tile = first; tile < stop; ++tile) {
     const int t1 = tile - first;
-    fetch(far, tile + (FAR ? 2 : 1), id);
-    id = page_of(tile + (FAR ? 3 : 2));
+    fetch(next, tile + 1, id);
+    id = page_of(tile + 2);
     if (threadIdx.x == 0) nan_tiles[(t1 + 2) & 3] = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -335,14 +358,14 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
       }
     }
     if constexpr (NV == 2) __syncthreads();   // before V of tile t - 1 gives way to t + 1
-  };
-  if constexpr (FAR) {
-    for (int tile = first; tile < stop; tile += 2) {
-      step(tile, two, one);
-      if (tile + 1 < stop) step(tile + 1, one, two);
-    }
-  } else {
-    for (int tile = first; tile < stop; ++tile) step(tile, one, one);
+  }
+  if (SEES == SEES_PREFIX && blind) {
+    m = -INFINITY;
+    sum = 0.0f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   }
   __syncthreads();
 

@@ -5,7 +5,9 @@
 
 namespace bfp {
 
-AttnKernel rest_rows_kernel(int tiles, int terms, int waves) { return rows_kernel_for<SEES_REST>(tiles, terms, waves); }
+AttnKernel rest_rows_kernel(int tiles, int terms, int waves, bool share) {
+  return rows_kernel_for<SEES_REST>(tiles, terms, waves, share);
+}
 AttnKernel rest_prompt_kernel(int tiles, int terms) { return prompt_kernel_for<SEES_REST>(tiles, terms); }
 
 }  // namespace bfp

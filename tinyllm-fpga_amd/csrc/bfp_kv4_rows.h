@@ -201,7 +201,8 @@ __device__ __forceinline__ bool arrive(unsigned long long *there, unsigned long 
 }
 
 // C: head tiles a lane group holds (hd <= 64 C); T: terms of a row (columns
-// R = 16 / T rows share); W: waves.
+// R = 16 / T rows share); W: waves; SHARE: a.stream says whether workgroups
+// share all tiles (W = 4).
 template <int C, int R, Kv4Sees SEES>
 __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, int head, int rt, uint32_t p0, int parts);
 
@@ -232,15 +233,23 @@ __device__ __forceinline__ void leave_sum(const Kv4AttnArgs &a, long long tok, i
   a.part_o[at * (16 * a.tiles) + d] = v;
 }
 
-template <int C, int T, int W, Kv4Sees SEES>
-__global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 2 : 1) void k_kv4_rows(Kv4AttnArgs a) {
+// Waves a SIMD that the registers leave room for.  Without shared work (which
+// takes 50 more) three of heads up to 128, four up to 64.
+constexpr int rows_per_simd(int C, int W, Kv4Sees sees, bool share) {
+  if (W > 8) return 4;
+  if (sees != SEES_ALL && !share && C <= 2) return C == 1 ? 4 : 3;
+  return C == 1 ? 3 : W > 4 || C == 2 ? 2 : 1;
+}
+
+template <int C, int T, int W, Kv4Sees SEES, bool SHARE>
+__global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv4_rows(Kv4AttnArgs a) {
   constexpr int R = 16 / T;
   constexpr bool PICK = SEES == SEES_PICKS;
   extern __shared__ __align__(16) char lds[];
   __shared__ Stream st;
   int seq, head, rt, split;
   uint32_t x = 0, x_stop = 1, piece = 0;
-  if (W == 4 && a.stream) {
+  if (SHARE && a.stream) {
     piece = stream_plan<SEES>(a, R, st);
     x = blockIdx.x * piece;
     const uint32_t all = st.before[a.b.n_seq];
@@ -269,7 +278,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
     KvSide<C> k, v;
     int id = -1;
     long long at = 0;
-    const bool early = SEES == SEES_ALL && !(W == 4 && a.stream) && a.window == 0;
+    const bool early = SEES == SEES_ALL && !(SHARE && a.stream) && a.window == 0;
     if (early) {
       id = kv4_page(pages, a.b.width, a.c.n_pages, (w * KEYS + 4 * r) >> a.page_shift);
       at = offset_of(w, id);
@@ -279,7 +288,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
     const RowsSeq sp = rows_seq<SEES>(a, R, seq);
     int from = 0, upto = sp.tiles, slot = -1;
     uint32_t begin = 0;
-    if (W == 4 && a.stream) {
+    if (SHARE && a.stream) {
       const uint32_t y = x - st.before[seq], group = y / sp.span(), off = y - group * sp.span();
       const uint32_t left = x_stop - x, whole = sp.span() - off, take = left < whole ? left : whole;
       begin = x - off;
@@ -317,14 +326,16 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
       lo_min = lo_min > sp.low ? lo_min : sp.low;
       lo_max = lo_max > sp.low ? lo_max : sp.low;
     }
+    bool blind = false;   // SEES_PREFIX: the row sees none of it; what is worked out for it is thrown away, not masked
     if constexpr (SEES == SEES_PREFIX) {   // rows of several sequences: by each one's position
       const int ends = key_hi(kv4_row_position<R>(a, sp.of, sp.row0 + (rr < rows ? rr : rows - 1) / G));
       lo = mine ? key_lo(ends, a.window) : 0;
       hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
-      hi_min = __builtin_amdgcn_readfirstlane(min_lanes<16>(mine ? hi : 0x7fffffff));
+      blind = hi <= lo;
+      hi_min = __builtin_amdgcn_readfirstlane(min_lanes<16>(blind ? 0x7fffffff : hi));
       hi_max = __builtin_amdgcn_readfirstlane(max_lanes<16>(hi));
-      lo_min = __builtin_amdgcn_readfirstlane(min_lanes<16>(mine ? lo : 0x7fffffff));
-      lo_max = __builtin_amdgcn_readfirstlane(max_lanes<16>(lo));
+      lo_min = __builtin_amdgcn_readfirstlane(min_lanes<16>(blind ? 0x7fffffff : lo));
+      lo_max = __builtin_amdgcn_readfirstlane(max_lanes<16>(blind ? 0 : lo));
     }
     const long long cap = (long long)a.b.width << a.page_shift;
     const int end = hi_max < cap ? hi_max : (int)cap;
@@ -588,6 +599,13 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
       }
     }
 
+    if (SEES == SEES_PREFIX && blind) {
+      m = -INFINITY;
+      sum = 0.0f;
+#pragma unroll
+      for (int d = 0; d < 4 * C; ++d) o[d] = f32x4{0, 0, 0, 0};
+    }
+
     // join the terms, then the waves
     sum += fpeer<16>(sum);
     sum += fpeer<32>(sum);
@@ -632,7 +650,7 @@ __global__ __launch_bounds__(64 * W, W > 8 ? 4 : C == 1 ? 3 : W > 4 || C == 2 ? 
         out_store(a.out, tok * a.out.row_stride + rh * a.out.head_stride + d, L == 0.0f ? 0.0f : acc / L);
       }
     }
-    if (!(W == 4 && a.stream)) return;
+    if (!(SHARE && a.stream)) return;
     if (slot >= 0) {
       // the row tile's parts are the pieces from p0 on
       const uint32_t p0 = begin / piece, parts = (begin + sp.tiles - 1) / piece - p0 + 1;
@@ -728,17 +746,25 @@ __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, i
     join_values<16, SEES>(a, sp, head, row_t, p0, parts, R, values, factor, total, top, sums);
 }
 
-template <int C, int W, Kv4Sees SEES>
+template <int C, int W, Kv4Sees SEES, bool SHARE = W == 4>
 static AttnKernel rows_kernel_of(int tiles, int terms) {
   const int R = 16 / terms;
   int lds = W * V_ROWS * v_pitch(C);
-  for (int n : {W * join_floats(R, tiles) * 4, (MAX_PARTS * R + 2 * R + 4096) * 4}) lds = n > lds ? n : lds;
-  return {terms == 1 ? k_kv4_rows<C, 1, W, SEES> : terms == 2 ? k_kv4_rows<C, 2, W, SEES> : k_kv4_rows<C, 4, W, SEES>, lds};
+  for (int n : {W * join_floats(R, tiles) * 4, SHARE ? (MAX_PARTS * R + 2 * R + 4096) * 4 : 0}) lds = n > lds ? n : lds;
+  return {terms == 1 ? k_kv4_rows<C, 1, W, SEES, SHARE> : terms == 2 ? k_kv4_rows<C, 2, W, SEES, SHARE> : k_kv4_rows<C, 4, W, SEES, SHARE>, lds};
 }
 
 template <Kv4Sees SEES>
-static AttnKernel rows_kernel_for(int tiles, int terms, int waves) {
+static AttnKernel rows_kernel_for(int tiles, int terms, int waves, bool share) {
   const int C = (tiles + 3) / 4;
+  if (SEES == SEES_ALL) share = true;   // whether or not they do: one kernel
+  if (waves == 4 && !share) {
+    constexpr bool SHARE = SEES == SEES_ALL;
+    return C == 1   ? rows_kernel_of<1, 4, SEES, SHARE>(tiles, terms)
+           : C == 2 ? rows_kernel_of<2, 4, SEES, SHARE>(tiles, terms)
+           : C == 3 ? rows_kernel_of<3, 4, SEES, SHARE>(tiles, terms)
+                    : rows_kernel_of<4, 4, SEES, SHARE>(tiles, terms);
+  }
   if (C == 1) return waves == 4 ? rows_kernel_of<1, 4, SEES>(tiles, terms) : rows_kernel_of<1, 16, SEES>(tiles, terms);
   if (C == 2) return waves == 4 ? rows_kernel_of<2, 4, SEES>(tiles, terms) : rows_kernel_of<2, 8, SEES>(tiles, terms);
   return C == 3 ? rows_kernel_of<3, 4, SEES>(tiles, terms) : rows_kernel_of<4, 4, SEES>(tiles, terms);

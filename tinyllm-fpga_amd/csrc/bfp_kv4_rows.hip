@@ -3,6 +3,6 @@
 
 namespace bfp {
 
-AttnKernel rows_kernel(int tiles, int terms, int waves) { return rows_kernel_for<SEES_ALL>(tiles, terms, waves); }
+AttnKernel rows_kernel(int tiles, int terms, int waves) { return rows_kernel_for<SEES_ALL>(tiles, terms, waves, true); }
 
 }  // namespace bfp
