@@ -194,8 +194,8 @@ static Kv4Plan plan_picks(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_ro
   const long long groups = rows * token_tiles * c.heads, most_groups = (long long)p.row_tiles * c.heads * b.n_seq;
   p.waves = rows_waves(tiles);
   if (key_tiles > 4 * p.waves || most_groups * p.waves > 0x3ffffff || groups > 256) {
-    p.waves = 4;
-    if (groups < 1024 && key_tiles > 16 && b.n_seq <= 256 && most_groups * (key_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
+    p.waves = groups > 1536 ? 2 : 4;
+    if (groups <= 256 && key_tiles > 16 && b.n_seq <= 256 && most_groups * (key_tiles + ROWS_EXTRA) < 0x7fffffffLL) {
       const long long most = groups * (key_tiles + ROWS_EXTRA) / 4 + 1, slots = tiles <= 4 ? 768 : tiles <= 8 ? 512 : 256;
       p.stream = (int)(most < slots ? most : slots);
       p.cells = 2 * (size_t)p.stream * R;

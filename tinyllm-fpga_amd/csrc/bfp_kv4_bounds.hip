@@ -166,7 +166,7 @@ __device__ __forceinline__ void group_sum(const bfp_rows &q, long long o, int gr
 // every fourth 16 pages, whose operands are loaded as they lie, the next ones
 // while these are multiplied.  Bound by the bytes of the bounds.
 template <int R, int K>
-__global__ __launch_bounds__(64 * SCORE_W) void k_kv4_score(Kv4PickArgs a) {
+__global__ __launch_bounds__(64 * SCORE_W, K <= 8 ? 4 : 2) void k_kv4_score(Kv4PickArgs a) {
   constexpr int T = R == 16 ? 3 : 1;
   __shared__ bf16x8 coefs[T * K * 64];
   __shared__ float waves[SCORE_W][16];
@@ -218,11 +218,8 @@ __global__ __launch_bounds__(64 * SCORE_W) void k_kv4_score(Kv4PickArgs a) {
     }
   }
   __syncthreads();
-  bf16x8 coef[T][K];
-#pragma unroll
-  for (int t = 0; t < T; ++t)
-#pragma unroll
-    for (int k = 0; k < K; ++k) coef[t][k] = coefs[(t * K + k) * 64 + lane];
+  // (read again for every tile: in registers those of 16 rows leave room for two waves a SIMD)
+  auto coef = [&](int t, int k) { return coefs[(t * K + k) * 64 + lane]; };
   const long long out = ((long long)seq * a.rows + (i - a.i0)) * a.c.heads + head;
   float most = 0.0f;
 #pragma unroll 1
@@ -231,13 +228,14 @@ __global__ __launch_bounds__(64 * SCORE_W) void k_kv4_score(Kv4PickArgs a) {
     for (int u = 0; u < 2; ++u) {   // the bytes of the tile after the next are asked for when this one's have been used
       const int first = p0 + u * STEP;
       if (first >= pages) break;
+      asm volatile("" ::: "memory");   // the coefficients stay in LDS
       f32x4 sc = {0, 0, 0, 0}, mag = {0, 0, 0, 0};
 #pragma unroll
       for (int k = 0; k < K; ++k) {
 #pragma unroll
-        for (int t = 0; t < T; ++t) sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][k], coef[t][k], sc, 0, 0, 0);
+        for (int t = 0; t < T; ++t) sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[u][k], coef(t, k), sc, 0, 0, 0);
         typedef unsigned u4 __attribute__((ext_vector_type(4)));
-        const u4 va = __builtin_bit_cast(u4, v[u][k]) & 0x7fff7fffu, ca = __builtin_bit_cast(u4, coef[0][k]) & 0x7fff7fffu;
+        const u4 va = __builtin_bit_cast(u4, v[u][k]) & 0x7fff7fffu, ca = __builtin_bit_cast(u4, coef(0, k)) & 0x7fff7fffu;
         mag = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, ca), mag, 0, 0, 0);
       }
       const unsigned long long there = __ballot(id >= 0);
@@ -764,14 +762,14 @@ int bfp_kv4_select_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const uin
   a.picks = picks;
   const score_fn score = p.R == 4 ? score_kernel<4>(cache->hd / 16) : score_kernel<16>(cache->hd / 16);
   const size_t lds = (size_t)(batch->width + 63) / 64 * 16 + (size_t)batch->width * 8;
-  // few workgroups: more waves each
-  const bool wide = pick_blocks * cache->heads <= 512;
-  const score_fn pick = wide ? k_kv4_pick<16> : k_kv4_pick<4>;
+  // few workgroups: more waves each (4084 rows of 1024 pages: 35 us with four, 56 with one)
+  const int W = pick_blocks * cache->heads <= 512 ? 16 : 4;
+  const score_fn pick = W == 16 ? k_kv4_pick<16> : k_kv4_pick<4>;
   if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void *)pick, hipFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024));
   for (a.i0 = 0; a.i0 < rows; a.i0 += p.rows) {
     hipLaunchKernelGGL(score, dim3((unsigned)(blocks * cache->heads)), dim3(64 * SCORE_W), 0, (hipStream_t)stream, a);
     BFP_TRY(launch_status(op));
-    hipLaunchKernelGGL(pick, dim3((unsigned)pick_blocks, cache->heads), dim3(wide ? 1024 : 256), lds, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(pick, dim3((unsigned)pick_blocks, cache->heads), dim3(64 * W), lds, (hipStream_t)stream, a);
     BFP_TRY(launch_status(op));
   }
   return BFP_OK;

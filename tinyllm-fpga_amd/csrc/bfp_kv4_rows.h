@@ -222,6 +222,37 @@ __device__ __forceinline__ int token_of(const Kv4AttnArgs &a, const RowTile &t, 
 template <Kv4Sees SEES>
 __device__ __forceinline__ int head_of(const Kv4AttnArgs &a, int rr) { return SEES == SEES_PICKS ? rr : rr % a.group; }
 
+// A lane's part of a column's query.
+__device__ __forceinline__ void pack_query(const float (&x)[16], bf16x8 (&qf)[2]) {
+  float y[8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int d = 0; d < 8; ++d) y[d] = x[8 * h + d];
+    qf[h] = pack8(y);
+  }
+}
+// All head tiles of it, their loads under way together: behind a branch on the
+// type each they follow one another.
+template <int C, int T, int TYPE>
+__device__ __forceinline__ void load_query(const Kv4AttnArgs &a, long long at, int tile0, bool mine, int t, bf16x8 (&qf)[C][2]) {
+  bfp_rows q = a.q;
+  q.type = TYPE;
+  float x[C][16];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int d = 0; d < 16; ++d) x[c][d] = 0.0f;
+    if (mine && tile0 + c < a.tiles) row_load_n(q, at + 16 * (tile0 + c), x[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int d = 0; d < 16; ++d) x[c][d] = query_term<T>(x[c][d], t) * a.q_sign;
+    pack_query(x[c], qf[c]);
+  }
+}
+
 // The workspace of a launch's own parts, and where unfinished rows go.
 template <Kv4Sees SEES>
 __device__ __forceinline__ float *slot_o(const Kv4AttnArgs &a) { return SEES >= SEES_PREFIX ? a.slot_o : a.part_o; }
@@ -346,25 +377,42 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
     const int32_t *list = PICK ? a.picks + ((long long)(sp.row0 + row_t.i) * a.c.heads + head) * a.n_picks : nullptr;
     const int sees = PICK ? key_hi(sp.at + row_t.i) : 0;
 
+    // the listed pages of a wave's first tiles are asked for before the queries
+    auto pick_of = [&](int tile) {
+      const int p = (int)(((long long)tile * KEYS + 4 * r) >> a.page_shift);
+      return tile < stop && p < a.n_picks ? list[p] : -1;
+    };
+    int tile = first + w;
+    int pick = -1, next_pick = -1, after_pick = -1;
+    if (PICK) {
+      pick = pick_of(tile);
+      next_pick = pick_of(tile + W);
+      after_pick = pick_of(tile + 2 * W);
+    }
+
     // the column's query, term t
     bf16x8 qf[C][2];
+    const long long q_at = (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride;
+    if constexpr (SEES == SEES_ALL) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float x[16];
-      if (mine && g * C + c < tiles) {
-        row_load_n(a.q, (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 16 * (g * C + c), x);
+      for (int c = 0; c < C; ++c) {
+        float x[16];
+        if (mine && g * C + c < tiles) {
+          row_load_n(a.q, q_at + 16 * (g * C + c), x);
 #pragma unroll
-        for (int d = 0; d < 16; ++d) x[d] = query_term<T>(x[d], t) * a.q_sign;
-      } else {
+          for (int d = 0; d < 16; ++d) x[d] = query_term<T>(x[d], t) * a.q_sign;
+        } else {
 #pragma unroll
-        for (int d = 0; d < 16; ++d) x[d] = 0.0f;
+          for (int d = 0; d < 16; ++d) x[d] = 0.0f;
+        }
+        pack_query(x, qf[c]);
       }
-      float y[8];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int d = 0; d < 8; ++d) y[d] = x[8 * h + d];
-        qf[c][h] = pack8(y);
+    } else {
+      switch (a.q.type) {
+        case BFP_F32: load_query<C, T, BFP_F32>(a, q_at, g * C, mine, t, qf); break;
+        case BFP_BF16: load_query<C, T, BFP_BF16>(a, q_at, g * C, mine, t, qf); break;
+        case BFP_F16: load_query<C, T, BFP_F16>(a, q_at, g * C, mine, t, qf); break;
+        default: load_query<C, T, BFP_TILES>(a, q_at, g * C, mine, t, qf); break;
       }
     }
 
@@ -386,22 +434,11 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
       return tile < stop && (unsigned)p < (unsigned)a.b.width ? pages[p] : -1;
     };
     auto known = [&](int raw) { return (unsigned)raw < (unsigned)a.c.n_pages ? raw : -1; };
-    // PICK: the listed page of a tile's keys, asked for three of the wave's tiles ahead, and its number
-    auto pick_of = [&](int tile) {
-      const int p = (int)(((long long)tile * KEYS + 4 * r) >> a.page_shift);
-      return tile < stop && p < a.n_picks ? list[p] : -1;
-    };
+    // PICK: the listed pages are asked for three of the wave's tiles ahead
     auto picked = [&](int pick) { return (unsigned)pick < (unsigned)a.b.width ? pages[pick] : -1; };
 
     // K of the next tile is asked for when this one's scores are done, V when
     // this one's has gone to LDS: no second set of registers
-    int tile = first + w;
-    int pick = -1, next_pick = -1, after_pick = -1;
-    if (PICK) {
-      pick = pick_of(tile);
-      next_pick = pick_of(tile + W);
-      after_pick = pick_of(tile + 2 * W);
-    }
     if (!early) {
       id = known(PICK ? picked(pick) : page_of(tile));
       at = offset_of(tile, id);
@@ -627,6 +664,51 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
     }
     __syncthreads();
     const float *jf = (const float *)lds;
+    if constexpr (SEES != SEES_ALL && !SHARE && W <= 4) {
+      // the rows' factors once, then eight values a thread: with few threads the
+      // factors for every 16 values cost 5 us more (two waves, 8 rows of 128)
+      float *factor = (float *)lds + W * stride, *top = factor + R * W, *total = top + R;
+      for (int u = threadIdx.x; u < 16 * R; u += 64 * W) {
+        const int row = u >> 4, k = u & 15;
+        const float mk = k < W ? jf[k * stride + row] : -INFINITY, M = max16(mk);
+        const float f = mk == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mk - M);
+        const float L = sum16(k < W ? f * jf[k * stride + 16 + row] : 0.0f);
+        if (k < W) factor[row * W + k] = f;
+        if (k == 0) top[row] = M, total[row] = L;
+      }
+      __syncthreads();
+      for (int u = threadIdx.x; u < R * 2 * tiles; u += 64 * W) {   // a tile's two halves in neighbouring lanes
+        const int row = u / (2 * tiles), d = 8 * (u - row * 2 * tiles);
+        if (rr0 + row >= rows) break;
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          const float f = factor[row * W + k];
+          const f32x4 *p = (const f32x4 *)(jf + k * stride + 32 + row * (hd + 4) + d);
+          const f32x4 x = p[0], y = p[1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] += f * x[e];
+            v[4 + e] += f * y[e];
+          }
+        }
+        const float L = total[row];
+        const long long tok = sp.row0 + token_of<SEES>(a, row_t, rr0 + row);
+        const int rh = head * G + head_of<SEES>(a, rr0 + row);
+        if (SEES >= SEES_PREFIX) {
+          const long long at = (tok * a.q.heads + rh) * a.sum_slots + a.sum_slot;
+          if (d == 0) a.part_ml[at] = make_float2(top[row], L);
+          float4 *p = (float4 *)(a.part_o + at * hd + d);
+          p[0] = make_float4(v[0], v[1], v[2], v[3]);
+          p[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = L == 0.0f ? 0.0f : v[e] / L;
+          out_store8(a.out, tok * a.out.row_stride + rh * a.out.head_stride + d, v, a.out_wide);
+        }
+      }
+      return;
+    }
     // 16 lanes to a row's tile; lane k of them works out wave k's factor
     const int l16 = threadIdx.x & 15;
     for (int u = threadIdx.x >> 4; u < R * tiles; u += 4 * W) {
@@ -750,13 +832,20 @@ template <int C, int W, Kv4Sees SEES, bool SHARE = W == 4>
 static AttnKernel rows_kernel_of(int tiles, int terms) {
   const int R = 16 / terms;
   int lds = W * V_ROWS * v_pitch(C);
-  for (int n : {W * join_floats(R, tiles) * 4, SHARE ? (MAX_PARTS * R + 2 * R + 4096) * 4 : 0}) lds = n > lds ? n : lds;
+  for (int n : {(W * join_floats(R, tiles) + (W <= 4 ? R * (W + 2) : 0)) * 4, SHARE ? (MAX_PARTS * R + 2 * R + 4096) * 4 : 0}) lds = n > lds ? n : lds;
   return {terms == 1 ? k_kv4_rows<C, 1, W, SEES, SHARE> : terms == 2 ? k_kv4_rows<C, 2, W, SEES, SHARE> : k_kv4_rows<C, 4, W, SEES, SHARE>, lds};
 }
 
 template <Kv4Sees SEES>
 static AttnKernel rows_kernel_for(int tiles, int terms, int waves, bool share) {
   const int C = (tiles + 3) / 4;
+  if constexpr (SEES == SEES_PICKS) {
+    if (waves == 2)
+      return C == 1   ? rows_kernel_of<1, 2, SEES>(tiles, terms)
+             : C == 2 ? rows_kernel_of<2, 2, SEES>(tiles, terms)
+             : C == 3 ? rows_kernel_of<3, 2, SEES>(tiles, terms)
+                      : rows_kernel_of<4, 2, SEES>(tiles, terms);
+  }
   if (SEES == SEES_ALL) share = true;   // whether or not they do: one kernel
   if (waves == 4 && !share) {
     constexpr bool SHARE = SEES == SEES_ALL;
