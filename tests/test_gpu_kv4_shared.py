@@ -202,6 +202,24 @@ def test_shared_groups_that_hold_nonsense(gpu):
     check(Shared(_int(bad), _int([-3, big_int]), _int([48])), keys, vals, [np.arange(n) // 16 != 1 for n in t.lens])
 
 
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("hd", [32, 128])
+def test_rows_past_all_positions(gpu, new, hd):
+    """Lengths near 2^31 with a window, so that a row's first key lies past
+    every table: nothing is seen, and nothing past the cache is read."""
+    import torch
+    from bfp.kv4 import Shared
+    t = Groups(8, [48], [0, 0, 0], [60 + new, 55 + new, 50 + new], [new] * 3, 16, 1, hd)
+    q, _ = _typed(t.s.rng.standard_normal((3 * new, 2, hd)), "f32")
+    for n in (2 ** 31 - 1, 2 ** 31 - 64, 0x7fff0000, 0x7fff0001):
+        t.batch.lens.fill_(n)
+        for window in (1, 63, 64):
+            for shared in (None, t.shared, Shared(t.shared.pages, t.shared.start, _int([n]))):
+                got = t.s.cache.attend(t.batch, q, shared=shared, window=window)
+                assert (got == 0).all()
+    torch.cuda.synchronize()
+
+
 def test_shared_is_attend_where_tables_agree(gpu):
     """Forked sequences of a pool: the group's table is the parent's."""
     import torch

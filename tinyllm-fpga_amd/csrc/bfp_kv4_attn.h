@@ -47,9 +47,9 @@ struct Kv4AttnArgs {
   // of the same rows and keys: workgroups go to the XCDs and their shader
   // engines in turn, whether one is ready sooner or not, so neighbours should
   // take equally long.
-  __device__ void place(int &seq, int &head, int &split, int &rt) const {
+  __device__ void place(uint32_t block, int &seq, int &head, int &split, int &rt) const {
     uint32_t u, h, s;
-    seq = (int)by_seq.div(blockIdx.x, u);
+    seq = (int)by_seq.div(block, u);
     u = by_head.div(u, h);
     rt = row_tiles - 1 - (int)by_split.div(u, s);
     split = (int)s;
@@ -128,7 +128,7 @@ __device__ __forceinline__ int kv4_shared_len(const Kv4AttnArgs &a, int b, int &
     (a.sh.start[mid] <= b ? g : past) = mid;
   }
   const int n = a.sh.len[g];
-  return a.sh.start[g] <= b && b < a.sh.start[g + 1] && n > 0 ? n : 0;
+  return a.sh.start[g] <= b && b < a.sh.start[g + 1] && n > 0 ? (n < KV4_MAX_POS ? n : KV4_MAX_POS) : 0;
 }
 __device__ __forceinline__ int kv4_shared_len(const Kv4AttnArgs &a, int b) {
   int g;
@@ -393,6 +393,14 @@ AttnKernel prefix_rows_kernel(int tiles, int terms, int waves, bool share);
 AttnKernel prefix_prompt_kernel(int tiles, int terms);
 AttnKernel rest_rows_kernel(int tiles, int terms, int waves, bool share);
 AttnKernel rest_prompt_kernel(int tiles, int terms);
+// Both parts of few rows in one launch, the prefix's workgroups first: they
+// have nothing to wait for in each other.
+typedef void (*attn_parts_fn)(Kv4AttnArgs prefix, Kv4AttnArgs rest, uint32_t prefix_blocks);
+struct PartsKernel {
+  attn_parts_fn fn;
+  int lds;
+};
+PartsKernel parts_kernel(int tiles, int prefix_terms, int rest_terms, int waves);
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }
 // Queues the kernel that joins what k_kv4_prompt left in pieces.

@@ -134,6 +134,7 @@ struct SharedPlan {
   Kv4Plan prefix, rest;
   bfp_kv4_batch groups;
   int slots, pieces;
+  bool joined;              // both parts in one launch
   long long blocks;         // of the first launch, where its pieces are shared out (0: its plan's)
   size_t sums, own, work;   // parts of rows; bytes of the launches' own parts
 };
@@ -150,10 +151,14 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   p.prefix = plan_keys(c, p.groups, q, out, prefix, true, 48);
   const long long cap = (long long)sh.width * c.page;
   p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len > 0 && sh.max_len < cap ? sh.max_len : cap), false, 16);
-  for (Kv4Plan *k : {&p.prefix, &p.rest}) {
-    const long long n = (long long)k->row_tiles * c.heads * (k == &p.rest ? b.n_seq : sh.n_groups);
-    if (!k->prompt && !k->stream && n > 256) k->waves = 4;
-  }
+  long long few = 0;   // workgroups of few rows that take all keys of a row tile: more than the card has CUs, then four waves each
+  for (const Kv4Plan *k : {&p.prefix, &p.rest})
+    if (!k->prompt && !k->stream) few += (long long)k->row_tiles * c.heads * (k == &p.rest ? b.n_seq : sh.n_groups);
+  for (Kv4Plan *k : {&p.prefix, &p.rest})
+    if (!k->prompt && !k->stream && few > 256) k->waves = 4;
+  // Both such, a prefix of few keys or rows and few keys behind it: one launch (5
+  // chats behind 304 tokens, 9 heads of 64: 23 us in two launches, 17 in one).
+  p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves;
   // Prompts' kernel, up to 64 groups: the device shares the keys out, whatever
   // the groups' lengths; no group has more splits than workgroups a KV head.
   p.pieces = p.blocks = 0;
@@ -263,7 +268,8 @@ static int check_work(const char *op, size_t need, const void *work, size_t work
   return BFP_OK;
 }
 
-static int launch_plan(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, hipStream_t s, long long blocks = 0) {
+// The arguments that follow from a plan, and how many workgroups it has.
+static int plan_args(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, long long &blocks) {
   a.splits = p.splits;
   a.chunk = p.chunk;
   a.stream = p.stream;
@@ -274,8 +280,18 @@ static int launch_plan(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const A
   if (blocks > 0x3ffffff / p.waves || each > 0x7fffffff)   // 2^32 threads
     return set_err(BFP_EINVAL, "%s: n_seq=%d of max_q=%d rows are too many for one call", op, a.b.n_seq, a.b.max_q);
   a.by_seq = FastDiv((uint32_t)each);
-  if (k.lds > 65536)   // one limit for a kernel, whatever the call
-    HIP_TRY(hipFuncSetAttribute((const void *)k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024));
+  return BFP_OK;
+}
+template <typename Fn>
+static int lds_limit(Fn fn, int lds) {
+  if (lds > 65536)   // one limit for a kernel, whatever the call
+    HIP_TRY(hipFuncSetAttribute((const void *)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 158 * 1024));
+  return BFP_OK;
+}
+
+static int launch_plan(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const AttnKernel &k, hipStream_t s, long long blocks = 0) {
+  BFP_TRY(plan_args(op, a, p, blocks));
+  BFP_TRY(lds_limit(k.fn, k.lds));
   hipLaunchKernelGGL(k.fn, dim3((unsigned)blocks), dim3(64 * p.waves), k.lds, s, a);
   return launch_status(op);
 }
@@ -378,6 +394,21 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
   Kv4AttnArgs g = a;
   g.b = p.groups;
   const Kv4Plan &one = p.prefix, &two = p.rest;
+  if (p.joined) {
+    long long n1 = 0, n2 = 0;
+    g.sum_slot = 0;
+    a.sum_slot = one.splits;
+    BFP_TRY(plan_args(op, g, one, n1));
+    BFP_TRY(plan_args(op, a, two, n2));
+    if (n1 + n2 > 0x3ffffff / one.waves)
+      return set_err(BFP_EINVAL, "%s: n_groups=%d and n_seq=%d are too many for one call", op, shared->n_groups, batch->n_seq);
+    const PartsKernel k = parts_kernel(a.tiles, one.terms, two.terms, one.waves);
+    BFP_TRY(lds_limit(k.fn, k.lds));
+    hipLaunchKernelGGL(k.fn, dim3((unsigned)(n1 + n2)), dim3(64 * one.waves), k.lds, s, g, a, (uint32_t)n1);
+    BFP_TRY(launch_status(op));
+    launch_join_shared(a, s);
+    return launch_status(op);
+  }
   BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms) : prefix_rows_kernel(a.tiles, one.terms, one.waves, one.stream > 0),
                       0, own, s, p.blocks));
   BFP_TRY(launch_part(op, a, two, two.prompt ? rest_prompt_kernel(a.tiles, two.terms) : rest_rows_kernel(a.tiles, two.terms, two.waves, two.stream > 0),

@@ -70,7 +70,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   if (SEES == SEES_PREFIX && a.pieces) {
     if (!a.piece(ROWS, seq, head, split, rt, splits, chunk)) return;
   } else {
-    a.place(seq, head, split, rt);
+    a.place(blockIdx.x, seq, head, split, rt);
   }
   Kv4Group of{};
   const Kv4Span sp = SEES == SEES_PREFIX ? kv4_group_span(a, seq, of)
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   const uint32_t page_tiles = (uint32_t)a.c.heads * tiles * a.c.page;   // at most 2^24
   auto fetch = [&](Bytes &x, int tile, int id) __attribute__((always_inline)) {
     x.there = (unsigned)id < (unsigned)a.c.n_pages;
-    const uint32_t slot = (uint32_t)(tile * KEYS + lane) & (a.c.page - 1);
+    const uint32_t slot = ((uint32_t)tile * KEYS + lane) & (a.c.page - 1);   // (unsigned: past the last tile)
     const unsigned long long at = (unsigned long long)(x.there ? (uint32_t)id : 0u) * page_tiles + slot;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {

@@ -273,7 +273,7 @@ constexpr int rows_per_simd(int C, int W, Kv4Sees sees, bool share) {
 }
 
 template <int C, int T, int W, Kv4Sees SEES, bool SHARE>
-__global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv4_rows(Kv4AttnArgs a) {
+__device__ __forceinline__ void rows_block(const Kv4AttnArgs &a, uint32_t block) {
   constexpr int R = 16 / T;
   constexpr bool PICK = SEES == SEES_PICKS;
   extern __shared__ __align__(16) char lds[];
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
   uint32_t x = 0, x_stop = 1, piece = 0;
   if (SHARE && a.stream) {
     piece = stream_plan<SEES>(a, R, st);
-    x = blockIdx.x * piece;
+    x = block * piece;
     const uint32_t all = st.before[a.b.n_seq];
     if (x >= all) return;
     x_stop = x + piece < all ? x + piece : all;
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
       seq += __popcll(__ballot(st.before[b + 1] <= x));
     seq = __builtin_amdgcn_readfirstlane(seq);
   } else {
-    a.place(seq, head, split, rt);
+    a.place(block, seq, head, split, rt);
   }
   const int G = a.group;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
@@ -301,8 +301,11 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
   bool begun = false;
   while (x < x_stop) {
     const int32_t *pages = a.b.pages + (long long)seq * a.b.width;
+    // Unsigned: of a wave that has no tile, whose first one may lie past 2^31 keys
+    // (the place of a signed overflow's result in its page is not defined).
+    auto slot_of = [&](int tile) { return (uint32_t)tile * KEYS + 4 * r; };
     auto offset_of = [&](int tile, int id) {
-      return kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, (tile * KEYS + 4 * r) & (a.c.page - 1));
+      return kv4_tile(id < 0 ? 0 : id, a.c.heads, head, tiles, 0, a.c.page, slot_of(tile) & (a.c.page - 1));
     };
     // Without a window a wave's first tile is known before the lengths are:
     // its page number and its bytes are on their way while those arrive.
@@ -331,7 +334,7 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
       }
       upto = from + (int)take < sp.tiles ? from + (int)take : sp.tiles;
       // the first part of a row tile's keys goes to the workgroup's second slot, any other to its first
-      if (from > 0 || upto < sp.tiles) slot = 2 * blockIdx.x + (from == 0 ? 1 : 0);
+      if (from > 0 || upto < sp.tiles) slot = 2 * block + (from == 0 ? 1 : 0);
       head = (int)(group % (uint32_t)a.c.heads);
       rt = (int)(group / (uint32_t)a.c.heads);
       if (begun) __syncthreads();   // the last round's sums have been read
@@ -430,8 +433,8 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
     // and looked at only when its bytes are asked for (8 sequences of 131072
     // tokens, 8 KV heads of 128: 151 us with one tile ahead, 149 so).
     auto page_of = [&](int tile) {
-      const int p = (tile * KEYS + 4 * r) >> a.page_shift;
-      return tile < stop && (unsigned)p < (unsigned)a.b.width ? pages[p] : -1;
+      const uint32_t p = slot_of(tile) >> a.page_shift;
+      return tile < stop && p < (unsigned)a.b.width ? pages[p] : -1;
     };
     auto known = [&](int raw) { return (unsigned)raw < (unsigned)a.c.n_pages ? raw : -1; };
     // PICK: the listed pages are asked for three of the wave's tiles ahead
@@ -739,7 +742,7 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
       stores_done();
       __syncthreads();
       if (w == 0) {
-        const bool all = arrive(a.there, a.number, p0, blockIdx.x - p0, parts);
+        const bool all = arrive(a.there, a.number, p0, block - p0, parts);
         if (lane == 0) st.last = all;
       }
       __syncthreads();
@@ -747,6 +750,21 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
     }
     while (x < x_stop && x == st.before[seq + 1]) ++seq;   // and past sequences without rows
   }
+}
+
+template <int C, int T, int W, Kv4Sees SEES, bool SHARE>
+__global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv4_rows(Kv4AttnArgs a) {
+  rows_block<C, T, W, SEES, SHARE>(a, blockIdx.x);
+}
+
+// Both parts of rows that share a prefix.
+template <int C, int T1, int T2, int W>
+__global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES_REST, false)) void k_kv4_parts(Kv4AttnArgs prefix, Kv4AttnArgs rest,
+                                                                                             uint32_t prefix_blocks) {
+  if (blockIdx.x < prefix_blocks)
+    rows_block<C, T1, W, SEES_PREFIX, false>(prefix, blockIdx.x);
+  else
+    rows_block<C, T2, W, SEES_REST, false>(rest, blockIdx.x - prefix_blocks);
 }
 
 // 64 E values of a part at a time, row after row; a lane has E of them under
@@ -828,11 +846,17 @@ __device__ void join_parts(const Kv4AttnArgs &a, char *lds, const RowsSeq &sp, i
     join_values<16, SEES>(a, sp, head, row_t, p0, parts, R, values, factor, total, top, sums);
 }
 
+static int rows_lds(int C, int W, int R, int tiles, bool share) {
+  int lds = W * V_ROWS * v_pitch(C);
+  for (int n : {(W * join_floats(R, tiles) + (W <= 4 ? R * (W + 2) : 0)) * 4, share ? (MAX_PARTS * R + 2 * R + 4096) * 4 : 0})
+    lds = n > lds ? n : lds;
+  return lds;
+}
+
 template <int C, int W, Kv4Sees SEES, bool SHARE = W == 4>
 static AttnKernel rows_kernel_of(int tiles, int terms) {
   const int R = 16 / terms;
-  int lds = W * V_ROWS * v_pitch(C);
-  for (int n : {(W * join_floats(R, tiles) + (W <= 4 ? R * (W + 2) : 0)) * 4, SHARE ? (MAX_PARTS * R + 2 * R + 4096) * 4 : 0}) lds = n > lds ? n : lds;
+  const int lds = rows_lds(C, W, R, tiles, SHARE);
   return {terms == 1 ? k_kv4_rows<C, 1, W, SEES, SHARE> : terms == 2 ? k_kv4_rows<C, 2, W, SEES, SHARE> : k_kv4_rows<C, 4, W, SEES, SHARE>, lds};
 }
 
@@ -857,6 +881,16 @@ static AttnKernel rows_kernel_for(int tiles, int terms, int waves, bool share) {
   if (C == 1) return waves == 4 ? rows_kernel_of<1, 4, SEES>(tiles, terms) : rows_kernel_of<1, 16, SEES>(tiles, terms);
   if (C == 2) return waves == 4 ? rows_kernel_of<2, 4, SEES>(tiles, terms) : rows_kernel_of<2, 8, SEES>(tiles, terms);
   return C == 3 ? rows_kernel_of<3, 4, SEES>(tiles, terms) : rows_kernel_of<4, 4, SEES>(tiles, terms);
+}
+
+template <int C, int W>
+static PartsKernel parts_kernel_of(int tiles, int t1, int t2) {
+  const int one = rows_lds(C, W, 16 / t1, tiles, false), two = rows_lds(C, W, 16 / t2, tiles, false);
+  return {t1 == 4   ? k_kv4_parts<C, 4, 4, W>
+          : t1 == 2 ? k_kv4_parts<C, 2, 2, W>
+          : t2 == 2 ? k_kv4_parts<C, 1, 2, W>
+                    : k_kv4_parts<C, 1, 1, W>,
+          one > two ? one : two};
 }
 
 }  // namespace bfp
