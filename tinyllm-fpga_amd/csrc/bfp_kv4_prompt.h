@@ -100,38 +100,34 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   const int first = tile0 + part.first, stop = tile0 + part.stop;
 
   // this lane's row, and what the wave's rows all see
-  int hi, lo, hi_min, lo_max;
+  int hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
+  const int wfirst = rr0 < rows ? rr0 : rows - 1, wlast = (rr0 + 32 < rows ? rr0 + 32 : rows) - 1;
+  int hi_min = key_hi(sp.at + wfirst / G), lo_max = key_lo(rr0 < rows ? key_hi(sp.at + wlast / G) : 0, a.window);
+  if (SEES == SEES_REST) {
+    lo = lo > low ? lo : low;
+    lo_max = lo_max > low ? lo_max : low;
+  }
   bool blind = false;   // SEES_PREFIX: the row sees none of it; what is worked out for it is thrown away, not masked
   bf16x8 qf[T][TB];
+  // SEES_PREFIX, whose rows are of several sequences: by each one's position
   auto take_rows = [&]() __attribute__((always_inline)) {
-    hi = mine ? key_hi(sp.at + i) : 0, lo = key_lo(hi, a.window);
-    const int wfirst = rr0 < rows ? rr0 : rows - 1, wlast = (rr0 + 32 < rows ? rr0 + 32 : rows) - 1;
-    hi_min = key_hi(sp.at + wfirst / G);
-    lo_max = key_lo(rr0 < rows ? key_hi(sp.at + wlast / G) : 0, a.window);
-    if constexpr (SEES == SEES_REST) {
-      lo = lo > low ? lo : low;
-      lo_max = lo_max > low ? lo_max : low;
-    }
-    if constexpr (SEES == SEES_PREFIX) {   // rows of several sequences: by each one's position
-      uint32_t rest;
-      const int row = (int)a.by_group.div((uint32_t)(mine ? rr : rows - 1), rest);
-      const int ends = key_hi(kv4_row_position<32>(a, of, sp.row0 + row));
-      lo = mine ? key_lo(ends, a.window) : 0;
-      hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
-      blind = hi <= lo;
-      hi_min = __builtin_amdgcn_readfirstlane(min_lanes<32>(blind ? 0x7fffffff : hi));
-      lo_max = __builtin_amdgcn_readfirstlane(max_lanes<32>(blind ? 0 : lo));
-    }
+    uint32_t rest;
+    const int row = (int)a.by_group.div((uint32_t)(mine ? rr : rows - 1), rest);
+    const int ends = key_hi(kv4_row_position<32>(a, of, sp.row0 + row));
+    lo = mine ? key_lo(ends, a.window) : 0;
+    hi = mine ? (ends < sp.at ? ends : sp.at) : 0;
+    blind = hi <= lo;
+    hi_min = __builtin_amdgcn_readfirstlane(min_lanes<32>(blind ? 0x7fffffff : hi));
+    lo_max = __builtin_amdgcn_readfirstlane(max_lanes<32>(blind ? 0 : lo));
     const long long q_at = (long long)(sp.row0 + i) * a.q.row_stride + qh * a.q.head_stride + 8 * h;
-    if constexpr (SEES == SEES_PREFIX) {
-      switch (a.q.type) {
-        case BFP_F32: prompt_query<TB, T, BFP_F32>(a, q_at, mine, qf); break;
-        case BFP_BF16: prompt_query<TB, T, BFP_BF16>(a, q_at, mine, qf); break;
-        case BFP_F16: prompt_query<TB, T, BFP_F16>(a, q_at, mine, qf); break;
-        default: prompt_query<TB, T, BFP_TILES>(a, q_at, mine, qf); break;
-      }
-      return;
+    switch (a.q.type) {
+      case BFP_F32: prompt_query<TB, T, BFP_F32>(a, q_at, mine, qf); break;
+      case BFP_BF16: prompt_query<TB, T, BFP_BF16>(a, q_at, mine, qf); break;
+      case BFP_F16: prompt_query<TB, T, BFP_F16>(a, q_at, mine, qf); break;
+      default: prompt_query<TB, T, BFP_TILES>(a, q_at, mine, qf); break;
     }
+  };
+  if constexpr (SEES != SEES_PREFIX) {
 #pragma unroll
     for (int c = 0; c < TB; ++c) {
       float x[8];
@@ -149,8 +145,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
         qf[t][c] = pack8(y);
       }
     }
-  };
-  if (SEES != SEES_PREFIX) take_rows();
+  }
 
   float m = -INFINITY, sum = 0.0f;
   f32x16 o[DT];
@@ -267,7 +262,7 @@ __global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs 
   int id = page_of(first);
   fetch(next, first, id);
   unsigned long long ok = next.ok;
-  if (SEES == SEES_PREFIX) take_rows();   // while the first tile is under way
+  if constexpr (SEES == SEES_PREFIX) take_rows();   // while the first tile is under way
   decode(next, 0);
   id = page_of(first + 1);
   __syncthreads();
