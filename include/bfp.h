@@ -656,9 +656,11 @@ size_t bfp_kv4_attn_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const
  * start[g] .. start[g+1]-1 of a batch have their first len[g] tokens in common,
  * position p of them in page pages[g*width + p/page].  start (n_groups + 1,
  * ascending), len (n_groups) and pages are device arrays of int32.  max_rows:
- * no group has more new rows (0: n_rows); max_len: none shares more (0: width
- * * page) -- it only chooses how the work is split.  Sequences outside every
- * group share nothing. */
+ * no group has more new rows (0: n_rows; rows past those are undefined);
+ * max_len: none shares more (0: width * page) -- it only chooses how the work
+ * is split.  With the batch's max_len it says how many tokens sequences have of
+ * their own: where some have far more than the difference, because they share
+ * less, leave it 0.  Sequences outside every group share nothing. */
 typedef struct bfp_kv4_shared {
   const int32_t *pages, *start, *len;
   int n_groups, width, max_rows, max_len;
@@ -667,7 +669,8 @@ typedef struct bfp_kv4_shared {
  * from the group's pages, once for all of the group's rows, and only the later
  * ones from each sequence's own: the entries of a sequence's table before
  * position len[g] are not looked at.  A row sees of the shared tokens those up
- * to its own position and within its window, as of any. */
+ * to its own position and within its window, as of any.  At most 2^26 - 16
+ * rows and query heads a sequence. */
 int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,
                           const bfp_rows *out, double scale, int window, void *work, size_t work_bytes, void *stream);
 size_t bfp_kv4_attn_shared_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,

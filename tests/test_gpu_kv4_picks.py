@@ -157,7 +157,7 @@ def test_select_equal_scores(gpu):
     """All pages alike, or alike in groups: the lower ones."""
     one = np.random.default_rng(1).standard_normal((4, 2, 2, 32))
     for kinds in (1, 4):
-        for lens, news in (([700, 64], [2, 2]), ([700], [30])):
+        for lens, news in (([700, 64], [2, 2]), ([700], [30]), ([700], [300]), ([3000, 5], [4, 1]), ([3000], [300])):
             s, buf, bounds, q, qv = _flat(lens, news, 16, 2, 32, 4, lambda rng, i: one[i * 7 % kinds])
             got = bounds.select(s.batch, q, 9, first=1, last=2).cpu().numpy()
             assert (got == choose(s, buf, qv, 2, 9, 1, 2)).all()
@@ -202,6 +202,28 @@ def test_select_extremes(gpu):
     assert (got[0] == want[0]).all() and (got[2:] == want[2:]).all()
     assert (got[1, 1] == want[1, 1]).all()      # the other KV head of the row with the infinity
     assert torch.isfinite(q).sum() == q.numel() - 1
+
+
+@pytest.mark.parametrize("width", [3000, 6200, 7000, 7943, 7944, 16384])
+def test_select_of_wide_tables(gpu, width):
+    """Scores of more and more pages in the workgroup's memory."""
+    import torch
+    from bfp.kv4 import Batch, Fp4Cache, PageBounds
+    cache = Fp4Cache(width, 16, 1, 16)
+    g = torch.Generator().manual_seed(width)
+    buf = torch.randint(-64, 65, (width, 1, 2, 16), generator=g).bfloat16()
+    order = torch.randperm(width, generator=g)
+    for rows in (1, 530):
+        batch = Batch(_int(order.numpy()[None]), _int([0, rows]), _int([16 * width]), max_q=rows)
+        q = torch.randint(-8, 9, (rows, 1, 16), generator=g).float().cuda()
+        got = PageBounds.from_buffer(cache, buf.cuda()).select(batch, q, 33, first=1, last=2).cpu()
+        b, x = buf[order].double(), q.double().cpu()
+        for t in {0, rows // 2, rows - 1}:
+            m = (16 * width - rows + t) // 16 + 1
+            score = ((x[t, 0].clamp(min=0) * b[:m, 0, 1]).sum(-1) + (x[t, 0].clamp(max=0) * b[:m, 0, 0]).sum(-1)).numpy()   # whole numbers
+            score[[0, m - 2, m - 1]] = np.inf
+            want = sorted(np.lexsort((np.arange(m), -score))[:33])
+            assert (got[t, 0].numpy() == want).all(), (rows, t)
 
 
 def test_select_leaves_other_rows(gpu):
@@ -250,6 +272,11 @@ PICKED = [  # lens, news, page, heads, hd, query heads, n, type, out type
     ([6000, 5000], [1, 1], 16, 1, 64, 3, 200, "f32", None),       # shared by many workgroups
     ([5000], [1], 64, 2, 128, 8, 70, "bf16", None),
     ([1200], [700], 16, 2, 64, 4, 4, "f16", None),                # many rows
+    ([1000], [900], 16, 2, 32, 2, 4, "bf16", None),               # and more
+    ([900], [800], 32, 2, 256, 2, 3, "f32", None),
+    ([9000], [1], 64, 2, 64, 4, 80, "bf16", None),                # long lists
+    ([2600, 1500], [1, 1], 64, 1, 256, 4, 20, "f16", None),
+    ([2600, 1500], [1, 2], 128, 1, 160, 20, 12, "tile", None),
 ]
 
 

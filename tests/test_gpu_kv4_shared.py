@@ -60,6 +60,8 @@ class Groups:
             mine = [b for b, x in enumerate(of) if x == k]
             bounds[k] = mine[0] if mine else bounds[k - 1] if k else 0
             bounds[k + 1] = mine[-1] + 1 if mine else bounds[k]
+        assert all(bounds[x] <= b < bounds[x + 1] for b, x in enumerate(of) if x >= 0)
+        assert not any(bounds[0] <= b < bounds[g] for b, x in enumerate(of) if x < 0)      # (between groups: one that shares 0)
         self.table = s.table[g:].copy()
         self.keys, self.vals, self.there = [], [], []
         for b, n in enumerate(lens):
@@ -100,6 +102,11 @@ CASES = [  # share, of, lens, news, page, heads, hd, query heads, type, result, 
     ([900, 700], [0] * 6 + [1] * 5, [950] * 6 + [790] * 5, [50] * 6 + [90] * 5, 64, 2, 64, 4, "f32", None, 0),
     ([900], [0] * 7, [960] * 7, [40] * 7, 16, 1, 192, 4, "f16", None, 0),
     ([600], [0] * 5, [700] * 5, [30] * 5, 128, 1, 256, 4, "bf16", None, 300),
+    ([900] * 70, list(range(70)), [940 + g for g in range(70)], [40] * 70, 32, 1, 32, 4, "bf16", None, 0),   # more groups than lanes, split
+    ([200, 100], [0] * 3 + [1] * 2, [441, 440, 450, 340, 350], [240] * 5, 16, 64, 16, 64, "bf16", None, 0),  # more row tiles than pieces
+    ([304], [0, 0, -1], [9000, 310, 5000], [1, 1, 1], 16, 1, 64, 2, "tile", None, 0),                        # long after the prefix
+    ([100], [0, 0], [3200, 2100], [60, 50], 32, 1, 64, 4, "bf16", None, 0),                                  # and split there
+    ([3000, 0, 10], [0, 1, 2], [3300, 2900, 400], [70, 60, 50], 64, 2, 128, 4, "f16", None, 500),
     ([40], [0] * 130, [41 + b % 7 for b in range(130)], [1] * 130, 16, 1, 16, 1, "f32", None, 0),            # more sequences than lanes
     ([33], [0] * 70, [34 + b % 5 if b % 3 else 0 for b in range(70)], [1 if b % 2 else 0 for b in range(70)], 16, 1, 32, 2, "f32", None, 7),
 ]
@@ -243,8 +250,12 @@ def test_shared_is_attend_where_tables_agree(gpu):
         cache.append(batch, rand(4, 2), rand(4, 2))
         q = rand(4, 6)
         a, b = cache.attend(batch, q), cache.attend(batch, q, shared=shared)
-        # each within 2^-16 of the largest value of the exact result at these sizes (scores up to 6, 153 keys)
-        assert (a - b).abs().max() <= 2.0 ** -15 * 4.0
+        keys, vals = cache.read(Batch(table, _int([0] + [int(x) for x in batch.lens.cumsum(0)]), batch.lens, max_q=200), int(batch.lens.sum()))
+        ends = np.concatenate([[0], np.cumsum(batch.lens.cpu().numpy())])
+        k, v = ([x[ends[b]:ends[b + 1]].double().cpu().numpy() for b in range(4)] for x in (keys, vals))
+        want, weight, big = ref.attend_all(q.double().cpu().numpy(), k, v, np.arange(5), batch.lens.cpu().numpy(), 3, 1 / 8, 0)
+        for got in (a, b):
+            assert (np.abs(got.double().cpu().numpy() - want) <= _bound(want, weight, big, 153, 64, "f32", "f32", 12)).all()
 
 
 @pytest.mark.parametrize("new", [1, 40])

@@ -56,6 +56,8 @@ def test_refuses_bad_calls():
         _refused(L, *_call(L, **kw))
     many = _batch(L, n_rows=2 ** 31 - 1)
     assert "too many" in _refused(L, *_call(L, cache=_cache(L, heads=1), batch=many, q=_rows(L, heads=8, rs=512), out=_rows(L, heads=8, rs=512)))
+    many = _batch(L, n_rows=1 << 23, max_q=1 << 23)     # a thread for each lane of the join
+    assert "too many" in _refused(L, *_call(L, cache=_cache(L, heads=1), batch=many, q=_rows(L, heads=8, rs=512), out=_rows(L, heads=8, rs=512)))
 
 
 def test_nothing_to_do_is_no_error():

@@ -78,10 +78,12 @@ class Shared(_rows.Fixed):
     start[g] .. start[g + 1] - 1 have lens[g] tokens in common, position p of
     them in page pages[g, p // page].  pages (groups, width), start (groups +
     1, ascending) and lens are int32 tensors on the device, read when a call
-    runs, as a Batch's.  max_rows: the most new rows a group has (0: all);
-    max_len: the most tokens one shares (0: the table's width), which only
-    chooses how the work is split.  Sequences outside every group share
-    nothing."""
+    runs, as a Batch's.  max_rows: the most new rows a group has (0: all; the
+    results of rows past those are undefined); max_len: the most tokens one
+    shares (0: the table's width), which only chooses how the work is split:
+    with the batch's max_len it says how many tokens sequences have of their
+    own, so leave it 0 where some share far less than others.  Sequences
+    outside every group share nothing."""
 
     def __init__(self, pages, start, lens, max_rows=0, max_len=0):
         if pages.dim() != 2 or pages.shape[1] < 1 or pages.shape[0] < 1:

@@ -149,8 +149,9 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   p.groups.max_q = sh.max_rows > 0 && sh.max_rows < b.n_rows ? sh.max_rows : b.n_rows;
   const long long prefix = keys_of(c, p.groups, window, 0);
   p.prefix = plan_keys(c, p.groups, q, out, prefix, true, 48);
+  // Without a hint the rest may be anything: the keys of a stream are shared out on the device.
   const long long cap = (long long)sh.width * c.page;
-  p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len > 0 && sh.max_len < cap ? sh.max_len : cap), false, 16);
+  p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len < cap ? sh.max_len : cap), false, 16);
   long long few = 0;   // workgroups of few rows that take all keys of a row tile: more than the card has CUs, then four waves each
   for (const Kv4Plan *k : {&p.prefix, &p.rest})
     if (!k->prompt && !k->stream) few += (long long)k->row_tiles * c.heads * (k == &p.rest ? b.n_seq : sh.n_groups);
@@ -331,6 +332,8 @@ static int check_shared(const char *op, const bfp_kv4_batch *b, const bfp_kv4_sh
     return set_err(BFP_EINVAL, "%s: width=%d pages of %d are more than %d positions", op, sh->width, c->page, KV4_MAX_POS);
   if ((long long)b->n_rows * (q->heads / c->heads) > 0x3fffffffLL && (sh->max_rows == 0 || (long long)sh->max_rows * (q->heads / c->heads) > 0x3fffffffLL))
     return set_err(BFP_EINVAL, "%s: groups of max_rows=%d rows of %d heads are too many", op, sh->max_rows, q->heads);
+  if ((long long)(b->max_q < b->n_rows ? b->max_q : b->n_rows) * q->heads > 0x3fffff0LL)   // the join: 2^32 threads
+    return set_err(BFP_EINVAL, "%s: max_q=%d rows of %d heads are too many", op, b->max_q, q->heads);
   return BFP_OK;
 }
 

@@ -765,7 +765,7 @@ int bfp_kv4_select_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const uin
   // few workgroups: more waves each (4084 rows of 1024 pages: 35 us with four, 56 with one)
   const int W = pick_blocks * cache->heads <= 512 ? 16 : 4;
   const score_fn pick = W == 16 ? k_kv4_pick<16> : k_kv4_pick<4>;
-  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void *)pick, hipFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024));
+  if (lds > 49152) HIP_TRY(hipFuncSetAttribute((const void *)pick, hipFuncAttributeMaxDynamicSharedMemorySize, 136 * 1024));
   for (a.i0 = 0; a.i0 < rows; a.i0 += p.rows) {
     hipLaunchKernelGGL(score, dim3((unsigned)(blocks * cache->heads)), dim3(64 * SCORE_W), 0, (hipStream_t)stream, a);
     BFP_TRY(launch_status(op));

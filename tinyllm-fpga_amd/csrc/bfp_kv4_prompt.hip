@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void k_kv4_join_shared(Kv4AttnArgs a) {
   const long long tok = sp.row0 + i, at = (tok * a.q.heads + qh) * a.sum_slots;
   const int hd = 16 * a.tiles;
   int g, before = 0;
-  if (kv4_shared_len(a, seq, g) > 0) before = a.split_of ? a.split_of[g] : a.prefix_slots;
+  if (kv4_shared_len(a, seq, g) > 0) before = a.split_of ? min(a.split_of[g], a.prefix_slots) : a.prefix_slots;
   const int n = before + a.sum_slots - a.prefix_slots;   // slot k of them
   auto slot = [&](int k) { return k < before ? k : k - before + a.prefix_slots; };
   const float2 ml = lane < n ? a.part_ml[at + slot(lane)] : make_float2(-INFINITY, 0.0f);
@@ -101,7 +101,7 @@ void launch_join_prompt(const Kv4AttnArgs &a, hipStream_t s) {
 }
 
 void launch_join_shared(const Kv4AttnArgs &a, hipStream_t s) {
-  const long long n = ((long long)a.b.max_q * a.q.heads + 3) / 4;
+  const long long n = ((long long)(a.b.max_q < a.b.n_rows ? a.b.max_q : a.b.n_rows) * a.q.heads + 3) / 4;
   hipLaunchKernelGGL(k_kv4_join_shared, dim3((unsigned)n, a.b.n_seq), dim3(256), 0, s, a);
 }
 
