@@ -390,7 +390,7 @@ AttnKernel picks_kernel(int tiles, int terms, int waves, bool share);
 AttnKernel prompt_kernel(int tiles, int terms);
 // Of a shared prefix, and of what lies behind it.
 AttnKernel prefix_rows_kernel(int tiles, int terms, int waves, bool share);
-AttnKernel prefix_prompt_kernel(int tiles, int terms);
+AttnKernel prefix_prompt_kernel(int tiles, int terms, bool pairs);
 AttnKernel rest_rows_kernel(int tiles, int terms, int waves, bool share);
 AttnKernel rest_prompt_kernel(int tiles, int terms);
 // Both parts of few rows in one launch, the prefix's workgroups first: they
@@ -403,6 +403,8 @@ struct PartsKernel {
 PartsKernel parts_kernel(int tiles, int prefix_terms, int rest_terms, int waves);
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }
+// Two workgroups of four waves a CU instead of one of eight: registers and LDS hold them.
+inline bool prompt_pairs(int tiles, int terms) { return tiles <= 6 && terms < 3; }
 // Queues the kernel that joins what k_kv4_prompt left in pieces.
 void launch_join_prompt(const Kv4AttnArgs &a, hipStream_t s);
 // The same of a row's two parts.

@@ -135,6 +135,7 @@ struct SharedPlan {
   bfp_kv4_batch groups;
   int slots, pieces;
   bool joined;              // both parts in one launch
+  bool pairs;               // the prompts' kernel with two workgroups a CU
   long long blocks;         // of the first launch, where its pieces are shared out (0: its plan's)
   size_t sums, own, work;   // parts of rows; bytes of the launches' own parts
 };
@@ -160,18 +161,27 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   // Both such, a prefix of few keys or rows and few keys behind it: one launch (5
   // chats behind 304 tokens, 9 heads of 64: 23 us in two launches, 17 in one).
   p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves;
-  // Prompts' kernel, up to 64 groups: the device shares the keys out, whatever
-  // the groups' lengths; no group has more splits than workgroups a KV head.
+  // Prompts' kernel: 128 rows a workgroup where that leaves fewer rows empty
+  // than 256 (groups of 320 rows, heads of 96, two terms: 217 us against 260; where
+  // both fill them alike 550 against 520).
+  const long long group_rows = (long long)p.groups.max_q * (q.heads / c.heads), in_8 = (group_rows + 255) / 256 * 256, in_4 = (group_rows + 127) / 128 * 128;
+  p.pairs = p.prefix.prompt && prompt_pairs(c.hd / 16, p.prefix.terms) && in_4 + in_4 / 8 < in_8;
+  if (p.pairs) {
+    p.prefix.waves = 4;
+    p.prefix.row_tiles = (int)(in_4 / 128);
+  }
+  // Up to 64 groups: the device shares the keys out, whatever the groups'
+  // lengths; no group has more splits than workgroups a KV head.
   p.pieces = p.blocks = 0;
   if (p.prefix.prompt && sh.n_groups <= 64) {
     const int group = q.heads / c.heads, rows = 32 * p.prefix.waves;
     const long long key_tiles = (prefix + KEYS - 1) / KEYS;
     const long long most = ((long long)b.n_rows * group + rows - 1) / rows * c.heads + (long long)sh.n_groups * c.heads;
-    int s = 256 / c.heads;
+    p.pieces = p.pairs ? 512 : 256;
+    int s = p.pieces / c.heads;
     if (s > key_tiles / 4) s = (int)(key_tiles / 4);
     p.prefix.splits = s < 1 ? 1 : s < 48 ? s : 48;
-    p.pieces = 256;
-    p.blocks = most > 256 ? most : 256;
+    p.blocks = most > p.pieces ? most : p.pieces;
   }
   p.slots = p.prefix.splits + p.rest.splits;
   p.sums = (size_t)b.n_rows * q.heads * p.slots;
@@ -412,7 +422,7 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
     launch_join_shared(a, s);
     return launch_status(op);
   }
-  BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms) : prefix_rows_kernel(a.tiles, one.terms, one.waves, one.stream > 0),
+  BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms, p.pairs) : prefix_rows_kernel(a.tiles, one.terms, one.waves, one.stream > 0),
                       0, own, s, p.blocks));
   BFP_TRY(launch_part(op, a, two, two.prompt ? rest_prompt_kernel(a.tiles, two.terms) : rest_rows_kernel(a.tiles, two.terms, two.waves, two.stream > 0),
                       one.splits, own, s));

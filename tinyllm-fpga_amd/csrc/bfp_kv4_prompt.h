@@ -61,7 +61,7 @@ __device__ __forceinline__ void prompt_query(const Kv4AttnArgs &a, long long at,
 // missing tiles are zeros in K, and columns of V whose results nobody
 // takes); T: terms; W: waves.
 template <int TB, int T, int W, Kv4Sees SEES>
-__global__ __launch_bounds__(64 * W, (W + 3) / 4) void k_kv4_prompt(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * W, W == 8 || (T < 3 && TB <= 6) ? 2 : 1) void k_kv4_prompt(Kv4AttnArgs a) {
   constexpr int ROWS = 32 * W, DT = TB / 2, UNITS = (TB + W - 1) / W;
   constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), NV = v_buffers(TB);
   extern __shared__ __align__(16) char lds[];
