@@ -204,6 +204,17 @@ def test_select_extremes(gpu):
     assert torch.isfinite(q).sum() == q.numel() - 1
 
 
+@pytest.mark.parametrize("news", [[1, 1], [7, 9]])
+def test_select_scores_below_float32(gpu, news):
+    """Scores that are minus infinity in float32 are pages all the same."""
+    def fill(rng, i):
+        return -2.0 ** 100 * rng.integers(1, 100, (2, 1, 32)).repeat(2, 1)
+    s, buf, bounds, q, qv = _flat([640, 320], news, 16, 2, 32, 4, fill)
+    q = (q.abs() + 0.5) * 2.0 ** 60
+    got = bounds.select(s.batch, q, 12, first=1, last=2).cpu().numpy()
+    assert (got == choose(s, buf, q.double().cpu().numpy(), 2, 12, 1, 2)).all()
+
+
 @pytest.mark.parametrize("width", [3000, 6200, 7000, 7943, 7944, 16384])
 def test_select_of_wide_tables(gpu, width):
     """Scores of more and more pages in the workgroup's memory."""

@@ -255,7 +255,7 @@ __global__ __launch_bounds__(64 * SCORE_W, K <= 8 ? 4 : 2) void k_kv4_score(Kv4P
         if (!mine || page >= pages || (R == 4 && col >= R)) continue;
         const bool ok = (there >> (4 * g + e)) & 1;
         if (ok) most = fabsf(x) < INFINITY ? fmaxf(most, m) : INFINITY;
-        a.score[out * a.b.width + page] = ok ? x : -INFINITY;
+        a.score[out * a.b.width + page] = ok ? fmaxf(x, -0x1.fffffep127f) : -INFINITY;   // -infinity: no page
       }
     }
   }
