@@ -670,7 +670,8 @@ typedef struct bfp_kv4_shared {
  * ones from each sequence's own: the entries of a sequence's table before
  * position len[g] are not looked at.  A row sees of the shared tokens those up
  * to its own position and within its window, as of any.  At most 2^26 - 16
- * rows and query heads a sequence. */
+ * rows and query heads a sequence.  Precision is bfp_kv4_attn_d's: each part is
+ * held in float32 until they are joined. */
 int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,
                           const bfp_rows *out, double scale, int window, void *work, size_t work_bytes, void *stream);
 size_t bfp_kv4_attn_shared_work(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const bfp_kv4_shared *shared, const bfp_rows *q,

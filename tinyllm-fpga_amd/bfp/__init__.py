@@ -8,7 +8,8 @@ Import the package with ``tinyllm-fpga_amd`` on ``sys.path``::
 
 Modules: ``api`` (the reference simulator's functions on the GPU),
 ``model`` (HBM-resident model, layer step and decode driver), ``rotary`` and ``kv4``
-(rotary positions, the paged 4-bit key/value cache and its attention), ``synth``
+(rotary positions, the paged 4-bit key/value cache and its attention, of shared
+prefixes and picked pages too), ``pages`` (who holds a cache's pages), ``synth``
 (seeded synthetic inputs), ``dims`` (model dimensions), ``_lib`` (ctypes
 binding of libbfp.so).
 """

@@ -82,7 +82,9 @@ class PagePool(_rows.Fixed):
     def reserve(self, batch, work=None):
         """A page for every entry of batch.pages that the batch's new rows lie
         in and that holds none (is outside [0, n_pages)): before append.  An
-        entry for which none is left becomes -1, and its rows have no slot."""
+        entry for which none is left becomes -1, and its rows have no slot.
+        A page that another entry holds too is not replaced: fork a sequence
+        that is cut back into one before it goes on."""
         if batch.device != self.device:
             raise ValueError(f"the batch is on {batch.device}, the pool on {self.device}")
         keep, p, size = self._work(work)

