@@ -136,11 +136,11 @@ __device__ __forceinline__ int own_page(const Kv4PickArgs &a, const Kv4Span &s, 
   return q < a.b.width ? q : a.b.width - 1;
 }
 
-// Eight values of P or N from offset o on, for query heads `stride` apart.
+// Eight values of N and P from offset o on, for query heads `stride` apart.
 // One branch on the type, so that the heads' loads are under way together
 // (behind a branch each they took a microsecond apiece).
 template <int TYPE>
-__device__ __forceinline__ void group_sum_of(bfp_rows q, long long o, long long stride, int group, bool upper, float (&sum)[8]) {
+__device__ __forceinline__ void group_sums_of(bfp_rows q, long long o, long long stride, int group, float (&N)[8], float (&P)[8]) {
   q.type = TYPE;
 #pragma unroll 4
   for (int h = 0; h < group; ++h) {
@@ -148,17 +148,18 @@ __device__ __forceinline__ void group_sum_of(bfp_rows q, long long o, long long 
     row_load_n(q, o + h * stride, x);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float y = upper ? fmaxf(x[e], 0.0f) : fminf(x[e], 0.0f);
-      sum[e] += x[e] == x[e] ? y : NAN;
+      const bool is = x[e] == x[e];
+      N[e] += is ? fminf(x[e], 0.0f) : NAN;
+      P[e] += is ? fmaxf(x[e], 0.0f) : NAN;
     }
   }
 }
-__device__ __forceinline__ void group_sum(const bfp_rows &q, long long o, int group, bool upper, float (&sum)[8]) {
+__device__ __forceinline__ void group_sums(const bfp_rows &q, long long o, int group, float (&N)[8], float (&P)[8]) {
   switch (q.type) {
-    case BFP_F32: group_sum_of<BFP_F32>(q, o, q.head_stride, group, upper, sum); break;
-    case BFP_BF16: group_sum_of<BFP_BF16>(q, o, q.head_stride, group, upper, sum); break;
-    case BFP_F16: group_sum_of<BFP_F16>(q, o, q.head_stride, group, upper, sum); break;
-    default: group_sum_of<BFP_TILES>(q, o, q.head_stride, group, upper, sum); break;
+    case BFP_F32: group_sums_of<BFP_F32>(q, o, q.head_stride, group, N, P); break;
+    case BFP_BF16: group_sums_of<BFP_BF16>(q, o, q.head_stride, group, N, P); break;
+    case BFP_F16: group_sums_of<BFP_F16>(q, o, q.head_stride, group, N, P); break;
+    default: group_sums_of<BFP_TILES>(q, o, q.head_stride, group, N, P); break;
   }
 }
 
@@ -167,9 +168,9 @@ __device__ __forceinline__ void group_sum(const bfp_rows &q, long long o, int gr
 // The waves share P and N, each works out some of the steps, and each takes
 // every fourth 16 pages, whose operands are loaded as they lie, the next ones
 // while these are multiplied.  One row: bound by the bytes of the bounds (8 rows
-// over up to 2048 pages, 8 heads of 128: 42 MB in 19 us, 2.2 TB/s; much of it is the
+// over up to 2048 pages, 8 heads of 128: 42 MB in 16 us, 2.6 TB/s; much of it is the
 // first loads and the queries' sums).  Many: by four products a step where one
-// is the score's (1021 rows of up to 1024 pages, 4 heads: 36 us).
+// is the score's (1021 rows of up to 1024 pages, 4 heads: 32 us).
 template <int R, int K>
 __global__ __launch_bounds__(64 * SCORE_W, K <= 8 ? 4 : 2) void k_kv4_score(Kv4PickArgs a) {
   constexpr int T = R == 16 ? 3 : 1;
@@ -200,27 +201,29 @@ __global__ __launch_bounds__(64 * SCORE_W, K <= 8 ? 4 : 2) void k_kv4_score(Kv4P
   bf16x8 v[2][K];
   fetch(id, v[0]);
   fetch(next_id, v[1]);
-  // a column: dims 32 k + 8 g .. + 7 of [N | P]
-#pragma unroll
-  for (int k0 = 0; k0 < K; k0 += SCORE_W) {
-    const int k = k0 + w;
-    if (K % SCORE_W && k >= K) break;
-    const int at = 32 * k + 8 * g;
-    const bool upper = at >= hd;
-    const int d = upper ? at - hd : at;
-    float sum[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] = 0.0f;
-    if (mine)
-      group_sum(a.q, (long long)(s.row0 + i) * a.q.row_stride + (long long)head * a.group * a.q.head_stride + d, a.group, upper, sum);
+  // a column: dims 32 k + 8 g .. + 7 of [N | P]; eight dims' N and P by one lane
+  auto put = [&](int at, const float (&sum)[8]) {
 #pragma unroll
     for (int t = 0; t < T; ++t) {
       const int term = R == 16 ? t : col / R;
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = term < 3 ? query_term<3>(sum[e], term) : 0.0f;
-      coefs[(t * K + k) * 64 + lane] = pack8(y);
+      coefs[(t * K + at / 32) * 64 + 16 * (at / 8 % 4) + col] = pack8(y);
     }
+  };
+  constexpr bool HALF = K <= SCORE_W;   // as many waves for N alone, and for P
+#pragma unroll
+  for (int k0 = 0; 2 * k0 < K; k0 += SCORE_W) {
+    const int d = 32 * (k0 + (HALF ? w / 2 : w)) + 8 * g;
+    if (d >= hd) break;
+    float N[8], P[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) N[e] = P[e] = 0.0f;
+    if (mine)
+      group_sums(a.q, (long long)(s.row0 + i) * a.q.row_stride + (long long)head * a.group * a.q.head_stride + d, a.group, N, P);
+    if (!HALF || w % 2 == 0) put(d, N);
+    if (!HALF || w % 2 == 1) put(hd + d, P);
   }
   __syncthreads();
   // (read again for every tile: in registers those of 16 rows leave room for two waves a SIMD)
@@ -666,9 +669,10 @@ static PickPlan plan_pick(const bfp_kv4 &c, const bfp_kv4_batch &b) {
   if (most >= 16) most = most / 16 * 16;
   p.rows = most < 1 ? 1 : most < (size_t)rows ? (int)most : rows;
   p.R = p.rows > 4 ? 16 : 4;
-  // a thousand workgroups, each with 64 pages or more
+  // 512 workgroups, each with 64 pages or more (1021 rows of 1024 pages, 4 heads: 34 us
+  // with a thousand, 32 so, 36 with 256; 7 rows of 2048, 8 heads: 17.1, 16.1, 19.5)
   const long long tiles = (long long)((p.rows + p.R - 1) / p.R) * c.heads * b.n_seq;
-  long long chunks = 1024 / tiles;
+  long long chunks = 512 / tiles;
   if (chunks > (b.width + 63) / 64) chunks = (b.width + 63) / 64;
   if (chunks > PICK_CHUNKS) chunks = PICK_CHUNKS;
   if (chunks < 1) chunks = 1;
