@@ -101,6 +101,9 @@ CASES = [  # share, of, lens, news, page, heads, hd, query heads, type, result, 
     ([4000], [0] * 40, [4000 + 3 * i + 1 for i in range(40)], [1] * 40, 32, 1, 64, 8, "bf16", None, 0),      # prompts' kernel, split
     ([1000, 700], [0] * 6 + [1] * 5, [1100] * 6 + [790] * 5, [13] * 6 + [14] * 5, 64, 2, 96, 8, "f16", None, 0),  # rows of one and a quarter workgroups
     ([1000], [0] * 7, [1100] * 7, [11] * 7, 16, 1, 32, 4, "bf16", None, 400),
+    ([6000, 900], [0] * 9 + [1] * 3, [6100] * 9 + [1000] * 3, [3] * 12, 64, 1, 128, 4, "bf16", None, 0),
+    ([6000], [0] * 9, [6100] * 9, [3] * 9, 16, 2, 112, 6, "f16", None, 0),
+    ([700], [0] * 9, [800] * 9, [10] * 9, 32, 1, 128, 3, "f16", None, 200),
     ([500] * 66, list(range(66)), [540 + g for g in range(66)], [20] * 66, 32, 1, 64, 16, "bf16", None, 0),
     ([900, 700], [0] * 6 + [1] * 5, [950] * 6 + [790] * 5, [50] * 6 + [90] * 5, 64, 2, 64, 4, "f32", None, 0),
     ([900], [0] * 7, [960] * 7, [40] * 7, 16, 1, 192, 4, "f16", None, 0),

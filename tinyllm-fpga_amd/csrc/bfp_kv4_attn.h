@@ -404,7 +404,7 @@ PartsKernel parts_kernel(int tiles, int prefix_terms, int rest_terms, int waves)
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }
 // Two workgroups of four waves a CU instead of one of eight: registers and LDS hold them.
-inline bool prompt_pairs(int tiles, int terms) { return tiles <= 6 && terms < 3; }
+inline bool prompt_pairs(int tiles, int terms) { return tiles <= 8 && terms < 3; }
 // Queues the kernel that joins what k_kv4_prompt left in pieces.
 void launch_join_prompt(const Kv4AttnArgs &a, hipStream_t s);
 // The same of a row's two parts.

@@ -98,6 +98,10 @@ static Kv4Plan plan_keys(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
         few.stream = (int)(most < slots ? most : slots);
         few.cells = 2 * (size_t)few.stream * R;
         few.us = each + R * c.hd / 128.0 + per_tile * groups * (seen + ROWS_EXTRA) / cus;   // joined by one workgroup
+        // A shared prefix takes 15 us more so (8 to 32 rows of 32 + 8 heads): heads of 128, 16384
+        // keys 42, 41, 52, 58 against the prompts' 27, 29, 30, 31; 65536 keys 65, 85, 106,
+        // 128 against 67, 68, 70, 71; heads of 64, 16384 keys 33 to 39 against 21 to 23.
+        if (whole) few.us += 15.0;
       }
     }
   }
@@ -162,8 +166,9 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   // chats behind 304 tokens, 9 heads of 64: 23 us in two launches, 15 in one).
   p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves;
   // Prompts' kernel: 128 rows a workgroup where that leaves fewer rows empty
-  // than 256 (groups of 320 rows, heads of 96, two terms: 217 us against 260; where
-  // both fill them alike 550 against 520).
+  // than 256 (groups of 320 rows, heads of 96, two terms: 217 us against 260; of 128
+  // rows, heads of 128, 65536 keys: 72 against 86; where both fill them alike 550
+  // against 520).
   const long long group_rows = (long long)p.groups.max_q * (q.heads / c.heads), in_8 = (group_rows + 255) / 256 * 256, in_4 = (group_rows + 127) / 128 * 128;
   p.pairs = p.prefix.prompt && prompt_pairs(c.hd / 16, p.prefix.terms) && in_4 + in_4 / 8 < in_8;
   if (p.pairs) {

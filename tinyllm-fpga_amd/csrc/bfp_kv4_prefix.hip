@@ -12,7 +12,8 @@ AttnKernel prefix_prompt_kernel(int tiles, int terms, bool pairs) {
   if (pairs)
     return tiles <= 2   ? prompt_kernel_of<2, 4, SEES_PREFIX>(terms)
            : tiles <= 4 ? prompt_kernel_of<4, 4, SEES_PREFIX>(terms)
-                        : prompt_kernel_of<6, 4, SEES_PREFIX>(terms);
+           : tiles <= 6 ? prompt_kernel_of<6, 4, SEES_PREFIX>(terms)
+                        : prompt_kernel_of<8, 4, SEES_PREFIX>(terms);
   return prompt_kernel_for<SEES_PREFIX>(tiles, terms);
 }
 

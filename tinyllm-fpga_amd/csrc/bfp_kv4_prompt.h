@@ -29,12 +29,14 @@ constexpr int pv_pitch(int tb) { return 64 * ((tb / 2) | 1); }
 // A tile of K, and of V with its exponent bytes (key, 16 tiles).
 constexpr int k_bytes(int tb) { return KEYS * pk_pitch(tb); }
 constexpr int v_bytes(int tb) { return KEYS * (pv_pitch(tb) + 16); }
-// Tiles of V held: with three, one barrier a tile is enough; the widest heads
-// leave room for two, and take a second barrier.
-constexpr int v_buffers(int tb) { return tb <= 12 ? 3 : 2; }
+// Two workgroups a CU: four waves of heads and terms for which there are eight too.
+constexpr bool in_pairs(int tb, int t, int w) { return w == 4 && t < 3 && tb <= 8; }
+// Tiles of V held: with three, one barrier a tile is enough; the widest heads,
+// and pairs of wide ones, leave room for two, and take a second barrier.
+constexpr int v_buffers(int tb, bool pair) { return tb <= (pair ? 6 : 12) ? 3 : 2; }
 constexpr int OUT_PITCH = 36;   // floats: 32 values of a row, on their way out
-constexpr int prompt_lds(int tb, int waves) {
-  const int in = 2 * k_bytes(tb) + v_buffers(tb) * v_bytes(tb), out = waves * (32 * OUT_PITCH + 64) * 4;
+constexpr int prompt_lds(int tb, int t, int waves) {
+  const int in = 2 * k_bytes(tb) + v_buffers(tb, in_pairs(tb, t, waves)) * v_bytes(tb), out = waves * (32 * OUT_PITCH + 64) * 4;
   return in > out ? in : out;
 }
 
@@ -66,9 +68,9 @@ __device__ __forceinline__ void prompt_query(const Kv4AttnArgs &a, long long at,
 // missing tiles are zeros in K, and columns of V whose results nobody
 // takes); T: terms; W: waves.
 template <int TB, int T, int W, Kv4Sees SEES>
-__global__ __launch_bounds__(64 * W, W == 8 || (T < 3 && TB <= 6) ? 2 : 1) void k_kv4_prompt(Kv4AttnArgs a) {
+__global__ __launch_bounds__(64 * W, W == 8 || in_pairs(TB, T, W) ? 2 : 1) void k_kv4_prompt(Kv4AttnArgs a) {
   constexpr int ROWS = 32 * W, DT = TB / 2, UNITS = (TB + W - 1) / W;
-  constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), NV = v_buffers(TB);
+  constexpr int KP = pk_pitch(TB), VP = pv_pitch(TB), NV = v_buffers(TB, in_pairs(TB, T, W));
   extern __shared__ __align__(16) char lds[];
   __shared__ int nan_tiles[4];
   int seq, head, rt, split, splits = a.splits, chunk = a.chunk;
@@ -439,7 +441,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || (T < 3 && TB <= 6) ? 2 : 1) void 
 template <int TB, int W, Kv4Sees SEES>
 static AttnKernel prompt_kernel_of(int terms) {
   return {terms == 1 ? k_kv4_prompt<TB, 1, W, SEES> : terms == 2 ? k_kv4_prompt<TB, 2, W, SEES> : k_kv4_prompt<TB, 3, 4, SEES>,
-          prompt_lds(TB, terms == 3 ? 4 : W)};
+          terms == 1 ? prompt_lds(TB, 1, W) : terms == 2 ? prompt_lds(TB, 2, W) : prompt_lds(TB, 3, 4)};
 }
 
 template <Kv4Sees SEES>
