@@ -104,6 +104,13 @@ CASES = [  # share, of, lens, news, page, heads, hd, query heads, type, result, 
     ([6000, 900], [0] * 9 + [1] * 3, [6100] * 9 + [1000] * 3, [3] * 12, 64, 1, 128, 4, "bf16", None, 0),
     ([6000], [0] * 9, [6100] * 9, [3] * 9, 16, 2, 112, 6, "f16", None, 0),
     ([700], [0] * 9, [800] * 9, [10] * 9, 32, 1, 128, 3, "f16", None, 200),
+    ([21000], [0] * 3, [21010, 21050, 21001], [1] * 3, 64, 8, 48, 8, "f16", None, 0),                        # few rows that share out their keys
+    ([27000], [0] * 2, [27001, 27300], [1, 2], 128, 1, 128, 2, "bf16", None, 0),
+    ([34000], [0] * 2, [34001, 34002], [1, 1], 256, 1, 256, 2, "f16", None, 0),
+    ([500], [0, 0], [6600, 6200], [300, 260], 64, 1, 64, 2, "bf16", None, 0),                                # prompts behind it, split
+    ([3000], [0] * 8, [3100] * 8, [40] * 8, 64, 1, 256, 4, "bf16", None, 700),
+    ([3100], [0] * 8, [3200] * 8, [40] * 8, 64, 1, 192, 4, "f16", None, 0),
+    ([2000], [0] * 8, [2100] * 8, [40] * 8, 32, 1, 240, 4, "f32", None, 0),
     ([500] * 66, list(range(66)), [540 + g for g in range(66)], [20] * 66, 32, 1, 64, 16, "bf16", None, 0),
     ([900, 700], [0] * 6 + [1] * 5, [950] * 6 + [790] * 5, [50] * 6 + [90] * 5, 64, 2, 64, 4, "f32", None, 0),
     ([900], [0] * 7, [960] * 7, [40] * 7, 16, 1, 192, 4, "f16", None, 0),
