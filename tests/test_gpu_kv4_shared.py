@@ -107,7 +107,7 @@ CASES = [  # share, of, lens, news, page, heads, hd, query heads, type, result, 
     ([21000], [0] * 3, [21010, 21050, 21001], [1] * 3, 64, 8, 48, 8, "f16", None, 0),                        # few rows that share out their keys
     ([27000], [0] * 2, [27001, 27300], [1, 2], 128, 1, 128, 2, "bf16", None, 0),
     ([34000], [0] * 2, [34001, 34002], [1, 1], 256, 1, 256, 2, "f16", None, 0),
-    ([500], [0, 0], [6600, 6200], [300, 260], 64, 1, 64, 2, "bf16", None, 0),                                # prompts behind it, split
+    ([500], [0, 0], [6600, 6200], [600, 560], 64, 1, 64, 2, "bf16", None, 0),                                # prompts behind it, split
     ([3000], [0] * 8, [3100] * 8, [40] * 8, 64, 1, 256, 4, "bf16", None, 700),
     ([3100], [0] * 8, [3200] * 8, [40] * 8, 64, 1, 192, 4, "f16", None, 0),
     ([2000], [0] * 8, [2100] * 8, [40] * 8, 32, 1, 240, 4, "f32", None, 0),
