@@ -400,7 +400,7 @@ struct PartsKernel {
   attn_parts_fn fn;
   int lds;
 };
-PartsKernel parts_kernel(int tiles, int prefix_terms, int rest_terms, int waves);
+PartsKernel parts_kernel(int tiles, int terms, int waves);
 inline int rows_waves(int tiles) { return tiles <= 4 ? 16 : tiles <= 8 ? 8 : 4; }
 inline int prompt_waves(int tiles, int terms) { return tiles <= 8 && terms < 3 ? 8 : 4; }
 // Two workgroups of four waves a CU instead of one of eight: registers and LDS hold them.

@@ -164,7 +164,9 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
     if (!k->prompt && !k->stream && few > 256) k->waves = 4;
   // Both such, a prefix of few keys or rows and few keys behind it: one launch (5
   // chats behind 304 tokens, 9 heads of 64: 23 us in two launches, 15 in one).
-  p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves;
+  // One kernel then, so as many terms in both: a row tile's rows follow from them.
+  p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves &&
+             p.prefix.terms == p.rest.terms;
   // Prompts' kernel: 128 rows a workgroup where that leaves fewer rows empty
   // than 256 (groups of 320 rows, heads of 96, two terms: 217 us against 260; of 128
   // rows, heads of 128, 65536 keys: 72 against 86; where both fill them alike 550
@@ -420,7 +422,7 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
     BFP_TRY(plan_args(op, a, two, n2));
     if (n1 + n2 > 0x3ffffff / one.waves)
       return set_err(BFP_EINVAL, "%s: n_groups=%d and n_seq=%d are too many for one call", op, shared->n_groups, batch->n_seq);
-    const PartsKernel k = parts_kernel(a.tiles, one.terms, two.terms, one.waves);
+    const PartsKernel k = parts_kernel(a.tiles, one.terms, one.waves);
     BFP_TRY(lds_limit(k.fn, k.lds));
     hipLaunchKernelGGL(k.fn, dim3((unsigned)(n1 + n2)), dim3(64 * one.waves), k.lds, s, g, a, (uint32_t)n1);
     BFP_TRY(launch_status(op));

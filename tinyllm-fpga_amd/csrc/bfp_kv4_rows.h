@@ -763,13 +763,13 @@ __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES, SHARE)) void k_kv
 }
 
 // Both parts of rows that share a prefix.
-template <int C, int T1, int T2, int W>
+template <int C, int T, int W>
 __global__ __launch_bounds__(64 * W, rows_per_simd(C, W, SEES_REST, false)) void k_kv4_parts(Kv4AttnArgs prefix, Kv4AttnArgs rest,
                                                                                              uint32_t prefix_blocks) {
   if (blockIdx.x < prefix_blocks)
-    rows_block<C, T1, W, SEES_PREFIX, false>(prefix, blockIdx.x);
+    rows_block<C, T, W, SEES_PREFIX, false>(prefix, blockIdx.x);
   else
-    rows_block<C, T2, W, SEES_REST, false>(rest, blockIdx.x - prefix_blocks);
+    rows_block<C, T, W, SEES_REST, false>(rest, blockIdx.x - prefix_blocks);
 }
 
 // 64 E values of a part at a time, row after row; a lane has E of them under
@@ -889,13 +889,9 @@ static AttnKernel rows_kernel_for(int tiles, int terms, int waves, bool share) {
 }
 
 template <int C, int W>
-static PartsKernel parts_kernel_of(int tiles, int t1, int t2) {
-  const int one = rows_lds(C, W, 16 / t1, tiles, false), two = rows_lds(C, W, 16 / t2, tiles, false);
-  return {t1 == 4   ? k_kv4_parts<C, 4, 4, W>
-          : t1 == 2 ? k_kv4_parts<C, 2, 2, W>
-          : t2 == 2 ? k_kv4_parts<C, 1, 2, W>
-                    : k_kv4_parts<C, 1, 1, W>,
-          one > two ? one : two};
+static PartsKernel parts_kernel_of(int tiles, int terms) {
+  return {terms == 4 ? k_kv4_parts<C, 4, W> : terms == 2 ? k_kv4_parts<C, 2, W> : k_kv4_parts<C, 1, W>,
+          rows_lds(C, W, 16 / terms, tiles, false)};
 }
 
 }  // namespace bfp
