@@ -32,3 +32,24 @@ def test_more_rows_outside_the_groups(gpu, most, mine, hd, hq, heads, hints):
     got = _attend(t, q).double().cpu().numpy()
     want, weight, big = t.want(qv, group, 1 / np.sqrt(hd), 0)
     assert (np.abs(got - want) <= _bound(want, weight, big, max(t.lens), hd, "bf16", "bf16", 9)).all()
+
+
+@pytest.mark.parametrize("seqs,new,share,hd,hq,heads", [(5, 1, 304, 64, 9, 3), (9, 2, 400, 128, 4, 1), (40, 1, 500, 64, 8, 1), (24, 1, 500, 128, 16, 4),
+                                                        (70, 8, 100, 32, 1, 1), (6, 4, 300, 192, 2, 1), (40, 1, 4000, 64, 8, 1)])
+def test_bits_are_those_of_calls_without_groups(gpu, seqs, new, share, hd, hq, heads):
+    """bfloat16 with up to 8 rows a KV head of a sequence: probabilities in two
+    terms (2^-16 off), however many rows the group has.  Results that lie
+    further from a rounding border than that and float32 may move them are the
+    exact ones rounded; probabilities in bfloat16 move them to either side."""
+    import torch
+    t = Groups(21, [share], [0] * seqs, [share + new + b % 5 for b in range(seqs)], [new] * seqs, 16, heads, hd)
+    q, qv = _typed(t.s.rng.standard_normal((t.rows, hq, hd)) * 0.01, "bf16")
+    _say(seqs, new, share, hd, hq, heads)
+    got = _attend(t, q).double().cpu().numpy()
+    want, weight, big = t.want(qv, hq // heads, 1 / np.sqrt(hd), 0)
+    off = ref.attend_bound(want, weight, big, max(t.lens), hd, 0, 2 * 2.0 ** -16)
+    assert (np.abs(got - want) <= off + HALF["bf16"] * np.abs(want)).all()
+    low, mid, high = (torch.from_numpy(x).bfloat16().double().numpy() for x in (want - off, want, want + off))
+    sure = low == high
+    assert share > 500 or sure.mean() > 0.02
+    assert (got[sure] == mid[sure]).all()

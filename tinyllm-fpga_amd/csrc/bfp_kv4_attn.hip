@@ -48,9 +48,10 @@ static long long keys_of(const bfp_kv4 &c, const bfp_kv4_batch &b, int window, l
 }
 
 // keys: of the longest sequence; whole: all rows see all of them, else up to
-// their own; most: splits.
+// their own; most: splits; row_terms: of every row, whatever the kernel (0:
+// each kernel's own).
 static Kv4Plan plan_keys(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_rows &q, const bfp_rows &out, long long keys, bool whole,
-                         int most) {
+                         int most, int row_terms = 0) {
   Kv4Plan p{};
   const int group = q.heads / c.heads, tiles = c.hd / 16;
   const long long rows = (long long)b.max_q * group;
@@ -78,7 +79,7 @@ static Kv4Plan plan_keys(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   {
     static const double itself[4] = {7.0, 7.5, 11.0, 13.0};
     few.prompt = false;
-    few.terms = terms_of(q, out, (int)(rows < 64 ? rows : 64));
+    few.terms = row_terms ? row_terms : terms_of(q, out, (int)(rows < 64 ? rows : 64));
     const int R = 16 / few.terms;
     few.row_tiles = (int)((rows + R - 1) / R);
     few.waves = rows_waves(tiles);
@@ -108,7 +109,7 @@ static Kv4Plan plan_keys(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
   {
     static const double itself[4] = {8.8, 12.0, 16.0, 20.0}, tile[4] = {1.4, 1.8, 2.1, 2.1};
     p.prompt = true;
-    p.terms = wide ? 3 : (q.type == BFP_BF16 && out.type == BFP_BF16 ? 1 : 2);
+    p.terms = wide ? 3 : row_terms ? row_terms : (q.type == BFP_BF16 && out.type == BFP_BF16 ? 1 : 2);
     p.waves = prompt_waves(tiles, p.terms);
     p.row_tiles = (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
     const long long groups = (long long)p.row_tiles * c.heads * b.n_seq;
@@ -152,11 +153,17 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
   p.groups.width = sh.width;
   p.groups.max_len = sh.max_len;
   p.groups.max_q = sh.max_rows > 0 && sh.max_rows < b.n_rows ? sh.max_rows : b.n_rows;
+  // Both parts in the terms that a sequence's rows have by themselves, however
+  // many the group has.  (64 samples of one problem, 4 rows a KV head, 256 a group,
+  // 16384 tokens: the prefix takes 49 us in two terms and 38 in one, which leaves
+  // bfloat16 results 1.3 times as far from the exact ones as without groups.)
+  const long long seq_rows = (long long)(b.max_q < b.n_rows ? b.max_q : b.n_rows) * (q.heads / c.heads);
+  const int terms = terms_of(q, out, (int)(seq_rows < 64 ? seq_rows : 64));
   const long long prefix = keys_of(c, p.groups, window, 0);
-  p.prefix = plan_keys(c, p.groups, q, out, prefix, true, 48);
+  p.prefix = plan_keys(c, p.groups, q, out, prefix, true, 48, terms);
   // Without a hint the rest may be anything: the keys of a stream are shared out on the device.
   const long long cap = (long long)sh.width * c.page;
-  p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len < cap ? sh.max_len : cap), false, 16);
+  p.rest = plan_keys(c, b, q, out, keys_of(c, b, window, sh.max_len < cap ? sh.max_len : cap), false, 16, terms);
   long long few = 0;   // workgroups of few rows that take all keys of a row tile: more than the card has CUs, then four waves each
   for (const Kv4Plan *k : {&p.prefix, &p.rest})
     if (!k->prompt && !k->stream) few += (long long)k->row_tiles * c.heads * (k == &p.rest ? b.n_seq : sh.n_groups);
@@ -164,9 +171,8 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
     if (!k->prompt && !k->stream && few > 256) k->waves = 4;
   // Both such, a prefix of few keys or rows and few keys behind it: one launch (5
   // chats behind 304 tokens, 9 heads of 64: 23 us in two launches, 15 in one).
-  // One kernel then, so as many terms in both: a row tile's rows follow from them.
-  p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves &&
-             p.prefix.terms == p.rest.terms;
+  // (One kernel then: a row tile's rows follow from the terms, which are the same.)
+  p.joined = !p.prefix.prompt && !p.prefix.stream && !p.rest.prompt && !p.rest.stream && p.prefix.waves == p.rest.waves;
   // Prompts' kernel: 128 rows a workgroup where that leaves fewer rows empty
   // than 256 (groups of 320 rows, heads of 96, two terms: 217 us against 260; of 128
   // rows, heads of 128, 65536 keys: 72 against 86; where both fill them alike 550
