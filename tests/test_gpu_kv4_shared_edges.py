@@ -53,3 +53,40 @@ def test_bits_are_those_of_calls_without_groups(gpu, seqs, new, share, hd, hq, h
     sure = low == high
     assert share > 500 or sure.mean() > 0.02
     assert (got[sure] == mid[sure]).all()
+
+
+def test_float32_is_as_exact_as_without_groups(gpu):
+    """Probabilities one by one: key j and value j are 1 in channel j and 0
+    elsewhere, so result j is 2^(q_j / 4) over the sum.  Scores are exact here, up
+    to 8 powers of two below the largest, and exponents at most 16 below 0
+    where the maximum goes 2^8 above it: each is rounded to 2^-21 and the
+    exponential to 2^-23 (uniformly: over the root of 3), the result twice to 2^-24:
+    2.1e-7 in all; a third more is allowed."""
+    import torch
+    rows, heads = 24, 3
+    t = Groups(4, [16], [0] * rows, [17] * rows, [1] * rows, 16, 1, 32)
+    c, s = t.s.cache, t.s
+    one_hot = np.zeros((2, 16, 8), np.uint8)                 # tile, slot, byte
+    one_hot[0, np.arange(16), np.arange(16) // 2] = 2 << (4 * (np.arange(16) % 2))
+    own = np.zeros((2, 16, 8), np.uint8)
+    own[1, 0, 0] = 2                                         # a row's own token: key 0, value 1 in channel 16
+    for x, mine in ((c.k, 0 * own), (c.v, own)):
+        x[int(s.table[0, 0]), 0] = torch.from_numpy(one_hot).cuda()
+        for b in range(rows):
+            x[int(t.table[b, 1]), 0] = torch.from_numpy(mine).cuda()
+    c.k_exp.fill_(127), c.v_exp.fill_(127)
+    q = np.zeros((rows, heads, 32))
+    q[:, :, :16] = s.rng.random((rows, heads, 16)) * 31
+    q, qv = _typed(q, "f32")
+    p = np.concatenate([2.0 ** (qv[:, :, :16] / 4), np.ones((rows, heads, 1))], -1)
+    want = p / p.sum(-1, keepdims=True)
+    plain = t.batch.pages.clone()
+    plain[:, 0] = int(s.table[0, 0])
+    for shared in (t.shared, None):
+        if shared is None:
+            t.batch.pages.copy_(plain)
+        got = c.attend(t.batch, q, scale=0.25 / 1.44269504088896340736, shared=shared).double().cpu().numpy()
+        assert (got[:, :, 17:] == 0).all()
+        off = got[:, :, :17] / want - 1
+        _say("float32", shared is not None, np.sqrt((off ** 2).mean()), np.abs(off).max())
+        assert np.sqrt((off ** 2).mean()) < 2.8e-7

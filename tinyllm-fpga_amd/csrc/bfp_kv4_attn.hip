@@ -407,7 +407,10 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
   const SharedPlan p = plan_shared(*cache, *batch, *shared, *q, *out, window);
   BFP_TRY(check_work(op, p.work, work, work_bytes));
   hipStream_t s = (hipStream_t)stream;
-  a.slack = fminf(2 * M_SLACK / a.scale2, 0x1p125f);   // few tiles a workgroup, whose first one sets the maximum: it is raised less often
+  // Few tiles a workgroup, whose first one sets the maximum: it is raised less
+  // often.  Not for rows in float32: exponents down to -32 are rounded to 2^-20, those
+  // to -16 to 2^-21, which is what probabilities are off there (2^-16 in two terms).
+  if (p.prefix.terms < 3) a.slack = fminf(2 * M_SLACK / a.scale2, 0x1p125f);
   a.sh = *shared;
   a.sh_seqs = batch->n_seq;
   a.sum_slots = p.slots;
