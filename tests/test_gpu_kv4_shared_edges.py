@@ -6,7 +6,7 @@ import pytest
 
 import kv4_ref as ref
 from test_gpu_kv4 import HALF, _dt, _int, _say, _typed
-from test_gpu_kv4_shared import Groups, _bound
+from test_gpu_kv4_shared import CASES, Groups, _bound
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,61 @@ def test_float32_is_as_exact_as_without_groups(gpu):
         off = got[:, :, :17] / want - 1
         _say("float32", shared is not None, np.sqrt((off ** 2).mean()), np.abs(off).max())
         assert np.sqrt((off ** 2).mean()) < 2.8e-7
+
+
+@pytest.mark.parametrize("hints", [True, False])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{c[0]}-{len(c[1])}-{c[4:]}")
+def test_every_part_that_is_joined_was_written(gpu, case, hints):
+    """Rows behind the last sequence, of more bytes than the scratch of the
+    others, are left alone and change no result."""
+    import torch
+    share, of, lens, news, page, heads, hd, hq, kind, out, window = case
+    t = Groups(43, share, of, lens, news, page, heads, hd, hints=hints, max_rows=None if hints else 0)
+    _say(case[0], case[4:], hints)
+    more = 70
+    q, qv = _typed(t.s.rng.standard_normal((t.rows + more, hq, hd)) * 1.5, kind)
+    res = out or ("f32" if kind == "tile" else kind)
+    to = torch.full((t.rows + more, hq, hd), 7.0, dtype=_dt(res), device="cuda")
+    size = t.s.cache.attend_work(t.batch, q, out=to, shared=t.shared, window=window)
+    work = torch.full(((size + 3) // 4,), float("nan"), device="cuda")
+    t.s.cache.attend(t.batch, q, out=to, shared=t.shared, window=window, work=work)
+    got = to.double().cpu().numpy()
+    want, weight, big = t.want(qv[:t.rows], hq // heads, 1 / np.sqrt(hd), window)
+    bound = _bound(want, weight, big, max(lens), hd, kind, res, t.rows * (hq // heads))
+    assert (np.abs(got[:t.rows] - want) <= bound).all() and (got[t.rows:] == 7).all()
+
+
+def test_parts_of_two_kinds_of_groups(gpu):
+    """Captured once; group ranges and lengths move from many row tiles, whose
+    keys stay whole, to few, whose keys are split, and back."""
+    import torch
+    t = Groups(44, [2000, 1500], [0] * 6 + [1] * 6, [2000 + 70 + b for b in range(6)] + [1600 + b for b in range(6)], [60] * 12, 16, 8, 64, max_rows=0)
+    q, qv = _typed(t.s.rng.standard_normal((t.rows, 32, 64)), "bf16")
+    out = torch.empty_like(q)
+    size = t.s.cache.attend_work(t.batch, q, shared=t.shared)
+    work = torch.full(((size + 3) // 4,), float("nan"), device="cuda")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            t.s.cache.attend(t.batch, q, shared=t.shared, out=out, work=work)
+    torch.cuda.synchronize()
+    table = t.table.copy()
+    for b in range(12):       # own pages that hold the shared tokens, for the sequences that are taken out of their group
+        whole = [2000, 1500][t.of[b]] // 16
+        table[b, :whole] = t.s.table[t.of[b], :whole]
+        if [2000, 1500][t.of[b]] % 16:
+            end, own = int(t.s.table[t.of[b], whole]), int(t.table[b, whole])
+            for x in (t.s.cache.k, t.s.cache.k_exp, t.s.cache.v, t.s.cache.v_exp):
+                x[own, :, :, :[2000, 1500][t.of[b]] % 16] = x[end, :, :, :[2000, 1500][t.of[b]] % 16]
+    t.batch.pages.copy_(_int(table))
+    want, weight, big = t.want(qv, 4, 1 / 8, 0)
+    bound = _bound(want, weight, big, max(t.lens), 64, "bf16", "bf16", 720 * 4)
+    for start in ([0, 6, 12], [5, 6, 7], [6, 6, 12], [0, 6, 6], [0, 6, 12]):
+        t.shared.start.copy_(_int(start))
+        out.fill_(float("nan"))
+        work.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (np.abs(out.double().cpu().numpy() - want) <= bound).all(), start

@@ -69,13 +69,15 @@ struct Kv4AttnArgs {
   int n_picks, token_tiles;
   // Shared prefixes.  SEES_PREFIX: b's sequences are the groups (pages, width,
   // n_seq, max_q), its start and len still the batch's.  Both launches leave
-  // unfinished rows in part_o [row][query head][slot][hd], sum_slots of them a
-  // row, from sum_slot on, and part_ml; k_kv4_rows its own parts in slot_o, slot_ml.
+  // unfinished rows in part_o [place][hd] and part_ml, the prefix's places first
+  // (prefix_place), then the rest's (rest_place); k_kv4_rows its own parts in slot_o,
+  // slot_ml.
   bfp_kv4_shared sh;
   int sh_seqs;   // sequences of the batch
-  int sum_slots, sum_slot;
-  int pieces, prefix_slots;   // k_kv4_prompt: workgroups that share the keys of up to 64 groups (0: splits of one length), and a row's slots
-  int32_t *split_of;   // with them: the splits of each group
+  int prefix_splits, rest_splits;   // at most, a row
+  long long rest_first;             // the rest's first place
+  int pieces, piece_shift, piece_blocks;   // k_kv4_prompt: workgroups that share the keys of up to 64 groups (0: splits of one length), log2 of each one's rows, and the launch's
+  int4 *piece_of;   // with them, of each group: splits, first workgroup, row tiles, first row
   float *slot_o;
   float2 *slot_ml;
 };
@@ -155,6 +157,18 @@ __device__ __forceinline__ int kv4_row_position(const Kv4AttnArgs &a, const Kv4G
   return p < 0 ? -1 : (int)(p < KV4_MAX_POS ? p : KV4_MAX_POS);
 }
 
+// Where a row's unfinished sums lie.  The prefix's, where pieces of the groups'
+// keys are shared out: by workgroup and row in it, since how many splits there are
+// depends on how many rows; else by row, head and split.
+__device__ __forceinline__ long long prefix_place(const Kv4AttnArgs &a, long long tok, int qh, int split) {
+  return (tok * a.q.heads + qh) * a.prefix_splits + split;
+}
+// The rest's: of row i of a sequence (k_kv4_prompt splits only what few row tiles see,
+// and rows that belong to no sequence should not take splits' room).
+__device__ __forceinline__ long long rest_place(const Kv4AttnArgs &a, int seq, int i, long long tok, int qh, int split) {
+  return a.rest_first + (a.rest_splits > 1 ? (((long long)seq * a.b.max_q + i) * a.q.heads + qh) * a.rest_splits + split : tok * a.q.heads + qh);
+}
+
 // Over N neighbouring lanes (16 or 32).
 template <int N>
 __device__ __forceinline__ int min_lanes(int v) {
@@ -168,16 +182,17 @@ template <int N>
 __device__ __forceinline__ int max_lanes(int v) { return -min_lanes<N>(-v); }
 
 // Workgroup blockIdx.x's part of the groups' prefixes, at most 64 of them,
-// where the longest takes its keys in prefix_slots splits at most: all workgroups
+// where the longest takes its keys in prefix_splits splits at most: all workgroups
 // take equally many tiles, whatever the groups' lengths, as long as a round of
 // them (a.pieces) has room for every row tile.  False: there is nothing for it.
 __device__ __forceinline__ bool Kv4AttnArgs::piece(int rows, int &g, int &head, int &split, int &rt, int &splits, int &chunk) const {
   const int lane = threadIdx.x & 63;
-  int units = 0, tiles = 0;   // row tiles x KV heads, and key tiles
+  int units = 0, tiles = 0, row0 = 0;   // row tiles x KV heads, key tiles, and the first row
   if (lane < b.n_seq) {
     Kv4Group x;
     const Kv4Span s = kv4_group_span(*this, lane, x);
     const int low = kv4_group_low(*this, x) / KEYS;
+    row0 = s.row0;
     units = (int)(((long long)s.n * group + rows - 1) / rows) * c.heads;
     tiles = s.at > low * KEYS ? (s.at + KEYS - 1) / KEYS - low : 1;
   }
@@ -186,7 +201,7 @@ __device__ __forceinline__ bool Kv4AttnArgs::piece(int rows, int &g, int &head, 
 #pragma unroll
   for (int d = 32; d > 0; d /= 2) most = max(most, __shfl_xor(most, d, 64));
   const int places = sum(min(units, 1 << 20));
-  int least = max((most + prefix_slots - 1) / prefix_slots, 4);
+  int least = max((most + prefix_splits - 1) / prefix_splits, 4);
   chunk = max(most, 1);
   if (places <= pieces && least < chunk) {   // the shortest pieces of which there are no more than `pieces`
     int too_short = least - 1;
@@ -196,13 +211,13 @@ __device__ __forceinline__ bool Kv4AttnArgs::piece(int rows, int &g, int &head, 
     }
   }
   const int mine = (tiles + chunk - 1) / chunk;
-  if (blockIdx.x == 0 && threadIdx.x < b.n_seq) split_of[lane] = mine;
   int up = units * mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     const int x = __shfl_up(up, d, 64);
     up += lane >= d ? x : 0;
   }
+  if (blockIdx.x == 0 && threadIdx.x < b.n_seq) piece_of[lane] = make_int4(mine, up - units * mine, units / c.heads, row0);
   const unsigned long long past = __ballot(up > (int)blockIdx.x);
   if (!past) return false;
   g = __ffsll((long long)past) - 1;

@@ -11,6 +11,7 @@
 // prompts multiply term by term.
 #include "bfp_kv4_attn.h"
 
+#include <algorithm>
 #include <atomic>
 #include <chrono>
 
@@ -138,11 +139,11 @@ static Kv4Plan plan_attn(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_row
 struct SharedPlan {
   Kv4Plan prefix, rest;
   bfp_kv4_batch groups;
-  int slots, pieces;
+  int pieces;               // k_kv4_prompt of up to 64 groups: workgroups that share the keys
+  long long blocks;         // and the launch's (0: its plan's)
   bool joined;              // both parts in one launch
   bool pairs;               // the prompts' kernel with two workgroups a CU
-  long long blocks;         // of the first launch, where its pieces are shared out (0: its plan's)
-  size_t sums, own, work;   // parts of rows; bytes of the launches' own parts
+  size_t prefix_sums, sums, own, work;   // parts of rows, of the prefix and in all; bytes of the launches' own parts
 };
 static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bfp_kv4_shared &sh, const bfp_rows &q, const bfp_rows &out,
                               int window) {
@@ -184,24 +185,31 @@ static SharedPlan plan_shared(const bfp_kv4 &c, const bfp_kv4_batch &b, const bf
     p.prefix.row_tiles = (int)(in_4 / 128);
   }
   // Up to 64 groups: the device shares the keys out, whatever the groups'
-  // lengths; no group has more splits than workgroups a KV head.
+  // lengths; no group has more splits than workgroups a KV head.  Either all
+  // row tiles' keys are whole, or they are split into `pieces` at most.  The
+  // launch has room for both, and each workgroup a place for its rows' sums:
+  // with places by row, as many as a row can have splits, 64 suffixes of 512
+  // tokens behind 16384 would take 18 GB of scratch instead of 1.1.
   p.pieces = p.blocks = 0;
   if (p.prefix.prompt && sh.n_groups <= 64) {
     const int group = q.heads / c.heads, rows = 32 * p.prefix.waves;
     const long long key_tiles = (prefix + KEYS - 1) / KEYS;
-    const long long most = ((long long)b.n_rows * group + rows - 1) / rows * c.heads + (long long)sh.n_groups * c.heads;
+    const long long in_groups = std::min<long long>(b.n_rows, (long long)sh.n_groups * p.groups.max_q);
+    const long long most = ((in_groups * group + rows - 1) / rows + sh.n_groups) * c.heads;
     p.pieces = p.pairs ? 512 : 256;
     int s = p.pieces / c.heads;
     if (s > key_tiles / 4) s = (int)(key_tiles / 4);
     p.prefix.splits = s < 1 ? 1 : s < 48 ? s : 48;
-    p.blocks = most > p.pieces ? most : p.pieces;
+    p.blocks = std::max(most, std::min<long long>(p.pieces, most * p.prefix.splits));
   }
-  p.slots = p.prefix.splits + p.rest.splits;
-  p.sums = (size_t)b.n_rows * q.heads * p.slots;
-  // (a split launch's parts are the rows', not its own)
-  const size_t one = p.prefix.splits > 1 ? 0 : p.prefix.work, two = p.rest.splits > 1 ? 0 : p.rest.work;
-  p.own = one > two ? one : two;
-  p.work = p.sums * (c.hd * sizeof(float) + sizeof(float2)) + p.own + 64 * sizeof(int32_t);
+  const size_t rows = (size_t)b.n_rows * q.heads;
+  p.prefix_sums = p.pieces ? (size_t)p.blocks * 32 * p.prefix.waves : rows * p.prefix.splits;
+  p.sums = p.prefix_sums + (p.rest.splits > 1 ? p.rest.cells : rows);
+  p.sums += p.sums & 1;   // (what lies behind float2s is 16-byte aligned)
+  // one launch after the other: the same room for the parts of few rows that share out their keys
+  p.own = std::max(p.prefix.stream ? p.prefix.work : 0, p.rest.stream ? p.rest.work : 0);
+  p.own = (p.own + 15) / 16 * 16;
+  p.work = p.sums * (c.hd * sizeof(float) + sizeof(float2)) + p.own + 64 * sizeof(int4);
   return p;
 }
 
@@ -331,10 +339,9 @@ static int launch_attn(const char *op, Kv4AttnArgs &a, const Kv4Plan &p, const A
   return launch_plan(op, a, p, k, s);
 }
 
-// One of the two parts: its slots of the rows' parts, and its own workspace.
-static int launch_part(const char *op, Kv4AttnArgs a, const Kv4Plan &p, const AttnKernel &k, int slot, void *own, hipStream_t s,
+// One of the two parts, with its own workspace.
+static int launch_part(const char *op, Kv4AttnArgs a, const Kv4Plan &p, const AttnKernel &k, void *own, hipStream_t s,
                        long long blocks = 0) {
-  a.sum_slot = slot;
   if (p.stream) {
     a.slot_o = (float *)own;
     a.slot_ml = (float2 *)((float *)own + p.cells * 16 * a.tiles);
@@ -413,20 +420,21 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
   if (p.prefix.terms < 3) a.slack = fminf(2 * M_SLACK / a.scale2, 0x1p125f);
   a.sh = *shared;
   a.sh_seqs = batch->n_seq;
-  a.sum_slots = p.slots;
+  a.prefix_splits = p.prefix.splits;
+  a.rest_splits = p.rest.splits;
+  a.rest_first = (long long)p.prefix_sums;
   a.part_o = (float *)work;
   a.part_ml = (float2 *)(a.part_o + p.sums * cache->hd);
   void *own = a.part_ml + p.sums;
-  a.split_of = p.pieces ? (int32_t *)((char *)own + p.own) : nullptr;
   a.pieces = p.pieces;
-  a.prefix_slots = p.prefix.splits;
+  a.piece_shift = __builtin_ctz((unsigned)(32 * p.prefix.waves));
+  a.piece_blocks = (int)p.blocks;
+  a.piece_of = (int4 *)((char *)own + p.own);
   Kv4AttnArgs g = a;
   g.b = p.groups;
   const Kv4Plan &one = p.prefix, &two = p.rest;
   if (p.joined) {
     long long n1 = 0, n2 = 0;
-    g.sum_slot = 0;
-    a.sum_slot = one.splits;
     BFP_TRY(plan_args(op, g, one, n1));
     BFP_TRY(plan_args(op, a, two, n2));
     if (n1 + n2 > 0x3ffffff / one.waves)
@@ -439,10 +447,9 @@ int bfp_kv4_attn_shared_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, cons
     return launch_status(op);
   }
   BFP_TRY(launch_part(op, g, one, one.prompt ? prefix_prompt_kernel(a.tiles, one.terms, p.pairs) : prefix_rows_kernel(a.tiles, one.terms, one.waves, one.stream > 0),
-                      0, own, s, p.blocks));
+                      own, s, p.blocks));
   BFP_TRY(launch_part(op, a, two, two.prompt ? rest_prompt_kernel(a.tiles, two.terms) : rest_rows_kernel(a.tiles, two.terms, two.waves, two.stream > 0),
-                      one.splits, own, s));
-  a.sum_slot = one.splits;
+                      own, s));
   launch_join_shared(a, s);
   return launch_status(op);
 }

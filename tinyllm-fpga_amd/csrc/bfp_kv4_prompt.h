@@ -394,7 +394,9 @@ __global__ __launch_bounds__(64 * W, W == 8 || in_pairs(TB, T, W) ? 2 : 1) void 
     const long long tok = sp.row0 + ri;
     const float L = ml[32 + row];
     if (SEES >= SEES_PREFIX) {
-      const long long at = (tok * a.q.heads + rh) * a.sum_slots + a.sum_slot + split;
+      const long long at = SEES == SEES_REST ? rest_place(a, seq, ri, tok, rh, split)
+                           : a.pieces        ? (long long)blockIdx.x * ROWS + 32 * w + row
+                                             : prefix_place(a, tok, rh, split);
       if (live[k] && piece == 0) a.part_ml[at] = make_float2(ml[row], L);
       to[k] = at * hd;
       over[k] = 1.0f;

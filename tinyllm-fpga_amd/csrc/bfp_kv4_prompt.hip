@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void k_kv4_join_prompt(Kv4AttnArgs a) {
 // are not there outside every group, and those of the rest.  A wave takes one
 // row and query head, 16 bytes a lane, so that several slots' values are
 // loaded at once, and four such loads are under way.  Bound by the slots' bytes
-// (64 rows of 32 heads of 128, 33 slots: 35 MB in 8.6 us).
+// (64 rows of 32 heads of 128, 33 slots: 35 MB in 8.9 us).
 __global__ __launch_bounds__(256) void k_kv4_join_shared(Kv4AttnArgs a) {
   __shared__ float rows[4][256];
   const int seq = blockIdx.y;
@@ -51,13 +51,27 @@ __global__ __launch_bounds__(256) void k_kv4_join_shared(Kv4AttnArgs a) {
   const int w = threadIdx.x >> 6, u = blockIdx.x * 4 + w, lane = threadIdx.x & 63;
   const int i = u / a.q.heads, qh = u % a.q.heads;
   if (i >= sp.n) return;   // (no barrier below)
-  const long long tok = sp.row0 + i, at = (tok * a.q.heads + qh) * a.sum_slots;
+  const long long tok = sp.row0 + i, rest = rest_place(a, seq, i, tok, qh, 0);
   const int hd = 16 * a.tiles;
-  int g, before = 0;
-  if (kv4_shared_len(a, seq, g) > 0) before = a.split_of ? min(a.split_of[g], a.prefix_slots) : a.prefix_slots;
-  const int n = before + a.sum_slots - a.prefix_slots;   // slot k of them
-  auto slot = [&](int k) { return k < before ? k : k - before + a.prefix_slots; };
-  const float2 ml = lane < n ? a.part_ml[at + slot(lane)] : make_float2(-INFINITY, 0.0f);
+  int g, before = 0;   // of its n parts the prefix's
+  long long place = prefix_place(a, tok, qh, 0), step = 1;   // where the first lies, and how far apart they are
+  if (kv4_shared_len(a, seq, g) > 0) {
+    before = a.prefix_splits;
+    if (a.pieces) {
+      const int4 of = a.piece_of[g];
+      uint32_t of_head;
+      const int head = (int)a.by_group.div((uint32_t)qh, of_head), row = (int)(tok - of.w) * a.group + (int)of_head;
+      const int rt = row >> a.piece_shift, tiles = of.z * a.c.heads, block = of.y + rt * a.c.heads + head;
+      before = min(of.x, a.prefix_splits);
+      place = ((long long)block << a.piece_shift) + (row & ((1 << a.piece_shift) - 1));
+      step = (long long)tiles << a.piece_shift;
+      // (rows past max_rows, groups that overlap: nobody took them)
+      if (row < 0 || rt >= of.z || of.y < 0 || block < 0 || block + (before - 1LL) * tiles >= a.piece_blocks) before = 0;
+    }
+  }
+  const int n = before + a.rest_splits;
+  auto slot = [&](int k) { return k < before ? place + k * step : rest + k - before; };
+  const float2 ml = lane < n ? a.part_ml[slot(lane)] : make_float2(-INFINITY, 0.0f);
   // lanes of a slot, slots at a time; this lane's
   const int lanes = hd / 4, each = 64 / lanes, mine = lane / lanes, d = 4 * (lane - mine * lanes);
   f32x4 acc = {0, 0, 0, 0}, x[4];
@@ -66,7 +80,7 @@ __global__ __launch_bounds__(256) void k_kv4_join_shared(Kv4AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {   // past the last slot: it again, with the factor 0 (its NaN, if it has one, is the row's anyway)
       const int k = k0 + e * each + mine;
-      x[e] = *(const f32x4 *)(a.part_o + (at + slot(k < n ? k : n - 1)) * hd + d);
+      x[e] = *(const f32x4 *)(a.part_o + slot(k < n ? k : n - 1) * hd + d);
     }
     if (k0 == 0) {   // while the first ones are under way
       M = wave_max(ml.x);

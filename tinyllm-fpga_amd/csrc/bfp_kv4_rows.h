@@ -263,8 +263,13 @@ template <Kv4Sees SEES>
 __device__ __forceinline__ float *slot_o(const Kv4AttnArgs &a) { return SEES >= SEES_PREFIX ? a.slot_o : a.part_o; }
 template <Kv4Sees SEES>
 __device__ __forceinline__ float2 *slot_ml(const Kv4AttnArgs &a) { return SEES >= SEES_PREFIX ? a.slot_ml : a.part_ml; }
+template <Kv4Sees SEES>
+__device__ __forceinline__ long long sum_place(const Kv4AttnArgs &a, long long tok, int qh) {   // (these launches split no row's keys)
+  return SEES == SEES_PREFIX ? prefix_place(a, tok, qh, 0) : rest_place(a, 0, 0, tok, qh, 0);
+}
+template <Kv4Sees SEES>
 __device__ __forceinline__ void leave_sum(const Kv4AttnArgs &a, long long tok, int qh, int d, float2 ml, float v) {
-  const long long at = (tok * a.q.heads + qh) * a.sum_slots + a.sum_slot;
+  const long long at = sum_place<SEES>(a, tok, qh);
   if (d == 0) a.part_ml[at] = ml;
   a.part_o[at * (16 * a.tiles) + d] = v;
 }
@@ -704,7 +709,7 @@ __device__ __forceinline__ void rows_block(const Kv4AttnArgs &a, uint32_t block)
         const long long tok = sp.row0 + token_of<SEES>(a, row_t, rr0 + row);
         const int rh = head * G + head_of<SEES>(a, rr0 + row);
         if (SEES >= SEES_PREFIX) {
-          const long long at = (tok * a.q.heads + rh) * a.sum_slots + a.sum_slot;
+          const long long at = sum_place<SEES>(a, tok, rh);
           if (d == 0) a.part_ml[at] = make_float2(top[row], L);
           float4 *p = (float4 *)(a.part_o + at * hd + d);
           p[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -735,7 +740,7 @@ __device__ __forceinline__ void rows_block(const Kv4AttnArgs &a, uint32_t block)
         if (d == 0) put(slot_ml<SEES>(a) + slot * R + row, make_float2(M, L));
         put(slot_o<SEES>(a) + ((long long)slot * R + row) * hd + d, acc);
       } else if (SEES >= SEES_PREFIX) {
-        leave_sum(a, tok, rh, d, make_float2(M, L), acc);
+        leave_sum<SEES>(a, tok, rh, d, make_float2(M, L), acc);
       } else {
         out_store(a.out, tok * a.out.row_stride + rh * a.out.head_stride + d, L == 0.0f ? 0.0f : acc / L);
       }
@@ -806,7 +811,7 @@ __device__ __forceinline__ void join_values(const Kv4AttnArgs &a, const RowsSeq 
       const long long tok = sp.row0 + token_of<SEES>(a, row_t, rr);
       const int qh = head * G + head_of<SEES>(a, rr);
       if (SEES >= SEES_PREFIX)
-        leave_sum(a, tok, qh, (v0 + u) % hd, make_float2(top[r], L), sum);
+        leave_sum<SEES>(a, tok, qh, (v0 + u) % hd, make_float2(top[r], L), sum);
       else
         out_store(a.out, tok * a.out.row_stride + qh * a.out.head_stride + (v0 + u) % hd, L == 0.0f ? 0.0f : sum / L);
     }
