@@ -745,15 +745,21 @@ size_t bfp_pages_work(const bfp_pages *pool, int n);
 int bfp_pages_copy_d(const bfp_pages *pool, const int32_t *src, const int32_t *dst, int n, void *stream);
 /* A page for every entry of the batch's table that its new rows lie in (as
  * bfp_kv4_append_d writes them) and that holds none; the entry becomes -1
- * where there is none left.  Writes batch->pages. */
+ * where there is none left.  Writes batch->pages.  What a page held stays in it:
+ * where an entry held none though the sequence has earlier tokens there (its
+ * page was not left when they were appended, or a parent had none), the new page
+ * does not hold those, and attention would take what it finds for them.  Such a
+ * sequence is given up, or goes on from its last whole page. */
 int bfp_pages_reserve_d(const bfp_pages *pool, const bfp_kv4_batch *batch, void *work, size_t work_bytes, void *stream);
 /* Branches: row i of out_pages (n x out_width) and out_len[i] go on from
  * sequence parents[i] of pages (n_seq x width) and len, which counts the
  * tokens that its pages hold.  Whole pages are shared (their refs rise); the
  * page in which the tokens end is copied to a page of its own.  Entries past
- * those are -1, also where no page was left for the copy, and what lies past
- * out_width is left out.  A parent outside [0, n_seq) gives an empty row.  What
- * out_pages held before is not looked at. */
+ * those are -1.  Where no page was left for the copy, its entry is -1 and
+ * out_len[i] ends with the whole pages: a program that keeps lengths of its own
+ * reads n_short before it goes on.  What lies past out_width is left out.  A
+ * parent outside [0, n_seq) gives an empty row.  What out_pages held before is
+ * not looked at. */
 int bfp_pages_fork_d(const bfp_pages *pool, const int32_t *pages, const int32_t *len, int n_seq, int width,
                      const int32_t *parents, int n, int32_t *out_pages, int32_t *out_len, int out_width, void *work,
                      size_t work_bytes, void *stream);

@@ -82,7 +82,10 @@ class PagePool(_rows.Fixed):
     def reserve(self, batch, work=None):
         """A page for every entry of batch.pages that the batch's new rows lie
         in and that holds none (is outside [0, n_pages)): before append.  An
-        entry for which none is left becomes -1, and its rows have no slot.
+        entry for which none is left becomes -1, and its rows have no slot:
+        once they have been appended the sequence is given up, or goes on
+        from its last whole page (a page that the entry is given later does
+        not hold them, but whatever was there).
         A page that another entry holds too is not replaced: fork a sequence
         that is cut back into one before it goes on."""
         if batch.device != self.device:
@@ -94,8 +97,9 @@ class PagePool(_rows.Fixed):
         """Branches: row i of the result goes on from sequence parents[i] of
         pages (sequences, width), of which lens tokens are cached.  Whole pages
         are shared; the page in which the tokens end is copied to one of its
-        own, in every cache.  Entries past those are -1, also where no page was
-        left for the copy.  A parent that does not exist gives an empty row.
+        own, in every cache.  Entries past those are -1.  Where no page was
+        left for the copy, its entry is -1 and the branch's length ends with
+        the whole pages.  A parent that does not exist gives an empty row.
         Returns (pages, lens), new tensors or `out`'s, whose pages are not
         given up first: free() them before."""
         p, n_seq, width = self._table(pages, "pages")

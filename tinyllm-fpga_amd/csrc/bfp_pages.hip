@@ -165,7 +165,8 @@ __device__ __forceinline__ int child_len(const ForkArgs &a, int i, const int32_t
   return n < 0 ? 0 : n < most ? n : most;
 }
 
-// The copies that the children need: src[i], dst[i] (-1: none).
+// The copies that the children need: src[i], dst[i] (-1: none; dst alone: no page
+// was left).
 __global__ __launch_bounds__(POOL_T) void k_pool_fork_plan(ForkArgs a) {
   __shared__ int waves[POOL_T / 64];
   int total = 0;
@@ -248,7 +249,9 @@ __device__ __forceinline__ void fork_tables(const ForkArgs &a, int blocks) {
       id = a.dst[i];
     }
     a.out_pages[e] = id;
-    if (p == 0) a.out_len[i] = n;
+    // without the copy it wanted, a child ends at its whole pages: a page that
+    // it is given later would hold another's tokens where its own are missing
+    if (p == 0) a.out_len[i] = a.src[i] >= 0 && a.dst[i] < 0 ? whole * a.page : n;
   }
 }
 
