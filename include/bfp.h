@@ -769,7 +769,7 @@ int bfp_pages_free_d(const bfp_pages *pool, int32_t *pages, long long n, void *s
 /* Moves the L pages that are held into pages 0 .. L-1: the k-th of those from
  * L on to the k-th free one below L, in every array, in refs and in the tables
  * (at most 16, all that hold any of the pool's).  An entry with a free page
- * from L on becomes -1.  *live = L (on the device). */
+ * becomes -1.  *live = L (on the device). */
 int bfp_pages_compact_d(const bfp_pages *pool, const bfp_page_table *tables, int n_tables, int32_t *live, void *work,
                         size_t work_bytes, void *stream);
 

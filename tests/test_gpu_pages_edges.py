@@ -59,3 +59,25 @@ def test_lengths_of_branches_that_lose_nothing(gpu):
         b.ref.fork(table, lens, [0, 1, 2], width)
         assert got.cpu().tolist() == lens
     b.check()
+
+
+@pytest.mark.parametrize("n_pages", [40, 5000])
+def test_compaction_clears_entries_of_free_pages(gpu, n_pages):
+    """A table whose pages were given up through another one names pages that
+    a compaction fills with others' tokens: its entries become -1, below the
+    held pages' number and above it."""
+    import torch
+    b = Both(n_pages, 16, heads=1, hd=16, layers=1)
+    rng = np.random.default_rng(n_pages)
+    held = rng.permutation(n_pages)[:n_pages // 2]
+    b.ref.refs[held] = 1
+    b.pool.refs.copy_(_int(b.ref.refs))
+    stale = np.array([[p for p in range(n_pages) if b.ref.refs[p] == 0]])
+    table = held[None].copy()
+    odd = np.array([[-1, -7, n_pages, 2 ** 31 - 1, -2 ** 31]])
+    dev = [_int(table), _int(stale), _int(odd)]
+    live = b.pool.compact(*dev)
+    assert int(live) == b.ref.compact(table)
+    assert (dev[0].cpu().numpy() == table).all()
+    assert (dev[1] == -1).all() and (dev[2].cpu().numpy() == odd).all()
+    b.check()

@@ -127,8 +127,9 @@ class PagePool(_rows.Fixed):
 
     def compact(self, *tables, work=None):
         """Move the held pages into the lowest ones and rewrite `tables` (at
-        most 16: all that hold any).  Returns their number, an int32 tensor (1)
-        on the device: pages from there on are free."""
+        most 16: all that hold any; entries with a free page become -1).
+        Returns the held pages' number, an int32 tensor (1) on the device:
+        pages from there on are free."""
         ts = (PageTableC * max(len(tables), 1))()
         for i, t in enumerate(tables):
             p, n, width = self._table(t, f"table {i}")

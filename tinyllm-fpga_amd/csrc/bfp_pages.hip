@@ -278,7 +278,8 @@ struct PoolTable {
   long long n;
 };
 struct CompactArgs {
-  int32_t *refs, *live, *moves, *src, *dst, *rank, *held;   // held: live pages of each chunk
+  // rank: of each page, -1 if it is free, and of those from L on which move is its; held: live pages of each chunk
+  int32_t *refs, *live, *moves, *src, *dst, *rank, *held;
   int n_pages, chunks;
   PoolTable table[POOL_TABLES];
   int n_tables;
@@ -349,10 +350,10 @@ __global__ __launch_bounds__(CHUNK_T) void k_pool_plan(CompactArgs a) {
     const bool is = (m >> k) & 1;
     if (id >= L) {
       if (is) a.src[r - below] = (int)id;
-      a.rank[id] = is ? r - below : -1;
     } else if (!is) {
       a.dst[id - r] = (int)id;
     }
+    a.rank[id] = !is ? -1 : id < L ? 0 : r - below;
     r += is;
   }
 }
@@ -363,9 +364,12 @@ __device__ __forceinline__ void compact_tables(const CompactArgs &a, int blocks)
   for (int t = 0; t < a.n_tables; ++t)
     for (long long e = first; e < a.table[t].n; e += step) {
       const int id = a.table[t].p[e];
-      if (id < L || id >= a.n_pages) continue;
-      const int k = a.rank[id];
-      a.table[t].p[e] = k < 0 ? -1 : a.dst[k];
+      if ((unsigned)id >= (unsigned)a.n_pages) continue;
+      const int k = a.rank[id];   // (the counts change in this launch)
+      if (k < 0)
+        a.table[t].p[e] = -1;   // free: another sequence's page lies there now, or none
+      else if (id >= L)
+        a.table[t].p[e] = a.dst[k];
     }
   for (long long k = first; k < n; k += step) {
     const int s = a.src[k];
