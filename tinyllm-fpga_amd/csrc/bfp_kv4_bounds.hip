@@ -117,6 +117,7 @@ struct Kv4PickArgs {
   bfp_rows q;
   const uint16_t *bounds;
   int group, i0, rows;        // rows i0 .. i0 + rows - 1 of every sequence
+  int products;               // that are added up to a score
   int n, first, last;         // pages to pick; of these the first and the last ones, whatever their scores
   int chunks, chunk;          // pieces of the pages, and how many pages each has
   FastDiv by_head, by_chunk, by_tile;
@@ -440,7 +441,7 @@ __device__ __forceinline__ double exact_score(const Kv4PickArgs &a, int id, int 
 
 // One row and KV head a workgroup of W waves.  Bound by its rounds of the
 // workgroup's waves, one after the other, each a barrier and a pass over LDS (64
-// rows and heads over 2048 pages 13 us, 4084 over 1024 35).  words: a bit for every page
+// rows and heads over 2048 pages 13 us, 4084 over 1024 36).  words: a bit for every page
 // that is taken, and for every one that may be; then the scores as keys, in
 // float32 and, of those at the border, in float64.
 template <int W>
@@ -505,12 +506,14 @@ __global__ __launch_bounds__(64 * W) void k_kv4_pick(Kv4PickArgs a) {
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < W; ++k) most = fmaxf(most, tops[k]);
-    // A product of 2 hd terms, 2^-23 of the sum of their magnitudes each (the
-    // matrix cores may cut); the second and third terms' sums, which are 2^-7
-    // and 2^-14 of the first's, P and N themselves (sums of the group's
-    // queries in float32, 2^-24 each) and the joining of the terms in what is
-    // added; magnitudes are of the first terms, at least 1 - 2^-7 of the whole.
-    const float e2 = 2.0f * (2 * a.c.hd + a.group + 16) * 0x1.06p-23f * most + 0x1p-120f;
+    // Every product that is added to a sum, 2^-23 of the sum of the magnitudes
+    // each (the matrix cores may cut): 2 hd, or three times as many where the
+    // terms go one after the other into one sum (a.products).  In what is
+    // added: P and N themselves (sums of the group's queries in float32, 2^-24
+    // each) and the joining of sums that hold a term each, of which the
+    // second and third are 2^-7 and 2^-14 of the first.  Magnitudes are of the
+    // first terms at least, 1 - 2^-7 of the whole.
+    const float e2 = 2.0f * (a.products + a.group + 16) * 0x1.06p-23f * most + 0x1p-120f;
     const bool exact_all = !(e2 < 0x1p120f);
     float A = 0.0f;
     if (!exact_all) {
@@ -762,6 +765,7 @@ int bfp_kv4_select_d(const bfp_kv4 *cache, const bfp_kv4_batch *batch, const uin
   a.bounds = bounds;
   a.group = q->heads / cache->heads;
   a.rows = p.rows;
+  a.products = (p.R == 16 ? 3 : 1) * 2 * cache->hd;
   a.n = n, a.first = first, a.last = last;
   a.chunks = p.chunks;
   a.chunk = p.chunk;
