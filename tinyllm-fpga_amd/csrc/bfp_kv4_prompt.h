@@ -12,8 +12,9 @@
 // read and decoded once for up to 256 of them.  As in prompts, exponentials and
 // products take turns (matrix cores busy 45%): three documents of up to 65536 tokens
 // with 239 rows of 16 heads behind them 200-234 us, 0.6 of the matrix product's rate
-// in two terms.  64 rows behind 16384 tokens: 38 us, of which the eight key tiles a
-// workgroup has are half, its first loads and its results the other.
+// in two terms.  64 samples' rows behind 16384 tokens, 256 a KV head: 49 us in two
+// terms, of which the eight key tiles a workgroup has are 30, its first loads and
+// its results the rest.
 #pragma once
 #include "bfp_kv4_attn.h"
 
